@@ -396,6 +396,25 @@ size_t tq_decode_noalloc_bytes(int B, int Hq, int Hkv, int n_split, const tq_lay
  * the first tq_decode_attn_paged_noalloc call on that device does nothing but launch.  Idempotent.         */
 int tq_noalloc_init(void);
 
+/* ---- the engine's paged exact cache -------------------------------------------------------------------------------
+ * k_cache / v_cache: blocks of 16 tokens, element (block, slot, h, :) at base + block*cs_blk + slot*cs_t + h*cs_h (in elements, the
+ * same for both), channels contiguous, `dtype`; bases and strides multiples of 16 bytes, cs_t up to 2^24 (TQ_EUNSUPPORTED otherwise); d a multiple of
+ * 64 up to 768.  block_table / bt_stride / seq_lens as tq_decode_attn_paged takes them, except that bt_stride 0 is TQ_EINVAL: a length
+ * beyond the row is cut to it, tokens of a block outside [0, num_blocks) have no weight.  The reference answers these calls through its
+ * engine's own backend (integration/vllm.py:290-318).
+ *
+ * tq_exact_decode: decode attention over the whole of that cache, exactly.  q (B, Hq, d), out (B, Hq, d) `dtype`, contiguous and on 16-byte
+ * boundaries; Hq / Hkv any whole number up to 1024; a sequence without tokens gives zeros.  max_len: a bound on seq_lens that the splits are
+ * planned for (longer ones are read whole, in larger shares).  n_split: 0, or how many workgroups share a sequence's tokens, up to 1024.
+ * weights (nullable): fp32, element (b, h, t) at base + b*w_b + h*w_h + t, weight_len tokens: every token's softmax weight, summed over the query
+ * heads of KV head h, is added to it (tokens from weight_len on have no place and are left out).  Summed in a fixed order.
+ * workspace: tq_exact_decode_bytes bytes (weight_len 0 without weights), 16-byte aligned, of this call alone until it has run.  0: sizes out of range. */
+size_t tq_exact_decode_bytes(int dtype, int B, int Hq, int Hkv, int d, int64_t max_len, int n_split, int64_t weight_len);
+int tq_exact_decode(const void *q, int dtype, int B, int Hq, int Hkv, int d, const void *k_cache, const void *v_cache,
+                    int64_t cs_blk, int64_t cs_t, int64_t cs_h, int64_t num_blocks, const int32_t *block_table, int bt_stride,
+                    const int32_t *seq_lens, float sm_scale, int64_t max_len, float *weights, int64_t w_b, int64_t w_h,
+                    int64_t weight_len, void *out, void *workspace, int n_split, void *stream);
+
 /* Log-sum-exp merge of n_parts partial results per (b, query head):
  * parts (B*Hq, n_parts, d+2) fp32 = [running max, sum of exp, un-normalised acc];
  * out (B*Hq, d) `dtype`.  The same operator a context-parallel shard exchange

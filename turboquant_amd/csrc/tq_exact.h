@@ -1,0 +1,69 @@
+// Attention over a paged EXACT cache: blocks of 16 tokens x KV heads x head_dim in fp32, fp16 or bf16, as a serving engine keeps them.
+#pragma once
+
+#include "tq_common.h"
+
+namespace tq {
+
+// A paged exact cache and the sequences in it.  Element strides; channels lie one behind another, rows start on 16-byte boundaries.
+struct ExactCache {
+  const void *k, *v;
+  int64_t s_blk, s_h;      // of a block, of a KV head
+  int32_t s_t;             // of a token
+  int32_t H, d;
+  int64_t num_blocks;
+  const int32_t* table;
+  const int32_t* lens;
+  int64_t table_step;      // entries from one sequence's row to the next; 0: one row for all
+  int32_t table_row;       // entries of a row
+};
+
+// tokens of sequence b that the cache can hold
+__device__ __forceinline__ int exact_len(const ExactCache& c, int b) {
+  const int64_t most = (int64_t)c.table_row * TQ_PAGE_TOKENS;
+  const int n = c.lens[b];
+  return n < 0 ? 0 : (n > most ? (int)most : n);
+}
+
+// Splits of a sequence: every workgroup takes `chunk` blocks of tokens, more of them only where a sequence would need more splits than there are
+// (a length beyond the bound that the host planned for).
+__host__ __device__ __forceinline__ int exact_blocks_per_split(int blocks, int n_split, int chunk) {
+  const int least = (blocks + n_split - 1) / n_split;
+  return least > chunk ? least : chunk;
+}
+__host__ __device__ __forceinline__ int exact_splits_used(int blocks, int n_split, int chunk) {
+  const int per = exact_blocks_per_split(blocks, n_split, chunk);
+  return (blocks + per - 1) / per;
+}
+
+constexpr int EXACT_HEADS = 16;                     // query heads of a workgroup: columns of a matrix instruction
+template <int DT> constexpr int exact_tokens() { return DT == TQ_F32 ? 16 : 32; }      // tokens of a wavefront's block
+
+struct ExactDecode {
+  ExactCache c;
+  const void* q;           // (B, Hq, d)
+  void* out;               // (B, Hq, d)
+  int32_t B, Hq, G, groups, n_split, chunk;
+  float scale2;            // scale x log2 e: the softmax is one of powers of two
+  float* acc;              // (B, Hq, n_split, d): numerators of a split; unused with one split
+  float2* ml;              // (B, Hq, n_split): its maximum (log2) and its sum
+  float* scores;           // (B, H, score_pages, G, 16) scaled scores (log2), for the weights; or null
+  int32_t score_pages;
+};
+
+struct ExactJoin {
+  const int32_t* lens;
+  int32_t table_row, B, Hq, H, G, d, n_split, chunk, block_tokens;
+  const float* acc;
+  const float2* ml;
+  void* out;
+  const float* scores;
+  int32_t score_pages;
+  float* weights;          // (B, H, L): element strides w_b, w_h
+  int64_t w_b, w_h;
+  int32_t L, weight_chunks;
+};
+
+template <int DT> int launch_exact_decode(const ExactDecode& a, hipStream_t stream);
+
+}  // namespace tq

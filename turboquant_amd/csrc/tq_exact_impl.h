@@ -1,0 +1,311 @@
+// The page-streaming kernel of decode attention over a paged exact cache (instantiated by one file per element type).
+//
+//   s[t] = scale q . k_t     out = sum_t exp(s[t] - m) v_t / sum_t exp(s[t] - m)     for the G query heads of a KV head at once
+//
+// A wavefront takes 32 tokens (fp32: 16) at a time, straight from memory into the operands of its matrix instructions - no shared memory, no
+// barrier in the loop:
+//   scores    tokens are rows, heads columns: a lane reads 16 bytes of the key of ONE token, which is its part of the row operand as it lies;
+//             the queries stay in registers as the column operand.  A lane gets scores of one head: four tokens of each sixteen.
+//   values    channels are rows, heads columns, tokens the contraction, in the order in which the lane holds the weights already: no weight
+//             changes its lane.  A lane reads 8 neighbouring channels (4 in the last 64 of an odd multiple of 64) of each of
+//             its 8 tokens - sixteen lanes a whole row - and turns the 8 x 8 block of halves around in registers (32 byte
+//             permutes a block of 128 channels); row r of channel tile t is channel 8 r + t, so the tiles need no exchange between lanes.
+//             fp32: a lane's four channels of a token are the row operands of four instructions as they are.
+//   softmax   one pass: running maximum and sum per head; a lane's accumulators all belong to its head, so a move of the maximum is a
+//             scalar of the lane.  Maximum, sum, scores and numerators are fp32; the weights are rounded to the cache's 16-bit type for the
+//             product (relative 2^-8 / 2^-11 at most, the size of the output's own rounding, and independent from token to token).
+// Tokens behind the length and those of a block number outside the cache have no weight; what lies in their slots is not used in any
+// product, so that NaN left there stays there.
+#pragma once
+
+#include "tq_exact.h"
+
+namespace tq {
+
+typedef float ex_f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t ex_u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t ex_u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 ex_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 ex_f16x8 __attribute__((ext_vector_type(8)));
+
+template <int DT>
+__device__ __forceinline__ ex_f32x4 ex_mfma(ex_u32x4 a, ex_u32x4 b, ex_f32x4 c) {
+  static_assert(DT == TQ_BF16 || DT == TQ_F16, "16-bit elements");
+  if constexpr (DT == TQ_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ex_bf16x8, a), __builtin_bit_cast(ex_bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ex_f16x8, a), __builtin_bit_cast(ex_f16x8, b), c, 0, 0, 0);
+}
+
+// two weights to the cache's type, nearest even
+template <int DT>
+__device__ __forceinline__ uint32_t ex_pack(float lo, float hi) {
+  if constexpr (DT == TQ_BF16) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const b2 r = {(__bf16)lo, (__bf16)hi};
+    return __builtin_bit_cast(uint32_t, r);
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 r = {(_Float16)lo, (_Float16)hi};
+    return __builtin_bit_cast(uint32_t, r);
+  }
+}
+
+// maximum / sum over the four lanes that hold a head (16 lanes apart)
+__device__ __forceinline__ float ex_quad_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float ex_quad_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Channel of accumulator element i (0..3) of channel tile `tile` in a lane of quarter `quarter`.
+// Chunks of 128 channels (16-bit types) or 64: rows of a chunk's tiles are 8 or 4 channels apart.
+template <int DT, int D>
+__device__ __forceinline__ int ex_channel(int tile, int quarter, int i) {
+  constexpr int WIDE = DT == TQ_F32 ? 0 : D / 128;          // chunks of 128
+  if (tile < WIDE * 8) return (tile >> 3) * 128 + (quarter * 4 + i) * 8 + (tile & 7);
+  const int t = tile - WIDE * 8;
+  return WIDE * 128 + (t >> 2) * 64 + (quarter * 4 + i) * 4 + (t & 3);
+}
+
+template <int DT, int D>
+constexpr int exact_waves_per_simd() { return D <= 128 ? (DT == TQ_F32 ? 3 : 4) : (D <= 256 ? 2 : 1); }
+
+template <int DT, int D>
+__global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_decode_kernel(const ExactDecode a) {
+  constexpr bool F32 = DT == TQ_F32;
+  constexpr int TB = exact_tokens<DT>(), PAGES = TB / TQ_PAGE_TOKENS;
+  constexpr int SIZE = F32 ? 4 : 2;
+  constexpr int KSTEPS = D * SIZE / 64;                      // 16-byte pieces that a lane reads of a key
+  constexpr int TILES = D / 16;                              // channel tiles
+  constexpr int WIDE = F32 ? 0 : D / 128, NARROW = (D - WIDE * 128) / 64;
+  using St = typename Elem<DT>::storage;
+
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  const int col = lane & 15, quarter = lane >> 4;            // head of the group; which four tokens of sixteen
+  int id = (int)blockIdx.x;
+  const int split = id % a.n_split; id /= a.n_split;
+  const int group = id % a.groups; id /= a.groups;
+  const int h = id % a.c.H, b = id / a.c.H;
+
+  const int len = exact_len(a.c, b);
+  const int blocks = (len + TB - 1) / TB;
+  const int per = exact_blocks_per_split(blocks, a.n_split, a.chunk);
+  const int first = split * per < blocks ? split * per : blocks, last = first + per < blocks ? first + per : blocks;
+  if (first >= last && a.n_split > 1) return;
+
+  const int head = group * EXACT_HEADS + col;                // of the KV head's G query heads
+  const bool live = head < a.G;
+  const int64_t row = (int64_t)b * a.Hq + h * a.G + head;
+  const int32_t* table = a.c.table + b * a.c.table_step;
+
+  ex_u32x4 Q[KSTEPS];
+#pragma unroll
+  for (int s = 0; s < KSTEPS; ++s) {
+    Q[s] = ex_u32x4{0, 0, 0, 0};
+    if (live) Q[s] = *(const ex_u32x4*)((const char*)a.q + (row * D) * SIZE + s * 64 + quarter * 16);
+  }
+  ex_f32x4 O[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) O[t] = ex_f32x4{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+  // fp16 weights are multiplied by 2^14, the largest power that holds them: without it a long context's many small ones would round to nothing
+  constexpr float LIFT = DT == TQ_F16 ? 14.0f : 0.0f;
+
+  for (int blk = first + wave; blk < last; blk += 4) {
+    // pages of the block: those behind the sequence or outside the cache give their tokens no weight
+    const int t0 = blk * TB;
+    const char *kp[PAGES], *vp[PAGES];
+    int valid[PAGES];                                        // tokens of the page that count
+    bool whole = true;
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p) {
+      const int left = len - t0 - p * TQ_PAGE_TOKENS;
+      valid[p] = left < 0 ? 0 : (left > TQ_PAGE_TOKENS ? TQ_PAGE_TOKENS : left);
+      int64_t page = left > 0 ? table[blk * PAGES + p] : 0;
+      if (page < 0 || page >= a.c.num_blocks) { page = 0; valid[p] = 0; }
+      whole &= valid[p] == TQ_PAGE_TOKENS;
+      const int64_t off = (page * a.c.s_blk + h * a.c.s_h) * SIZE;
+      kp[p] = (const char*)a.c.k + off;
+      vp[p] = (const char*)a.c.v + off;
+    }
+    // ---- scores ----
+    const uint32_t krow = (uint32_t)col * (uint32_t)a.c.s_t * SIZE + quarter * 16;
+    ex_f32x4 S[PAGES];
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p) {
+      S[p] = ex_f32x4{0, 0, 0, 0};
+      const bool there = whole || col < valid[p];
+#pragma unroll
+      for (int s = 0; s < KSTEPS; ++s) {
+        ex_u32x4 kf = {0, 0, 0, 0};
+        if (there) kf = *(const ex_u32x4*)(kp[p] + krow + s * 64);
+        if constexpr (F32) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            S[p] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[i]), __uint_as_float(Q[s][i]), S[p], 0, 0, 0);
+        } else {
+          S[p] = ex_mfma<DT>(kf, Q[s], S[p]);
+        }
+      }
+    }
+    // ---- weights of this lane's head: tokens quarter * 4 + i of each page ----
+    float top = -INFINITY, pr[PAGES][4];
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float s2 = S[p][i] * a.scale2;
+        pr[p][i] = whole || quarter * 4 + i < valid[p] ? s2 : -INFINITY;
+        top = fmaxf(top, pr[p][i]);
+      }
+    if (a.scores && live) {
+#pragma unroll
+      for (int p = 0; p < PAGES; ++p) {
+        const int page = blk * PAGES + p;
+        if (page < a.score_pages)
+          *(ex_f32x4*)(a.scores + ((((int64_t)b * a.c.H + h) * a.score_pages + page) * a.G + head) * TQ_PAGE_TOKENS + quarter * 4) =
+              ex_f32x4{pr[p][0], pr[p][1], pr[p][2], pr[p][3]};
+      }
+    }
+    top = fmaxf(m, ex_quad_max(top));
+    if (__any(top > m)) {
+      const float move = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+      l *= move;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) O[t] *= move;
+      m = top;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m - LIFT;
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pr[p][i] = __builtin_amdgcn_exp2f(pr[p][i] - ref);
+        l += pr[p][i];
+      }
+    // ---- values ----
+    const uint32_t vrow = (uint32_t)(quarter * 4) * (uint32_t)a.c.s_t * SIZE;
+    const uint32_t step = (uint32_t)a.c.s_t * SIZE;
+    if constexpr (F32) {
+#pragma unroll
+      for (int c = 0; c < NARROW; ++c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ex_f32x4 x = {0, 0, 0, 0};
+          if (whole || quarter * 4 + i < valid[0]) x = *(const ex_f32x4*)(vp[0] + vrow + i * step + (c * 64 + col * 4) * SIZE);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) O[c * 4 + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t], pr[0][i], O[c * 4 + t], 0, 0, 0);
+        }
+      }
+    } else {
+      ex_u32x4 P;
+#pragma unroll
+      for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) P[p * 2 + i] = ex_pack<DT>(pr[p][2 * i], pr[p][2 * i + 1]);
+#pragma unroll
+      for (int c = 0; c < WIDE; ++c) {
+        ex_u32x4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = ex_u32x4{0, 0, 0, 0};
+          if (whole || quarter * 4 + (i & 3) < valid[i >> 2])
+            x[i] = *(const ex_u32x4*)(vp[i >> 2] + vrow + (i & 3) * step + (c * 128 + col * 8) * SIZE);
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          ex_u32x4 f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            f[j] = __builtin_amdgcn_perm(x[2 * j + 1][t >> 1], x[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+          O[c * 8 + t] = ex_mfma<DT>(f, P, O[c * 8 + t]);
+        }
+      }
+      if constexpr (NARROW > 0) {
+        ex_u32x2 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = ex_u32x2{0, 0};
+          if (whole || quarter * 4 + (i & 3) < valid[i >> 2])
+            x[i] = *(const ex_u32x2*)(vp[i >> 2] + vrow + (i & 3) * step + (WIDE * 128 + col * 4) * SIZE);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          ex_u32x4 f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            f[j] = __builtin_amdgcn_perm(x[2 * j + 1][t >> 1], x[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+          O[WIDE * 8 + t] = ex_mfma<DT>(f, P, O[WIDE * 8 + t]);
+        }
+      }
+    }
+  }
+
+  // ---- the four wavefronts of the workgroup: to a common maximum, then summed pairwise (2, 3 -> 0, 1 -> 0) ----
+  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ __align__(16) ex_f32x4 s_acc[2][TILES][64];
+  l = ex_quad_sum(l);
+  if (quarter == 0) { s_m[wave][col] = m; s_l[wave][col] = l; }
+  __syncthreads();
+  const float M = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
+  const float ref = M == -INFINITY ? 0.0f : M;
+  const float f = __builtin_amdgcn_exp2f(m - ref);
+  float sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) sum += s_l[w][col] * __builtin_amdgcn_exp2f(s_m[w][col] - ref);
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) O[t] *= f;
+  if (wave >= 2)
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) s_acc[wave - 2][t][lane] = O[t];
+  __syncthreads();
+  if (wave < 2)
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) O[t] += s_acc[wave][t][lane];
+  __syncthreads();
+  if (wave == 1)
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) s_acc[0][t][lane] = O[t];
+  __syncthreads();
+  if (wave != 0 || !live) return;
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) O[t] += s_acc[0][t][lane];
+  if (quarter == 0) a.ml[row * a.n_split + split] = make_float2(M - LIFT, sum);
+  const bool one = a.n_split == 1;
+  const float inv = one ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+  float* acc = one ? nullptr : a.acc + (row * a.n_split + split) * D;
+  St* out = (St*)a.out + row * D;
+#pragma unroll
+  for (int t = 0; t < TILES; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = ex_channel<DT, D>(t, quarter, i);
+      if (one) Elem<DT>::store(out, c, O[t][i] * inv);
+      else acc[c] = O[t][i];
+    }
+}
+
+template <int DT>
+int launch_exact_decode(const ExactDecode& a, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)a.n_split * a.groups * a.c.H * a.B)), block(256);
+#define TQ_EXACT_D(D) \
+  case D: exact_decode_kernel<DT, D><<<grid, block, 0, stream>>>(a); break
+  switch (a.c.d) {
+    TQ_EXACT_D(64); TQ_EXACT_D(128); TQ_EXACT_D(192); TQ_EXACT_D(256); TQ_EXACT_D(320); TQ_EXACT_D(384);
+    TQ_EXACT_D(448); TQ_EXACT_D(512); TQ_EXACT_D(576); TQ_EXACT_D(640); TQ_EXACT_D(704); TQ_EXACT_D(768);
+    default: return TQ_EUNSUPPORTED;
+  }
+#undef TQ_EXACT_D
+  TQ_CHECK_LAUNCH();
+  return TQ_OK;
+}
+
+}  // namespace tq
