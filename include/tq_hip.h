@@ -415,6 +415,38 @@ int tq_exact_decode(const void *q, int dtype, int B, int Hq, int Hkv, int d, con
                     const int32_t *seq_lens, float sm_scale, int64_t max_len, float *weights, int64_t w_b, int64_t w_h,
                     int64_t weight_len, void *out, void *workspace, int n_split, void *stream);
 
+/* What a prompt's newest queries make of the tokens of that cache: the softmax weights of the newest min(window, rows of the sequence, seq_lens[b])
+ * queries of every sequence, causal among themselves, summed over them and the query heads of KV head h, are added to weights (as in
+ * tq_exact_decode).  q (rows, Hq, d) contiguous, 16-byte aligned; sequence b's rows are query_start_loc[b] .. query_start_loc[b + 1] - 1 (device, B + 1
+ * entries; what lies outside 0 .. rows is left out), the last of them at position seq_lens[b] - 1.  window up to 1024.  Values are not read. */
+size_t tq_exact_window_bytes(int dtype, int B, int Hq, int Hkv, int d, int window, int64_t max_len);
+int tq_exact_window(const void *q, int dtype, int64_t rows, const int32_t *query_start_loc, int B, int Hq, int Hkv, int d,
+                    int window, const void *k_cache, int64_t cs_blk, int64_t cs_t, int64_t cs_h, int64_t num_blocks,
+                    const int32_t *block_table, int bt_stride, const int32_t *seq_lens, float sm_scale, int64_t max_len,
+                    float *weights, int64_t w_b, int64_t w_h, int64_t weight_len, void *workspace, void *stream);
+
+/* Which tokens stay when sequences of more than `budget` tokens are cut to it, per sequence and KV head: first those with a position below
+ * `sinks` or from seen[b] - recent on, then by weight (NaN last, +inf as the largest number), of two alike the one in the lower slot.
+ * A slot below the budget whose token goes is a hole; the k-th hole takes the k-th of the tokens that stay behind the budget, the others stay
+ * where they are.  weights / positions: fp32 / int32 (B, H, L), element (b, h, slot) at base + b*.._b + h*.._h + slot; seq_lens and seen
+ * (tokens that a sequence has had in all; NULL: seq_lens) are device int32 (B,); lengths above L are cut to L.  1 <= budget, sinks + recent <= budget.
+ * Written: lens_out (B,) = min(length, budget); count (B, H) moves; dst / src (B, H, moves) slots, ascending, -1 from count on, moves at
+ * least max(1, min(budget, L - budget)); weights_out / positions_out (B, H, L), which may be the inputs themselves (same address and strides):
+ * those of the tokens that stay, then 0 and the positions that the next tokens will have.
+ * tq_move_tokens_exact, tq_move_tokens_pool: carry the moves out in an exact cache (all strides in elements) / in the compressed pages of
+ * the same block numbers (`budget`: the one of the selection).  A sequence's pages must be its own: tokens are overwritten in place.  Moves that
+ * touch a page outside the table row or the cache are left out.                                                                   */
+int tq_evict_select(const float *weights, int64_t w_b, int64_t w_h, const int32_t *positions, int64_t p_b, int64_t p_h,
+                    const int32_t *seq_lens, const int32_t *seen, int B, int H, int L, int budget, int sinks, int recent,
+                    int moves, int32_t *lens_out, int32_t *count, int32_t *dst, int32_t *src, float *weights_out, int64_t wo_b,
+                    int64_t wo_h, int32_t *positions_out, int64_t po_b, int64_t po_h, void *stream);
+int tq_move_tokens_exact(void *k_cache, void *v_cache, int dtype, int d, int64_t cs_blk, int64_t cs_t, int64_t cs_h,
+                         int64_t num_blocks, const int32_t *block_table, int bt_stride, const int32_t *count, const int32_t *dst,
+                         const int32_t *src, int B, int H, int moves, void *stream);
+int tq_move_tokens_pool(uint8_t *pool, int64_t num_pages, const tq_page_layout *layout, const int32_t *block_table, int bt_stride,
+                        const int32_t *count, const int32_t *dst, const int32_t *src, int B, int H, int moves, int budget,
+                        void *stream);
+
 /* Log-sum-exp merge of n_parts partial results per (b, query head):
  * parts (B*Hq, n_parts, d+2) fp32 = [running max, sum of exp, un-normalised acc];
  * out (B*Hq, d) `dtype`.  The same operator a context-parallel shard exchange

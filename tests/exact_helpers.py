@@ -102,3 +102,69 @@ def check_decode(seqs, q, got, scale, weights_before=None, weights_after=None, k
             allowed[:, :m] = w_err[:, :m] + 2 * STEP32 * (want[:, :m].abs() + w[:, :m])
             off = (after - want).abs()
             assert (off <= allowed).all(), f"weights of sequence {b}: off by {float((off / allowed.clamp_min(1e-30)).max()):.3g} of what is allowed"
+
+
+def window64(seqs, q, starts, window, scale, keep=None, lens=None):
+    """Weights (B, H, longest) that the newest `window` rows of q (rows, Hq, d) give in 64 bits, and their bound (attention64's for
+    a weight; a sum over `rows` of them adds a half step each)."""
+    lens = seqs.lens if lens is None else lens
+    L = max(1, *lens)
+    H, d = seqs.H, seqs.d
+    out, err = (torch.zeros(len(lens), H, L, dtype=torch.float64) for _ in range(2))
+    for b, n in enumerate(lens):
+        run = max(0, min(starts[b + 1], q.shape[0]) - max(starts[b], 0))
+        W = min(window, run, n)
+        end = min(starts[b + 1], q.shape[0])
+        for w in range(W):
+            m = n - W + w + 1
+            kp = None if keep is None else keep[b][:m]
+            _, p, _, p_err = attention64(q[end - W + w], seqs.k64[b][:m], seqs.v64[b][:m], scale, kp)
+            out[b, :, :m] += p
+            err[b, :, :m] += p_err + W * q.shape[1] // H * STEP32 * p
+    return out, err
+
+
+def check_weights(got, before, add, err):
+    L = got.shape[2]
+    add, err = add[:, :, :L], err[:, :, :L]
+    want = before.double().clone()
+    want[:, :, : add.shape[2]] += add
+    allowed = torch.zeros_like(want)
+    allowed[:, :, : add.shape[2]] = err + 2 * STEP32 * (want[:, :, : add.shape[2]].abs() + add)
+    off = (got.cpu().double() - want).abs()
+    assert torch.isfinite(got).all()
+    assert (off <= allowed).all(), f"off by {float((off / allowed.clamp_min(1e-30)).max()):.3g} of what is allowed"
+
+
+def evict64(weights, positions, lens, seen, budget, sinks, recent):
+    """select_evictions by its definition, sequence by sequence, on lists."""
+    B, H, L = weights.shape
+    new_w, new_p = torch.zeros_like(weights), torch.empty_like(positions)
+    moves = max(1, min(budget, L - budget))
+    count = torch.zeros(B, H, dtype=torch.int32)
+    dst, src = (torch.full((B, H, moves), -1, dtype=torch.int32) for _ in range(2))
+    left = []
+    for b in range(B):
+        n = max(0, min(int(lens[b]), L))
+        had = int(lens[b]) if seen is None else int(seen[b])
+        left.append(min(n, budget))
+        for h in range(H):
+            w, p = weights[b, h, :n].tolist(), positions[b, h, :n].tolist()
+
+            def key(i):
+                if p[i] < sinks or p[i] >= had - recent:
+                    return 2, 0.0
+                x = w[i]
+                return 1, -math.inf if x != x else min(x, torch.finfo(torch.float32).max)
+            kept = set(sorted(range(n), key=lambda i: (-key(i)[0], -key(i)[1], i))[:budget])
+            holes = [i for i in range(min(n, budget)) if i not in kept]
+            movers = [i for i in range(budget, n) if i in kept]
+            assert len(holes) == len(movers)
+            where = {i: i for i in kept if i < budget} | dict(zip(holes, movers))
+            for to, of in where.items():
+                new_w[b, h, to], new_p[b, h, to] = weights[b, h, of], positions[b, h, of]
+            new_p[b, h, left[-1]:] = torch.arange(had, had + L - left[-1], dtype=torch.int32)
+            count[b, h] = len(holes)
+            dst[b, h, :len(holes)] = torch.tensor(holes, dtype=torch.int32)
+            src[b, h, :len(holes)] = torch.tensor(movers, dtype=torch.int32)
+    return torch.tensor(left, dtype=torch.int32), count, dst, src, new_w, new_p

@@ -112,6 +112,13 @@ _SIGNATURES = {
     "tq_exact_decode_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i64, _i, _i64]),
     "tq_exact_decode": (C.c_int, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i, _vp, _f, _i64, _vp, _i64, _i64, _i64, _vp, _vp,
                                   _i, _vp]),
+    "tq_exact_window_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i, _i64]),
+    "tq_exact_window": (C.c_int, [_vp, _i, _i64, _vp, _i, _i, _i, _i, _i, _vp, _i64, _i64, _i64, _i64, _vp, _i, _vp, _f, _i64, _vp, _i64, _i64, _i64,
+                                  _vp, _vp]),
+    "tq_evict_select": (C.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp,
+                                  _i64, _i64, _vp]),
+    "tq_move_tokens_exact": (C.c_int, [_vp, _vp, _i, _i, _i64, _i64, _i64, _i64, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "tq_move_tokens_pool": (C.c_int, [_vp, _i64, C.POINTER(TqPageLayout), _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "tq_decode_merge": (C.c_int, [_vp, _i64, _i, _i, _i, _vp, _vp]),
     "tq_time_next_page_kernel": (None, [_vp, _vp]),
     "tq_time_next_key_kernel": (None, [_vp, _vp]),
@@ -254,6 +261,13 @@ def ordinary(*tensors) -> bool:
                 return False
             device = at
     return True
+
+
+def changed(*tensors):
+    """Tell autograd that a kernel wrote to these tensors in place."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

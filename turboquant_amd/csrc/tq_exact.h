@@ -64,6 +64,10 @@ struct ExactJoin {
   int32_t L, weight_chunks;
 };
 
+// what the entry points check of a cache, and its description
+int exact_cache_init(ExactCache* c, const void* k, const void* v, int dtype, int H, int d, int64_t s_blk, int64_t s_t, int64_t s_h, int64_t num_blocks,
+                     const int32_t* table, int bt_stride, const int32_t* lens);
+
 template <int DT> int launch_exact_decode(const ExactDecode& a, hipStream_t stream);
 
 }  // namespace tq

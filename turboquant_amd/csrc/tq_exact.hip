@@ -144,7 +144,6 @@ static bool exact_plan(ExactPlan* p, int dtype, int B, int Hq, int Hkv, int d, i
   return grid <= INT32_MAX && join <= INT32_MAX;
 }
 
-// checks of a paged exact cache; `c` filled but for its sequences
 int exact_cache_init(ExactCache* c, const void* k, const void* v, int dtype, int H, int d, int64_t s_blk, int64_t s_t, int64_t s_h, int64_t num_blocks,
                      const int32_t* table, int bt_stride, const int32_t* lens) {
   if (!k || !v || !table || !lens) return TQ_ENULL;

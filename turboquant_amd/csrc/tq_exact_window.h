@@ -1,0 +1,32 @@
+// The weight that a prompt's newest queries give to the tokens of a paged exact cache.
+#pragma once
+
+#include "tq_exact.h"
+
+namespace tq {
+
+struct ExactWindow {
+  ExactCache c;                  // (its values are not read)
+  const void* q;                 // (rows, Hq, d)
+  const int32_t* starts;         // (B + 1): the rows of each sequence
+  int64_t rows;
+  int32_t B, Hq, G, W;           // W: newest rows of a sequence that count, at most
+  int32_t row_tiles, tile_waves, row_groups;     // tiles of 16 (query, head) rows at most; wavefronts side by side on them; turns that they take
+  int32_t n_split, chunk;        // as in decode
+  float scale2;
+  float2* ml;                    // (B, H, parts, row_tiles * 16): maximum (log2) and sum of a row over a part of the tokens
+  float2* stat;                  // (B, H, row_tiles * 16): of all tokens: maximum and 1 / sum
+  int32_t parts;
+  float* weights;
+  int64_t w_b, w_h;
+  int32_t L;
+};
+
+template <int DT> int launch_exact_window(const ExactWindow& a, bool add, hipStream_t stream);
+
+// row tiles that a wavefront holds as operands (and how many registers that takes: 4 d / 32 a tile, fp32 twice as many)
+__host__ __device__ constexpr int window_tiles(int dt, int d) {
+  return dt == TQ_F32 ? (d <= 64 ? 4 : (d <= 128 ? 2 : 1)) : (d <= 128 ? 4 : (d <= 256 ? 2 : 1));
+}
+
+}  // namespace tq

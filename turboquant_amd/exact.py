@@ -15,9 +15,11 @@ from typing import Optional
 import torch
 
 from . import _ffi
+from .eviction import Evictions
 from .paged import PAGE_TOKENS
 
 MAX_HEAD_DIM = 768
+MAX_WINDOW = 1024
 
 
 def _require_plain(t: torch.Tensor, name: str) -> None:
@@ -139,6 +141,8 @@ class ExactPagedCache:
                 *self._strides[:3], self.num_blocks, table.data_ptr(), bt_stride, lens.data_ptr(), float(scale), int(max_len),
                 w_ptr, w_b, w_h, w_len, out.data_ptr(), workspace.data_ptr(), splits, _ffi.stream_ptr(self.device)),
                 "tq_exact_decode")
+        if weights is not None:
+            _ffi.changed(weights)
         return out
 
     def _decode_bytes(self, B, Hq, max_len, splits, weight_len) -> int:
@@ -152,6 +156,68 @@ class ExactPagedCache:
     def workspace(self, B: int, Hq: int, max_len: int, n_split: Optional[int] = None, weight_len: int = 0) -> torch.Tensor:
         """A workspace for decode steps of this size; weight_len: the last dimension of `weights`, 0 without them."""
         return torch.empty(self._decode_bytes(B, Hq, max_len, n_split or 0, weight_len) // 4, dtype=torch.float32, device=self.device)
+
+    def add_window_weights(self, query: torch.Tensor, query_start_loc: torch.Tensor, block_table: torch.Tensor,
+                           seq_lens: torch.Tensor, weights: torch.Tensor, window: int, scale: Optional[float] = None,
+                           max_len: Optional[int] = None) -> torch.Tensor:
+        """Add to `weights` (as in decode_attention) the softmax weight that the newest `window` queries of every sequence
+        give to its tokens, summed over those queries and the query heads of a KV head: what there is to evict by
+        before the first token is decoded.  query (rows, Hq, d) holds the rows of an engine's step, sequence b's from
+        query_start_loc[b] to query_start_loc[b + 1], the last of them at position seq_lens[b] - 1; a query sees the tokens up
+        to its own.  A sequence with fewer rows gives those, one without rows nothing."""
+        _ffi.require_gpu(query, "query")
+        if query.dim() != 3:
+            raise ValueError("query must be (rows, Hq, d)")
+        rows, Hq, d = query.shape
+        if d != self.head_dim or Hq == 0 or Hq % self.num_kv_heads:
+            raise ValueError(f"Incompatible GQA shapes: Q={Hq}, H_kv={self.num_kv_heads}, d={d}")
+        if query.dtype != self.dtype or query.device != self.device:
+            raise TypeError("the query must have the cache's dtype and live on its GPU")
+        _require_plain(query, "query")
+        if query_start_loc.dim() != 1 or query_start_loc.shape[0] < 1:
+            raise ValueError("query_start_loc must have one entry more than there are sequences")
+        B = query_start_loc.shape[0] - 1
+        table, bt_stride, lens = self._sequences(block_table, seq_lens, B)
+        self._weights(weights, B)
+        if not 1 <= window <= MAX_WINDOW:
+            raise ValueError(f"window must be 1 .. {MAX_WINDOW}, got {window}")
+        if scale is None:
+            scale = 1.0 / math.sqrt(d)
+        if max_len is None:
+            max_len = table.shape[-1] * PAGE_TOKENS
+        if B == 0 or rows == 0:
+            return weights
+        query = query.contiguous()
+        if query.data_ptr() % 16:
+            query = query.clone()
+        starts = query_start_loc.to(device=self.device, dtype=torch.int32).contiguous()
+        need = _ffi.lib().tq_exact_window_bytes(self._tag, B, Hq, self.num_kv_heads, d, int(window), int(max_len)) if max_len >= 0 else 0
+        if need == 0:
+            raise ValueError(f"no plan for {B} sequences of {Hq} query heads, window {window}, max_len {max_len}")
+        workspace = torch.empty(need // 4, dtype=torch.float32, device=self.device)
+        with _ffi.on_device(self.device):
+            _ffi.check(_ffi.lib().tq_exact_window(
+                query.data_ptr(), self._tag, rows, starts.data_ptr(), B, Hq, self.num_kv_heads, d, int(window), self.key_cache.data_ptr(),
+                *self._strides[:3], self.num_blocks, table.data_ptr(), bt_stride, lens.data_ptr(), float(scale), int(max_len),
+                weights.data_ptr(), weights.stride(0), weights.stride(1), weights.shape[2], workspace.data_ptr(),
+                _ffi.stream_ptr(self.device)), "tq_exact_window")
+        _ffi.changed(weights)
+        return weights
+
+    # ---- eviction --------------------------------------------------------------------------------------------------------
+    def move_tokens(self, evictions: Evictions, block_table: torch.Tensor) -> None:
+        """Carry out the moves of `select_evictions` in these blocks, in place.  The sequences' blocks must be their own: a
+        block that two sequences share would change for both."""
+        count, dst, src, table, bt_stride = evictions.for_cache(block_table, self.num_kv_heads, self.device)
+        B, H, moves = dst.shape
+        if B == 0:
+            return
+        with _ffi.on_device(self.device):
+            _ffi.check(_ffi.lib().tq_move_tokens_exact(
+                self.key_cache.data_ptr(), self.value_cache.data_ptr(), self._tag, self.head_dim, *self._strides[:3], self.num_blocks,
+                table.data_ptr(), bt_stride, count.data_ptr(), dst.data_ptr(), src.data_ptr(), B, H, moves, _ffi.stream_ptr(self.device)),
+                "tq_move_tokens_exact")
+        _ffi.changed(self.key_cache, self.value_cache)
 
     def _check_workspace(self, workspace: torch.Tensor, need: int) -> None:
         _ffi.require_gpu(workspace, "workspace")

@@ -17,6 +17,7 @@ from typing import Optional
 import torch
 
 from . import _ffi
+from .eviction import Evictions
 from .quantizer import TurboQuantProd
 
 PAGE_TOKENS = _ffi.TQ_PAGE_TOKENS
@@ -450,6 +451,20 @@ class PagedKVPool:
                 key_cache.stride(1), key_cache.stride(2), int(ring_rows), out.data_ptr(), workspace.data_ptr(),
                 n_split, _ffi.stream_ptr(self.device)), "tq_decode_attn_paged_ring")
         return out
+
+    # ---- eviction ---------------------------------------------------------------
+    def move_tokens(self, evictions: Evictions, block_table: torch.Tensor) -> None:
+        """Carry out the moves of `select_evictions` in the compressed pages of block_table (B, max_pages), in place: codes,
+        norms and scales go along as they are.  The sequences' pages must be their own."""
+        count, dst, src, table, bt_stride = evictions.for_cache(block_table, self.num_kv_heads, self.device)
+        B, H, moves = dst.shape
+        if B == 0:
+            return
+        with _ffi.on_device(self.device):
+            _ffi.check(_ffi.lib().tq_move_tokens_pool(
+                self.data.data_ptr(), self.num_pages, C.byref(self.layout), table.data_ptr(), bt_stride, count.data_ptr(), dst.data_ptr(),
+                src.data_ptr(), B, H, moves, evictions.budget, _ffi.stream_ptr(self.device)), "tq_move_tokens_pool")
+        _ffi.changed(self.data)
 
 
 # what a native call goes past
