@@ -51,6 +51,30 @@ struct ExactDecode {
   int32_t score_pages;
 };
 
+// Which part of the work a workgroup takes.  Workgroups go to the eight dies in turn: the groups of heads of one part, which read the same keys and
+// values, go to one die one after another; the splits of a sequence go to different ones (with as many pairs of sequence and KV head as
+// dies, or splits as dies, a long sequence would otherwise be one die's work).
+__host__ __device__ __forceinline__ int64_t exact_grid(const ExactDecode& a) {
+  const int64_t parts = (int64_t)a.n_split * a.c.H * a.B;
+  return a.groups == 1 ? parts : (parts + 7) / 8 * 8 * a.groups;
+}
+__device__ __forceinline__ bool exact_place(const ExactDecode& a, int* split, int* group, int* h, int* b) {
+  const unsigned pairs = (unsigned)(a.c.H * a.B);
+  unsigned id = blockIdx.x, part = id;
+  *group = 0;
+  if (a.groups > 1) {
+    const unsigned turn = id >> 3;
+    *group = (int)(turn % (unsigned)a.groups);
+    part = (turn / (unsigned)a.groups) * 8 + (id & 7);
+    if (part >= pairs * (unsigned)a.n_split) return false;
+  }
+  const unsigned s = part / pairs, pair = (part - s * pairs + s) % pairs;
+  *split = (int)s;
+  *h = (int)(pair % (unsigned)a.c.H);
+  *b = (int)(pair / (unsigned)a.c.H);
+  return true;
+}
+
 struct ExactJoin {
   const int32_t* lens;
   int32_t table_row, B, Hq, H, G, d, n_split, chunk, block_tokens;

@@ -124,7 +124,7 @@ static bool exact_plan(ExactPlan* p, int dtype, int B, int Hq, int Hkv, int d, i
   const int64_t blocks = std::max<int64_t>(1, (max_len + p->block_tokens - 1) / p->block_tokens);
   int64_t n = n_split;
   if (n == 0) {
-    const int64_t resident = 256 * (d <= 128 ? (dtype == TQ_F32 ? 3 : 4) : (d <= 256 ? 2 : 1));
+    const int64_t resident = 256 * (d <= 64 ? 4 : (d <= 128 ? 3 : (d <= 256 ? 2 : 1)));
     n = std::max((resident + pairs - 1) / pairs, (max_len + 1023) / 1024);
     n = std::min<int64_t>(std::min<int64_t>(n, (blocks + 3) / 4), JOIN_MAX_SPLITS);
   }
@@ -140,7 +140,7 @@ static bool exact_plan(ExactPlan* p, int dtype, int B, int Hq, int Hkv, int d, i
   p->acc_at = at;     at = round256(at + (p->n_split > 1 ? rows * p->n_split * d * sizeof(float) : 0));
   p->scores_at = at;  at = round256(at + (size_t)B * Hkv * p->score_pages * G * TQ_PAGE_TOKENS * sizeof(float));
   p->bytes = at;
-  const int64_t grid = pairs * p->n_split, join = (int64_t)rows + (int64_t)B * Hkv * ((score_len + JOIN_TOKENS - 1) / JOIN_TOKENS);
+  const int64_t grid = (pairs * p->n_split + 8 * p->groups), join = (int64_t)rows + (int64_t)B * Hkv * ((score_len + JOIN_TOKENS - 1) / JOIN_TOKENS);
   return grid <= INT32_MAX && join <= INT32_MAX;
 }
 

@@ -76,7 +76,28 @@ __device__ __forceinline__ int ex_channel(int tile, int quarter, int i) {
 }
 
 template <int DT, int D>
-constexpr int exact_waves_per_simd() { return D <= 128 ? (DT == TQ_F32 ? 3 : 4) : (D <= 256 ? 2 : 1); }
+constexpr int exact_waves_per_simd() { return D <= 64 ? 4 : (D <= 128 ? 3 : (D <= 256 ? 2 : 1)); }
+
+// A block's pages: where they lie, and how many of their tokens count (none of a page behind the sequence or outside the cache: its loads
+// go to block 0, which is there, and what they bring is masked)
+template <int PAGES>
+struct ExactPages {
+  int64_t at[PAGES];                                         // byte offset of the KV head's first row
+  int valid[PAGES];
+  bool whole;
+  __device__ __forceinline__ void find(const ExactCache& c, const int32_t* table, int len, int blk, int h, int size) {
+    whole = true;
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p) {
+      const int left = len - (blk * PAGES + p) * TQ_PAGE_TOKENS;
+      valid[p] = left < 0 ? 0 : (left > TQ_PAGE_TOKENS ? TQ_PAGE_TOKENS : left);
+      int64_t page = left > 0 ? table[blk * PAGES + p] : 0;
+      if (page < 0 || page >= c.num_blocks) { page = 0; valid[p] = 0; }
+      whole &= valid[p] == TQ_PAGE_TOKENS;
+      at[p] = (page * c.s_blk + h * c.s_h) * size;
+    }
+  }
+};
 
 template <int DT, int D>
 __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_decode_kernel(const ExactDecode a) {
@@ -86,14 +107,15 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
   constexpr int KSTEPS = D * SIZE / 64;                      // 16-byte pieces that a lane reads of a key
   constexpr int TILES = D / 16;                              // channel tiles
   constexpr int WIDE = F32 ? 0 : D / 128, NARROW = (D - WIDE * 128) / 64;
+  constexpr int VTOKENS = F32 ? 4 : 8;                       // tokens of a lane
+  constexpr bool AHEAD = D <= 256;                           // keys and values are read a block ahead (above, their registers are the accumulators')
+  constexpr bool QUERIES_IN_LDS = D == 256;                  // (two wavefronts per SIMD: 256 registers)
   using St = typename Elem<DT>::storage;
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int col = lane & 15, quarter = lane >> 4;            // head of the group; which four tokens of sixteen
-  int id = (int)blockIdx.x;
-  const int split = id % a.n_split; id /= a.n_split;
-  const int group = id % a.groups; id /= a.groups;
-  const int h = id % a.c.H, b = id / a.c.H;
+  int split, group, h, b;
+  if (!exact_place(a, &split, &group, &h, &b)) return;
 
   const int len = exact_len(a.c, b);
   const int blocks = (len + TB - 1) / TB;
@@ -106,11 +128,19 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
   const int64_t row = (int64_t)b * a.Hq + h * a.G + head;
   const int32_t* table = a.c.table + b * a.c.table_step;
 
-  ex_u32x4 Q[KSTEPS];
+  __shared__ ex_u32x4 s_q[QUERIES_IN_LDS ? KSTEPS : 1][64];
+  ex_u32x4 Q[QUERIES_IN_LDS ? 1 : KSTEPS];
+  const auto query = [&](int s) __attribute__((always_inline)) {
+    ex_u32x4 x = {0, 0, 0, 0};
+    if (live) x = *(const ex_u32x4*)((const char*)a.q + (row * D) * SIZE + s * 64 + quarter * 16);
+    return x;
+  };
+  if constexpr (QUERIES_IN_LDS) {
+    for (int s = wave; s < KSTEPS; s += 4) s_q[s][lane] = query(s);
+    __syncthreads();
+  } else {
 #pragma unroll
-  for (int s = 0; s < KSTEPS; ++s) {
-    Q[s] = ex_u32x4{0, 0, 0, 0};
-    if (live) Q[s] = *(const ex_u32x4*)((const char*)a.q + (row * D) * SIZE + s * 64 + quarter * 16);
+    for (int s = 0; s < KSTEPS; ++s) Q[s] = query(s);
   }
   ex_f32x4 O[TILES];
 #pragma unroll
@@ -119,43 +149,75 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
   // fp16 weights are multiplied by 2^14, the largest power that holds them: without it a long context's many small ones would round to nothing
   constexpr float LIFT = DT == TQ_F16 ? 14.0f : 0.0f;
 
-  for (int blk = first + wave; blk < last; blk += 4) {
-    // pages of the block: those behind the sequence or outside the cache give their tokens no weight
-    const int t0 = blk * TB;
-    const char *kp[PAGES], *vp[PAGES];
-    int valid[PAGES];                                        // tokens of the page that count
-    bool whole = true;
+  const uint32_t step = (uint32_t)a.c.s_t * SIZE;
+  const uint32_t krow = (uint32_t)col * step + quarter * 16, vrow = (uint32_t)(quarter * 4) * step;
+  ex_u32x4 K[PAGES][KSTEPS];
+  ex_u32x4 V[WIDE > 0 ? WIDE : 1][VTOKENS];                  // (fp32: one chunk of 64 after another, below)
+  ex_u32x2 VN[VTOKENS];
+  ex_f32x4 VF[F32 ? NARROW : 1][4];
+  const auto load_key = [&](const ExactPages<PAGES>& at, int p, int s) __attribute__((always_inline)) {
+    K[p][s] = *(const ex_u32x4*)((const char*)a.c.k + at.at[p] + krow + s * 64);
+  };
+  const auto load_keys = [&](const ExactPages<PAGES>& at) __attribute__((always_inline)) {
 #pragma unroll
-    for (int p = 0; p < PAGES; ++p) {
-      const int left = len - t0 - p * TQ_PAGE_TOKENS;
-      valid[p] = left < 0 ? 0 : (left > TQ_PAGE_TOKENS ? TQ_PAGE_TOKENS : left);
-      int64_t page = left > 0 ? table[blk * PAGES + p] : 0;
-      if (page < 0 || page >= a.c.num_blocks) { page = 0; valid[p] = 0; }
-      whole &= valid[p] == TQ_PAGE_TOKENS;
-      const int64_t off = (page * a.c.s_blk + h * a.c.s_h) * SIZE;
-      kp[p] = (const char*)a.c.k + off;
-      vp[p] = (const char*)a.c.v + off;
+    for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+      for (int s = 0; s < KSTEPS; ++s) load_key(at, p, s);
+  };
+  const auto load_chunk = [&](const ExactPages<PAGES>& at, int c) __attribute__((always_inline)) {      // of 128 channels (fp32: 64)
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) VF[c][i] = *(const ex_f32x4*)((const char*)a.c.v + at.at[0] + vrow + i * step + (c * 64 + col * 4) * SIZE);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) V[c][i] = *(const ex_u32x4*)((const char*)a.c.v + at.at[i >> 2] + vrow + (i & 3) * step + (c * 128 + col * 8) * SIZE);
     }
-    // ---- scores ----
-    const uint32_t krow = (uint32_t)col * (uint32_t)a.c.s_t * SIZE + quarter * 16;
+  };
+  const auto load_narrow = [&](const ExactPages<PAGES>& at) __attribute__((always_inline)) {
+    if constexpr (!F32 && NARROW > 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) VN[i] = *(const ex_u32x2*)((const char*)a.c.v + at.at[i >> 2] + vrow + (i & 3) * step + (WIDE * 128 + col * 4) * SIZE);
+    }
+  };
+  constexpr int CHUNKS = F32 ? NARROW : WIDE;
+  const auto load_values = [&](const ExactPages<PAGES>& at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) load_chunk(at, c);
+    load_narrow(at);
+  };
+
+  ExactPages<PAGES> now, next;
+  if (first + wave < last) {
+    now.find(a.c, table, len, first + wave, h, SIZE);
+    if constexpr (AHEAD) {
+      load_keys(now);
+      load_values(now);
+    }
+  }
+  for (int blk = first + wave; blk < last; blk += 4) {
+    const bool more = blk + 4 < last;
+    if (more) next.find(a.c, table, len, blk + 4, h, SIZE);
+    int q_lane = lane;
+    if constexpr (QUERIES_IN_LDS) asm volatile("" : "+v"(q_lane));        // (the compiler would read them once, into registers that are not there)
+    // ---- scores; the next block's keys are on their way as soon as this one's are used ----
     ex_f32x4 S[PAGES];
 #pragma unroll
     for (int p = 0; p < PAGES; ++p) {
       S[p] = ex_f32x4{0, 0, 0, 0};
-      const bool there = whole || col < valid[p];
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) {
-        ex_u32x4 kf = {0, 0, 0, 0};
-        if (there) kf = *(const ex_u32x4*)(kp[p] + krow + s * 64);
+        if constexpr (!AHEAD) load_key(now, p, s);
+        const ex_u32x4 q = QUERIES_IN_LDS ? s_q[QUERIES_IN_LDS ? s : 0][q_lane] : Q[QUERIES_IN_LDS ? 0 : s];
         if constexpr (F32) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            S[p] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[i]), __uint_as_float(Q[s][i]), S[p], 0, 0, 0);
+            S[p] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(K[p][s][i]), __uint_as_float(q[i]), S[p], 0, 0, 0);
         } else {
-          S[p] = ex_mfma<DT>(kf, Q[s], S[p]);
+          S[p] = ex_mfma<DT>(K[p][s], q, S[p]);
         }
       }
     }
+    if (AHEAD && more) load_keys(next);
     // ---- weights of this lane's head: tokens quarter * 4 + i of each page ----
     float top = -INFINITY, pr[PAGES][4];
 #pragma unroll
@@ -163,7 +225,7 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float s2 = S[p][i] * a.scale2;
-        pr[p][i] = whole || quarter * 4 + i < valid[p] ? s2 : -INFINITY;
+        pr[p][i] = now.whole || quarter * 4 + i < now.valid[p] ? s2 : -INFINITY;
         top = fmaxf(top, pr[p][i]);
       }
     if (a.scores && live) {
@@ -191,19 +253,20 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
         pr[p][i] = __builtin_amdgcn_exp2f(pr[p][i] - ref);
         l += pr[p][i];
       }
-    // ---- values ----
-    const uint32_t vrow = (uint32_t)(quarter * 4) * (uint32_t)a.c.s_t * SIZE;
-    const uint32_t step = (uint32_t)a.c.s_t * SIZE;
+    // ---- values; those of tokens without weight are put to zero, since NaN times nothing is NaN ----
     if constexpr (F32) {
 #pragma unroll
-      for (int c = 0; c < NARROW; ++c) {
+      for (int c = 0; c < CHUNKS; ++c) {
+        if constexpr (!AHEAD) load_chunk(now, c);
+        if (!now.whole) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          ex_f32x4 x = {0, 0, 0, 0};
-          if (whole || quarter * 4 + i < valid[0]) x = *(const ex_f32x4*)(vp[0] + vrow + i * step + (c * 64 + col * 4) * SIZE);
-#pragma unroll
-          for (int t = 0; t < 4; ++t) O[c * 4 + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t], pr[0][i], O[c * 4 + t], 0, 0, 0);
+          for (int i = 0; i < 4; ++i)
+            if (quarter * 4 + i >= now.valid[0]) VF[c][i] = ex_f32x4{0, 0, 0, 0};
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) O[c * 4 + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(VF[c][i][t], pr[0][i], O[c * 4 + t], 0, 0, 0);
       }
     } else {
       ex_u32x4 P;
@@ -212,41 +275,41 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
 #pragma unroll
         for (int i = 0; i < 2; ++i) P[p * 2 + i] = ex_pack<DT>(pr[p][2 * i], pr[p][2 * i + 1]);
 #pragma unroll
-      for (int c = 0; c < WIDE; ++c) {
-        ex_u32x4 x[8];
+      for (int c = 0; c < CHUNKS; ++c) {
+        if constexpr (!AHEAD) load_chunk(now, c);
+        if (!now.whole) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = ex_u32x4{0, 0, 0, 0};
-          if (whole || quarter * 4 + (i & 3) < valid[i >> 2])
-            x[i] = *(const ex_u32x4*)(vp[i >> 2] + vrow + (i & 3) * step + (c * 128 + col * 8) * SIZE);
+          for (int i = 0; i < 8; ++i)
+            if (quarter * 4 + (i & 3) >= now.valid[i >> 2]) V[c][i] = ex_u32x4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
           ex_u32x4 f;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            f[j] = __builtin_amdgcn_perm(x[2 * j + 1][t >> 1], x[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+            f[j] = __builtin_amdgcn_perm(V[c][2 * j + 1][t >> 1], V[c][2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
           O[c * 8 + t] = ex_mfma<DT>(f, P, O[c * 8 + t]);
         }
       }
       if constexpr (NARROW > 0) {
-        ex_u32x2 x[8];
+        if constexpr (!AHEAD) load_narrow(now);
+        if (!now.whole) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = ex_u32x2{0, 0};
-          if (whole || quarter * 4 + (i & 3) < valid[i >> 2])
-            x[i] = *(const ex_u32x2*)(vp[i >> 2] + vrow + (i & 3) * step + (WIDE * 128 + col * 4) * SIZE);
+          for (int i = 0; i < 8; ++i)
+            if (quarter * 4 + (i & 3) >= now.valid[i >> 2]) VN[i] = ex_u32x2{0, 0};
         }
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           ex_u32x4 f;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            f[j] = __builtin_amdgcn_perm(x[2 * j + 1][t >> 1], x[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+            f[j] = __builtin_amdgcn_perm(VN[2 * j + 1][t >> 1], VN[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
           O[WIDE * 8 + t] = ex_mfma<DT>(f, P, O[WIDE * 8 + t]);
         }
       }
     }
+    if (AHEAD && more) load_values(next);
+    now = next;
   }
 
   // ---- the four wavefronts of the workgroup: to a common maximum, then summed pairwise (2, 3 -> 0, 1 -> 0) ----
@@ -295,7 +358,7 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
 
 template <int DT>
 int launch_exact_decode(const ExactDecode& a, hipStream_t stream) {
-  const dim3 grid((unsigned)((int64_t)a.n_split * a.groups * a.c.H * a.B)), block(256);
+  const dim3 grid((unsigned)exact_grid(a)), block(256);
 #define TQ_EXACT_D(D) \
   case D: exact_decode_kernel<DT, D><<<grid, block, 0, stream>>>(a); break
   switch (a.c.d) {
