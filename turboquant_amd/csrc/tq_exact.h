@@ -85,7 +85,7 @@ struct ExactJoin {
   int32_t score_pages;
   float* weights;          // (B, H, L): element strides w_b, w_h
   int64_t w_b, w_h;
-  int32_t L, weight_chunks;
+  int32_t L, weight_chunks, weight_tokens;
 };
 
 // what the entry points check of a cache, and its description

@@ -6,19 +6,63 @@
 namespace tq {
 
 // ---- splits -> outputs, scores -> weights ---------------------------------------------------------------------------------------------
-// Row workgroups (first of the grid, none with a single split): out = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i over a row's splits.
-// Weight workgroups: weights[b, h, t] += sum over the heads of h of 2^(s_t - M) / sum, a thread per token, heads in order: no atomics, the same
+// Rows (the first workgroups of the grid, none with a single split): out = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i over a row's splits.
+// Weights: weights[b, h, t] += sum over the heads of h of 2^(s_t - M) / sum, a thread per token, heads in order: no atomics, the same
 // result every time.  Both only need what the page kernel left, so that they share a launch.
-constexpr int JOIN_MAX_SPLITS = 1024, JOIN_TOKENS = 1024;
+constexpr int JOIN_MAX_SPLITS = 1024, JOIN_FEW = 16;
 
-template <int DT>
-__device__ __forceinline__ void exact_join_row(const ExactJoin& a, int row, float* s_f, float* s_red) {
-  const int tid = (int)threadIdx.x, b = row / a.Hq;
+__device__ __forceinline__ int join_len(const ExactJoin& a, int b) {
   const int64_t most = (int64_t)a.table_row * TQ_PAGE_TOKENS;
-  const int n = a.lens[b], len = n < 0 ? 0 : (n > most ? (int)most : n);
-  const int used = exact_splits_used((len + a.block_tokens - 1) / a.block_tokens, a.n_split, a.chunk);
+  const int n = a.lens[b];
+  return n < 0 ? 0 : (n > most ? (int)most : n);
+}
+__device__ __forceinline__ int join_used(const ExactJoin& a, int len) {
+  return exact_splits_used((len + a.block_tokens - 1) / a.block_tokens, a.n_split, a.chunk);
+}
+template <int DT>
+__device__ __forceinline__ void join_store(void* out, int64_t at, const float4& x) {
+  if constexpr (DT == TQ_F32) {
+    *(float4*)((float*)out + at) = x;
+  } else {
+    Elem<DT>::store(out, at, x.x);
+    Elem<DT>::store(out, at + 1, x.y);
+    Elem<DT>::store(out, at + 2, x.z);
+    Elem<DT>::store(out, at + 3, x.w);
+  }
+}
+
+// Few splits: a wavefront per row, a lane knows the factor of its split.
+template <int DT>
+__device__ __forceinline__ void exact_join_few(const ExactJoin& a, int row) {
+  const int lane = (int)threadIdx.x & 63;
+  const int used = join_used(a, join_len(a, row / a.Hq));
+  const float2 ml = lane < used ? a.ml[(int64_t)row * a.n_split + lane] : make_float2(-INFINITY, 0.0f);
+  const float top = wave_max_fast(ml.x), ref = top == -INFINITY ? 0.0f : top;
+  const float f = __builtin_amdgcn_exp2f(ml.x - ref), sum = wave_sum_fast(f * ml.y), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const int quads = a.d >> 2;
+  for (int q = lane; q < quads; q += 64) {
+    const float4* acc = (const float4*)(a.acc + (int64_t)row * a.n_split * a.d) + q;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (int i0 = 0; i0 < used; i0 += 8) {                   // eight on their way at a time, the last one over again behind the end
+      float4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = acc[(int64_t)(i0 + i < used ? i0 + i : used - 1) * quads];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float g = i0 + i < used ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (i0 + i) & 63)) : 0.0f;
+        o.x = fmaf(g, x[i].x, o.x); o.y = fmaf(g, x[i].y, o.y); o.z = fmaf(g, x[i].z, o.z); o.w = fmaf(g, x[i].w, o.w);
+      }
+    }
+    join_store<DT>(a.out, (int64_t)row * a.d + q * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+  }
+}
+
+// Many splits: a workgroup per row and 64 channels, sixteen lanes to a split, sixteen splits at a time.
+template <int DT>
+__device__ __forceinline__ void exact_join_many(const ExactJoin& a, int row, int slice, float* s_f, float* s_red, float4* s_o) {
+  const int tid = (int)threadIdx.x;
+  const int used = join_used(a, join_len(a, row / a.Hq));
   const float2* ml = a.ml + (int64_t)row * a.n_split;
-  // (every thread for itself: the maximum and the sum are a few hundred values of the L1)
   float top = -INFINITY;
   for (int i = tid; i < used; i += 256) top = fmaxf(top, ml[i].x);
   top = wave_max_fast(top);
@@ -28,85 +72,110 @@ __device__ __forceinline__ void exact_join_row(const ExactJoin& a, int row, floa
   const float ref = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f;
   for (int i = tid; i < used; i += 256) {
-    const float f = __builtin_amdgcn_exp2f(ml[i].x - ref);
+    const float2 x = ml[i];
+    const float f = __builtin_amdgcn_exp2f(x.x - ref);
     s_f[i] = f;
-    sum += f * ml[i].y;
+    sum += f * x.y;
   }
   sum = wave_sum_fast(sum);
+  if ((tid & 63) == 0) s_red[4 + (tid >> 6)] = sum;
   __syncthreads();
-  if ((tid & 63) == 0) s_red[tid >> 6] = sum;
-  __syncthreads();
-  sum = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
+  sum = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-
-  // four channels per thread; as many threads as are left share the splits
-  const int quads = a.d >> 2, shares = 256 / quads, share = tid / quads, quad = tid - share * quads;
+  const int quad = tid & 15, share = tid >> 4;
+  const float* acc = a.acc + (int64_t)row * a.n_split * a.d + slice * 64 + quad * 4;
   float4 o = make_float4(0, 0, 0, 0);
-  if (share < shares) {
-    const float4* acc = (const float4*)(a.acc + (int64_t)row * a.n_split * a.d) + quad;
-    for (int i = share; i < used; i += shares) {
-      const float4 x = acc[(int64_t)i * quads];
-      const float f = s_f[i];
-      o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
-    }
+#pragma unroll 8
+  for (int i = share; i < used; i += 16) {
+    const float4 x = *(const float4*)(acc + (int64_t)i * a.d);
+    const float f = s_f[i];
+    o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
   }
-  __shared__ float4 s_o[256];
   s_o[tid] = o;
   __syncthreads();
   if (share != 0) return;
-  for (int i = 1; i < shares; ++i) {
-    const float4 x = s_o[i * quads + quad];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) {
+    const float4 x = s_o[i * 16 + quad];
     o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
   }
-  const int64_t at = (int64_t)row * a.d + quad * 4;
-  Elem<DT>::store(a.out, at, o.x * inv);
-  Elem<DT>::store(a.out, at + 1, o.y * inv);
-  Elem<DT>::store(a.out, at + 2, o.z * inv);
-  Elem<DT>::store(a.out, at + 3, o.w * inv);
+  join_store<DT>(a.out, (int64_t)row * a.d + slice * 64 + quad * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
+// A thread's four tokens are neighbours: sixteen bytes of each head's scores.
 __device__ __forceinline__ void exact_add_weights(const ExactJoin& a, int id, float2* s_head) {
   const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int chunk = id % a.weight_chunks; id /= a.weight_chunks;
   const int h = id % a.H, b = id / a.H;
-  const int64_t most = (int64_t)a.table_row * TQ_PAGE_TOKENS;
-  const int n = a.lens[b], held = n < 0 ? 0 : (n > most ? (int)most : n);
-  const int len = held < a.L ? held : a.L;
-  const int t0 = chunk * JOIN_TOKENS;
+  const int held = join_len(a, b), len = held < a.L ? held : a.L;
+  const int t0 = chunk * a.weight_tokens;
   if (t0 >= len) return;
-  const int used = exact_splits_used((held + a.block_tokens - 1) / a.block_tokens, a.n_split, a.chunk);
+  const int used = join_used(a, held);
   for (int g = wave; g < a.G; g += 4) {
     const float2* ml = a.ml + ((int64_t)b * a.Hq + h * a.G + g) * a.n_split;
-    float top = -INFINITY, sum = 0.0f;
-    for (int i = lane; i < used; i += 64) top = fmaxf(top, ml[i].x);
+    float2 x = lane < used ? ml[lane] : make_float2(-INFINITY, 0.0f);
+    float top = x.x;
+    for (int i = lane + 64; i < used; i += 64) top = fmaxf(top, ml[i].x);
     top = wave_max_fast(top);
     const float ref = top == -INFINITY ? 0.0f : top;
-    for (int i = lane; i < used; i += 64) sum += ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - ref);
+    float sum = x.y * __builtin_amdgcn_exp2f(x.x - ref);
+    for (int i = lane + 64; i < used; i += 64) sum += ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - ref);
     sum = wave_sum_fast(sum);
     if (lane == 0) s_head[g] = make_float2(ref, sum == 0.0f ? 0.0f : 1.0f / sum);
   }
   __syncthreads();
-  float* w = a.weights + b * a.w_b + h * a.w_h;
-  for (int t = t0 + tid; t < t0 + JOIN_TOKENS && t < len; t += 256) {
+  for (int t = t0 + tid * 4; t < t0 + a.weight_tokens && t < len; t += 1024) {
     const float* s = a.scores + (((int64_t)b * a.H + h) * a.score_pages + (t >> 4)) * a.G * TQ_PAGE_TOKENS + (t & 15);
-    float add = 0.0f;
-    for (int g = 0; g < a.G; ++g) add += __builtin_amdgcn_exp2f(s[g * TQ_PAGE_TOKENS] - s_head[g].x) * s_head[g].y;
-    w[t] += add;
+    float4 add = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int g = 0; g < a.G; ++g) {
+      const float4 x = *(const float4*)(s + g * TQ_PAGE_TOKENS);
+      const float2 r = s_head[g];
+      add.x = fmaf(__builtin_amdgcn_exp2f(x.x - r.x), r.y, add.x);
+      add.y = fmaf(__builtin_amdgcn_exp2f(x.y - r.x), r.y, add.y);
+      add.z = fmaf(__builtin_amdgcn_exp2f(x.z - r.x), r.y, add.z);
+      add.w = fmaf(__builtin_amdgcn_exp2f(x.w - r.x), r.y, add.w);
+    }
+    float* w = a.weights + b * a.w_b + h * a.w_h + t;
+    const int n = len - t;
+    w[0] += add.x;
+    if (n > 1) w[1] += add.y;
+    if (n > 2) w[2] += add.z;
+    if (n > 3) w[3] += add.w;
   }
 }
 
 template <int DT>
-__global__ void __launch_bounds__(256) exact_join_kernel(const ExactJoin a, int rows) {
+__global__ void __launch_bounds__(256) exact_join_kernel(const ExactJoin a, int row_groups) {
   __shared__ float2 s_two[JOIN_MAX_SPLITS];
-  __shared__ float s_red[4];
-  const int id = (int)blockIdx.x;
-  if (id < rows) exact_join_row<DT>(a, id, (float*)s_two, s_red);
-  else exact_add_weights(a, id - rows, s_two);
+  __shared__ float s_red[8];
+  __shared__ float4 s_o[256];
+  int id = (int)blockIdx.x;
+  if (id >= row_groups) {
+    exact_add_weights(a, id - row_groups, s_two);
+  } else if (a.n_split <= JOIN_FEW) {
+    id = id * 4 + ((int)threadIdx.x >> 6);
+    if (id < a.B * a.Hq) exact_join_few<DT>(a, id);
+  } else {
+    const int slices = a.d >> 6;
+    exact_join_many<DT>(a, id / slices, id % slices, (float*)s_two, s_red, s_o);
+  }
+}
+
+// Tokens of a weight workgroup: more than 1024 only where that leaves 2048 workgroups (a workgroup that finds its part of a short sequence empty
+// still has to be dispatched: 96 sequences of 61 .. 8190 tokens, 8 KV heads: 26 us with 6144 workgroups, 20 with 2304)
+static int64_t join_tokens(int64_t pairs, int64_t len) {
+  const int64_t groups = pairs * ((len + 1023) / 1024);
+  return 1024 * std::max<int64_t>(1, std::min<int64_t>(groups / 2048, 64));
+}
+// workgroups that join rows
+static int64_t join_groups(int64_t rows, int n_split, int d) {
+  return n_split <= 1 ? 0 : (n_split <= JOIN_FEW ? (rows + 3) / 4 : rows * (d / 64));
 }
 
 // ---- how a call is split ----------------------------------------------------------------------------------------------------------------
 struct ExactPlan {
-  int groups, n_split, chunk, block_tokens, score_pages;
+  int groups, n_split, chunk, block_tokens, score_pages, weight_tokens;
   size_t ml_at, acc_at, scores_at, bytes;
 };
 
@@ -133,6 +202,7 @@ static bool exact_plan(ExactPlan* p, int dtype, int B, int Hq, int Hkv, int d, i
   if (n_split == 0) chunk = (chunk + 3) & ~(int64_t)3;                  // (a block for each of the four wavefronts)
   p->n_split = (int)std::max<int64_t>(1, (blocks + chunk - 1) / chunk);
   p->chunk = (int)chunk;
+  p->weight_tokens = (int)join_tokens((int64_t)B * Hkv, score_len);
   p->score_pages = (int)((score_len + TQ_PAGE_TOKENS - 1) / TQ_PAGE_TOKENS);
   const size_t rows = (size_t)B * Hq;
   size_t at = 0;
@@ -140,7 +210,7 @@ static bool exact_plan(ExactPlan* p, int dtype, int B, int Hq, int Hkv, int d, i
   p->acc_at = at;     at = round256(at + (p->n_split > 1 ? rows * p->n_split * d * sizeof(float) : 0));
   p->scores_at = at;  at = round256(at + (size_t)B * Hkv * p->score_pages * G * TQ_PAGE_TOKENS * sizeof(float));
   p->bytes = at;
-  const int64_t grid = (pairs * p->n_split + 8 * p->groups), join = (int64_t)rows + (int64_t)B * Hkv * ((score_len + JOIN_TOKENS - 1) / JOIN_TOKENS);
+  const int64_t grid = (pairs * p->n_split + 8 * p->groups), join = join_groups((int64_t)rows, p->n_split, d) + (int64_t)B * Hkv * ((score_len + p->weight_tokens - 1) / p->weight_tokens);
   return grid <= INT32_MAX && join <= INT32_MAX;
 }
 
@@ -197,9 +267,10 @@ extern "C" int tq_exact_decode(const void* q, int dtype, int B, int Hq, int Hkv,
   j.lens = seq_lens; j.table_row = a.c.table_row; j.B = B; j.Hq = Hq; j.H = Hkv; j.G = a.G; j.d = d; j.n_split = p.n_split; j.chunk = p.chunk;
   j.block_tokens = p.block_tokens; j.acc = a.acc; j.ml = a.ml; j.out = out; j.scores = a.scores; j.score_pages = p.score_pages;
   j.weights = weights; j.w_b = w_b; j.w_h = w_h; j.L = p.score_pages ? (int)weight_len : 0;
-  j.weight_chunks = (j.L + JOIN_TOKENS - 1) / JOIN_TOKENS;
-  const int rows = p.n_split > 1 ? B * Hq : 0;
-  const dim3 grid((unsigned)(rows + B * Hkv * j.weight_chunks)), block(256);
+  j.weight_tokens = p.weight_tokens;
+  j.weight_chunks = (j.L + j.weight_tokens - 1) / j.weight_tokens;
+  const int rows = (int)join_groups((int64_t)B * Hq, p.n_split, d);
+  const dim3 grid((unsigned)(rows + (int64_t)B * Hkv * j.weight_chunks)), block(256);
   if (dtype == TQ_F32) exact_join_kernel<TQ_F32><<<grid, block, 0, st>>>(j, rows);
   else if (dtype == TQ_F16) exact_join_kernel<TQ_F16><<<grid, block, 0, st>>>(j, rows);
   else exact_join_kernel<TQ_BF16><<<grid, block, 0, st>>>(j, rows);
