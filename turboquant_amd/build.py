@@ -18,7 +18,7 @@ HOST = os.path.join(HERE, "_tq_host.so")           # (imported by _ffi.py, where
 SOURCES = ["tq_decode_mfma_d128.hip", "tq_decode_mfma_d128_f16.hip", "tq_decode_mfma_d64.hip", "tq_decode_mfma_d64_f16.hip",
            "tq_decode_mfma_d256.hip", "tq_quantize_mfma.hip", "tq_quantize_wide.hip", "tq_decode_wide.hip", "tq_decode_heads.hip",
            "tq_quantize.hip", "tq_score.hip", "tq_decode.hip", "tq_decode_mfma.hip", "tq_exact_bf16.hip", "tq_exact_f16.hip",
-           "tq_exact_f32.hip", "tq_exact.hip", "tq_exact_window_bf16.hip", "tq_exact_window_f16.hip", "tq_exact_window_f32.hip",
+           "tq_exact_f32.hip", "tq_exact_heads_bf16.hip", "tq_exact_heads_f16.hip", "tq_exact.hip", "tq_exact_window_bf16.hip", "tq_exact_window_f16.hip", "tq_exact_window_f32.hip",
            "tq_exact_window.hip", "tq_evict.hip", "tq_probe.hip"]
 
 # packed-fp32 instructions stay off: some of their forms have produced wrong

@@ -1,6 +1,8 @@
 // Attention over a paged EXACT cache: blocks of 16 tokens x KV heads x head_dim in fp32, fp16 or bf16, as a serving engine keeps them.
 #pragma once
 
+#include <atomic>
+
 #include "tq_common.h"
 
 namespace tq {
@@ -93,5 +95,17 @@ int exact_cache_init(ExactCache* c, const void* k, const void* v, int dtype, int
                      const int32_t* table, int bt_stride, const int32_t* lens);
 
 template <int DT> int launch_exact_decode(const ExactDecode& a, hipStream_t stream);
+template <int DT> int launch_exact_heads(const ExactDecode& a, int tile_waves, hipStream_t stream);
+
+// a kernel may use more than 64 KB of LDS once it is told so, on every device for itself
+inline int exact_allow_lds(const void* kern, int bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  if (const hipError_t e = hipGetDevice(&dev)) return (int)e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (ready.load(std::memory_order_relaxed) & bit) return TQ_OK;
+  if (const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return (int)e;
+  ready.fetch_or(bit, std::memory_order_relaxed);
+  return TQ_OK;
+}
 
 }  // namespace tq

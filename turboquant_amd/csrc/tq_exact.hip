@@ -175,6 +175,7 @@ static int64_t join_groups(int64_t rows, int n_split, int d) {
 
 // ---- how a call is split ----------------------------------------------------------------------------------------------------------------
 struct ExactPlan {
+  int tile_waves;                     // 0: the kernel of sixteen heads; else tiles of sixteen heads that a workgroup serves
   int groups, n_split, chunk, block_tokens, score_pages, weight_tokens;
   size_t ml_at, acc_at, scores_at, bytes;
 };
@@ -188,18 +189,22 @@ static bool exact_plan(ExactPlan* p, int dtype, int B, int Hq, int Hkv, int d, i
   const int G = Hq / Hkv;
   if (G > JOIN_MAX_SPLITS) return false;
   p->block_tokens = dtype == TQ_F32 ? 16 : 32;
-  p->groups = (G + EXACT_HEADS - 1) / EXACT_HEADS;
+  const int tiles = (G + EXACT_HEADS - 1) / EXACT_HEADS;
+  const bool shared = dtype != TQ_F32 && tiles > 1 && d <= 576;
+  p->tile_waves = !shared ? 0 : (tiles > 4 ? 8 : (tiles > 2 ? 4 : 2));
+  p->groups = shared ? (tiles + p->tile_waves - 1) / p->tile_waves : tiles;
   const int64_t pairs = std::max<int64_t>(1, (int64_t)B * Hkv * p->groups);
   const int64_t blocks = std::max<int64_t>(1, (max_len + p->block_tokens - 1) / p->block_tokens);
   int64_t n = n_split;
   if (n == 0) {
-    const int64_t resident = 256 * (d <= 64 ? 4 : (d <= 128 ? 3 : (d <= 256 ? 2 : 1)));
+    const int64_t resident = 256 * (shared ? (d > 256 ? 1 : 2) : (d <= 64 ? 4 : (d <= 128 ? 3 : (d <= 256 ? 2 : 1))));
     n = std::max((resident + pairs - 1) / pairs, (max_len + 1023) / 1024);
+    if (shared) n = (resident + pairs - 1) / pairs;
     n = std::min<int64_t>(std::min<int64_t>(n, (blocks + 3) / 4), JOIN_MAX_SPLITS);
   }
   n = std::max<int64_t>(1, std::min(n, blocks));
   int64_t chunk = (blocks + n - 1) / n;
-  if (n_split == 0) chunk = (chunk + 3) & ~(int64_t)3;                  // (a block for each of the four wavefronts)
+  if (n_split == 0 && !shared) chunk = (chunk + 3) & ~(int64_t)3;                  // (a block for each of the four wavefronts)
   p->n_split = (int)std::max<int64_t>(1, (blocks + chunk - 1) / chunk);
   p->chunk = (int)chunk;
   p->weight_tokens = (int)join_tokens((int64_t)B * Hkv, score_len);
@@ -259,8 +264,12 @@ extern "C" int tq_exact_decode(const void* q, int dtype, int B, int Hq, int Hkv,
   a.scores = p.score_pages ? (float*)(ws + p.scores_at) : nullptr;
   a.score_pages = p.score_pages;
   hipStream_t st = (hipStream_t)stream;
-  const int done = dtype == TQ_F32 ? launch_exact_decode<TQ_F32>(a, st)
-                                   : (dtype == TQ_F16 ? launch_exact_decode<TQ_F16>(a, st) : launch_exact_decode<TQ_BF16>(a, st));
+  int done;
+  if (p.tile_waves)
+    done = dtype == TQ_F16 ? launch_exact_heads<TQ_F16>(a, p.tile_waves, st) : launch_exact_heads<TQ_BF16>(a, p.tile_waves, st);
+  else
+    done = dtype == TQ_F32 ? launch_exact_decode<TQ_F32>(a, st)
+                           : (dtype == TQ_F16 ? launch_exact_decode<TQ_F16>(a, st) : launch_exact_decode<TQ_BF16>(a, st));
   if (done) return done;
   if (p.n_split == 1 && !p.score_pages) return TQ_OK;
   ExactJoin j{};

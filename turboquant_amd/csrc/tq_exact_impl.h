@@ -65,14 +65,38 @@ __device__ __forceinline__ float ex_quad_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Channel of accumulator element i (0..3) of channel tile `tile` in a lane of quarter `quarter`.
-// Chunks of 128 channels (16-bit types) or 64: rows of a chunk's tiles are 8 or 4 channels apart.
-template <int DT, int D>
+// Channel of accumulator element i (0..3) of channel tile `tile` in a lane of quarter `quarter`: WIDE chunks of 128 channels, whose tiles'
+// rows are 8 channels apart, then chunks of 64, 4 apart.
+template <int WIDE>
 __device__ __forceinline__ int ex_channel(int tile, int quarter, int i) {
-  constexpr int WIDE = DT == TQ_F32 ? 0 : D / 128;          // chunks of 128
   if (tile < WIDE * 8) return (tile >> 3) * 128 + (quarter * 4 + i) * 8 + (tile & 7);
   const int t = tile - WIDE * 8;
   return WIDE * 128 + (t >> 2) * 64 + (quarter * 4 + i) * 4 + (t & 3);
+}
+template <int DT, int D> constexpr int ex_wide() { return DT == TQ_F32 ? 0 : D / 128; }
+
+// A wavefront's accumulators of one head: the output, or the split's numerators with its maximum and sum.  The tiles of a chunk hold
+// neighbouring channels, so that a lane writes 16 bytes at a time.
+template <int DT, int D, int WIDE = ex_wide<DT, D>()>
+__device__ __forceinline__ void exact_store(const ExactDecode& a, const ex_f32x4* O, float top, float sum, int64_t row, int split, int quarter) {
+  if (quarter == 0) a.ml[row * a.n_split + split] = make_float2(top, sum);
+  const bool one = a.n_split == 1;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  float* acc = a.acc + (row * a.n_split + split) * D;
+#pragma unroll
+  for (int t = 0; t < D / 16; t += 4)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = ex_channel<WIDE>(t, quarter, i);         // and the three after it
+      const ex_f32x4 x = {O[t][i], O[t + 1][i], O[t + 2][i], O[t + 3][i]};
+      if (!one) {
+        *(ex_f32x4*)(acc + c) = x;
+      } else if constexpr (DT == TQ_F32) {
+        *(ex_f32x4*)((float*)a.out + row * D + c) = x * inv;
+      } else {
+        *(ex_u32x2*)((uint16_t*)a.out + row * D + c) = ex_u32x2{ex_pack<DT>(x[0] * inv, x[1] * inv), ex_pack<DT>(x[2] * inv, x[3] * inv)};
+      }
+    }
 }
 
 template <int DT, int D>
@@ -106,11 +130,10 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
   constexpr int SIZE = F32 ? 4 : 2;
   constexpr int KSTEPS = D * SIZE / 64;                      // 16-byte pieces that a lane reads of a key
   constexpr int TILES = D / 16;                              // channel tiles
-  constexpr int WIDE = F32 ? 0 : D / 128, NARROW = (D - WIDE * 128) / 64;
+  constexpr int WIDE = ex_wide<DT, D>(), NARROW = (D - WIDE * 128) / 64;
   constexpr int VTOKENS = F32 ? 4 : 8;                       // tokens of a lane
   constexpr bool AHEAD = D <= 256;                           // keys and values are read a block ahead (above, their registers are the accumulators')
   constexpr bool QUERIES_IN_LDS = D == 256;                  // (two wavefronts per SIMD: 256 registers)
-  using St = typename Elem<DT>::storage;
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int col = lane & 15, quarter = lane >> 4;            // head of the group; which four tokens of sixteen
@@ -341,19 +364,7 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
   if (wave != 0 || !live) return;
 #pragma unroll
   for (int t = 0; t < TILES; ++t) O[t] += s_acc[0][t][lane];
-  if (quarter == 0) a.ml[row * a.n_split + split] = make_float2(M - LIFT, sum);
-  const bool one = a.n_split == 1;
-  const float inv = one ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
-  float* acc = one ? nullptr : a.acc + (row * a.n_split + split) * D;
-  St* out = (St*)a.out + row * D;
-#pragma unroll
-  for (int t = 0; t < TILES; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = ex_channel<DT, D>(t, quarter, i);
-      if (one) Elem<DT>::store(out, c, O[t][i] * inv);
-      else acc[c] = O[t][i];
-    }
+  exact_store<DT, D>(a, O, M - LIFT, sum, row, split, quarter);
 }
 
 template <int DT>
