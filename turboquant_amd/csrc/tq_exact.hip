@@ -191,7 +191,7 @@ static bool exact_plan(ExactPlan* p, int dtype, int B, int Hq, int Hkv, int d, i
   p->block_tokens = dtype == TQ_F32 ? 16 : 32;
   const int tiles = (G + EXACT_HEADS - 1) / EXACT_HEADS;
   const bool shared = dtype != TQ_F32 && tiles > 1 && d <= 576;
-  p->tile_waves = !shared ? 0 : (tiles > 4 ? 8 : (tiles > 2 ? 4 : 2));
+  p->tile_waves = !shared ? 0 : (tiles > 4 && d <= 256 ? 8 : (tiles > 2 ? 4 : 2));
   p->groups = shared ? (tiles + p->tile_waves - 1) / p->tile_waves : tiles;
   const int64_t pairs = std::max<int64_t>(1, (int64_t)B * Hkv * p->groups);
   const int64_t blocks = std::max<int64_t>(1, (max_len + p->block_tokens - 1) / p->block_tokens);

@@ -19,15 +19,28 @@ namespace tq {
 __device__ __forceinline__ void ex_to_lds(const void* from, uint32_t m0) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(m0) : "memory", "m0");
 }
+__device__ __forceinline__ void ex_row_to_lds(const void* base, uint32_t off, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(m0) : "memory", "m0");
+}
 __device__ __forceinline__ void ex_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// Values of more than 512 channels are read 64 channels at a time, 16 registers instead of 32 (with 128, 30 of 256 were spilled, and a wait for a spilled
+// Where a block's rows lie in LDS, in 16-byte pieces.  Up to 448 channels they follow one another, and a load takes 64 pieces wherever a row ends.  512 and
+// 576 channels: a load takes the first 64 pieces of ONE row, whose address is the wavefront's (a scalar and the lane's constant; with divisions by
+// the length of a row the loads were 250 of a block's 815 vector instructions), and with 576 another takes the last 8 of eight rows.
+// Values of 576 channels are read 64 channels at a time, 16 registers instead of 32 (with 128, 30 of 256 were spilled, and a wait for a spilled
 // register is one for the next block): 8 bytes a lane, so that four rows should be half the banks apart.
-__host__ __device__ constexpr int heads_wide(int d) { return d > 512 ? 0 : d / 128; }
-__host__ __device__ constexpr int heads_key_row(int d) { return d / 8 + 1; }
-__host__ __device__ constexpr int heads_value_row(int d) { return d / 8 + (heads_wide(d) ? 1 : 2); }
-__host__ __device__ constexpr int heads_loads(int d) { return (32 * heads_value_row(d) + 63) / 64; }          // of a block's keys, or values
-__host__ __device__ constexpr int heads_lds(int d) { return 4 * heads_loads(d) * 1024; }
+template <int D>
+struct HeadsLds {
+  static constexpr bool ROWS = D >= 512;
+  static constexpr int WIDE = D / 128;         // chunks of 128 value channels
+  static constexpr int PIECES = D / 8;
+  static constexpr int KROW = (ROWS ? 64 : PIECES) + 1, VROW = (ROWS ? 64 : PIECES) + (WIDE ? 1 : 2);
+  static constexpr int LOADS = ROWS ? 32 + (PIECES > 64 ? 4 : 0) : (32 * VROW + 63) / 64;                  // of a block's keys, or values
+  static constexpr int KTAIL = 32 * KROW * 16, VTAIL = 32 * VROW * 16;                                     // bytes before the rows' ends
+  static constexpr int KBYTES = ROWS ? KTAIL + (LOADS - 32) * 1024 : LOADS * 1024, VBYTES = ROWS ? VTAIL + (LOADS - 32) * 1024 : LOADS * 1024;
+  static constexpr int BYTES = 2 * (KBYTES + VBYTES);
+  static_assert(PIECES == 72 || PIECES <= 64, "the ends of eight rows fill a load");
+};
 
 // the value, computed where it stands: what is made of it does not stay in registers from one turn to the next
 __device__ __forceinline__ int ex_anew(int x) {
@@ -37,11 +50,11 @@ __device__ __forceinline__ int ex_anew(int x) {
 
 template <int DT, int D, int TW>
 __global__ void __launch_bounds__(TW * 64, TW == 8 || D <= 256 ? 2 : 1) exact_heads_kernel(const ExactDecode a) {
-  constexpr int KSTEPS = D / 32, TILES = D / 16, WIDE = heads_wide(D), NARROW = (D - WIDE * 128) / 64;
-  constexpr int KROW = heads_key_row(D), VROW = heads_value_row(D), LOADS = heads_loads(D), BUF = LOADS * 1024;
-  static_assert((32 * KROW + 63) / 64 <= LOADS, "keys take no more loads than values");
-  constexpr float LIFT = DT == TQ_F16 ? 14.0f : 0.0f;        // (as in tq_exact_impl.h)
-  extern __shared__ __align__(16) unsigned char s_blocks[];  // [2 turns][keys, values][LOADS KB]
+  using Lds = HeadsLds<D>;
+  constexpr int KSTEPS = D / 32, TILES = D / 16, WIDE = Lds::WIDE, NARROW = (D - WIDE * 128) / 64;
+  constexpr int KROW = Lds::KROW, VROW = Lds::VROW, LOADS = Lds::LOADS, TURN = Lds::KBYTES + Lds::VBYTES;
+  constexpr int DEPTH = D > 256 ? 16 : 8;                    // key operands on their way from LDS
+  extern __shared__ __align__(16) unsigned char s_blocks[];  // [2 turns][keys, values]
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   int split, group, h, b;
@@ -71,46 +84,117 @@ __global__ void __launch_bounds__(TW * 64, TW == 8 || D <= 256 ? 2 : 1) exact_he
   float m = -INFINITY, l = 0.0f;
 
   ExactPages<2> now, next;
+  const uint32_t head_off = (uint32_t)((int)threadIdx.x & 63) * 16;        // a lane's part of a row
   const auto fetch = [&](const ExactPages<2>& at, int turn) __attribute__((always_inline)) {
-    const int ln = ex_anew((int)threadIdx.x & 63);           // (the places in a block are computed anew: there are no registers to keep them in)
+    if constexpr (Lds::ROWS) {
+      // wavefront w takes rows w, w + TW ... of each page; an address is the last one plus TW rows
 #pragma unroll
-    for (int i = 0; i < 2 * LOADS; i += TW) {
-      const int n = i + wave;                                // this wavefront's load: keys first
-      if (2 * LOADS % TW != 0 && n >= 2 * LOADS) break;
-      const bool value = n >= LOADS;
-      const int k = value ? n - LOADS : n, piece = k * 64 + ln;
-      int r = value ? piece / VROW : piece / KROW, p = piece - r * (value ? VROW : KROW);
-      r = r < 32 ? r : 31;                                   // (what fills the last load up, and the pieces between two rows: of no use, but there)
-      p = p < D / 8 ? p : D / 8 - 1;
-      const char* from = (const char*)(value ? a.c.v : a.c.k) + (r < 16 ? at.at[0] : at.at[1]) + ((uint32_t)(r & 15) * step + (uint32_t)p * 16);
-      ex_to_lds(from, lds0 + (uint32_t)(turn * 2 * BUF + n * 1024));
-      if constexpr (D > 512) __builtin_amdgcn_sched_barrier(0);
+      for (int side = 0; side < 2; ++side)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const char* from = (const char*)(side ? a.c.v : a.c.k) + at.at[p] + (uint32_t)wave * step;
+          const int row_bytes = (side ? VROW : KROW) * 16;
+          uint32_t to = lds0 + (uint32_t)(turn * TURN + (side ? Lds::KBYTES : 0) + (p * 16 + wave) * row_bytes);
+#pragma unroll
+          for (int i = 0; i < 16 / TW; ++i) {
+            ex_row_to_lds(from, head_off, to);
+            from += (uint64_t)(step * TW);
+            to += TW * row_bytes;
+          }
+        }
+      if constexpr (LOADS > 32) {
+        // the ends of rows r .. r + 7: keys of both pages, then values; a key's pieces change places by its row, for the banks
+        const int ln = ex_anew((int)threadIdx.x & 63);
+#pragma unroll
+        for (int i = 0; i < 8; i += TW) {
+          const int n = i + wave, r = (n & 3) * 8;
+          const bool value = n >= 4;
+          const uint32_t off = (uint32_t)((r & 8) + (ln >> 3)) * step + (64 + (value ? ln & 7 : (ln & 7) ^ (ln >> 3))) * 16;
+          const uint32_t to = lds0 + (uint32_t)(turn * TURN + (value ? Lds::KBYTES + Lds::VTAIL : Lds::KTAIL) + r * 128);
+          ex_row_to_lds((const char*)(value ? a.c.v : a.c.k) + (r < 16 ? at.at[0] : at.at[1]), off, to);
+        }
+      }
+    } else {
+      const int ln = ex_anew((int)threadIdx.x & 63);         // (places are computed anew: there are no registers to keep them in)
+#pragma unroll
+      for (int i = 0; i < 2 * LOADS; i += TW) {
+        const int n = i + wave;                              // this wavefront's load: keys first
+        if (2 * LOADS % TW != 0 && n >= 2 * LOADS) break;
+        const bool value = n >= LOADS;
+        const int k = value ? n - LOADS : n, piece = k * 64 + ln;
+        int r = value ? piece / VROW : piece / KROW, p = piece - r * (value ? VROW : KROW);
+        r = r < 32 ? r : 31;                                 // (what fills the last load up, and the pieces between two rows: of no use, but there)
+        p = p < Lds::PIECES ? p : Lds::PIECES - 1;
+        const char* from = (const char*)(value ? a.c.v : a.c.k) + (r < 16 ? at.at[0] : at.at[1]) + ((uint32_t)(r & 15) * step + (uint32_t)p * 16);
+        ex_to_lds(from, lds0 + (uint32_t)(turn * TURN + (value ? Lds::KBYTES : 0) + k * 1024));
+      }
     }
   };
+  // table entries are read two blocks ahead, as vector loads behind a block's own: they have arrived with it
+  int32_t entry[2] = {-1, -1};
   if (first < last) {
     now.find(a.c, table, len, first, h, 2);
     fetch(now, 0);
+    ExactPages<2>::entries(entry, table, len, first + 1);
   }
   for (int blk = first, turn = 0; blk < last; ++blk, turn ^= 1) {
     ex_arrived();
     __syncthreads();
     if (blk + 1 < last) {
-      next.find(a.c, table, len, blk + 1, h, 2);
+      entry[0] = __builtin_amdgcn_readfirstlane(entry[0]);
+      entry[1] = __builtin_amdgcn_readfirstlane(entry[1]);
+      next.place(a.c, entry, len, blk + 1, h, 2);
       fetch(next, turn ^ 1);
+      ExactPages<2>::entries(entry, table, len, blk + 2);
+    }
+    if (!now.whole) {
+      // values of tokens without weight are put to zero where they lie, since NaN times nothing is NaN
+#pragma unroll 1
+      for (int r = 0; r < 32; ++r) {
+        if ((r & 15) < (r < 16 ? now.valid[0] : now.valid[1])) continue;
+        unsigned char* to = s_blocks + turn * TURN + Lds::KBYTES;
+        for (int p = (int)threadIdx.x; p < Lds::PIECES; p += TW * 64)
+          *(ex_u32x4*)(to + (p < 64 || !Lds::ROWS ? (r * VROW + p) * 16 : Lds::VTAIL + r * 128 + (p - 64) * 16)) = ex_u32x4{0, 0, 0, 0};
+      }
+      __syncthreads();
     }
     const int lane = ex_anew((int)threadIdx.x & 63), col = lane & 15, quarter = lane >> 4;
     // (a lane's first key and value piece: all others are constants away)
-    const unsigned char *kb = s_blocks + (turn * 2 * BUF + (col * KROW + quarter) * 16), *vb = s_blocks + (turn * 2 * BUF + BUF + (quarter * 4 * VROW + col) * 16);
+    const unsigned char* kb = s_blocks + (turn * TURN + (col * KROW + quarter) * 16);
+    const unsigned char* vb = s_blocks + (turn * TURN + Lds::KBYTES + quarter * 4 * VROW * 16);
     // ---- scores ----
+    const auto key = [&](int p, int s) __attribute__((always_inline)) {
+      if (Lds::ROWS && s >= 16)                              // the last eight pieces
+        return *(const ex_u32x4*)(s_blocks + turn * TURN + Lds::KTAIL + (p * 16 + col) * 128 + ((((s - 16) * 4 + quarter) ^ (col & 7)) * 16));
+      return *(const ex_u32x4*)(kb + (p * 16 * KROW + s * 4) * 16);
+    };
+    const auto value = [&](int c, int i) __attribute__((always_inline)) {                  // chunk of 128 channels, token
+      return *(const ex_u32x4*)(vb + (((i >> 2) * 16 + (i & 3)) * VROW + c * 16) * 16 + col * 16);
+    };
+    const auto value_end = [&](int i) __attribute__((always_inline)) {                     // the last 64 channels
+      const int r = (i >> 2) * 16 + (i & 3);                 // (and quarter * 4)
+      if (Lds::ROWS) return *(const ex_u32x2*)(s_blocks + turn * TURN + Lds::KBYTES + Lds::VTAIL + r * 128 + quarter * 512 + col * 8);
+      return *(const ex_u32x2*)(vb + (r * VROW + WIDE * 16) * 16 + col * 8);
+    };
+    // (the compiler would read each operand right before its use and wait for it: the order is held down by the barriers for the scheduler)
+    constexpr int N = 2 * KSTEPS, PRE = N < DEPTH ? N : DEPTH;
     ex_f32x4 S[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    ex_u32x4 kf[PRE];
 #pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) {
+    for (int i = 0; i < PRE; ++i) kf[i] = key(i & 1, i >> 1);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
-        S[p] = ex_mfma<DT>(*(const ex_u32x4*)(kb + (p * 16 * KROW + s * 4) * 16), Q[s], S[p]);
-      if (D > 256 && s & 1) __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < N; ++i) {
+      S[i & 1] = ex_mfma<DT>(kf[i % PRE], Q[i >> 1], S[i & 1]);
+      if (i + PRE < N) kf[i % PRE] = key((i + PRE) & 1, (i + PRE) >> 1);
+      if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_barrier(0);                       // (values are not read into registers that keys still need)
+    ex_u32x4 x[2][8];
+    if constexpr (WIDE > 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[0][i] = value(0, i);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     // ---- weights ----
     float top = -INFINITY, pr[2][4];
 #pragma unroll
@@ -131,14 +215,17 @@ __global__ void __launch_bounds__(TW * 64, TW == 8 || D <= 256 ? 2 : 1) exact_he
       }
     }
     top = fmaxf(m, ex_quad_max(top));
-    if (__any(top > m)) {
+    if (__any(top > m + EX_SLACK)) {
       const float move = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
       l *= move;
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) O[t] *= move;
+      for (int t = 0; t < TILES; ++t) {
+        if constexpr (D > 256) asm volatile("" : "+a"(O[t]));  // (they lie in the other half of the registers and would be copied out in every turn)
+        O[t] *= move;
+      }
       m = top;
     }
-    const float ref = m == -INFINITY ? 0.0f : m - LIFT;
+    const float ref = m == -INFINITY ? 0.0f : m - ex_lift<DT>();
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -152,46 +239,46 @@ __global__ void __launch_bounds__(TW * 64, TW == 8 || D <= 256 ? 2 : 1) exact_he
 #pragma unroll
       for (int i = 0; i < 2; ++i) P[p * 2 + i] = ex_pack<DT>(pr[p][2 * i], pr[p][2 * i + 1]);
     // ---- values ----
+    ex_u32x2 y[8];
 #pragma unroll
     for (int c = 0; c < WIDE; ++c) {
-      ex_u32x4 x[8];
+      if (c + 1 < WIDE) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = *(const ex_u32x4*)(vb + (((i >> 2) * 16 + (i & 3)) * VROW + c * 16) * 16);
-        if (!now.whole && quarter * 4 + (i & 3) >= now.valid[i >> 2]) x[i] = ex_u32x4{0, 0, 0, 0};
+        for (int i = 0; i < 8; ++i) x[(c + 1) & 1][i] = value(c + 1, i);
+      } else if constexpr (NARROW > 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = value_end(i);
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
+        const ex_u32x4* v = x[c & 1];
         ex_u32x4 f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = __builtin_amdgcn_perm(x[2 * j + 1][t >> 1], x[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+        for (int j = 0; j < 4; ++j) f[j] = __builtin_amdgcn_perm(v[2 * j + 1][t >> 1], v[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
         O[c * 8 + t] = ex_mfma<DT>(f, P, O[c * 8 + t]);
       }
-      if constexpr (D > 256) __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    if constexpr (NARROW > 0) {
+      if constexpr (WIDE == 0) {
 #pragma unroll
-    for (int c = 0; c < NARROW; ++c) {
-      ex_u32x2 x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = *(const ex_u32x2*)(vb - col * 8 + (((i >> 2) * 16 + (i & 3)) * VROW + WIDE * 16 + c * 8) * 16);
-        if (!now.whole && quarter * 4 + (i & 3) >= now.valid[i >> 2]) x[i] = ex_u32x2{0, 0};
+        for (int i = 0; i < 8; ++i) y[i] = value_end(i);
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         ex_u32x4 f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = __builtin_amdgcn_perm(x[2 * j + 1][t >> 1], x[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
-        O[WIDE * 8 + c * 4 + t] = ex_mfma<DT>(f, P, O[WIDE * 8 + c * 4 + t]);
+        for (int j = 0; j < 4; ++j) f[j] = __builtin_amdgcn_perm(y[2 * j + 1][t >> 1], y[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+        O[WIDE * 8 + t] = ex_mfma<DT>(f, P, O[WIDE * 8 + t]);
       }
-      if constexpr (D > 256) __builtin_amdgcn_sched_barrier(0);
     }
     now = next;
   }
   l = ex_quad_sum(l);
   const int lane = (int)threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
   if (head0 + col >= a.G) return;
-  exact_store<DT, D, WIDE>(a, O, m - LIFT, l, row0 + col, split, quarter);
+  exact_store<DT, D, WIDE>(a, O, m - ex_lift<DT>(), l, row0 + col, split, quarter);
 }
 
 template <int DT>
@@ -201,13 +288,13 @@ int launch_exact_heads(const ExactDecode& a, int tw, hipStream_t stream) {
   {                                                                                                                         \
     const auto kern = exact_heads_kernel<DT, D, TW>;                                                                        \
     static std::atomic<uint64_t> ready{0};                                                                                  \
-    if (const int rc = exact_allow_lds((const void*)kern, heads_lds(D), ready)) return rc;                                  \
-    kern<<<grid, block, heads_lds(D), stream>>>(a);                                                                         \
+    if (const int rc = exact_allow_lds((const void*)kern, HeadsLds<D>::BYTES, ready)) return rc;                                  \
+    kern<<<grid, block, HeadsLds<D>::BYTES, stream>>>(a);                                                                         \
     break;                                                                                                                  \
   }
 #define TQ_HEADS_D(D)                                                                 \
   case D:                                                                             \
-    if (tw == 8) TQ_HEADS_TW(D, 8)                                                    \
+    if constexpr (D <= 256) if (tw == 8) TQ_HEADS_TW(D, 8)                            \
     if (tw == 4) TQ_HEADS_TW(D, 4)                                                    \
     TQ_HEADS_TW(D, 2)
   switch (a.c.d) {

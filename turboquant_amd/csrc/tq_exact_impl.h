@@ -65,6 +65,12 @@ __device__ __forceinline__ float ex_quad_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// The reference of the powers of two moves up when a head's maximum has passed it by more than 2^EX_SLACK, not with every new maximum: accumulators
+// are multiplied seldom, and weights are up to 2^EX_SLACK large.  fp16 weights are multiplied by 2^6 besides, which keeps the largest
+// under fp16's 2^16: without it a long context's many small ones would round to nothing.
+constexpr float EX_SLACK = 8.0f;
+template <int DT> __device__ __forceinline__ constexpr float ex_lift() { return DT == TQ_F16 ? 6.0f : 0.0f; }
+
 // Channel of accumulator element i (0..3) of channel tile `tile` in a lane of quarter `quarter`: WIDE chunks of 128 channels, whose tiles'
 // rows are 8 channels apart, then chunks of 64, 4 apart.
 template <int WIDE>
@@ -110,12 +116,24 @@ struct ExactPages {
   int valid[PAGES];
   bool whole;
   __device__ __forceinline__ void find(const ExactCache& c, const int32_t* table, int len, int blk, int h, int size) {
+    int32_t entry[PAGES];
+    entries(entry, table, len, blk);
+    place(c, entry, len, blk, h, size);
+  }
+  static __device__ __forceinline__ void entries(int32_t* entry, const int32_t* table, int len, int blk) {
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p) {
+      const int page = blk * PAGES + p;
+      entry[p] = page * TQ_PAGE_TOKENS < len ? table[page] : -1;
+    }
+  }
+  __device__ __forceinline__ void place(const ExactCache& c, const int32_t* entry, int len, int blk, int h, int size) {
     whole = true;
 #pragma unroll
     for (int p = 0; p < PAGES; ++p) {
       const int left = len - (blk * PAGES + p) * TQ_PAGE_TOKENS;
       valid[p] = left < 0 ? 0 : (left > TQ_PAGE_TOKENS ? TQ_PAGE_TOKENS : left);
-      int64_t page = left > 0 ? table[blk * PAGES + p] : 0;
+      int64_t page = entry[p];
       if (page < 0 || page >= c.num_blocks) { page = 0; valid[p] = 0; }
       whole &= valid[p] == TQ_PAGE_TOKENS;
       at[p] = (page * c.s_blk + h * c.s_h) * size;
@@ -169,8 +187,6 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
 #pragma unroll
   for (int t = 0; t < TILES; ++t) O[t] = ex_f32x4{0, 0, 0, 0};
   float m = -INFINITY, l = 0.0f;
-  // fp16 weights are multiplied by 2^14, the largest power that holds them: without it a long context's many small ones would round to nothing
-  constexpr float LIFT = DT == TQ_F16 ? 14.0f : 0.0f;
 
   const uint32_t step = (uint32_t)a.c.s_t * SIZE;
   const uint32_t krow = (uint32_t)col * step + quarter * 16, vrow = (uint32_t)(quarter * 4) * step;
@@ -261,14 +277,14 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
       }
     }
     top = fmaxf(m, ex_quad_max(top));
-    if (__any(top > m)) {
+    if (__any(top > m + EX_SLACK)) {
       const float move = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
       l *= move;
 #pragma unroll
       for (int t = 0; t < TILES; ++t) O[t] *= move;
       m = top;
     }
-    const float ref = m == -INFINITY ? 0.0f : m - LIFT;
+    const float ref = m == -INFINITY ? 0.0f : m - ex_lift<DT>();
 #pragma unroll
     for (int p = 0; p < PAGES; ++p)
 #pragma unroll
@@ -364,7 +380,7 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
   if (wave != 0 || !live) return;
 #pragma unroll
   for (int t = 0; t < TILES; ++t) O[t] += s_acc[0][t][lane];
-  exact_store<DT, D>(a, O, M - LIFT, sum, row, split, quarter);
+  exact_store<DT, D>(a, O, M - ex_lift<DT>(), sum, row, split, quarter);
 }
 
 template <int DT>
