@@ -13,7 +13,9 @@ struct ExactWindow {
   int32_t B, Hq, G, W;           // W: newest rows of a sequence that count, at most
   int32_t row_tiles, tile_waves, row_groups;     // tiles of 16 (query, head) rows at most; wavefronts side by side on them; turns that they take
   int32_t n_split, chunk;        // as in decode
-  float scale2;
+  int32_t waves;                 // of a workgroup: 4 or 8
+  float scale2;                  // |scale| log2 e, positive
+  uint32_t flip;                 // the sign bits of the queries' elements, for a negative scale
   float2* ml;                    // (B, H, parts, row_tiles * 16): maximum (log2) and sum of a row over a part of the tokens
   float2* stat;                  // (B, H, row_tiles * 16): of all tokens: maximum and 1 / sum
   int32_t parts;
@@ -24,9 +26,13 @@ struct ExactWindow {
 
 template <int DT> int launch_exact_window(const ExactWindow& a, bool add, hipStream_t stream);
 
-// row tiles that a wavefront holds as operands (and how many registers that takes: 4 d / 32 a tile, fp32 twice as many)
+// row tiles that a wavefront holds as operands: d / 8 registers each, fp32 twice as many
 __host__ __device__ constexpr int window_tiles(int dt, int d) {
-  return dt == TQ_F32 ? (d <= 64 ? 4 : (d <= 128 ? 2 : 1)) : (d <= 128 ? 4 : (d <= 256 ? 2 : 1));
+  return dt == TQ_F32 ? (d <= 64 ? 4 : (d <= 128 ? 2 : 1)) : (d <= 256 ? 4 : (d <= 512 ? 2 : 1));
 }
+__host__ __device__ constexpr int window_waves_per_simd(int dt, int d, int waves) { return dt != TQ_F32 && d <= 128 ? (waves == 4 ? 3 : (d <= 64 ? 4 : 2)) : 2; }
+// bytes of a block's keys (32 tokens, fp32 16) in LDS, and of all blocks that a workgroup may hold
+__host__ __device__ constexpr int window_block_bytes(int d) { return 64 * d; }
+constexpr int WINDOW_LDS = 96 * 1024;
 
 }  // namespace tq

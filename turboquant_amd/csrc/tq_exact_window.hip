@@ -2,29 +2,40 @@
 #include "tq_exact_window.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace tq {
 
-// stat[r] = (M, 1 / sum_i 2^(m_i - M) l_i) over the parts of a row; a row that sees nothing has no weight to give
-__global__ void __launch_bounds__(256) exact_window_join_kernel(const float2* ml, float2* stat, int parts, int padded, int64_t rows,
-                                                                ExactCache c, int block_tokens, int n_split, int chunk, int token_waves) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * padded) return;
-  const int64_t row = i / padded;
-  const int r = (int)(i - row * padded), len = exact_len(c, (int)(row / c.H));
+// stat[r] = (M, 1 / sum_i 2^(m_i - M) l_i) over the parts of a row; a row that sees nothing has no weight to give.  Sixteen rows a workgroup, sixteen
+// threads a row.
+__global__ void __launch_bounds__(256) exact_window_join_kernel(const float2* ml, float2* stat, int parts, int padded, ExactCache c, int block_tokens,
+                                                                int n_split, int chunk, int token_waves) {
+  __shared__ float s_top[16][17], s_sum[16][17];
+  const int r = (int)threadIdx.x & 15, share = (int)threadIdx.x >> 4;
+  const int64_t at = (int64_t)blockIdx.x * 16, row = at / padded;
+  const int in = (int)(at - row * padded) + r, len = exact_len(c, (int)(row / c.H));
   const int used = exact_splits_used((len + block_tokens - 1) / block_tokens, n_split, chunk) * token_waves;
+  const float2* x = ml + row * parts * padded + in;
   float top = -INFINITY, sum = 0.0f;
-  for (int p = 0; p < used; ++p) top = fmaxf(top, ml[(row * parts + p) * padded + r].x);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  for (int p = 0; p < used; ++p) {
-    const float2 x = ml[(row * parts + p) * padded + r];
-    sum += x.y * __builtin_amdgcn_exp2f(x.x - ref);
+  for (int p = share; p < used; p += 16) {
+    const float2 v = x[(int64_t)p * padded];
+    const float now = fmaxf(top, v.x), ref = now == -INFINITY ? 0.0f : now;
+    sum = sum * __builtin_amdgcn_exp2f(top - ref) + v.y * __builtin_amdgcn_exp2f(v.x - ref);
+    top = now;
   }
-  stat[i] = make_float2(ref, sum == 0.0f ? 0.0f : 1.0f / sum);
+  s_top[share][r] = top;
+  s_sum[share][r] = sum;
+  __syncthreads();
+  if (share != 0) return;
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, s_top[i][r]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  sum = 0.0f;
+  for (int i = 0; i < 16; ++i) sum += s_sum[i][r] * __builtin_amdgcn_exp2f(s_top[i][r] - ref);
+  stat[at + r] = make_float2(ref, sum == 0.0f ? 0.0f : 1.0f / sum);
 }
 
 struct WindowPlan {
-  int row_tiles, tile_waves, row_groups, n_split, chunk, block_tokens, parts;
+  int row_tiles, waves, tile_waves, row_groups, n_split, chunk, block_tokens, parts;
   size_t ml_at, stat_at, bytes;
 };
 
@@ -34,15 +45,19 @@ static bool window_plan(WindowPlan* p, int dtype, int B, int Hq, int Hkv, int d,
   const int G = Hq / Hkv, NT = window_tiles(dtype, d);
   p->block_tokens = dtype == TQ_F32 ? 16 : 32;
   p->row_tiles = (W * G + 15) / 16;
-  p->tile_waves = p->row_tiles > 2 * NT ? 4 : (p->row_tiles > NT ? 2 : 1);
+  p->tile_waves = p->row_tiles > 4 * NT ? 8 : (p->row_tiles > 2 * NT ? 4 : (p->row_tiles > NT ? 2 : 1));
   p->row_groups = (p->row_tiles + p->tile_waves * NT - 1) / (p->tile_waves * NT);
   const int64_t blocks = std::max<int64_t>(1, (max_len + p->block_tokens - 1) / p->block_tokens);
   const int64_t pairs = std::max<int64_t>(1, (int64_t)B * Hkv);
-  const int64_t token_waves = 4 / p->tile_waves;
-  // four workgroups a compute unit of the second pass, up to 1024 tokens each; a block for every wavefront of a workgroup at least
-  int64_t n = std::max((1024 + pairs - 1) / pairs, (max_len + 1023) / 1024);
-  n = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(n, (blocks + 4 * token_waves - 1) / (4 * token_waves)), 4096));
-  const int64_t chunk = (blocks + n - 1) / n;
+  // the wavefronts that are left stand side by side on the tokens, as far as two turns of their blocks take no more than 64 KB (one block: any size)
+  const int64_t token_waves = p->tile_waves >= 4 ? 1 : std::max(1, std::min(4 / p->tile_waves, 32768 / window_block_bytes(d)));
+  p->waves = (int)(p->tile_waves * token_waves);
+  // twice as many workgroups as the card holds: sequences differ in length (nine of 17 .. 4099 tokens, 16 / 2 heads of 256, a pass: 33 us with once as
+  // many, 24 with twice, 24 with three times; four of 32768, 32 / 8 heads of 128, where nothing differs: 74, 81, 85); a block for every wavefront at least
+  const int64_t resident = 256 * 4 * window_waves_per_simd(dtype, d, p->waves == 8 ? 8 : 4) / p->waves;
+  int64_t n = std::max(2 * resident / pairs, (max_len + 4095) / 4096);
+  n = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(n, (blocks + token_waves - 1) / token_waves), 4096));
+  const int64_t chunk = ((blocks + n - 1) / n + token_waves - 1) / token_waves * token_waves;
   p->chunk = (int)chunk;
   p->n_split = (int)((blocks + chunk - 1) / chunk);
   p->parts = (int)(p->n_split * token_waves);
@@ -50,7 +65,7 @@ static bool window_plan(WindowPlan* p, int dtype, int B, int Hq, int Hkv, int d,
   p->ml_at = 0;
   p->stat_at = (rows * p->parts * sizeof(float2) + 255) & ~(size_t)255;
   p->bytes = p->stat_at + std::max<size_t>(256, (rows * sizeof(float2) + 255) & ~(size_t)255);
-  return pairs * p->n_split * p->row_groups <= INT32_MAX && (int64_t)((rows + 255) / 256) <= INT32_MAX;
+  return pairs * p->n_split * p->row_groups <= INT32_MAX && (int64_t)(rows / 16) <= INT32_MAX;
 }
 
 }  // namespace tq
@@ -78,7 +93,10 @@ extern "C" int tq_exact_window(const void* q, int dtype, int64_t rows, const int
   if ((uintptr_t)workspace & 15) return TQ_EINVAL;
   a.q = q; a.starts = query_start_loc; a.rows = rows; a.B = B; a.Hq = Hq; a.G = Hq / Hkv; a.W = window;
   a.row_tiles = p.row_tiles; a.tile_waves = p.tile_waves; a.row_groups = p.row_groups; a.n_split = p.n_split; a.chunk = p.chunk; a.parts = p.parts;
-  a.scale2 = sm_scale * 1.4426950408889634f;
+  // (not zero: a hidden score of -inf stays one)
+  a.scale2 = std::max(std::fabs(sm_scale) * 1.4426950408889634f, 1.17549435e-38f);
+  a.flip = std::signbit(sm_scale) ? (dtype == TQ_F32 ? 0x80000000u : 0x80008000u) : 0u;
+  a.waves = p.waves;
   a.ml = (float2*)((char*)workspace + p.ml_at);
   a.stat = (float2*)((char*)workspace + p.stat_at);
   a.weights = weights; a.w_b = w_b; a.w_h = w_h; a.L = (int)weight_len;
@@ -87,9 +105,8 @@ extern "C" int tq_exact_window(const void* q, int dtype, int64_t rows, const int
   int done = pass(a, false, st);
   if (done) return done;
   const int padded = p.row_tiles * 16;
-  const int64_t all = (int64_t)B * Hkv * padded;
-  exact_window_join_kernel<<<dim3((unsigned)((all + 255) / 256)), dim3(256), 0, st>>>(a.ml, a.stat, p.parts, padded, (int64_t)B * Hkv, a.c, p.block_tokens,
-                                                                                      p.n_split, p.chunk, 4 / p.tile_waves);
+  exact_window_join_kernel<<<dim3((unsigned)((int64_t)B * Hkv * p.row_tiles)), dim3(256), 0, st>>>(a.ml, a.stat, p.parts, padded, a.c, p.block_tokens, p.n_split,
+                                                                                                   p.chunk, p.waves / p.tile_waves);
   TQ_CHECK_LAUNCH();
   return pass(a, true, st);
 }

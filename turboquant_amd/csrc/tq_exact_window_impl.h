@@ -5,33 +5,46 @@
 //   second  weights[t] += sum_r 2^(s_rt - m_r) / l_r
 //
 // The scores are computed twice rather than stored: at W = 32 and 32 heads of 128 a token's scores are 4 KB per KV head and its key 256 bytes.
-// Tokens are rows of the matrix instruction and come from memory as they lie, as in decode; (query, head) rows are its columns and stay in
-// registers, window_tiles() tiles of 16 per wavefront.  The four wavefronts of a workgroup stand side by side on the tiles, or, with few of them,
-// on the tokens.  In the first pass a lane keeps maximum and sum of its own tokens (four of each sixteen) and joins them with the three other lanes of its
+// Tokens are rows of the matrix instruction, (query, head) rows its columns; those stay in registers, window_tiles() tiles of 16 per wavefront.  The
+// wavefronts of a workgroup stand side by side on the tiles, and, with few of those, on the tokens.  Keys lie in LDS twice, filled by LDS-direct loads
+// a turn ahead: read from memory as operands, they came from the L1 once for every wavefront, 16 lines of 64 bytes a load, and that was the bound.
+// In the first pass a lane keeps maximum and sum of its own tokens (four of each sixteen) and joins them with the three other lanes of its
 // row at the end; in the second it sums its columns' weights of its tokens, over the tiles in registers, over lanes once per block.
 #pragma once
 
-#include "tq_exact_impl.h"
+#include "tq_exact_heads_impl.h"
 #include "tq_exact_window.h"
 
 namespace tq {
 
 constexpr int WINDOW_TOKENS = 1024;             // tokens whose sums a workgroup of the second pass holds at a time
 
-template <int DT, int D, bool ADD>
-__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) exact_window_kernel(const ExactWindow a) {
+// A block's keys in LDS: rows one behind another, a row's 16-byte pieces in an order of its own, so that the sixteen rows of an operand lie in
+// different banks: with an even number of bank widths to a row, piece p of row r is the (p ^ r)-th of its sixteen; with an odd one, the
+// (p ^ r / 2)-th of its eight.
+template <int PIECES>
+__device__ __forceinline__ int window_place(int p, int r) {
+  return PIECES % 16 == 0 ? p ^ (r & 15) : p ^ (r >> 1 & 7);
+}
+
+template <int DT, int D, int WAVES, bool ADD>
+__global__ void __launch_bounds__(WAVES * 64, window_waves_per_simd(DT, D, WAVES)) exact_window_kernel(const ExactWindow a) {
   constexpr bool F32 = DT == TQ_F32;
   constexpr int TB = exact_tokens<DT>(), PAGES = TB / TQ_PAGE_TOKENS, SIZE = F32 ? 4 : 2;
-  constexpr int KSTEPS = D * SIZE / 64, NT = window_tiles(DT, D);
-  __shared__ float s_w[ADD ? 4 : 1][ADD ? WINDOW_TOKENS : 1];
+  constexpr int KSTEPS = D * SIZE / 64, NT = window_tiles(DT, D), PIECES = D * SIZE / 16;
+  constexpr int BLOCK = window_block_bytes(D), PAGE_LOADS = PIECES / 4;        // LDS-direct loads of a page: 64 pieces each
+  extern __shared__ __align__(16) unsigned char s_keys[];    // [2 turns][wavefronts side by side on tokens][BLOCK]
+  __shared__ float s_w[ADD ? WAVES : 1][ADD ? WINDOW_TOKENS : 1];
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int col = lane & 15, quarter = lane >> 4;
-  int id = (int)blockIdx.x;
-  const int split = id % a.n_split; id /= a.n_split;
+  unsigned id = blockIdx.x;
   int group0 = 0, groups = a.row_groups;
-  if (!ADD) { group0 = id % a.row_groups; id /= a.row_groups; groups = 1; }
-  const int h = id % a.c.H, b = id / a.c.H;
+  if (!ADD) { group0 = (int)(id % (unsigned)a.row_groups); id /= (unsigned)a.row_groups; groups = 1; }
+  // (splits of a sequence on different dies, as in decode)
+  const unsigned pairs = (unsigned)(a.c.H * a.B);
+  const int split = (int)(id / pairs), pair = (int)((id % pairs + (unsigned)split) % pairs);
+  const int h = pair % a.c.H, b = pair / a.c.H;
 
   const int len = exact_len(a.c, b);
   const int blocks = (len + TB - 1) / TB, per = exact_blocks_per_split(blocks, a.n_split, a.chunk);
@@ -44,31 +57,57 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) exact_window_kernel(con
   int W = a.W < len ? a.W : len;
   W = run < W ? (int)run : W;
   const int n_rows = W * a.G;
-  const int tile_wave = wave % a.tile_waves, token_wave = wave / a.tile_waves, token_waves = 4 / a.tile_waves;
+  const int tile_wave = wave % a.tile_waves, token_wave = wave / a.tile_waves, token_waves = a.waves / a.tile_waves;
   const int32_t* table = a.c.table + b * a.c.table_step;
   const int64_t row_at = (int64_t)b * a.c.H + h;
   const int padded = a.row_tiles * 16;
   if (first >= last || n_rows == 0) return;                  // (the same for the whole workgroup)
+  const uint32_t step = (uint32_t)a.c.s_t * SIZE, lds0 = (uint32_t)(uintptr_t)s_keys;
+
+  // A turn: token_waves blocks from `blk` on.  Lane l knows the table entry of the turn's page l; -1: behind the sequence.
+  const auto entries = [&](int blk) __attribute__((always_inline)) {
+    const int page = blk * PAGES + lane;
+    return lane < token_waves * PAGES && page * TQ_PAGE_TOKENS < len ? table[page] : -1;
+  };
+  const auto page_of = [&](int entry, int p) __attribute__((always_inline)) {
+    const int64_t x = __builtin_amdgcn_readlane(entry, p);
+    return x < 0 || x >= a.c.num_blocks ? (int64_t)-1 : x;
+  };
+  const auto fetch = [&](int entry, int turn) __attribute__((always_inline)) {
+    for (int n = wave; n < token_waves * PAGES * PAGE_LOADS; n += a.waves) {
+      const int p = n / PAGE_LOADS, k = n - p * PAGE_LOADS;  // page of the turn, load of the page
+      int64_t page = page_of(entry, p);
+      page = page < 0 ? 0 : page;                            // (a block that is there; its tokens are masked)
+      const int piece = k * 64 + lane, r = piece / PIECES, at = piece - r * PIECES;
+      const uint32_t off = (uint32_t)r * step + (uint32_t)window_place<PIECES>(at, r) * 16;
+      ex_row_to_lds((const char*)a.c.k + (page * a.c.s_blk + h * a.c.s_h) * SIZE, off,
+                    lds0 + (uint32_t)(turn * token_waves * BLOCK + p * (PAGE_LOADS * 1024) + k * 1024));
+    }
+  };
 
   for (int sub = first; sub < last; sub += ADD ? WINDOW_TOKENS / TB : last - first) {
     const int sub_end = ADD && sub + WINDOW_TOKENS / TB < last ? sub + WINDOW_TOKENS / TB : last;
     if (ADD) {
       __syncthreads();
-      for (int i = (int)threadIdx.x; i < 4 * WINDOW_TOKENS; i += 256) s_w[0][i] = 0.0f;
+      for (int i = (int)threadIdx.x; i < (sub_end - sub) * TB; i += a.waves * 64)
+        for (int k = 0; k < a.tile_waves; ++k) s_w[k][i] = 0.0f;
       __syncthreads();
     }
     for (int grp = group0; grp < group0 + groups; ++grp) {
+      if (grp * a.tile_waves * NT * 16 >= n_rows) break;     // (the same for the whole workgroup)
       const int tile0 = (grp * a.tile_waves + tile_wave) * NT;
-      if (tile0 * 16 >= n_rows) continue;                    // (no barrier inside)
+      const bool busy = tile0 * 16 < n_rows;                 // (a wavefront without rows still fetches and waits with the others)
+      if (ADD && grp > group0) __syncthreads();              // (the turns of the group before have been read)
+      int entry = entries(sub);
+      fetch(entry, 0);
+      int entry_next = entries(sub + token_waves);
       ex_u32x4 Q[NT][KSTEPS];
-      int end[NT];                                           // tokens that the row of this lane's column sees
-      float mx[NT], sm[NT];                                  // first pass: maximum and sum; second: maximum and 1 / sum of the row
+      float mx[NT], sm[NT];                                  // first pass: maximum (unscaled) and sum; second: maximum (log2) and 1 / sum of the row
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int r = (tile0 + t) * 16 + col;
         const bool live = r < n_rows;
         const int w = live ? r / a.G : 0, g = r - w * a.G;
-        end[t] = live ? len - W + w + 1 : 0;
         mx[t] = ADD ? 0.0f : -INFINITY;
         sm[t] = 0.0f;
         if (ADD && live) {
@@ -80,34 +119,41 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) exact_window_kernel(con
         for (int s = 0; s < KSTEPS; ++s) {
           Q[t][s] = ex_u32x4{0, 0, 0, 0};
           if (live) Q[t][s] = *(const ex_u32x4*)((const char*)a.q + (((r1 - W + w) * a.Hq + h * a.G + g) * D) * SIZE + s * 64 + quarter * 16);
+          Q[t][s] ^= a.flip;                                 // (a negative scale is the queries')
         }
       }
       const bool full_tiles = (tile0 + NT) * 16 <= n_rows;
-      for (int blk = sub + token_wave; blk < sub_end; blk += token_waves) {
-        const int t0 = blk * TB;
-        bool whole = full_tiles && t0 + TB <= len - W + 1;   // every row sees every token
-        const char* kp[PAGES];
+      for (int turn0 = sub, turn = 0; turn0 < sub_end; turn0 += token_waves, turn ^= 1) {
+        ex_arrived();
+        __syncthreads();                                     // everybody's loads of this turn are there, everybody is done with the other
+        const int now = entry;
+        if (turn0 + token_waves < sub_end) {
+          entry = entry_next;
+          fetch(entry, turn ^ 1);
+          entry_next = entries(turn0 + 2 * token_waves);
+        }
+        const int blk = turn0 + token_wave, t0 = blk * TB;
+        if (!busy || blk >= sub_end) continue;
         int valid[PAGES];
+        bool whole = full_tiles && t0 + TB <= len - W + 1;   // every row sees every token
 #pragma unroll
         for (int p = 0; p < PAGES; ++p) {
           const int left = len - t0 - p * TQ_PAGE_TOKENS;
-          valid[p] = left < 0 ? 0 : (left > TQ_PAGE_TOKENS ? TQ_PAGE_TOKENS : left);
-          int64_t page = left > 0 ? table[blk * PAGES + p] : 0;
-          if (page < 0 || page >= a.c.num_blocks) { page = 0; valid[p] = 0; }
+          valid[p] = page_of(now, token_wave * PAGES + p) < 0 || left < 0 ? 0 : (left > TQ_PAGE_TOKENS ? TQ_PAGE_TOKENS : left);
           whole &= valid[p] == TQ_PAGE_TOKENS;
-          kp[p] = (const char*)a.c.k + (page * a.c.s_blk + h * a.c.s_h) * SIZE;
         }
-        const uint32_t krow = (uint32_t)col * (uint32_t)a.c.s_t * SIZE + quarter * 16;
+        const unsigned char* keys = s_keys + (turn * token_waves + token_wave) * BLOCK;
+        const auto key = [&](int p, int s) __attribute__((always_inline)) {
+          return *(const ex_u32x4*)(keys + ((p * 16 + col) * PIECES + window_place<PIECES>(s * 4 + quarter, col)) * 16);
+        };
         ex_f32x4 S[NT][PAGES];
 #pragma unroll
         for (int p = 0; p < PAGES; ++p) {
-          const bool there = whole || col < valid[p];
 #pragma unroll
           for (int t = 0; t < NT; ++t) S[t][p] = ex_f32x4{0, 0, 0, 0};
 #pragma unroll
           for (int s = 0; s < KSTEPS; ++s) {
-            ex_u32x4 kf = {0, 0, 0, 0};
-            if (there) kf = *(const ex_u32x4*)(kp[p] + krow + s * 64);
+            const ex_u32x4 kf = key(p, s);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               if constexpr (F32) {
@@ -120,17 +166,21 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) exact_window_kernel(con
             }
           }
         }
-        // scores in powers of two; hidden ones have no weight
+        // hidden scores have no weight; blocks that every row sees whole are left as they are
+        if (!whole) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+          for (int t = 0; t < NT; ++t) {
+            const int r = (tile0 + t) * 16 + col;
+            const int end = r < n_rows ? len - W + r / a.G + 1 : 0;          // tokens that the row of this lane's column sees
 #pragma unroll
-          for (int p = 0; p < PAGES; ++p)
+            for (int p = 0; p < PAGES; ++p)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int in = quarter * 4 + i;
-              const float s2 = S[t][p][i] * a.scale2;
-              S[t][p][i] = whole || (in < valid[p] && t0 + p * TQ_PAGE_TOKENS + in < end[t]) ? s2 : -INFINITY;
-            }
+              for (int i = 0; i < 4; ++i) {
+                const int in = quarter * 4 + i;
+                if (!(in < valid[p] && t0 + p * TQ_PAGE_TOKENS + in < end)) S[t][p][i] = -INFINITY;
+              }
+          }
+        }
         if constexpr (!ADD) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -139,40 +189,40 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) exact_window_kernel(con
             for (int p = 0; p < PAGES; ++p)
 #pragma unroll
               for (int i = 0; i < 4; ++i) top = fmaxf(top, S[t][p][i]);
-            const float ref = top == -INFINITY ? 0.0f : top;
-            float sum = sm[t] * __builtin_amdgcn_exp2f(mx[t] - ref);
+            const float ref = top == -INFINITY ? 0.0f : top * a.scale2;
+            float sum = sm[t] * __builtin_amdgcn_exp2f(fmaf(mx[t], a.scale2, -ref));
 #pragma unroll
             for (int p = 0; p < PAGES; ++p)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(S[t][p][i] - ref);
+              for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(fmaf(S[t][p][i], a.scale2, -ref));
             sm[t] = sum;
             mx[t] = top;
           }
         } else {
-          ex_f32x4 add[PAGES];
 #pragma unroll
           for (int p = 0; p < PAGES; ++p) {
-            add[p] = ex_f32x4{0, 0, 0, 0};
+            ex_f32x4 add = {0, 0, 0, 0};
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) add[p][i] = fmaf(__builtin_amdgcn_exp2f(S[t][p][i] - mx[t]), sm[t], add[p][i]);
+              for (int i = 0; i < 4; ++i) add[i] = fmaf(__builtin_amdgcn_exp2f(fmaf(S[t][p][i], a.scale2, -mx[t])), sm[t], add[i]);
             // over the sixteen rows of the tiles
 #pragma unroll
-            for (int i = 0; i < 4; ++i) add[p][i] = lanes_sum_dpp<16>(add[p][i]);
+            for (int i = 0; i < 4; ++i) add[i] = lanes_sum_dpp<16>(add[i]);
             if (col == 0) {
-              float* to = &s_w[wave][(blk - sub) * TB + p * TQ_PAGE_TOKENS + quarter * 4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) to[i] += add[p][i];
+              ex_f32x4* to = (ex_f32x4*)&s_w[tile_wave][(blk - sub) * TB + p * TQ_PAGE_TOKENS + quarter * 4];
+              *to += add;
             }
           }
         }
       }
       if constexpr (!ADD) {
+        if (!busy) continue;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const float top = ex_quad_max(mx[t]), ref = top == -INFINITY ? 0.0f : top;
-          const float sum = ex_quad_sum(sm[t] * __builtin_amdgcn_exp2f(mx[t] - ref));
+          const float mine = mx[t] == -INFINITY ? -INFINITY : mx[t] * a.scale2;
+          const float top = ex_quad_max(mine), ref = top == -INFINITY ? 0.0f : top;
+          const float sum = ex_quad_sum(sm[t] * __builtin_amdgcn_exp2f(mine - ref));
           const int r = (tile0 + t) * 16 + col;
           if (quarter == 0 && r < n_rows) a.ml[(row_at * a.parts + split * token_waves + token_wave) * padded + r] = make_float2(top, sum);
         }
@@ -181,9 +231,11 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) exact_window_kernel(con
     if constexpr (ADD) {
       __syncthreads();
       float* w = a.weights + b * a.w_b + h * a.w_h;
-      for (int i = (int)threadIdx.x; i < (sub_end - sub) * TB; i += 256) {
+      for (int i = (int)threadIdx.x; i < (sub_end - sub) * TB; i += a.waves * 64) {
         const int t = sub * TB + i;
-        if (t < len && t < a.L) w[t] += (s_w[0][i] + s_w[1][i]) + (s_w[2][i] + s_w[3][i]);
+        float add = 0.0f;
+        for (int k = 0; k < a.tile_waves; ++k) add += s_w[k][i];
+        if (t < len && t < a.L) w[t] += add;
       }
     }
   }
@@ -191,18 +243,29 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) exact_window_kernel(con
 
 template <int DT>
 int launch_exact_window(const ExactWindow& a, bool add, hipStream_t stream) {
-  const dim3 grid((unsigned)((int64_t)a.n_split * (add ? 1 : a.row_groups) * a.c.H * a.B)), block(256);
+  const dim3 grid((unsigned)((int64_t)a.n_split * (add ? 1 : a.row_groups) * a.c.H * a.B)), block(a.waves * 64);
+  const int lds = 2 * a.waves / a.tile_waves * window_block_bytes(a.c.d);
+#define TQ_WINDOW(D, WAVES, ADD)                                                                                            \
+  {                                                                                                                         \
+    const auto kern = exact_window_kernel<DT, D, WAVES, ADD>;                                                               \
+    static std::atomic<uint64_t> ready{0};                                                                                  \
+    if (const int rc = exact_allow_lds((const void*)kern, WINDOW_LDS, ready)) return rc;                                    \
+    kern<<<grid, block, lds, stream>>>(a);                                                                                  \
+    break;                                                                                                                  \
+  }
 #define TQ_WINDOW_D(D)                                                                \
   case D:                                                                             \
-    if (add) exact_window_kernel<DT, D, true><<<grid, block, 0, stream>>>(a);         \
-    else exact_window_kernel<DT, D, false><<<grid, block, 0, stream>>>(a);            \
-    break
+    if (a.waves == 8 && add) TQ_WINDOW(D, 8, true)                                    \
+    if (a.waves == 8) TQ_WINDOW(D, 8, false)                                          \
+    if (add) TQ_WINDOW(D, 4, true)                                                    \
+    TQ_WINDOW(D, 4, false)
   switch (a.c.d) {
-    TQ_WINDOW_D(64); TQ_WINDOW_D(128); TQ_WINDOW_D(192); TQ_WINDOW_D(256); TQ_WINDOW_D(320); TQ_WINDOW_D(384);
-    TQ_WINDOW_D(448); TQ_WINDOW_D(512); TQ_WINDOW_D(576); TQ_WINDOW_D(640); TQ_WINDOW_D(704); TQ_WINDOW_D(768);
+    TQ_WINDOW_D(64) TQ_WINDOW_D(128) TQ_WINDOW_D(192) TQ_WINDOW_D(256) TQ_WINDOW_D(320) TQ_WINDOW_D(384)
+    TQ_WINDOW_D(448) TQ_WINDOW_D(512) TQ_WINDOW_D(576) TQ_WINDOW_D(640) TQ_WINDOW_D(704) TQ_WINDOW_D(768)
     default: return TQ_EUNSUPPORTED;
   }
 #undef TQ_WINDOW_D
+#undef TQ_WINDOW
   TQ_CHECK_LAUNCH();
   return TQ_OK;
 }
