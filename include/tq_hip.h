@@ -432,14 +432,16 @@ int tq_exact_window(const void *q, int dtype, int64_t rows, const int32_t *query
  * (tokens that a sequence has had in all; NULL: seq_lens) are device int32 (B,); lengths above L are cut to L.  1 <= budget, sinks + recent <= budget.
  * Written: lens_out (B,) = min(length, budget); count (B, H) moves; dst / src (B, H, moves) slots, ascending, -1 from count on, moves at
  * least max(1, min(budget, L - budget)); weights_out / positions_out (B, H, L), which may be the inputs themselves (same address and strides):
- * those of the tokens that stay, then 0 and the positions that the next tokens will have.
+ * those of the tokens that stay, then 0 and the positions that the next tokens will have.  workspace: tq_evict_select_bytes bytes, 16-byte
+ * aligned (0 bytes: not looked at), of this call alone until it has run.
  * tq_move_tokens_exact, tq_move_tokens_pool: carry the moves out in an exact cache (all strides in elements) / in the compressed pages of
  * the same block numbers (`budget`: the one of the selection).  A sequence's pages must be its own: tokens are overwritten in place.  Moves that
  * touch a page outside the table row or the cache are left out.                                                                   */
+size_t tq_evict_select_bytes(int B, int H, int L, int budget, int moves);
 int tq_evict_select(const float *weights, int64_t w_b, int64_t w_h, const int32_t *positions, int64_t p_b, int64_t p_h,
                     const int32_t *seq_lens, const int32_t *seen, int B, int H, int L, int budget, int sinks, int recent,
                     int moves, int32_t *lens_out, int32_t *count, int32_t *dst, int32_t *src, float *weights_out, int64_t wo_b,
-                    int64_t wo_h, int32_t *positions_out, int64_t po_b, int64_t po_h, void *stream);
+                    int64_t wo_h, int32_t *positions_out, int64_t po_b, int64_t po_h, void *workspace, void *stream);
 int tq_move_tokens_exact(void *k_cache, void *v_cache, int dtype, int d, int64_t cs_blk, int64_t cs_t, int64_t cs_h,
                          int64_t num_blocks, const int32_t *block_table, int bt_stride, const int32_t *count, const int32_t *dst,
                          const int32_t *src, int B, int H, int moves, void *stream);

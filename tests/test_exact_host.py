@@ -78,7 +78,7 @@ def test_window_of_nothing_launches_nothing():
 
 def select_args(**kw):
     a = dict(w=P, w_b=80, w_h=40, pos=P, p_b=80, p_h=40, lens=P, seen=None, B=2, H=2, L=40, budget=20, sinks=4, recent=3, moves=20, lens_out=P, count=P,
-             dst=P, src=P, w_out=P, wo_b=80, wo_h=40, pos_out=P, po_b=80, po_h=40, stream=None)
+             dst=P, src=P, w_out=P, wo_b=80, wo_h=40, pos_out=P, po_b=80, po_h=40, workspace=None, stream=None)
     assert set(kw) <= set(a)
     return list({**a, **kw}.values())
 
@@ -87,7 +87,7 @@ def select_args(**kw):
     *((dict([(n, None)]), -3) for n in ("w", "pos", "lens", "lens_out", "count", "dst", "src", "w_out", "pos_out")),
     (dict(B=-1), -1), (dict(H=0), -1), (dict(L=0), -1), (dict(budget=0), -1), (dict(sinks=-1), -1), (dict(recent=-1), -1),
     (dict(sinks=10, recent=11), -1), (dict(sinks=2 ** 31 - 1, recent=2 ** 31 - 1), -1), (dict(moves=19), -1), (dict(w_b=-1), -1), (dict(po_h=-1), -1),
-    (dict(B=2 ** 20, H=2 ** 12), -1),
+    (dict(B=2 ** 20, H=2 ** 12), -1), (dict(L=2 ** 30 + 1, budget=1, sinks=0, recent=0), -1), (dict(L=40000), -3), (dict(L=40000, workspace=P + 8), -1),
 ])
 def test_select_refuses(bad, rc):
     assert _ffi.lib().tq_evict_select(*select_args(**bad)) == rc

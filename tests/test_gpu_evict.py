@@ -61,7 +61,15 @@ def test_who_stays(gpu, L, budget, kind):
 @pytest.mark.parametrize("L,budget", [(40000, 1000), (131072, 16384), (150001, 75000)])
 def test_long_rows(gpu, L, budget):
     for kind in ("sums", "ties", "close"):
-        check(weights_of(1, 2, L, 1, kind), in_order(1, 2, L), [L - 3], budget, sinks=16, recent=100)
+        check(weights_of(1, 2, L, 1, kind), in_order(1, 2, L), [L - 3], budget, sinks=16, recent=100, out="inputs" if kind == "ties" else None)
+
+
+@pytest.mark.parametrize("L,budget", [(16384, 5), (16385, 5), (16385, 16384), (4096, 4095), (4097, 100), (32769, 32768), (33000, 8192), (50000, 8193), (40000, 20000)])
+def test_rows_at_the_ends_of_their_parts(gpu, L, budget):
+    """One workgroup and several, budgets at and off a part's end, and rows of a batch that are within the budget beside others."""
+    for kind, sinks, recent in (("sums", 0, 0), ("equal", min(4, budget), 0), ("odd", 0, min(budget, 1000))):
+        w, pos = weights_of(3, 1, L, budget, kind), in_order(3, 1, L)
+        check(w, pos, [L, min(L, budget + 1), budget - 1], budget, sinks=sinks, recent=recent, out="inputs" if kind == "equal" else None)
 
 
 def test_lengths_within_the_budget_and_of_nothing(gpu):

@@ -11,7 +11,10 @@
 
 namespace tq {
 
-constexpr int SEL_THREADS = 1024, SEL_BINS = 2048;
+constexpr int SEL_BINS = 2048;
+// the digits of a key, from the highest: 11, 11 and 10 bits
+__host__ __device__ constexpr int sel_low(int pass) { return pass == 0 ? 21 : (pass == 1 ? 10 : 0); }
+__host__ __device__ constexpr int sel_bits(int pass) { return pass == 2 ? 10 : 11; }
 
 struct EvictSelect {
   const float* w;  int64_t w_b, w_h;            // (B, H, L) in
@@ -31,7 +34,59 @@ __device__ __forceinline__ uint32_t evict_key(float w, int pos, int sinks, int n
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// One row: its pointers and numbers
+struct EvictRow {
+  const float* w;
+  const int32_t* pos;
+  float* w_out;
+  int32_t *pos_out, *dst, *src;
+  int64_t row;
+  int b, h, n, left, seen, newest;
+  __device__ __forceinline__ EvictRow(const EvictSelect& a, int r) {
+    row = r; h = r % a.H; b = r / a.H;
+    const int held = a.lens[b];
+    n = held < 0 ? 0 : (held > a.L ? a.L : held);
+    left = n < a.budget ? n : a.budget;
+    seen = a.seen ? a.seen[b] : held;
+    const int64_t from = (int64_t)seen - a.recent;
+    newest = from < INT32_MIN ? INT32_MIN : (int)from;
+    w = a.w + b * a.w_b + h * a.w_h;
+    pos = a.pos + b * a.p_b + h * a.p_h;
+    w_out = a.w_out + b * a.wo_b + h * a.wo_h;
+    pos_out = a.pos_out + b * a.po_b + h * a.po_h;
+    dst = a.dst + row * a.moves;
+    src = a.src + row * a.moves;
+  }
+};
+
+// Weights and positions of a wavefront's J x 64 slots from `base` on (of slot 0 from `end` on).  All loads first, none behind a condition: one memory
+// latency, not J of them.
+template <int J>
+__device__ __forceinline__ void sel_load(float (&w)[J], int (&pos)[J], const EvictRow& r, int base, int end) {
+  const int lane = (int)threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int i = base + j * 64 + lane, at = i < end ? i : 0;
+    w[j] = r.w[at];
+    pos[j] = r.pos[at];
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) asm volatile("" : "+v"(w[j]), "+v"(pos[j]));
+}
+// counts a key's digit; a wavefront whose keys all fall into one bin adds once (sums that are all alike would be 64 turns of one address)
+__device__ __forceinline__ void sel_count(uint32_t* bins, bool in, uint32_t digit) {
+  const uint64_t who = __ballot(in);
+  if (who == 0) return;
+  const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)digit, __builtin_ctzll(who));
+  if (__ballot(in && digit == first) == who) {
+    if (((int)threadIdx.x & 63) == __builtin_ctzll(who)) atomicAdd(&bins[first], (uint32_t)__popcll(who));
+  } else if (in) {
+    atomicAdd(&bins[digit], 1u);
+  }
+}
+
 // inclusive sum over the workgroup's threads; *total = all of it
+template <int THREADS>
 __device__ __forceinline__ uint32_t sel_scan(uint32_t v, uint32_t* s_wave, uint32_t* total) {
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
 #pragma unroll
@@ -44,7 +99,7 @@ __device__ __forceinline__ uint32_t sel_scan(uint32_t v, uint32_t* s_wave, uint3
   __syncthreads();
   uint32_t before = 0, all = 0;
 #pragma unroll
-  for (int i = 0; i < SEL_THREADS / 64; ++i) {
+  for (int i = 0; i < THREADS / 64; ++i) {
     const uint32_t x = s_wave[i];
     if (i < wave) before += x;
     all += x;
@@ -53,92 +108,381 @@ __device__ __forceinline__ uint32_t sel_scan(uint32_t v, uint32_t* s_wave, uint3
   return before + v;
 }
 
-__global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictSelect a) {
-  __shared__ uint32_t s_bin[SEL_BINS];
-  __shared__ uint32_t s_wave[SEL_THREADS / 64];
-  __shared__ uint32_t s_found[2];
-  const int tid = (int)threadIdx.x, h = (int)blockIdx.x % a.H, b = (int)blockIdx.x / a.H;
-  const int held = a.lens[b], n = held < 0 ? 0 : (held > a.L ? a.L : held);
-  const int seen = a.seen ? a.seen[b] : held;
-  const int64_t newest64 = (int64_t)seen - a.recent;
-  const int newest = newest64 < INT32_MIN ? INT32_MIN : (int)newest64;
-  const float* w = a.w + b * a.w_b + h * a.w_h;
-  const int32_t* pos = a.pos + b * a.p_b + h * a.p_h;
-  float* w_out = a.w_out + b * a.wo_b + h * a.wo_h;
-  int32_t* pos_out = a.pos_out + b * a.po_b + h * a.po_h;
-  const int64_t row = (int64_t)b * a.H + h;
-  int32_t *dst = a.dst + row * a.moves, *src = a.src + row * a.moves;
-  const int left = n < a.budget ? n : a.budget;
-  if (h == 0 && tid == 0) a.lens_out[b] = left;
+// The bin, from the highest down, in which the count reaches `want`: s_found = {bin, how many of it are wanted}.  count(bin): keys in it.
+template <int THREADS, class Count>
+__device__ __forceinline__ void sel_find(uint32_t want, Count count, uint32_t* s_wave, uint32_t* s_found) {
+  constexpr int EACH = SEL_BINS / THREADS;
+  const int hi = SEL_BINS - 1 - EACH * (int)threadIdx.x;
+  uint32_t c[EACH], mine = 0, total;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) { c[i] = count(hi - i); mine += c[i]; }
+  uint32_t before = sel_scan<THREADS>(mine, s_wave, &total) - mine;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    if (before < want && want <= before + c[i]) {
+      s_found[0] = (uint32_t)(hi - i);
+      s_found[1] = want - before;
+    }
+    before += c[i];
+  }
+  __syncthreads();
+}
 
+// exclusive sum over the wavefronts of two counts that each of them has, in slot order
+template <int WAVES>
+__device__ __forceinline__ uint2 sel_waves(uint2 v, uint2* s_two, uint2* total) {
+  const int wave = (int)threadIdx.x >> 6;
+  __syncthreads();
+  if (((int)threadIdx.x & 63) == 0) s_two[wave] = v;
+  __syncthreads();
+  uint2 before = make_uint2(0, 0), all = before;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    const uint2 x = s_two[i];
+    if (i < wave) { before.x += x.x; before.y += x.y; }
+    all.x += x.x; all.y += x.y;
+  }
+  *total = all;
+  return before;
+}
+
+// Keys of a wavefront's J x 64 neighbouring slots in registers: who of them stays, and the lists.  `ties`: keys equal to `last` in front of these slots;
+// `holes`, `movers`: in front of the wavefront's slots, found by `offsets` from its own numbers.  put(slot, rank, mover, j).  Returns bit j: slot j stays.
+template <int J, class Offsets, class Put>
+__device__ __forceinline__ uint32_t sel_lists(const uint32_t (&k)[J], int base, int n, int budget, uint32_t last, uint32_t want, uint32_t ties, Offsets offsets, Put put) {
+  const int lane = (int)threadIdx.x & 63;
+  const uint64_t below = (1ull << lane) - 1;
+  uint32_t stays = 0, holes = 0, movers = 0;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int i = base + j * 64 + lane;
+    const bool in = i < n, tie = in && k[j] == last;
+    const uint64_t t = __ballot(tie);
+    const bool keep = in && (k[j] > last || (tie && ties + (uint32_t)__popcll(t & below) < want));
+    ties += (uint32_t)__popcll(t);
+    stays |= (uint32_t)keep << j;
+    holes += (uint32_t)__popcll(__ballot(in && !keep && i < budget));
+    movers += (uint32_t)__popcll(__ballot(keep && i >= budget));
+  }
+  const uint2 at = offsets(make_uint2(holes, movers));
+  holes = at.x; movers = at.y;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int i = base + j * 64 + lane;
+    const bool keep = stays >> j & 1, hole = i < n && !keep && i < budget, mover = keep && i >= budget;
+    const uint64_t hb = __ballot(hole), mb = __ballot(mover);
+    if (hole) put(i, holes + (uint32_t)__popcll(hb & below), false, j);
+    if (mover) put(i, movers + (uint32_t)__popcll(mb & below), true, j);
+    holes += (uint32_t)__popcll(hb);
+    movers += (uint32_t)__popcll(mb);
+  }
+  return stays;
+}
+
+// ---- a row in one workgroup: its keys are read once and stay in registers ----
+// `each` (up to J): 64 slots per wavefront and step, so that all wavefronts have some.
+template <int THREADS, int J>
+__global__ void __launch_bounds__(THREADS) evict_row_kernel(const EvictSelect a, int each) {
+  constexpr int WAVES = THREADS / 64, BATCH = J < 8 ? J : 8;
+  __shared__ uint32_t s_bin[SEL_BINS];
+  __shared__ uint32_t s_wave[WAVES], s_found[2];
+  __shared__ uint2 s_two[WAVES];
+  const int tid = (int)threadIdx.x, lane = tid & 63, base = (tid >> 6) * (each * 64);
+  const EvictRow r(a, (int)blockIdx.x);
+  if (r.h == 0 && tid == 0) a.lens_out[r.b] = r.left;
   uint32_t moved = 0;
-  if (n > a.budget && a.budget > 0) {
-    // ---- the key of the last one that stays: three digits, from the highest ----
-    uint32_t want = (uint32_t)a.budget, prefix = 0;
-    int low = 21;                               // lowest bit of the digit
+  if (r.n > a.budget) {
+    const int end = base + each * 64 < r.n ? base + each * 64 : r.n;          // of this wavefront's slots
+    uint32_t k[J];
+    {
+      float w[J];
+      int pos[J];
+      sel_load<J>(w, pos, r, base, end);
+#pragma unroll
+      for (int j = 0; j < J; ++j) k[j] = base + j * 64 + lane < end ? evict_key(w[j], pos[j], a.sinks, r.newest) : 0u;
+    }
+    uint32_t want = (uint32_t)a.budget, last = 0;
+#pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
-      const int bits = pass == 2 ? 10 : 11, above = low + bits;
-      for (int i = tid; i < SEL_BINS; i += SEL_THREADS) s_bin[i] = 0;
+      const int low = sel_low(pass), above = low + sel_bits(pass);
+      for (int i = tid; i < SEL_BINS; i += THREADS) s_bin[i] = 0;
       __syncthreads();
-      for (int i = tid; i < n; i += SEL_THREADS) {
-        const uint32_t k = evict_key(w[i], pos[i], a.sinks, newest);
-        if (above == 32 || (k >> above) == (prefix >> above)) atomicAdd(&s_bin[(k >> low) & ((1u << bits) - 1)], 1u);
-      }
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        sel_count(s_bin, base + j * 64 + lane < end && (pass == 0 || (k[j] >> (above & 31)) == (last >> (above & 31))), (k[j] >> low) & ((1u << sel_bits(pass)) - 1));
       __syncthreads();
-      // from the highest bin down: the one in which the count reaches what is wanted
-      const int hi = SEL_BINS - 1 - 2 * tid;    // this thread's two bins, in that order
-      const uint32_t c0 = s_bin[hi], c1 = s_bin[hi - 1];
-      uint32_t total;
-      const uint32_t upto = sel_scan(c0 + c1, s_wave, &total), before = upto - c0 - c1;
-      if (before < want && want <= upto) {
-        const bool first = want <= before + c0;
-        s_found[0] = (uint32_t)(first ? hi : hi - 1);
-        s_found[1] = want - (first ? before : before + c0);
-      }
-      __syncthreads();
-      prefix |= s_found[0] << low;
-      want = s_found[1];                        // of the keys equal so far
-      low = pass == 0 ? 10 : 0;
+      sel_find<THREADS>(want, [&](int bin) { return s_bin[bin]; }, s_wave, s_found);
+      last |= s_found[0] << low;
+      want = s_found[1];
     }
-    // ---- in slot order: who stays, holes and movers ----
-    uint32_t ties = 0, holes = 0, movers = 0;
-    for (int i0 = 0; i0 < n; i0 += SEL_THREADS) {
-      const int i = i0 + tid;
-      const bool in = i < n;
-      const uint32_t k = in ? evict_key(w[i], pos[i], a.sinks, newest) : 0u;
-      const bool tie = in && k == prefix;
-      uint32_t total;
-      const uint32_t rank = ties + sel_scan(tie, s_wave, &total);       // 1 for the first
-      ties += total;
-      const bool stays = in && (k > prefix || (tie && rank <= want));
-      const bool hole = in && !stays && i < a.budget, mover = stays && i >= a.budget;
-      const uint32_t at = sel_scan((uint32_t)hole | (uint32_t)mover << 16, s_wave, &total);
-      const uint32_t hr = holes + (at & 0xffff), mr = movers + (at >> 16);
-      if (hole) dst[hr - 1] = i;
-      if (mover) src[mr - 1] = i;
-      holes += total & 0xffff;
-      movers += total >> 16;
-    }
-    moved = movers;
+    // ties in front of this wavefront's slots
+    uint32_t ties = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) ties += (uint32_t)__popcll(__ballot(base + j * 64 + lane < end && k[j] == last));
+    uint2 total;
+    ties = sel_waves<WAVES>(make_uint2(ties, 0), s_two, &total).x;
+    sel_lists<J>(k, base, end, a.budget, last, want, ties, [&](uint2 mine) { return sel_waves<WAVES>(mine, s_two, &total); },
+                 [&](int slot, uint32_t rank, bool mover, int) { (mover ? r.src : r.dst)[rank] = slot; });
+    moved = total.y;
   }
-  if (tid == 0) a.count[row] = (int32_t)moved;
-  for (int i = (int)moved + tid; i < a.moves; i += SEL_THREADS) dst[i] = src[i] = -1;
-  // ---- weights and positions of who stays: in place first, then the movers, then the slots that are free now ----
-  if (w_out != w)
-    for (int i = tid; i < left; i += SEL_THREADS) w_out[i] = w[i];
-  if (pos_out != pos)
-    for (int i = tid; i < left; i += SEL_THREADS) pos_out[i] = pos[i];
-  __syncthreads();
-  for (int i = tid; i < (int)moved; i += SEL_THREADS) {
-    const int to = dst[i], of = src[i];
-    w_out[to] = w[of];
-    pos_out[to] = pos[of];
+  if (tid == 0) a.count[r.row] = (int32_t)moved;
+  for (int i = (int)moved + tid; i < a.moves; i += THREADS) r.dst[i] = r.src[i] = -1;
+  // ---- weights and positions of who stays: in place first (holes too), then the movers, then the slots that are free now ----
+  if (r.w_out != r.w || r.pos_out != r.pos) {
+    for (int j0 = 0; j0 < each; j0 += BATCH) {
+      const int from = base + j0 * 64, end = base + each * 64 < r.left ? base + each * 64 : r.left;
+      float w[BATCH];
+      int pos[BATCH];
+      sel_load<BATCH>(w, pos, r, from, end);
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const int i = from + j * 64 + lane;
+        if (i < end && r.w_out != r.w) r.w_out[i] = w[j];
+        if (i < end && r.pos_out != r.pos) r.pos_out[i] = pos[j];
+      }
+    }
   }
   __syncthreads();
-  for (int i = left + tid; i < a.L; i += SEL_THREADS) {
-    w_out[i] = 0.0f;
-    pos_out[i] = seen + (i - left);
+  for (int i0 = 0; i0 < (int)moved; i0 += THREADS * 4) {
+    int to[4], of[4], pos[4];
+    float w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j * THREADS + tid, at = i < (int)moved ? i : 0;
+      to[j] = r.dst[at];
+      of[j] = r.src[at];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { w[j] = r.w[of[j]]; pos[j] = r.pos[of[j]]; }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(w[j]), "+v"(pos[j]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j * THREADS + tid < (int)moved) {
+        r.w_out[to[j]] = w[j];
+        r.pos_out[to[j]] = pos[j];
+      }
   }
+  __syncthreads();
+  for (int i = r.left + tid; i < a.L; i += THREADS) {
+    r.w_out[i] = 0.0f;
+    r.pos_out[i] = r.seen + (i - r.left);
+  }
+}
+
+// ---- a long row in several workgroups ----
+// A part is up to PART slots, all below the budget or none.  Three launches count the digits, each part into bins of its own (no atomics on memory, nothing to
+// clear); a launch finds the digit of the one before by summing the parts.  A fourth writes the lists: what lies in front of a part follows
+// from the parts' counts of larger keys and of ties.  It copies who stays where it is, movers leave their weight and position in the workspace, and a
+// fifth puts those where the holes are and clears the slots behind the budget; weights and positions may be rewritten in place, since nothing is read
+// from them there.
+constexpr int PART_THREADS = 1024, PART_J = 8, PART = PART_THREADS * PART_J, PART_WAVES = PART_THREADS / 64;
+
+struct EvictParts {
+  int32_t below, parts;                         // parts below the budget, and in all
+  uint32_t* bins;                               // (3 passes, rows, parts, SEL_BINS)
+  uint32_t* larger;                             // (rows, parts): keys known to be larger than the last that stays
+  uint32_t* found;                              // (3 passes, rows, 2)
+  float* moved_w;                               // (rows, moves)
+  int32_t* moved_pos;
+};
+
+__device__ __forceinline__ void part_slots(const EvictSelect& a, const EvictParts& q, const EvictRow& r, int part, int* first, int* end) {
+  const int64_t from = part < q.below ? (int64_t)part * PART : (int64_t)a.budget + (int64_t)(part - q.below) * PART;
+  const int64_t to = part < q.below && from + PART > a.budget ? a.budget : from + PART;
+  *first = (int)(from < r.n ? from : r.n);
+  *end = (int)(to < r.n ? to : r.n);
+}
+
+// (pass 3: the lists)
+template <int PASS>
+__global__ void __launch_bounds__(PART_THREADS) evict_part_kernel(const EvictSelect a, const EvictParts q) {
+  __shared__ uint32_t s_bin[SEL_BINS];
+  __shared__ uint32_t s_wave[PART_WAVES], s_found[2];
+  __shared__ uint2 s_two[PART_WAVES], s_part[PART_WAVES];
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int part = (int)(blockIdx.x % (unsigned)q.parts);
+  const EvictRow r(a, (int)(blockIdx.x / (unsigned)q.parts));
+  const int64_t rows = (int64_t)a.B * a.H;
+  if (PASS == 0 && part == 0 && r.h == 0 && tid == 0) a.lens_out[r.b] = r.left;
+  if (r.n <= a.budget) return;                  // (the last launch does what there is to do)
+  int first, end;
+  part_slots(a, q, r, part, &first, &end);
+  uint32_t want = (uint32_t)a.budget, last = 0;
+  if constexpr (PASS > 0) {
+#pragma unroll
+    for (int p = 0; p + 1 < PASS; ++p) {        // digits that earlier launches have found
+      const uint32_t* f = q.found + (p * rows + r.row) * 2;
+      last |= f[0] << sel_low(p);
+      want = f[1];
+    }
+    const uint32_t* bins = q.bins + (((PASS - 1) * rows + r.row) * q.parts) * SEL_BINS;
+    sel_find<PART_THREADS>(want, [&](int bin) {
+      uint32_t n = 0;
+#pragma unroll 8
+      for (int p = 0; p < q.parts; ++p) n += bins[(int64_t)p * SEL_BINS + bin];
+      return n;
+    }, s_wave, s_found);
+    const uint32_t digit = s_found[0];
+    last |= digit << sel_low(PASS - 1);
+    want = s_found[1];
+    if (PASS < 3) {
+      // every part's own: how many of its keys are larger by this digit
+      uint32_t n = 0, total;
+#pragma unroll
+      for (int u = 0; u < SEL_BINS / PART_THREADS; ++u) {
+        const int i = u * PART_THREADS + tid;
+        const uint32_t c = bins[(int64_t)part * SEL_BINS + i];
+        n += i > (int)digit ? c : 0;
+      }
+      sel_scan<PART_THREADS>(n, s_wave, &total);
+      if (tid == 0) {
+        uint32_t* larger = q.larger + r.row * q.parts + part;
+        *larger = PASS == 1 ? total : *larger + total;
+        if (part == 0) {
+          uint32_t* f = q.found + ((PASS - 1) * rows + r.row) * 2;
+          f[0] = digit;
+          f[1] = want;
+        }
+      }
+    }
+  }
+  const int base = first + wave * (PART_J * 64);
+  uint32_t k[PART_J];
+  float w[PART_J];
+  int pos[PART_J];
+  sel_load<PART_J>(w, pos, r, base, end);
+#pragma unroll
+  for (int j = 0; j < PART_J; ++j) k[j] = base + j * 64 + lane < end ? evict_key(w[j], pos[j], a.sinks, r.newest) : 0u;
+  if constexpr (PASS < 3) {
+    constexpr int LOW = sel_low(PASS), ABOVE = (LOW + sel_bits(PASS)) & 31;
+    for (int i = tid; i < SEL_BINS; i += PART_THREADS) s_bin[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PART_J; ++j)
+      sel_count(s_bin, base + j * 64 + lane < end && (PASS == 0 || (k[j] >> ABOVE) == (last >> ABOVE)), (k[j] >> LOW) & ((1u << sel_bits(PASS)) - 1));
+    __syncthreads();
+    uint32_t* mine = q.bins + ((PASS * rows + r.row) * q.parts + part) * SEL_BINS;
+    for (int i = tid; i < SEL_BINS; i += PART_THREADS) mine[i] = s_bin[i];
+  } else {
+    // parts in slot order: keys that stay for sure and ties of each, sixteen parts at a time; what lies in front of this one
+    const uint32_t digit = last & ((1u << sel_bits(2)) - 1);
+    const uint32_t* bins = q.bins + ((2 * rows + r.row) * q.parts) * SEL_BINS;
+    uint32_t ties = 0, ties_here = 0, holes = 0, movers = 0, all = 0;
+    for (int p0 = 0; p0 < q.parts; p0 += PART_WAVES) {
+      const int p = p0 + wave;
+      uint32_t n = 0, t = 0;
+      if (p < q.parts) {
+#pragma unroll
+        for (int u = 0; u < (1 << sel_bits(2)) / 64; ++u) {
+          const int i = u * 64 + lane;
+          const uint32_t c = bins[(int64_t)p * SEL_BINS + i];
+          n += i > (int)digit ? c : 0;
+          t += i == (int)digit ? c : 0;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) { n += __shfl_xor(n, o, 64); t += __shfl_xor(t, o, 64); }
+        n += q.larger[r.row * q.parts + p];
+      }
+      __syncthreads();
+      if (lane == 0) s_part[wave] = make_uint2(n, t);
+      __syncthreads();
+      for (int i = 0; i < PART_WAVES && p0 + i < q.parts; ++i) {
+        const uint2 x = s_part[i];
+        const uint32_t kept = x.x + (want > ties_here ? (want - ties_here < x.y ? want - ties_here : x.y) : 0);
+        int f, e;
+        part_slots(a, q, r, p0 + i, &f, &e);
+        if (p0 + i < part) {
+          ties += x.y;
+          if (p0 + i < q.below) holes += (uint32_t)(e - f) - kept;
+          else movers += kept;
+        }
+        if (p0 + i >= q.below) all += kept;
+        ties_here += x.y;
+      }
+    }
+    uint32_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < PART_J; ++j) mine += (uint32_t)__popcll(__ballot(base + j * 64 + lane < end && k[j] == last));
+    uint2 total;
+    ties += sel_waves<PART_WAVES>(make_uint2(mine, 0), s_two, &total).x;
+    const uint32_t stays = sel_lists<PART_J>(k, base, end, a.budget, last, want, ties, [&](uint2 x) {
+      const uint2 at = sel_waves<PART_WAVES>(x, s_two, &total);
+      return make_uint2(holes + at.x, movers + at.y);
+    }, [&](int slot, uint32_t rank, bool mover, int j) {
+      (mover ? r.src : r.dst)[rank] = slot;
+      if (mover) {
+        q.moved_w[r.row * a.moves + rank] = w[j];
+        q.moved_pos[r.row * a.moves + rank] = pos[j];
+      }
+    });
+    if (part < q.below) {
+#pragma unroll
+      for (int j = 0; j < PART_J; ++j)
+        if (stays >> j & 1) {
+          const int i = base + j * 64 + lane;
+          if (r.w_out != r.w) r.w_out[i] = w[j];
+          if (r.pos_out != r.pos) r.pos_out[i] = pos[j];
+        }
+    }
+    if (part == 0 && tid == 0) a.count[r.row] = (int32_t)all;
+  }
+}
+
+// A thread for some of a row's numbers: its move of that number, its slot of that number if it is free or the row is left as it is, its place in the
+// lists of moves if there is none.
+constexpr int FINISH_SHARE = 1024;
+__global__ void __launch_bounds__(256) evict_finish_kernel(const EvictSelect a, const EvictParts q, int shares) {
+  const int share = (int)(blockIdx.x % (unsigned)shares);
+  const EvictRow r(a, (int)(blockIdx.x / (unsigned)shares));
+  const bool cut = r.n > a.budget;
+  const int moved = cut ? a.count[r.row] : 0;
+  if (share == 0 && threadIdx.x == 0 && !cut) a.count[r.row] = 0;
+  constexpr int J = FINISH_SHARE / 256;
+  int i[J], to[J], pos[J];
+  float w[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    i[j] = share * FINISH_SHARE + j * 256 + (int)threadIdx.x;
+    const bool move = i[j] < moved, copy = !cut && i[j] < r.left;
+    to[j] = move ? r.dst[i[j]] : i[j];
+    w[j] = move ? q.moved_w[r.row * a.moves + i[j]] : (copy ? r.w[i[j]] : 0.0f);
+    pos[j] = move ? q.moved_pos[r.row * a.moves + i[j]] : (copy ? r.pos[i[j]] : 0);
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    if (i[j] < moved || (!cut && i[j] < r.left)) {
+      r.w_out[to[j]] = w[j];
+      r.pos_out[to[j]] = pos[j];
+    }
+    if (i[j] >= r.left && i[j] < a.L) {
+      r.w_out[i[j]] = 0.0f;
+      r.pos_out[i[j]] = r.seen + (i[j] - r.left);
+    }
+    if (i[j] >= moved && i[j] < a.moves) r.dst[i[j]] = r.src[i[j]] = -1;
+  }
+}
+
+// Slots of a row in one workgroup (32 rows of 32768: 53 us with one workgroup of 1024 threads each, 45 in parts)
+constexpr int ROW_SLOTS = 16384;
+
+struct EvictPlan { int below, parts, shares; size_t bins_at, larger_at, found_at, w_at, pos_at, bytes; };
+static EvictPlan evict_plan(int64_t rows, int L, int budget, int moves) {
+  EvictPlan p{};
+  if (L <= ROW_SLOTS) return p;
+  const int64_t front = std::min(L, budget);
+  p.below = (int)((front + PART - 1) / PART);
+  p.parts = p.below + (int)((L - front + PART - 1) / PART);
+  p.shares = (int)(((int64_t)L + FINISH_SHARE - 1) / FINISH_SHARE);
+  size_t at = 0;
+  const auto take = [&](size_t n) { const size_t here = at; at = (at + n + 255) & ~(size_t)255; return here; };
+  p.bins_at = take((size_t)3 * rows * p.parts * SEL_BINS * 4);
+  p.larger_at = take((size_t)rows * p.parts * 4);
+  p.found_at = take((size_t)3 * rows * 2 * 4);
+  p.w_at = take((size_t)rows * moves * 4);
+  p.pos_at = take((size_t)rows * moves * 4);
+  p.bytes = at;
+  return p;
 }
 
 // ---- the moves ----------------------------------------------------------------------------------------------------------------------------
@@ -286,19 +630,51 @@ static int move_list(MoveList* m, const int32_t* count, const int32_t* dst, cons
 
 }  // namespace tq
 
+extern "C" size_t tq_evict_select_bytes(int B, int H, int L, int budget, int moves) {
+  if (B <= 0 || H <= 0 || L <= 0 || budget <= 0 || moves <= 0) return 0;
+  return tq::evict_plan((int64_t)B * H, L, budget, moves).bytes;
+}
+
 extern "C" int tq_evict_select(const float* weights, int64_t w_b, int64_t w_h, const int32_t* positions, int64_t p_b, int64_t p_h, const int32_t* seq_lens,
                                const int32_t* seen, int B, int H, int L, int budget, int sinks, int recent, int moves, int32_t* lens_out, int32_t* count,
                                int32_t* dst, int32_t* src, float* weights_out, int64_t wo_b, int64_t wo_h, int32_t* positions_out, int64_t po_b,
-                               int64_t po_h, void* stream) {
+                               int64_t po_h, void* workspace, void* stream) {
   using namespace tq;
   if (!weights || !positions || !seq_lens || !lens_out || !count || !dst || !src || !weights_out || !positions_out) return TQ_ENULL;
   if (B < 0 || H <= 0 || L <= 0 || budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget) return TQ_EINVAL;
-  if (w_b < 0 || w_h < 0 || p_b < 0 || p_h < 0 || wo_b < 0 || wo_h < 0 || po_b < 0 || po_h < 0 || L > INT32_MAX - 2 * SEL_THREADS) return TQ_EINVAL;
+  if (w_b < 0 || w_h < 0 || p_b < 0 || p_h < 0 || wo_b < 0 || wo_h < 0 || po_b < 0 || po_h < 0 || L > (1 << 30)) return TQ_EINVAL;
   if (moves < std::max(1, std::min(budget, L - budget)) || (int64_t)B * H > INT32_MAX) return TQ_EINVAL;
   if (B == 0) return TQ_OK;
-  EvictSelect a{weights, w_b, w_h, positions, p_b, p_h, seq_lens, seen, B, H, L, budget, sinks, recent, moves, lens_out, count, dst, src,
-                weights_out, wo_b, wo_h, positions_out, po_b, po_h};
-  evict_select_kernel<<<dim3((unsigned)(B * H)), dim3(SEL_THREADS), 0, (hipStream_t)stream>>>(a);
+  const EvictSelect a{weights, w_b, w_h, positions, p_b, p_h, seq_lens, seen, B, H, L, budget, sinks, recent, moves, lens_out, count, dst, src,
+                      weights_out, wo_b, wo_h, positions_out, po_b, po_h};
+  hipStream_t st = (hipStream_t)stream;
+  const int64_t rows = (int64_t)B * H;
+  if (L <= ROW_SLOTS) {
+    const dim3 grid((unsigned)rows);
+    const auto each = [&](int threads) { return (L + threads - 1) / threads; };
+    if (L <= 1024) evict_row_kernel<256, 4><<<grid, dim3(256), 0, st>>>(a, each(256));
+    else if (L <= 4096) evict_row_kernel<512, 8><<<grid, dim3(512), 0, st>>>(a, each(512));
+    else evict_row_kernel<1024, 16><<<grid, dim3(1024), 0, st>>>(a, each(1024));
+    TQ_CHECK_LAUNCH();
+    return TQ_OK;
+  }
+  const EvictPlan p = evict_plan(rows, L, budget, moves);
+  if (!workspace) return TQ_ENULL;
+  if ((uintptr_t)workspace & 15) return TQ_EINVAL;
+  if (rows * p.parts > INT32_MAX || rows * p.shares > INT32_MAX) return TQ_EINVAL;
+  char* ws = (char*)workspace;
+  const EvictParts q{p.below, p.parts, (uint32_t*)(ws + p.bins_at), (uint32_t*)(ws + p.larger_at), (uint32_t*)(ws + p.found_at), (float*)(ws + p.w_at),
+                     (int32_t*)(ws + p.pos_at)};
+  const dim3 grid((unsigned)(rows * p.parts)), block(PART_THREADS);
+  evict_part_kernel<0><<<grid, block, 0, st>>>(a, q);
+  TQ_CHECK_LAUNCH();
+  evict_part_kernel<1><<<grid, block, 0, st>>>(a, q);
+  TQ_CHECK_LAUNCH();
+  evict_part_kernel<2><<<grid, block, 0, st>>>(a, q);
+  TQ_CHECK_LAUNCH();
+  evict_part_kernel<3><<<grid, block, 0, st>>>(a, q);
+  TQ_CHECK_LAUNCH();
+  evict_finish_kernel<<<dim3((unsigned)(rows * p.shares)), dim3(256), 0, st>>>(a, q, p.shares);
   TQ_CHECK_LAUNCH();
   return TQ_OK;
 }

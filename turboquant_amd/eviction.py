@@ -116,12 +116,14 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
     got = Evictions(whole(B), whole(B, H), whole(B, H, moves), whole(B, H, moves), new_w, new_p, budget)
     if B == 0:
         return got
+    need = _ffi.lib().tq_evict_select_bytes(B, H, L, budget, moves)
+    workspace = torch.empty(need // 4, dtype=torch.float32, device=dev) if need else None
     with _ffi.on_device(dev):
         _ffi.check(_ffi.lib().tq_evict_select(
             weights.data_ptr(), weights.stride(0), weights.stride(1), positions.data_ptr(), positions.stride(0), positions.stride(1),
             lens.data_ptr(), _ffi.ptr(had), B, H, L, budget, sinks, recent, moves, got.lens.data_ptr(), got.count.data_ptr(),
             got.dst.data_ptr(), got.src.data_ptr(), new_w.data_ptr(), new_w.stride(0), new_w.stride(1), new_p.data_ptr(), new_p.stride(0),
-            new_p.stride(1), _ffi.stream_ptr(dev)), "tq_evict_select")
+            new_p.stride(1), _ffi.ptr(workspace), _ffi.stream_ptr(dev)), "tq_evict_select")
     if out is not None:
         _ffi.changed(new_w, new_p)
     return got
