@@ -23,7 +23,9 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <array>
+#include <cmath>
 #include <optional>
 #include <vector>
 
@@ -54,11 +56,20 @@ struct Library {
   decltype(&tq_cache_scores_rows) cache_scores_rows;
   decltype(&tq_cache_attend_bytes) cache_attend_bytes;
   decltype(&tq_cache_attend) cache_attend;
+  decltype(&tq_exact_decode_bytes) exact_decode_bytes;
+  decltype(&tq_exact_decode) exact_decode;
+  decltype(&tq_exact_window_bytes) exact_window_bytes;
+  decltype(&tq_exact_window) exact_window;
+  decltype(&tq_evict_select_bytes) evict_select_bytes;
+  decltype(&tq_evict_select) evict_select;
+  decltype(&tq_move_tokens_exact) move_tokens_exact;
 } g_lib{};
 constexpr const char* kNames[] = {"tq_quantize_keys", "tq_dequant_keys", "tq_score", "tq_ring_write", "tq_append_kv_paged",
                                   "tq_append_kv_newest", "tq_decode_workspace_bytes", "tq_decode_attn_paged", "tq_decode_attn_paged_by_length",
                                   "tq_decode_attn_paged_ring", "tq_decode_attn_paged_ring_by_length", "tq_cache_append_bytes",
-                                  "tq_cache_append", "tq_cache_scores_rows", "tq_cache_attend_bytes", "tq_cache_attend"};
+                                  "tq_cache_append", "tq_cache_scores_rows", "tq_cache_attend_bytes", "tq_cache_attend",
+                                  "tq_exact_decode_bytes", "tq_exact_decode", "tq_exact_window_bytes", "tq_exact_window",
+                                  "tq_evict_select_bytes", "tq_evict_select", "tq_move_tokens_exact"};
 static_assert(sizeof(Library) == sizeof(kNames) / sizeof(kNames[0]) * sizeof(void*), "a pointer per name, in order");
 bool g_bound = false;
 
@@ -507,6 +518,176 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   });
 }
 
+// ---- the engine's paged exact cache ---------------------------------------------------------------------------------------------
+
+// Key and value blocks (blocks, 16, H, d) as ExactPagedCache takes them
+struct Blocks {
+  at::Tensor k, v;
+  int64_t n = 0, H = 0, d = 0;
+  int tag = -1;
+  bool take(Plain& p, PyObject* key, PyObject* value) {
+    k = p.take(key); v = p.take(value);
+    if (!p.ok || k.dim() != 4 || k.sizes() != v.sizes() || k.strides() != v.strides() || k.scalar_type() != v.scalar_type() || k.size(1) != TQ_PAGE_TOKENS ||
+        k.stride(3) != 1)
+      return false;
+    tag = dtype_tag(k.scalar_type());
+    n = k.size(0); H = k.size(2); d = k.size(3);
+    if (tag < 0 || n == 0 || H == 0 || H > INT_MAX || d <= 0 || d % 64 || d > 768) return false;
+    const int64_t piece = 16 / (int64_t)k.element_size();
+    return k.stride(0) % piece == 0 && k.stride(1) % piece == 0 && k.stride(2) % piece == 0 && k.stride(1) <= 1 << 24 &&
+           (((uintptr_t)k.data_ptr() | (uintptr_t)v.data_ptr()) & 15) == 0;
+  }
+};
+// Block table and lengths of B sequences
+struct Sequences {
+  at::Tensor table, lens;
+  int64_t B = 0, stride = 0, row = 0;
+  bool take(Plain& p, PyObject* bt, PyObject* seq, int64_t batch, bool shared) {
+    table = p.take(bt); lens = p.take(seq);
+    B = batch;
+    if (!p.ok || !dense_as(table, at::kInt) || !dense_as(lens, at::kInt) || lens.dim() != 1 || lens.size(0) != B) return false;
+    if (table.dim() == 2 ? table.size(0) != B : !shared || table.dim() != 1) return false;
+    row = table.size(-1);
+    stride = table.dim() == 1 ? -row : row;
+    return row > 0 && row <= INT_MAX;
+  }
+  const int32_t* entries() const { return (const int32_t*)table.data_ptr(); }
+  const int32_t* lengths() const { return (const int32_t*)lens.data_ptr(); }
+};
+// (B, H, L), slots contiguous, no two elements in one place
+bool slots_of(const at::Tensor& t, at::ScalarType dt, int64_t B, int64_t H) {
+  if (t.scalar_type() != dt || t.dim() != 3 || t.size(0) != B || t.size(1) != H || t.size(2) <= 0 || t.size(2) > INT_MAX || t.stride(2) != 1) return false;
+  const int64_t L = t.size(2), b = t.stride(0), h = t.stride(1);
+  if (B > 1 && H > 1) return b >= h ? h >= L && b >= h * (H - 1) + L : b >= L && h >= b * (B - 1) + L;
+  return B > 1 ? b >= L : H <= 1 || h >= L;
+}
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+// a number, or None (`none`)
+double real_arg(PyObject* o, double none) { return o == Py_None ? none : PyFloat_AsDouble(o); }
+int64_t int_or(PyObject* o, int64_t none) { return o == Py_None ? none : PyLong_AsLongLong(o); }
+
+// exact_cache(key blocks, value blocks) -> (tag, blocks, H, d, three strides)
+PyObject* exact_cache(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return entry<2>(args, n_args, [](PyObject* const* a) -> PyObject* {
+    Plain p;
+    Blocks c;
+    if (!c.take(p, a[0], a[1])) return nullptr;
+    return Py_BuildValue("iLLL(LLL)", c.tag, (long long)c.n, (long long)c.H, (long long)c.d, (long long)c.k.stride(0), (long long)c.k.stride(1),
+                         (long long)c.k.stride(2));
+  });
+}
+
+// exact_decode(query (B, Hq, d), block table, lengths, key blocks, value blocks, scale or None, longest or None, weights or None) -> attention
+PyObject* exact_decode(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return entry<8>(args, n_args, [](PyObject* const* a) -> PyObject* {
+    Plain p;
+    Blocks c;
+    Sequences s;
+    if (!c.take(p, a[3], a[4])) return nullptr;
+    const at::Tensor q = p.take(a[0]);
+    if (!p.ok || q.dim() != 3 || q.size(2) != c.d || q.scalar_type() != c.k.scalar_type() || !q.is_contiguous() || ((uintptr_t)q.data_ptr() & 15)) return nullptr;
+    const int64_t B = q.size(0), Hq = q.size(1);
+    if (B == 0 || B > INT_MAX || Hq == 0 || Hq > INT_MAX || Hq % c.H || !s.take(p, a[1], a[2], B, true)) return nullptr;
+    const double scale = real_arg(a[5], 1.0 / std::sqrt((double)c.d));
+    const int64_t longest = int_or(a[6], s.row * TQ_PAGE_TOKENS);
+    at::Tensor w;
+    int64_t w_len = 0;
+    if (a[7] != Py_None) {
+      w = p.take(a[7]);
+      if (!p.ok || !slots_of(w, at::kFloat, B, c.H)) return nullptr;
+      w_len = std::min(w.size(2), s.row * TQ_PAGE_TOKENS);
+    }
+    if (PyErr_Occurred() || longest < 0) return nullptr;
+    const size_t need = g_lib.exact_decode_bytes(c.tag, (int)B, (int)Hq, (int)c.H, (int)c.d, longest, 0, w_len);
+    if (need == 0) return nullptr;
+    const at::Tensor ws = p.fresh({(int64_t)(need / 4)}, at::kFloat), out = p.fresh(q.sizes(), q.scalar_type());
+    if (unlocked(g_lib.exact_decode, q.data_ptr(), c.tag, (int)B, (int)Hq, (int)c.H, (int)c.d, c.k.data_ptr(), c.v.data_ptr(), c.k.stride(0), c.k.stride(1),
+                 c.k.stride(2), c.n, s.entries(), (int)s.stride, s.lengths(), (float)scale, longest, w_len ? (float*)w.data_ptr() : nullptr,
+                 w_len ? w.stride(0) : 0, w_len ? w.stride(1) : 0, w_len, out.data_ptr(), ws.data_ptr(), 0, p.stream()) != TQ_OK)
+      return nullptr;
+    if (w_len) written(w);
+    return THPVariable_Wrap(out);
+  });
+}
+
+// exact_window(query (rows, Hq, d), starts, block table, lengths, key blocks, value blocks, weights, window, scale or None, longest or None) -> True
+PyObject* exact_window(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return entry<10>(args, n_args, [](PyObject* const* a) -> PyObject* {
+    Plain p;
+    Blocks c;
+    Sequences s;
+    if (!c.take(p, a[4], a[5])) return nullptr;
+    const at::Tensor q = p.take(a[0]), starts = p.take(a[1]), w = p.take(a[6]);
+    if (!p.ok || q.dim() != 3 || q.size(2) != c.d || q.scalar_type() != c.k.scalar_type() || !q.is_contiguous() || ((uintptr_t)q.data_ptr() & 15)) return nullptr;
+    if (!dense_as(starts, at::kInt) || starts.dim() != 1 || starts.size(0) < 2 || starts.size(0) > INT_MAX) return nullptr;
+    const int64_t rows = q.size(0), Hq = q.size(1), B = starts.size(0) - 1, window = int_arg(a[7]);
+    if (rows == 0 || Hq == 0 || Hq > INT_MAX || Hq % c.H || !s.take(p, a[2], a[3], B, true) || !slots_of(w, at::kFloat, B, c.H)) return nullptr;
+    const double scale = real_arg(a[8], 1.0 / std::sqrt((double)c.d));
+    const int64_t longest = int_or(a[9], s.row * TQ_PAGE_TOKENS);
+    if (PyErr_Occurred() || longest < 0 || window < 1 || window > 1024) return nullptr;
+    const size_t need = g_lib.exact_window_bytes(c.tag, (int)B, (int)Hq, (int)c.H, (int)c.d, (int)window, longest);
+    if (need == 0) return nullptr;
+    const at::Tensor ws = p.fresh({(int64_t)(need / 4)}, at::kFloat);
+    if (unlocked(g_lib.exact_window, q.data_ptr(), c.tag, rows, (const int32_t*)starts.data_ptr(), (int)B, (int)Hq, (int)c.H, (int)c.d, (int)window,
+                 c.k.data_ptr(), c.k.stride(0), c.k.stride(1), c.k.stride(2), c.n, s.entries(), (int)s.stride, s.lengths(), (float)scale, longest,
+                 (float*)w.data_ptr(), w.stride(0), w.stride(1), w.size(2), ws.data_ptr(), p.stream()) != TQ_OK)
+      return nullptr;
+    written(w);
+    Py_RETURN_TRUE;
+  });
+}
+
+// evict_select(weights, positions (B, H, L), lengths, seen or None, budget, sinks, recent) -> (lengths, count, dst, src, weights, positions)
+PyObject* evict_select(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return entry<7>(args, n_args, [](PyObject* const* a) -> PyObject* {
+    Plain p;
+    const at::Tensor w = p.take(a[0]), pos = p.take(a[1]), lens = p.take(a[2]);
+    const at::Tensor seen = a[3] == Py_None ? lens : p.take(a[3]);
+    const int64_t budget = int_arg(a[4]), sinks = int_arg(a[5]), recent = int_arg(a[6]);
+    if (!p.ok || PyErr_Occurred() || w.dim() != 3 || w.numel() == 0 || w.sizes() != pos.sizes() || w.scalar_type() != at::kFloat || pos.scalar_type() != at::kInt ||
+        w.stride(2) != 1 || pos.stride(2) != 1)
+      return nullptr;
+    const int64_t B = w.size(0), H = w.size(1), L = w.size(2);
+    if (!dense_as(lens, at::kInt) || lens.dim() != 1 || lens.size(0) != B || !dense_as(seen, at::kInt) || seen.dim() != 1 || seen.size(0) != B) return nullptr;
+    if (B > INT_MAX || H > INT_MAX || L > INT_MAX || budget < 1 || budget > INT_MAX || sinks < 0 || recent < 0 || sinks > budget || recent > budget - sinks) return nullptr;
+    const int64_t moves = std::max<int64_t>(1, std::min(budget, L - budget));
+    const at::Tensor out = p.fresh({B}, at::kInt), count = p.fresh({B, H}, at::kInt), dst = p.fresh({B, H, moves}, at::kInt), src = p.fresh({B, H, moves}, at::kInt),
+                     new_w = p.fresh({B, H, L}, at::kFloat), new_p = p.fresh({B, H, L}, at::kInt);
+    const size_t need = g_lib.evict_select_bytes((int)B, (int)H, (int)L, (int)budget, (int)moves);
+    at::Tensor ws;
+    if (need) ws = p.fresh({(int64_t)(need / 4)}, at::kFloat);
+    if (unlocked(g_lib.evict_select, (const float*)w.data_ptr(), w.stride(0), w.stride(1), (const int32_t*)pos.data_ptr(), pos.stride(0), pos.stride(1),
+                 (const int32_t*)lens.data_ptr(), (const int32_t*)seen.data_ptr(), (int)B, (int)H, (int)L, (int)budget, (int)sinks, (int)recent, (int)moves,
+                 (int32_t*)out.data_ptr(), (int32_t*)count.data_ptr(), (int32_t*)dst.data_ptr(), (int32_t*)src.data_ptr(), (float*)new_w.data_ptr(), H * L, L,
+                 (int32_t*)new_p.data_ptr(), H * L, L, need ? ws.data_ptr() : nullptr, p.stream()) != TQ_OK)
+      return nullptr;
+    return tuple({out, count, dst, src, new_w, new_p});
+  });
+}
+
+// move_exact(key blocks, value blocks, block table, count, dst, src) -> True
+PyObject* move_exact(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return entry<6>(args, n_args, [](PyObject* const* a) -> PyObject* {
+    Plain p;
+    Blocks c;
+    if (!c.take(p, a[0], a[1])) return nullptr;
+    const at::Tensor table = p.take(a[2]), count = p.take(a[3]), dst = p.take(a[4]), src = p.take(a[5]);
+    if (!p.ok || !dense_as(dst, at::kInt) || !dense_as(src, at::kInt) || !dense_as(count, at::kInt) || !dense_as(table, at::kInt)) return nullptr;
+    if (dst.dim() != 3 || dst.size(1) != c.H || src.sizes() != dst.sizes() || count.dim() != 2 || count.size(0) != dst.size(0) || count.size(1) != c.H) return nullptr;
+    const int64_t B = dst.size(0), moves = dst.size(2);
+    if (B == 0 || B > INT_MAX || moves > INT_MAX || table.dim() != 2 || table.size(0) != B || table.size(1) == 0 || table.size(1) > INT_MAX) return nullptr;
+    if (unlocked(g_lib.move_tokens_exact, c.k.data_ptr(), c.v.data_ptr(), c.tag, (int)c.d, c.k.stride(0), c.k.stride(1), c.k.stride(2), c.n,
+                 (const int32_t*)table.data_ptr(), (int)table.size(1), (const int32_t*)count.data_ptr(), (const int32_t*)dst.data_ptr(),
+                 (const int32_t*)src.data_ptr(), (int)B, (int)c.H, (int)moves, p.stream()) != TQ_OK)
+      return nullptr;
+    written(c.k);
+    written(c.v);
+    Py_RETURN_TRUE;
+  });
+}
+
 // bind({name: address}): the library's functions
 PyObject* bind(PyObject*, PyObject* arg) {
   if (!PyDict_Check(arg)) { PyErr_SetString(PyExc_TypeError, "bind takes a dict of addresses"); return nullptr; }
@@ -528,6 +709,8 @@ PyMethodDef kMethods[] = {
     TQ_FAST(ring_write, "rows into the ring"), TQ_FAST(append, "tokens into pages"), TQ_FAST(decode, "a decode step"),
     TQ_FAST(decode_ring, "a decode step, exact tokens in place"), TQ_FAST(cache_append, "a token into the cache object"),
     TQ_FAST(cache_scores, "scores of the cache object"), TQ_FAST(cache_attend, "weighted values of the cache object"),
+    TQ_FAST(exact_cache, "an exact cache's blocks"), TQ_FAST(exact_decode, "a decode step over an exact cache"),
+    TQ_FAST(exact_window, "a window's weights"), TQ_FAST(evict_select, "who stays"), TQ_FAST(move_exact, "moves in an exact cache"),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tq_host", "host side of small calls", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -36,11 +36,11 @@ class Evictions(NamedTuple):
         _ffi.require_gpu(block_table, "block_table")
         if block_table.device != device or self.dst.device != device:
             raise ValueError(f"the cache lives on {device}, the evictions on {self.dst.device}, block_table on {block_table.device}")
-        table = block_table.contiguous()
+        table = block_table.contiguous().resolve_neg()
         return self.count, self.dst, self.src, table, table.shape[1]
 
 
-def _own_rows(t: torch.Tensor) -> bool:
+def own_rows(t: torch.Tensor) -> bool:
     """Whether no two elements of t (B, H, L), slots contiguous, lie in one place."""
     reach = t.shape[2]
     for stride, size in sorted((t.stride(i), t.shape[i]) for i in (0, 1) if t.shape[i] > 1):
@@ -69,6 +69,11 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
     Tokens that stay and lie within the first `budget` slots do not move, those behind fill the holes in ascending order, so the slots are not
     in order of position afterwards (attention does not ask).  The inputs are left as they are; out=(weights, positions)
     takes the new ones instead of new tensors, the inputs themselves included."""
+    fast = _ffi.native()
+    if fast is not None and out is None:
+        done = fast.evict_select(weights, positions, seq_lens, seen, budget, sinks, recent)
+        if done is not None:
+            return Evictions(*done, budget)
     _ffi.require_gpu(weights, "weights")
     _ffi.require_gpu(positions, "positions")
     if weights.dim() != 3 or weights.shape != positions.shape or 0 in weights.shape[1:]:
@@ -85,13 +90,13 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
     for name, t in (("seq_lens", seq_lens), ("seen", seen)):
         if t is not None and t.shape != (B,):
             raise ValueError(f"{name} must have one entry for each of {B} sequences")
-    weights = weights.detach()
+    weights, positions = weights.detach().resolve_neg(), positions.resolve_neg()
     if weights.stride(2) != 1 and L > 1:
         weights = weights.contiguous()
     if positions.stride(2) != 1 and L > 1:
         positions = positions.contiguous()
-    lens = seq_lens.to(device=dev, dtype=torch.int32).contiguous()
-    had = None if seen is None else seen.to(device=dev, dtype=torch.int32).contiguous()
+    lens = seq_lens.to(device=dev, dtype=torch.int32).contiguous().resolve_neg()
+    had = None if seen is None else seen.to(device=dev, dtype=torch.int32).contiguous().resolve_neg()
     if out is None:
         new_w, new_p = (torch.empty(B, H, L, dtype=t.dtype, device=dev) for t in (weights, positions))
     else:
@@ -99,9 +104,11 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
         for new, old, name in ((new_w, weights, "weights"), (new_p, positions, "positions")):
             if new.shape != old.shape or new.dtype != old.dtype or new.device != dev or (new.stride(2) != 1 and L > 1):
                 raise ValueError(f"out must hold {name} (B, H, L) like the input's, slots contiguous")
+            if new.is_neg():
+                raise ValueError(f"out {name} is negated lazily: its memory does not hold its values")
             if torch.is_grad_enabled() and new.requires_grad:
                 raise RuntimeError(f"out {name} requires a gradient")
-            if not _own_rows(new):
+            if not own_rows(new):
                 raise ValueError(f"out {name} must not overlap itself")
             same = new.data_ptr() == old.data_ptr() and new.stride() == old.stride()
             for other in (weights, positions):

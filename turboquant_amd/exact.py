@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _ffi
-from .eviction import Evictions
+from .eviction import Evictions, own_rows
 from .paged import PAGE_TOKENS
 
 MAX_HEAD_DIM = 768
@@ -32,6 +32,13 @@ class ExactPagedCache:
     boundaries; the object holds the two tensors and nothing else."""
 
     def __init__(self, key_cache: torch.Tensor, value_cache: torch.Tensor):
+        self.key_cache, self.value_cache = key_cache, value_cache
+        fast = _ffi.native()
+        known = None if fast is None else fast.exact_cache(key_cache, value_cache)
+        if known is not None:
+            self._tag, self.num_blocks, self.num_kv_heads, self.head_dim, self._strides = known
+            self.dtype, self.device = key_cache.dtype, key_cache.device
+            return
         _ffi.require_gpu(key_cache, "key_cache")
         _ffi.require_gpu(value_cache, "value_cache")
         if key_cache.dim() != 4 or key_cache.shape != value_cache.shape or key_cache.shape[1] != PAGE_TOKENS:
@@ -43,12 +50,13 @@ class ExactPagedCache:
         self.num_blocks, _, self.num_kv_heads, self.head_dim = key_cache.shape
         if self.head_dim % 64 or not 0 < self.head_dim <= MAX_HEAD_DIM or self.num_kv_heads == 0 or self.num_blocks == 0:
             raise ValueError(f"head_dim must be a multiple of 64 up to {MAX_HEAD_DIM}, got a cache of shape {tuple(key_cache.shape)}")
+        if any(t.is_neg() or t._is_zerotensor() for t in (key_cache, value_cache)):
+            raise ValueError("key_cache and value_cache must hold their values: a lazily negated tensor does not")
         self._strides = key_cache.stride()
         piece = 16 // key_cache.element_size()
         if (value_cache.stride() != self._strides or self._strides[3] != 1 or any(s % piece for s in self._strides[:3]) or
                 self._strides[1] > 1 << 24 or key_cache.data_ptr() % 16 or value_cache.data_ptr() % 16):
             raise ValueError("key_cache and value_cache need the same strides, contiguous channels and rows on 16-byte boundaries")
-        self.key_cache, self.value_cache = key_cache, value_cache
 
     @classmethod
     def from_engine(cls, kv_cache: torch.Tensor) -> "ExactPagedCache":
@@ -69,8 +77,8 @@ class ExactPagedCache:
         _ffi.require_gpu(block_table, "block_table")
         if block_table.device != self.device:
             raise ValueError(f"block_table lives on {block_table.device}, the cache on {self.device}")
-        table = block_table.contiguous()
-        lens = seq_lens.to(device=self.device, dtype=torch.int32).contiguous()
+        table = block_table.contiguous().resolve_neg()
+        lens = seq_lens.to(device=self.device, dtype=torch.int32).contiguous().resolve_neg()
         return table, (-table.shape[0] if table.dim() == 1 else table.shape[1]), lens
 
     def _weights(self, weights: torch.Tensor, batch: int) -> None:
@@ -79,14 +87,10 @@ class ExactPagedCache:
             raise TypeError("weights must be float32 on the cache's GPU")
         if weights.dim() != 3 or tuple(weights.shape[:2]) != (batch, self.num_kv_heads) or weights.shape[2] == 0:
             raise ValueError(f"weights must be ({batch}, {self.num_kv_heads}, tokens)")
-        if weights.stride(2) != 1:
-            raise ValueError("weights need contiguous tokens")
-        sizes = sorted((weights.stride(i), weights.shape[i]) for i in (0, 1) if weights.shape[i] > 1)
-        reach = weights.shape[2]
-        for stride, size in sizes:
-            if stride < reach:
-                raise ValueError("weights must not overlap themselves")
-            reach = stride * (size - 1) + reach
+        if weights.stride(2) != 1 or weights.is_neg():
+            raise ValueError("weights need contiguous tokens, and memory that holds their values")
+        if not own_rows(weights):
+            raise ValueError("weights must not overlap themselves")
         _require_plain(weights, "weights")
 
     # ---- read ----------------------------------------------------------------------------------------------------------
@@ -101,6 +105,11 @@ class ExactPagedCache:
         head, is added in place (tokens from L on have no place in it).  max_len bounds the lengths for the plan of the
         splits: without it the width of the table does.  The `workspace` of a step (`workspace()`) belongs to it alone until
         it has run: graphs that may run at the same time need one each."""
+        fast = _ffi.native()
+        if fast is not None and n_split is None and workspace is None and out is None:
+            done = fast.exact_decode(query, block_table, seq_lens, self.key_cache, self.value_cache, scale, max_len, weights)
+            if done is not None:
+                return done
         _ffi.require_gpu(query, "query")
         if query.dim() != 3:
             raise ValueError("query must be (B, Hq, d)")
@@ -113,7 +122,7 @@ class ExactPagedCache:
         table, bt_stride, lens = self._sequences(block_table, seq_lens, B)
         if scale is None:
             scale = 1.0 / math.sqrt(d)
-        query = query.contiguous()
+        query = query.contiguous().resolve_neg()
         if query.data_ptr() % 16:
             query = query.clone()
         if out is None:
@@ -165,6 +174,10 @@ class ExactPagedCache:
         before the first token is decoded.  query (rows, Hq, d) holds the rows of an engine's step, sequence b's from
         query_start_loc[b] to query_start_loc[b + 1], the last of them at position seq_lens[b] - 1; a query sees the tokens up
         to its own.  A sequence with fewer rows gives those, one without rows nothing."""
+        fast = _ffi.native()
+        if fast is not None and fast.exact_window(query, query_start_loc, block_table, seq_lens, self.key_cache, self.value_cache, weights,
+                                                  window, scale, max_len):
+            return weights
         _ffi.require_gpu(query, "query")
         if query.dim() != 3:
             raise ValueError("query must be (rows, Hq, d)")
@@ -187,10 +200,10 @@ class ExactPagedCache:
             max_len = table.shape[-1] * PAGE_TOKENS
         if B == 0 or rows == 0:
             return weights
-        query = query.contiguous()
+        query = query.contiguous().resolve_neg()
         if query.data_ptr() % 16:
             query = query.clone()
-        starts = query_start_loc.to(device=self.device, dtype=torch.int32).contiguous()
+        starts = query_start_loc.to(device=self.device, dtype=torch.int32).contiguous().resolve_neg()
         need = _ffi.lib().tq_exact_window_bytes(self._tag, B, Hq, self.num_kv_heads, d, int(window), int(max_len)) if max_len >= 0 else 0
         if need == 0:
             raise ValueError(f"no plan for {B} sequences of {Hq} query heads, window {window}, max_len {max_len}")
@@ -208,6 +221,9 @@ class ExactPagedCache:
     def move_tokens(self, evictions: Evictions, block_table: torch.Tensor) -> None:
         """Carry out the moves of `select_evictions` in these blocks, in place.  The sequences' blocks must be their own: a
         block that two sequences share would change for both."""
+        fast = _ffi.native()
+        if fast is not None and fast.move_exact(self.key_cache, self.value_cache, block_table, evictions.count, evictions.dst, evictions.src):
+            return
         count, dst, src, table, bt_stride = evictions.for_cache(block_table, self.num_kv_heads, self.device)
         B, H, moves = dst.shape
         if B == 0:
