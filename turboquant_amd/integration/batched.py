@@ -27,6 +27,11 @@ prefill steps).  Modes are those of `integration.vllm`:
   full_tq       decode steps are answered from the pool alone; prefill by the
                 backend, or by dense causal attention over the step's own K/V
                 when the engine's cache was never allocated (`no_alloc`)
+
+The first `exact_layers` layers may stay uncompressed: their decode steps are answered from the engine's paged cache, all of it exactly
+(`ExactPagedCache`).  And a cache may be cut: `track_weights` has every layer sum the attention weight that its tokens get - the newest
+`window` queries of every prompt step, and in exact layers every decode step -, and `evict_batched` keeps the sinks, the newest and the heaviest
+of a sequence's tokens, in the engine's blocks and in the pages alike.  The engine goes on with the lengths that it returns.
 """
 
 from __future__ import annotations
@@ -40,6 +45,8 @@ import torch
 import torch.nn.functional as F
 
 from .. import _ffi
+from ..eviction import select_evictions
+from ..exact import ExactPagedCache
 from ..paged import APPEND, PAGE_TOKENS, PagedKVPool
 from ..quantizer import TurboQuantProd
 from . import vllm as _single
@@ -57,22 +64,29 @@ def _host_list(meta, name):
 
 @dataclass
 class BatchedLayerState:
-    """One attention layer: its quantiser and the compressed pool that shadows the engine's blocks."""
+    """One attention layer: its quantiser and the compressed pool that shadows the engine's blocks (None: the layer stays exact)."""
     config: LayerConfig
-    quantizer: TurboQuantProd
-    pool: PagedKVPool
+    quantizer: Optional[TurboQuantProd]
+    pool: Optional[PagedKVPool]
     tokens_written: int = 0
     decode_steps: int = 0
+    weights: Optional[torch.Tensor] = None                     # (B, H_kv, tokens): what every slot's token has been given so far
+    positions: Optional[torch.Tensor] = None                   # (B, H_kv, tokens): where in the sequence it stood
+    window: int = 0
 
     @property
     def supports_hybrid(self) -> bool:
-        return True
+        """Whether the engine's cache may be freed (an exact layer has nothing else)."""
+        return self.pool is not None
 
     # ---- write -------------------------------------------------------------------
     def write(self, key: torch.Tensor, value: torch.Tensor, meta) -> None:
         """Quantise this step's tokens (n, H_kv, d) into the pages their sequences own."""
         cfg = self.config
         n = int(meta.num_actual_tokens)
+        if self.pool is None:                                  # the engine's own cache has them
+            self.tokens_written += n
+            return
         k = key[:n].reshape(n, cfg.num_kv_heads, cfg.head_dim)
         v = value[:n].reshape(n, cfg.num_kv_heads, cfg.head_dim)
         table = meta.block_table
@@ -93,6 +107,8 @@ class BatchedLayerState:
         sequences of `block_table`: tokens [0, seq_lens[b]) of every sequence, read in place through the
         block table and written to the pages of the same numbers (the batch counterpart of
         capture.py:187-217, without the gather copy)."""
+        if self.pool is None:
+            raise RuntimeError("an exact layer has no pages to write to")
         self.pool.append_from_blocks(kv_cache[0], kv_cache[1], block_table, block_table, seq_lens,
                                      max_tokens=max_tokens)
         self.tokens_written += int(seq_lens.sum())
@@ -123,6 +139,9 @@ class BatchedLayerState:
         """One query token per sequence, (B, H_q, d) -> (B, H_q, d)."""
         self.decode_steps += 1
         cfg = self.config
+        if self.pool is None:
+            return ExactPagedCache.from_engine(kv_cache).decode_attention(query, meta.block_table, meta.seq_lens, scale=scale, weights=self.weights,
+                                                                          max_len=getattr(meta, "max_seq_len", None))
         if (hybrid and cfg.ring_capacity > 0 and torch.is_tensor(kv_cache) and kv_cache.dim() == 5 and
                 kv_cache.shape[0] == 2 and tuple(kv_cache.shape[2:]) == (PAGE_TOKENS, cfg.num_kv_heads, cfg.head_dim) and
                 kv_cache.dtype == query.dtype and cfg.ring_capacity <= 1024 and
@@ -139,8 +158,35 @@ class BatchedLayerState:
         return self.pool.decode_attention(query, meta.block_table, hist, scale=scale, recent_k=rk, recent_v=rv,
                                           recent_len=rlen, max_len=getattr(meta, "max_seq_len", None))
 
+    # ---- eviction ------------------------------------------------------------------
+    def track(self, batch: int, max_len: int, window: int) -> None:
+        """Sum weights from now on, for `batch` sequences (rows of the step's block table) of up to max_len tokens."""
+        shape = (batch, self.config.num_kv_heads, max_len)
+        self.weights = torch.zeros(shape, dtype=torch.float32, device=self.config.device)
+        self.positions = torch.arange(max_len, dtype=torch.int32, device=self.config.device).expand(shape).contiguous()
+        self.window = window
+
+    def observe(self, query: torch.Tensor, meta, kv_cache: torch.Tensor, scale: Optional[float] = None) -> None:
+        """Add the weights that the newest queries of every sequence in this step give; query (rows, H_q, d)."""
+        ExactPagedCache.from_engine(kv_cache).add_window_weights(query, meta.query_start_loc, meta.block_table, meta.seq_lens, self.weights,
+                                                                 window=self.window, scale=scale, max_len=getattr(meta, "max_seq_len", None))
+
+    def evict(self, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int, seen: Optional[torch.Tensor] = None, sinks: int = 4,
+              recent: int = 0, kv_cache: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Cut every sequence to `budget` tokens (`select_evictions`), in the engine's cache (2, num_blocks, 16, H_kv, d), if there is one, and in
+        this layer's pages; returns the lengths that are left."""
+        if self.weights is None:
+            raise RuntimeError("nothing has been tracked: track_weights comes first")
+        e = select_evictions(self.weights, self.positions, seq_lens, budget, seen=seen, sinks=sinks, recent=recent,
+                             out=(self.weights, self.positions))
+        if kv_cache is not None:
+            ExactPagedCache.from_engine(kv_cache).move_tokens(e, block_table)
+        if self.pool is not None:
+            self.pool.move_tokens(e, block_table)
+        return e.lens
+
     def memory_bytes(self) -> int:
-        return self.pool.data.numel()
+        return 0 if self.pool is None else self.pool.data.numel()
 
 
 class _BatchedLayerHooks:
@@ -194,6 +240,9 @@ class _BatchedLayerHooks:
             return passthrough()
         self.state.write(key, value, attn_metadata)
         n = int(attn_metadata.num_actual_tokens)
+        if self.state.weights is not None and int(attn_metadata.max_query_len) > 1:
+            cfg = self.state.config
+            self.state.observe(query[:n].reshape(n, cfg.num_query_heads, cfg.head_dim), attn_metadata, kv_cache, getattr(impl, "scale", None))
         if mode == MODE_CAPTURE_ONLY:
             return passthrough()
         if int(attn_metadata.max_query_len) > 1:               # prefill (or a mixed step): exact attention
@@ -210,10 +259,14 @@ class _BatchedLayerHooks:
 def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, value_bits: int = 2,
                           value_group_size: int = 32, ring_capacity: int = 128, initial_layers_count: int = 4,
                           initial_layers_key_bits: Optional[int] = None, mode: str = MODE_CAPTURE_ONLY,
-                          no_alloc: bool = False, dtype: torch.dtype = torch.bfloat16) -> Dict[str, BatchedLayerState]:
+                          no_alloc: bool = False, dtype: torch.dtype = torch.bfloat16,
+                          exact_layers: int = 0) -> Dict[str, BatchedLayerState]:
     """Hook every standard attention layer of `model_runner` with a compressed pool of `num_blocks`
     16-token pages (the engine's block count); returns {layer name: BatchedLayerState}.  Bit widths are
-    assigned as by `install_hooks` (integration/vllm.py:333-359).  Latent-attention layers are left alone."""
+    assigned as by `install_hooks` (integration/vllm.py:333-359).  The first `exact_layers` of them get no pool: their
+    decode steps are answered from the engine's cache.  Latent-attention layers are left alone."""
+    if exact_layers and no_alloc:
+        raise ValueError("exact layers are answered from the engine's cache, which no_alloc leaves out")
     _single.set_mode(mode)
     if initial_layers_key_bits is None:
         initial_layers_key_bits = min(key_bits + 1, 4)
@@ -232,9 +285,11 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
                           key_bits=initial_layers_key_bits if idx < initial_layers_count else key_bits,
                           value_bits=value_bits, value_group_size=min(value_group_size, head_dim),
                           ring_capacity=ring_capacity, layer_idx=idx, backend_kind="flash", device=device)
-        tq = TurboQuantProd(head_dim, bits=cfg.key_bits, device=device, seed=42 + 7 * idx)
-        pool = PagedKVPool(tq, cfg.num_kv_heads, num_blocks, value_bits=value_bits,
-                           value_group_size=cfg.value_group_size, dtype=dtype, device=device)
+        tq = pool = None
+        if idx >= exact_layers:
+            tq = TurboQuantProd(head_dim, bits=cfg.key_bits, device=device, seed=42 + 7 * idx)
+            pool = PagedKVPool(tq, cfg.num_kv_heads, num_blocks, value_bits=value_bits,
+                               value_group_size=cfg.value_group_size, dtype=dtype, device=device)
         state = BatchedLayerState(config=cfg, quantizer=tq, pool=pool)
         states[name] = state
         has_update = hasattr(impl, "do_kv_cache_update")
@@ -249,6 +304,31 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
     model_runner._tq_no_alloc = no_alloc
     logger.info("[TurboQuant] Batched hooks on %d layers (mode=%s, no_alloc=%s)", len(states), mode, no_alloc)
     return states
+
+
+def track_weights(model_runner, batch: int, max_len: int, window: int = 32) -> None:
+    """Have every hooked layer sum the attention weight of its tokens from now on: `batch` rows of the block table, up to max_len tokens each.  A
+    prompt step adds what its newest `window` queries give, read from the engine's cache; a decode step adds its own in exact layers."""
+    if getattr(model_runner, "_tq_no_alloc", False):
+        raise ValueError("weights are summed over the engine's cache, which no_alloc leaves out")
+    if not 1 <= window <= 1024:
+        raise ValueError(f"window must be 1 .. 1024, got {window}")
+    for state in model_runner._tq_layer_states.values():
+        state.track(batch, max_len, window)
+
+
+def evict_batched(model_runner, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int, seen: Optional[torch.Tensor] = None,
+                  sinks: int = 4, recent: int = 0) -> torch.Tensor:
+    """Cut every sequence to `budget` tokens in every hooked layer, each KV head by its own weights; returns the lengths (B,) that all layers have
+    now.  seq_lens (B,) tokens held, seen (B,) tokens had in all (None: nothing was cut before).  Blocks behind the new lengths are the
+    engine's to give away.  A sequence's blocks must be its own (no prefix shared with another)."""
+    ctx = model_runner.compilation_config.static_forward_context
+    lens = seq_lens
+    for name, state in model_runner._tq_layer_states.items():
+        caches = getattr(ctx[name], "kv_cache", None)
+        cache = caches[0] if caches and torch.is_tensor(caches[0]) and caches[0].dim() == 5 else None
+        lens = state.evict(block_table, seq_lens, budget, seen=seen, sinks=sinks, recent=recent, kv_cache=cache)
+    return lens
 
 
 def get_batched_stats(model_runner) -> dict:

@@ -143,6 +143,7 @@ class MinimalRunner:
         perm = torch.randperm(self.num_blocks, generator=torch.Generator().manual_seed(seed + 1))
         self.block_table = perm.view(batch, self.blocks_per_seq).to(torch.int32).to(self.device)
         self.seq_lens = [0] * batch
+        self.evicted = [0] * batch             # tokens that have left a sequence's cache: positions go on counting them
 
     # ---- metadata ------------------------------------------------------------------
     def metadata(self, new_tokens: Sequence[int]) -> StepMetadata:
@@ -178,7 +179,7 @@ class MinimalRunner:
         T = tokens.shape[0]
         if positions is None:
             lens, qsl = meta.seq_lens_cpu.tolist(), meta.query_start_loc_cpu.tolist()
-            positions = torch.cat([torch.arange(L - (qsl[b + 1] - qsl[b]), L) for b, L in enumerate(lens)]).to(self.device)
+            positions = torch.cat([torch.arange(L - (qsl[b + 1] - qsl[b]), L) + self.evicted[b] for b, L in enumerate(lens)]).to(self.device)
         x = self.embed[tokens]
         hq, hkv, d = self.hq, self.hkv, self.d
         for lay in self.layers:
@@ -204,7 +205,21 @@ class MinimalRunner:
     def decode_step(self, tokens: torch.Tensor) -> torch.Tensor:
         """tokens (B,): one new token per sequence."""
         meta = self.decode_metadata()
-        return self.step(tokens, meta, positions=(meta.seq_lens - 1).long())
+        positions = (meta.seq_lens - 1).long()
+        if any(self.evicted):
+            positions = positions + torch.tensor(self.evicted, device=self.device)
+        return self.step(tokens, meta, positions=positions)
+
+    def evict(self, budget: int, sinks: int = 4, recent: int = 0) -> None:
+        """Cut every sequence's cache to `budget` tokens by the weights that the batched hooks have summed (integration.batched
+        .track_weights); the sequences keep their blocks and fill them again."""
+        from .batched import evict_batched
+        lens = torch.tensor(self.seq_lens, dtype=torch.int32)
+        seen = lens + torch.tensor(self.evicted, dtype=torch.int32)
+        left = evict_batched(self, self.block_table, lens.to(self.device), budget, seen=seen.to(self.device), sinks=sinks, recent=recent)
+        now = left.tolist()
+        self.evicted = [e + n - m for e, n, m in zip(self.evicted, self.seq_lens, now)]
+        self.seq_lens = now
 
     # ---- the decode step as a HIP graph ----------------------------------------------
     def capture_decode_step(self, max_seq_len: int, first_tokens: torch.Tensor):
@@ -230,6 +245,8 @@ class MinimalRunner:
                                     + pos % BLOCK)
             return self.step(tokens, meta, positions=pos)
 
+        if any(self.evicted):
+            raise RuntimeError("sequences that have been cut are not captured: their positions are not their lengths")
         host_lens = list(self.seq_lens)
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
