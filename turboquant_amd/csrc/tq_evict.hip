@@ -89,11 +89,11 @@ __device__ __forceinline__ void sel_count(uint32_t* bins, bool in, uint32_t digi
 template <int THREADS>
 __device__ __forceinline__ uint32_t sel_scan(uint32_t v, uint32_t* s_wave, uint32_t* total) {
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t x = __shfl_up(v, o, 64);
-    if (lane >= o) v += x;
-  }
+  // within rows of sixteen lanes, then the rows' ends into the rows behind them
+#define TQ_SCAN_STEP(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, true)
+  TQ_SCAN_STEP(0x111, 0xF); TQ_SCAN_STEP(0x112, 0xF); TQ_SCAN_STEP(0x114, 0xF); TQ_SCAN_STEP(0x118, 0xF);
+  TQ_SCAN_STEP(0x142, 0xA); TQ_SCAN_STEP(0x143, 0xC);
+#undef TQ_SCAN_STEP
   __syncthreads();                              // (s_wave may still be read from the call before)
   if (lane == 63) s_wave[wave] = v;
   __syncthreads();
@@ -147,9 +147,11 @@ __device__ __forceinline__ uint2 sel_waves(uint2 v, uint2* s_two, uint2* total) 
 }
 
 // Keys of a wavefront's J x 64 neighbouring slots in registers: who of them stays, and the lists.  `ties`: keys equal to `last` in front of these slots;
-// `holes`, `movers`: in front of the wavefront's slots, found by `offsets` from its own numbers.  put(slot, rank, mover, j).  Returns bit j: slot j stays.
-template <int J, class Offsets, class Put>
-__device__ __forceinline__ uint32_t sel_lists(const uint32_t (&k)[J], int base, int n, int budget, uint32_t last, uint32_t want, uint32_t ties, Offsets offsets, Put put) {
+// `holes`, `movers`: in front of the wavefront's slots, found by `offsets` from its own numbers.  mover(slot, rank, j) for all of the wavefront's movers,
+// between(), hole(slot, rank, j) for its holes.  Returns bit j: slot j stays.
+template <int J, class Offsets, class Mover, class Between, class Hole>
+__device__ __forceinline__ uint32_t sel_lists(const uint32_t (&k)[J], int base, int n, int budget, uint32_t last, uint32_t want, uint32_t ties, Offsets offsets,
+                                              Mover mover, Between between, Hole hole) {
   const int lane = (int)threadIdx.x & 63;
   const uint64_t below = (1ull << lane) - 1;
   uint32_t stays = 0, holes = 0, movers = 0;
@@ -158,8 +160,11 @@ __device__ __forceinline__ uint32_t sel_lists(const uint32_t (&k)[J], int base, 
     const int i = base + j * 64 + lane;
     const bool in = i < n, tie = in && k[j] == last;
     const uint64_t t = __ballot(tie);
-    const bool keep = in && (k[j] > last || (tie && ties + (uint32_t)__popcll(t & below) < want));
-    ties += (uint32_t)__popcll(t);
+    bool keep = in && k[j] > last;
+    if (t) {
+      keep = keep || (tie && ties + (uint32_t)__popcll(t & below) < want);
+      ties += (uint32_t)__popcll(t);
+    }
     stays |= (uint32_t)keep << j;
     holes += (uint32_t)__popcll(__ballot(in && !keep && i < budget));
     movers += (uint32_t)__popcll(__ballot(keep && i >= budget));
@@ -169,38 +174,47 @@ __device__ __forceinline__ uint32_t sel_lists(const uint32_t (&k)[J], int base, 
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int i = base + j * 64 + lane;
-    const bool keep = stays >> j & 1, hole = i < n && !keep && i < budget, mover = keep && i >= budget;
-    const uint64_t hb = __ballot(hole), mb = __ballot(mover);
-    if (hole) put(i, holes + (uint32_t)__popcll(hb & below), false, j);
-    if (mover) put(i, movers + (uint32_t)__popcll(mb & below), true, j);
-    holes += (uint32_t)__popcll(hb);
-    movers += (uint32_t)__popcll(mb);
+    const bool is = (stays >> j & 1) && i >= budget;
+    const uint64_t who = __ballot(is);
+    if (who == 0) continue;                     // (the wavefront as one)
+    if (is) mover(i, movers + (uint32_t)__popcll(who & below), j);
+    movers += (uint32_t)__popcll(who);
+  }
+  between();
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int i = base + j * 64 + lane;
+    const bool is = i < n && !(stays >> j & 1) && i < budget;
+    const uint64_t who = __ballot(is);
+    if (who == 0) continue;
+    if (is) hole(i, holes + (uint32_t)__popcll(who & below), j);
+    holes += (uint32_t)__popcll(who);
   }
   return stays;
 }
 
-// ---- a row in one workgroup: its keys are read once and stay in registers ----
+// ---- a row in one workgroup: its weights and positions are read once and stay in registers, movers meet their holes in LDS ----
 // `each` (up to J): 64 slots per wavefront and step, so that all wavefronts have some.
 template <int THREADS, int J>
 __global__ void __launch_bounds__(THREADS) evict_row_kernel(const EvictSelect a, int each) {
-  constexpr int WAVES = THREADS / 64, BATCH = J < 8 ? J : 8;
+  constexpr int WAVES = THREADS / 64;
   __shared__ uint32_t s_bin[SEL_BINS];
   __shared__ uint32_t s_wave[WAVES], s_found[2];
   __shared__ uint2 s_two[WAVES];
+  __shared__ float2 s_mover[THREADS * J / 2];   // weight and position (as it is) of the n-th; no more than half of the slots move
   const int tid = (int)threadIdx.x, lane = tid & 63, base = (tid >> 6) * (each * 64);
   const EvictRow r(a, (int)blockIdx.x);
   if (r.h == 0 && tid == 0) a.lens_out[r.b] = r.left;
   uint32_t moved = 0;
+  const int end = base + each * 64 < r.n ? base + each * 64 : r.n;            // of this wavefront's slots
+  float w[J];
+  int pos[J];
+  if (r.n > 0) sel_load<J>(w, pos, r, base, end);
+  uint32_t stays = 0xffffffffu;
   if (r.n > a.budget) {
-    const int end = base + each * 64 < r.n ? base + each * 64 : r.n;          // of this wavefront's slots
     uint32_t k[J];
-    {
-      float w[J];
-      int pos[J];
-      sel_load<J>(w, pos, r, base, end);
 #pragma unroll
-      for (int j = 0; j < J; ++j) k[j] = base + j * 64 + lane < end ? evict_key(w[j], pos[j], a.sinks, r.newest) : 0u;
-    }
+    for (int j = 0; j < J; ++j) k[j] = base + j * 64 + lane < end ? evict_key(w[j], pos[j], a.sinks, r.newest) : 0u;
     uint32_t want = (uint32_t)a.budget, last = 0;
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
@@ -221,53 +235,36 @@ __global__ void __launch_bounds__(THREADS) evict_row_kernel(const EvictSelect a,
     for (int j = 0; j < J; ++j) ties += (uint32_t)__popcll(__ballot(base + j * 64 + lane < end && k[j] == last));
     uint2 total;
     ties = sel_waves<WAVES>(make_uint2(ties, 0), s_two, &total).x;
-    sel_lists<J>(k, base, end, a.budget, last, want, ties, [&](uint2 mine) { return sel_waves<WAVES>(mine, s_two, &total); },
-                 [&](int slot, uint32_t rank, bool mover, int) { (mover ? r.src : r.dst)[rank] = slot; });
+    stays = sel_lists<J>(k, base, end, a.budget, last, want, ties, [&](uint2 mine) { return sel_waves<WAVES>(mine, s_two, &total); },
+                         [&](int slot, uint32_t rank, int j) {
+                           r.src[rank] = slot;
+                           s_mover[rank] = make_float2(w[j], __int_as_float(pos[j]));
+                         },
+                         [] { __syncthreads(); },
+                         [&](int slot, uint32_t rank, int) {
+                           const float2 x = s_mover[rank];
+                           r.dst[rank] = slot;
+                           r.w_out[slot] = x.x;
+                           r.pos_out[slot] = __float_as_int(x.y);
+                         });
     moved = total.y;
   }
-  if (tid == 0) a.count[r.row] = (int32_t)moved;
-  for (int i = (int)moved + tid; i < a.moves; i += THREADS) r.dst[i] = r.src[i] = -1;
-  // ---- weights and positions of who stays: in place first (holes too), then the movers, then the slots that are free now ----
-  if (r.w_out != r.w || r.pos_out != r.pos) {
-    for (int j0 = 0; j0 < each; j0 += BATCH) {
-      const int from = base + j0 * 64, end = base + each * 64 < r.left ? base + each * 64 : r.left;
-      float w[BATCH];
-      int pos[BATCH];
-      sel_load<BATCH>(w, pos, r, from, end);
+  // Who stays in place, the slots that are free now, the ends of the lists.  (In place, too: every wavefront has its slots in registers - where a row is
+  // cut, behind barriers; where it is not, no slot that is written has been read.)
 #pragma unroll
-      for (int j = 0; j < BATCH; ++j) {
-        const int i = from + j * 64 + lane;
-        if (i < end && r.w_out != r.w) r.w_out[i] = w[j];
-        if (i < end && r.pos_out != r.pos) r.pos_out[i] = pos[j];
-      }
+  for (int j = 0; j < J; ++j) {
+    const int i = base + j * 64 + lane;
+    if (i < end && i < r.left && (stays >> j & 1)) {
+      if (r.w_out != r.w) r.w_out[i] = w[j];
+      if (r.pos_out != r.pos) r.pos_out[i] = pos[j];
     }
   }
-  __syncthreads();
-  for (int i0 = 0; i0 < (int)moved; i0 += THREADS * 4) {
-    int to[4], of[4], pos[4];
-    float w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j * THREADS + tid, at = i < (int)moved ? i : 0;
-      to[j] = r.dst[at];
-      of[j] = r.src[at];
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { w[j] = r.w[of[j]]; pos[j] = r.pos[of[j]]; }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(w[j]), "+v"(pos[j]));
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i0 + j * THREADS + tid < (int)moved) {
-        r.w_out[to[j]] = w[j];
-        r.pos_out[to[j]] = pos[j];
-      }
-  }
-  __syncthreads();
   for (int i = r.left + tid; i < a.L; i += THREADS) {
     r.w_out[i] = 0.0f;
     r.pos_out[i] = r.seen + (i - r.left);
   }
+  if (tid == 0) a.count[r.row] = (int32_t)moved;
+  for (int i = (int)moved + tid; i < a.moves; i += THREADS) r.dst[i] = r.src[i] = -1;
 }
 
 // ---- a long row in several workgroups ----
@@ -308,6 +305,15 @@ __global__ void __launch_bounds__(PART_THREADS) evict_part_kernel(const EvictSel
   if (r.n <= a.budget) return;                  // (the last launch does what there is to do)
   int first, end;
   part_slots(a, q, r, part, &first, &end);
+  const int base = first + wave * (PART_J * 64);
+  float w[PART_J];                              // (on their way while the digits are found)
+  int pos[PART_J];
+#pragma unroll
+  for (int j = 0; j < PART_J; ++j) {
+    const int i = base + j * 64 + lane, at = i < end ? i : 0;
+    w[j] = r.w[at];
+    pos[j] = r.pos[at];
+  }
   uint32_t want = (uint32_t)a.budget, last = 0;
   if constexpr (PASS > 0) {
 #pragma unroll
@@ -347,11 +353,7 @@ __global__ void __launch_bounds__(PART_THREADS) evict_part_kernel(const EvictSel
       }
     }
   }
-  const int base = first + wave * (PART_J * 64);
   uint32_t k[PART_J];
-  float w[PART_J];
-  int pos[PART_J];
-  sel_load<PART_J>(w, pos, r, base, end);
 #pragma unroll
   for (int j = 0; j < PART_J; ++j) k[j] = base + j * 64 + lane < end ? evict_key(w[j], pos[j], a.sinks, r.newest) : 0u;
   if constexpr (PASS < 3) {
@@ -387,17 +389,15 @@ __global__ void __launch_bounds__(PART_THREADS) evict_part_kernel(const EvictSel
       __syncthreads();
       if (lane == 0) s_part[wave] = make_uint2(n, t);
       __syncthreads();
-      for (int i = 0; i < PART_WAVES && p0 + i < q.parts; ++i) {
-        const uint2 x = s_part[i];
+#pragma unroll
+      for (int i = 0; i < PART_WAVES; ++i) {
+        const uint2 x = s_part[i];              // (of parts that are not there: nothing)
         const uint32_t kept = x.x + (want > ties_here ? (want - ties_here < x.y ? want - ties_here : x.y) : 0);
-        int f, e;
-        part_slots(a, q, r, p0 + i, &f, &e);
-        if (p0 + i < part) {
-          ties += x.y;
-          if (p0 + i < q.below) holes += (uint32_t)(e - f) - kept;
-          else movers += kept;
-        }
-        if (p0 + i >= q.below) all += kept;
+        const bool front = p0 + i < part, low = p0 + i < q.below;
+        ties += front ? x.y : 0;
+        holes += front && low ? (uint32_t)(p0 + i + 1 < q.below ? PART : a.budget - (q.below - 1) * PART) - kept : 0;
+        movers += front && !low ? kept : 0;
+        all += low ? 0 : kept;
         ties_here += x.y;
       }
     }
@@ -409,13 +409,11 @@ __global__ void __launch_bounds__(PART_THREADS) evict_part_kernel(const EvictSel
     const uint32_t stays = sel_lists<PART_J>(k, base, end, a.budget, last, want, ties, [&](uint2 x) {
       const uint2 at = sel_waves<PART_WAVES>(x, s_two, &total);
       return make_uint2(holes + at.x, movers + at.y);
-    }, [&](int slot, uint32_t rank, bool mover, int j) {
-      (mover ? r.src : r.dst)[rank] = slot;
-      if (mover) {
-        q.moved_w[r.row * a.moves + rank] = w[j];
-        q.moved_pos[r.row * a.moves + rank] = pos[j];
-      }
-    });
+    }, [&](int slot, uint32_t rank, int j) {
+      r.src[rank] = slot;
+      q.moved_w[r.row * a.moves + rank] = w[j];
+      q.moved_pos[r.row * a.moves + rank] = pos[j];
+    }, [] {}, [&](int slot, uint32_t rank, int) { r.dst[rank] = slot; });
     if (part < q.below) {
 #pragma unroll
       for (int j = 0; j < PART_J; ++j)
