@@ -11,6 +11,8 @@
 //     without conflicts.
 #pragma once
 
+#include <type_traits>
+
 #include "tq_exact_impl.h"
 
 namespace tq {
@@ -85,68 +87,66 @@ __global__ void __launch_bounds__(TW * 64, TW == 8 || D <= 256 ? 2 : 1) exact_he
 
   ExactPages<2> now, next;
   const uint32_t head_off = (uint32_t)((int)threadIdx.x & 63) * 16;        // a lane's part of a row
-  const auto fetch = [&](const ExactPages<2>& at, int turn) __attribute__((always_inline)) {
+  // This wavefront's loads of a block, NL of them, number u.  (Issued in a row they hold it up for 128 clocks each, 2300 of a block's 7000: they are spread
+  // over the block before.)
+  constexpr int ROW_LOADS = 64 / TW, END_LOADS = LOADS > 32 ? 8 / TW : 0;
+  constexpr int NL = Lds::ROWS ? ROW_LOADS + END_LOADS : (2 * LOADS + TW - 1) / TW;
+  const auto fetch = [&](const ExactPages<2>& at, int turn, int u) __attribute__((always_inline)) {
     if constexpr (Lds::ROWS) {
-      // wavefront w takes rows w, w + TW ... of each page; an address is the last one plus TW rows
-#pragma unroll
-      for (int side = 0; side < 2; ++side)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const char* from = (const char*)(side ? a.c.v : a.c.k) + at.at[p] + (uint32_t)wave * step;
-          const int row_bytes = (side ? VROW : KROW) * 16;
-          uint32_t to = lds0 + (uint32_t)(turn * TURN + (side ? Lds::KBYTES : 0) + (p * 16 + wave) * row_bytes);
-#pragma unroll
-          for (int i = 0; i < 16 / TW; ++i) {
-            ex_row_to_lds(from, head_off, to);
-            from += (uint64_t)(step * TW);
-            to += TW * row_bytes;
-          }
-        }
-      if constexpr (LOADS > 32) {
+      if (u < ROW_LOADS) {
+        // row wave + i TW of a page: keys of both pages, then values
+        const int side = u / (ROW_LOADS / 2), p = u / (ROW_LOADS / 4) & 1, i = u % (ROW_LOADS / 4);
+        const int row = wave + i * TW, row_bytes = (side ? VROW : KROW) * 16;
+        ex_row_to_lds((const char*)(side ? a.c.v : a.c.k) + at.at[p] + (uint64_t)((uint32_t)row * step), head_off,
+                      lds0 + (uint32_t)(turn * TURN + (side ? Lds::KBYTES : 0) + (p * 16 + row) * row_bytes));
+      } else {
         // the ends of rows r .. r + 7: keys of both pages, then values; a key's pieces change places by its row, for the banks
         const int ln = ex_anew((int)threadIdx.x & 63);
-#pragma unroll
-        for (int i = 0; i < 8; i += TW) {
-          const int n = i + wave, r = (n & 3) * 8;
-          const bool value = n >= 4;
-          const uint32_t off = (uint32_t)((r & 8) + (ln >> 3)) * step + (64 + (value ? ln & 7 : (ln & 7) ^ (ln >> 3))) * 16;
-          const uint32_t to = lds0 + (uint32_t)(turn * TURN + (value ? Lds::KBYTES + Lds::VTAIL : Lds::KTAIL) + r * 128);
-          ex_row_to_lds((const char*)(value ? a.c.v : a.c.k) + (r < 16 ? at.at[0] : at.at[1]), off, to);
-        }
+        const int n = (u - ROW_LOADS) * TW + wave, r = (n & 3) * 8;
+        const bool value = n >= 4;
+        const uint32_t off = (uint32_t)((r & 8) + (ln >> 3)) * step + (64 + (value ? ln & 7 : (ln & 7) ^ (ln >> 3))) * 16;
+        const uint32_t to = lds0 + (uint32_t)(turn * TURN + (value ? Lds::KBYTES + Lds::VTAIL : Lds::KTAIL) + r * 128);
+        ex_row_to_lds((const char*)(value ? a.c.v : a.c.k) + (r < 16 ? at.at[0] : at.at[1]), off, to);
       }
     } else {
+      const int n = u * TW + wave;                           // keys first
+      if (2 * LOADS % TW != 0 && n >= 2 * LOADS) return;
       const int ln = ex_anew((int)threadIdx.x & 63);         // (places are computed anew: there are no registers to keep them in)
-#pragma unroll
-      for (int i = 0; i < 2 * LOADS; i += TW) {
-        const int n = i + wave;                              // this wavefront's load: keys first
-        if (2 * LOADS % TW != 0 && n >= 2 * LOADS) break;
-        const bool value = n >= LOADS;
-        const int k = value ? n - LOADS : n, piece = k * 64 + ln;
-        int r = value ? piece / VROW : piece / KROW, p = piece - r * (value ? VROW : KROW);
-        r = r < 32 ? r : 31;                                 // (what fills the last load up, and the pieces between two rows: of no use, but there)
-        p = p < Lds::PIECES ? p : Lds::PIECES - 1;
-        const char* from = (const char*)(value ? a.c.v : a.c.k) + (r < 16 ? at.at[0] : at.at[1]) + ((uint32_t)(r & 15) * step + (uint32_t)p * 16);
-        ex_to_lds(from, lds0 + (uint32_t)(turn * TURN + (value ? Lds::KBYTES : 0) + k * 1024));
-      }
+      const bool value = n >= LOADS;
+      const int k = value ? n - LOADS : n, piece = k * 64 + ln;
+      int r = value ? piece / VROW : piece / KROW, p = piece - r * (value ? VROW : KROW);
+      r = r < 32 ? r : 31;                                   // (what fills the last load up, and the pieces between two rows: of no use, but there)
+      p = p < Lds::PIECES ? p : Lds::PIECES - 1;
+      const char* from = (const char*)(value ? a.c.v : a.c.k) + (r < 16 ? at.at[0] : at.at[1]) + ((uint32_t)(r & 15) * step + (uint32_t)p * 16);
+      ex_to_lds(from, lds0 + (uint32_t)(turn * TURN + (value ? Lds::KBYTES : 0) + k * 1024));
     }
   };
   // table entries are read two blocks ahead, as vector loads behind a block's own: they have arrived with it
   int32_t entry[2] = {-1, -1};
   if (first < last) {
     now.find(a.c, table, len, first, h, 2);
-    fetch(now, 0);
+#pragma unroll
+    for (int u = 0; u < NL; ++u) fetch(now, 0, u);
     ExactPages<2>::entries(entry, table, len, first + 1);
   }
-  for (int blk = first, turn = 0; blk < last; ++blk, turn ^= 1) {
+  const auto block = [&](auto more, int blk, int turn) __attribute__((always_inline)) {
     ex_arrived();
     __syncthreads();
-    if (blk + 1 < last) {
+    constexpr bool MORE = decltype(more)::value;
+    constexpr int STEPS = 2 * KSTEPS + TILES;                // matrix instructions of a block
+    if constexpr (MORE) {
       entry[0] = __builtin_amdgcn_readfirstlane(entry[0]);
       entry[1] = __builtin_amdgcn_readfirstlane(entry[1]);
       next.place(a.c, entry, len, blk + 1, h, 2);
-      fetch(next, turn ^ 1);
       ExactPages<2>::entries(entry, table, len, blk + 2);
     }
+    const auto load_ahead = [&](int g) __attribute__((always_inline)) {        // behind matrix instruction g
+      if constexpr (MORE) {
+#pragma unroll
+        for (int u = 0; u < NL; ++u)
+          if (u >= NL * g / STEPS && u < NL * (g + 1) / STEPS) fetch(next, turn ^ 1, u);
+      }
+    };
     if (!now.whole) {
       // values of tokens without weight are put to zero where they lie, since NaN times nothing is NaN
 #pragma unroll 1
@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(TW * 64, TW == 8 || D <= 256 ? 2 : 1) exact_he
     for (int i = 0; i < N; ++i) {
       S[i & 1] = ex_mfma<DT>(kf[i % PRE], Q[i >> 1], S[i & 1]);
       if (i + PRE < N) kf[i % PRE] = key((i + PRE) & 1, (i + PRE) >> 1);
+      load_ahead(i);
       if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
     }
     ex_u32x4 x[2][8];
@@ -257,6 +258,7 @@ __global__ void __launch_bounds__(TW * 64, TW == 8 || D <= 256 ? 2 : 1) exact_he
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = __builtin_amdgcn_perm(v[2 * j + 1][t >> 1], v[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
         O[c * 8 + t] = ex_mfma<DT>(f, P, O[c * 8 + t]);
+        load_ahead(N + c * 8 + t);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -271,10 +273,14 @@ __global__ void __launch_bounds__(TW * 64, TW == 8 || D <= 256 ? 2 : 1) exact_he
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = __builtin_amdgcn_perm(y[2 * j + 1][t >> 1], y[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
         O[WIDE * 8 + t] = ex_mfma<DT>(f, P, O[WIDE * 8 + t]);
+        load_ahead(N + WIDE * 8 + t);
       }
     }
     now = next;
-  }
+  };
+  int turn = 0;
+  for (int blk = first; blk + 1 < last; ++blk, turn ^= 1) block(std::true_type{}, blk, turn);
+  if (first < last) block(std::false_type{}, last - 1, turn);
   l = ex_quad_sum(l);
   const int lane = (int)threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
   if (head0 + col >= a.G) return;
