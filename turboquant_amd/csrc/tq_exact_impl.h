@@ -120,11 +120,13 @@ struct ExactPages {
     entries(entry, table, len, blk);
     place(c, entry, len, blk, h, size);
   }
+  // (no condition around the loads: behind one they would be waited for at once.  Pages behind the sequence have its last entry, and no tokens.)
   static __device__ __forceinline__ void entries(int32_t* entry, const int32_t* table, int len, int blk) {
+    const int last = len > 0 ? (len - 1) / TQ_PAGE_TOKENS : 0;
 #pragma unroll
     for (int p = 0; p < PAGES; ++p) {
       const int page = blk * PAGES + p;
-      entry[p] = page * TQ_PAGE_TOKENS < len ? table[page] : -1;
+      entry[p] = table[page < last ? page : last];
     }
   }
   __device__ __forceinline__ void place(const ExactCache& c, const int32_t* entry, int len, int blk, int h, int size) {

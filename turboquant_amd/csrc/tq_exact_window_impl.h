@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(WAVES * 64, window_waves_per_simd(DT, D, WAVES
   const int split = (int)(id / pairs), pair = (int)((id % pairs + (unsigned)split) % pairs);
   const int h = pair % a.c.H, b = pair / a.c.H;
 
-  const int len = exact_len(a.c, b);
+  const int len = __builtin_amdgcn_readfirstlane(exact_len(a.c, b));
   const int blocks = (len + TB - 1) / TB, per = exact_blocks_per_split(blocks, a.n_split, a.chunk);
   const int first = split * per < blocks ? split * per : blocks, last = first + per < blocks ? first + per : blocks;
   // the rows of the window
@@ -64,10 +64,12 @@ __global__ void __launch_bounds__(WAVES * 64, window_waves_per_simd(DT, D, WAVES
   if (first >= last || n_rows == 0) return;                  // (the same for the whole workgroup)
   const uint32_t step = (uint32_t)a.c.s_t * SIZE, lds0 = (uint32_t)(uintptr_t)s_keys;
 
-  // A turn: token_waves blocks from `blk` on.  Lane l knows the table entry of the turn's page l; -1: behind the sequence.
+  // A turn: token_waves blocks from `blk` on.  Lane l knows the table entry of the turn's page l (behind the sequence, where nothing counts, its
+  // last; a condition around the load would have it waited for at once, and with it the keys that are on their way).
+  const int last_page = (len - 1) / TQ_PAGE_TOKENS;
   const auto entries = [&](int blk) __attribute__((always_inline)) {
     const int page = blk * PAGES + lane;
-    return lane < token_waves * PAGES && page * TQ_PAGE_TOKENS < len ? table[page] : -1;
+    return table[page < last_page ? page : last_page];
   };
   const auto page_of = [&](int entry, int p) __attribute__((always_inline)) {
     const int64_t x = __builtin_amdgcn_readlane(entry, p);
