@@ -129,11 +129,9 @@ __global__ void __launch_bounds__(WAVES * 64, window_waves_per_simd(DT, D, WAVES
         ex_arrived();
         __syncthreads();                                     // everybody's loads of this turn are there, everybody is done with the other
         const int now = entry;
-        if (turn0 + token_waves < sub_end) {
-          entry = entry_next;
-          fetch(entry, turn ^ 1);
-          entry_next = entries(turn0 + 2 * token_waves);
-        }
+        entry = entry_next;
+        if (turn0 + token_waves < sub_end) fetch(entry, turn ^ 1);
+        entry_next = entries(turn0 + 2 * token_waves);       // (always: behind a condition it would be waited for)
         const int blk = turn0 + token_wave, t0 = blk * TB;
         if (!busy || blk >= sub_end) continue;
         int valid[PAGES];
