@@ -71,20 +71,32 @@ __global__ void __launch_bounds__(WAVES * 64, window_waves_per_simd(DT, D, WAVES
     const int page = blk * PAGES + lane;
     return table[page < last_page ? page : last_page];
   };
-  const auto page_of = [&](int entry, int p) __attribute__((always_inline)) {
-    const int64_t x = __builtin_amdgcn_readlane(entry, p);
-    return x < 0 || x >= a.c.num_blocks ? (int64_t)-1 : x;
+  const uint32_t in_cache = a.c.num_blocks < 0x80000000ll ? (uint32_t)a.c.num_blocks : 0x80000000u;
+  const auto there = [&](int entry, int p) __attribute__((always_inline)) { return (uint32_t)__builtin_amdgcn_readlane(entry, p) < in_cache; };
+  // A wavefront's loads of a turn are numbers wave, wave + waves, ...: page n / PAGE_LOADS, 64 pieces of it.  A lane's place in its page is the same in
+  // every turn; the first FIXED of them stay in registers (computed anew they were 40 instructions a load, and the loads a quarter of a turn).
+  constexpr int FIXED = 5;
+  const int turn_loads = token_waves * PAGES * PAGE_LOADS;
+  const char* head = (const char*)a.c.k + h * a.c.s_h * SIZE;
+  const uint64_t block_bytes = (uint64_t)a.c.s_blk * SIZE;
+  const auto place = [&](int n) __attribute__((always_inline)) {
+    const int piece = n % PAGE_LOADS * 64 + lane, r = piece / PIECES, at = piece - r * PIECES;
+    return (uint32_t)r * step + (uint32_t)window_place<PIECES>(at, r) * 16;
+  };
+  uint32_t fixed[FIXED];
+#pragma unroll
+  for (int i = 0; i < FIXED; ++i) fixed[i] = place(wave + i * a.waves);
+  const auto load = [&](int entry, int turn, int n, uint32_t off) __attribute__((always_inline)) {
+    const int p = n / PAGE_LOADS;
+    uint32_t page = (uint32_t)__builtin_amdgcn_readlane(entry, p);
+    page = page < in_cache ? page : 0;                       // (a block that is there; its tokens are masked)
+    ex_row_to_lds(head + page * block_bytes, off, lds0 + (uint32_t)(turn * token_waves * BLOCK + n * 1024));
   };
   const auto fetch = [&](int entry, int turn) __attribute__((always_inline)) {
-    for (int n = wave; n < token_waves * PAGES * PAGE_LOADS; n += a.waves) {
-      const int p = n / PAGE_LOADS, k = n - p * PAGE_LOADS;  // page of the turn, load of the page
-      int64_t page = page_of(entry, p);
-      page = page < 0 ? 0 : page;                            // (a block that is there; its tokens are masked)
-      const int piece = k * 64 + lane, r = piece / PIECES, at = piece - r * PIECES;
-      const uint32_t off = (uint32_t)r * step + (uint32_t)window_place<PIECES>(at, r) * 16;
-      ex_row_to_lds((const char*)a.c.k + (page * a.c.s_blk + h * a.c.s_h) * SIZE, off,
-                    lds0 + (uint32_t)(turn * token_waves * BLOCK + p * (PAGE_LOADS * 1024) + k * 1024));
-    }
+#pragma unroll
+    for (int i = 0; i < FIXED; ++i)
+      if (wave + i * a.waves < turn_loads) load(entry, turn, wave + i * a.waves, fixed[i]);
+    for (int n = wave + FIXED * a.waves; n < turn_loads; n += a.waves) load(entry, turn, n, place(n));
   };
 
   for (int sub = first; sub < last; sub += ADD ? WINDOW_TOKENS / TB : last - first) {
@@ -139,7 +151,7 @@ __global__ void __launch_bounds__(WAVES * 64, window_waves_per_simd(DT, D, WAVES
 #pragma unroll
         for (int p = 0; p < PAGES; ++p) {
           const int left = len - t0 - p * TQ_PAGE_TOKENS;
-          valid[p] = page_of(now, token_wave * PAGES + p) < 0 || left < 0 ? 0 : (left > TQ_PAGE_TOKENS ? TQ_PAGE_TOKENS : left);
+          valid[p] = !there(now, token_wave * PAGES + p) || left < 0 ? 0 : (left > TQ_PAGE_TOKENS ? TQ_PAGE_TOKENS : left);
           whole &= valid[p] == TQ_PAGE_TOKENS;
         }
         const unsigned char* keys = s_keys + (turn * token_waves + token_wave) * BLOCK;
