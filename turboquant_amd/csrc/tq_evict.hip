@@ -85,37 +85,50 @@ __device__ __forceinline__ void sel_count(uint32_t* bins, bool in, uint32_t digi
   }
 }
 
+// inclusive sum over a wavefront's lanes: within rows of sixteen, then the rows' ends into the rows behind them
+__device__ __forceinline__ uint32_t lanes_scan16(uint32_t v) {
+#define TQ_SCAN_STEP(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, true)
+  TQ_SCAN_STEP(0x111, 0xF); TQ_SCAN_STEP(0x112, 0xF); TQ_SCAN_STEP(0x114, 0xF); TQ_SCAN_STEP(0x118, 0xF);
+  return v;
+}
+__device__ __forceinline__ uint32_t lanes_scan(uint32_t v) {
+  v = lanes_scan16(v);
+  TQ_SCAN_STEP(0x142, 0xA); TQ_SCAN_STEP(0x143, 0xC);
+#undef TQ_SCAN_STEP
+  return v;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+
+// Sums over the wavefronts in front of this one, and over all, of a count that each of them has.  (Up to sixteen, a lane each: in a workgroup of a
+// thousand threads an instruction that all of them execute takes sixteen clocks.)
+template <int WAVES>
+__device__ __forceinline__ uint32_t sel_before(const uint32_t* s_wave, uint32_t* total) {
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const uint32_t v = lanes_scan16(lane < WAVES ? s_wave[lane] : 0u);
+  *total = lane_of(v, WAVES - 1);
+  return wave > 0 ? lane_of(v, wave - 1) : 0u;
+}
+
 // inclusive sum over the workgroup's threads; *total = all of it
 template <int THREADS>
 __device__ __forceinline__ uint32_t sel_scan(uint32_t v, uint32_t* s_wave, uint32_t* total) {
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  // within rows of sixteen lanes, then the rows' ends into the rows behind them
-#define TQ_SCAN_STEP(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, true)
-  TQ_SCAN_STEP(0x111, 0xF); TQ_SCAN_STEP(0x112, 0xF); TQ_SCAN_STEP(0x114, 0xF); TQ_SCAN_STEP(0x118, 0xF);
-  TQ_SCAN_STEP(0x142, 0xA); TQ_SCAN_STEP(0x143, 0xC);
-#undef TQ_SCAN_STEP
+  v = lanes_scan(v);
   __syncthreads();                              // (s_wave may still be read from the call before)
-  if (lane == 63) s_wave[wave] = v;
+  if (((int)threadIdx.x & 63) == 63) s_wave[(int)threadIdx.x >> 6] = v;
   __syncthreads();
-  uint32_t before = 0, all = 0;
-#pragma unroll
-  for (int i = 0; i < THREADS / 64; ++i) {
-    const uint32_t x = s_wave[i];
-    if (i < wave) before += x;
-    all += x;
-  }
-  *total = all;
-  return before + v;
+  return sel_before<THREADS / 64>(s_wave, total) + v;
 }
 
-// The bin, from the highest down, in which the count reaches `want`: s_found = {bin, how many of it are wanted}.  count(bin): keys in it.
-template <int THREADS, class Count>
-__device__ __forceinline__ void sel_find(uint32_t want, Count count, uint32_t* s_wave, uint32_t* s_found) {
+// The bin, from the highest down, in which the count reaches `want`: s_found = {bin, how many of it are wanted}.  counts(bin, c): c[i] = keys in bin - i, for
+// as many as a thread has.
+template <int THREADS, class Counts>
+__device__ __forceinline__ void sel_find(uint32_t want, Counts counts, uint32_t* s_wave, uint32_t* s_found) {
   constexpr int EACH = SEL_BINS / THREADS;
   const int hi = SEL_BINS - 1 - EACH * (int)threadIdx.x;
   uint32_t c[EACH], mine = 0, total;
+  counts(hi, c);
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) { c[i] = count(hi - i); mine += c[i]; }
+  for (int i = 0; i < EACH; ++i) mine += c[i];
   uint32_t before = sel_scan<THREADS>(mine, s_wave, &total) - mine;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
@@ -128,21 +141,18 @@ __device__ __forceinline__ void sel_find(uint32_t want, Count count, uint32_t* s
   __syncthreads();
 }
 
-// exclusive sum over the wavefronts of two counts that each of them has, in slot order
+// sums over the wavefronts in front, in slot order, of two counts that each of them has, and over all
 template <int WAVES>
-__device__ __forceinline__ uint2 sel_waves(uint2 v, uint2* s_two, uint2* total) {
-  const int wave = (int)threadIdx.x >> 6;
+__device__ __forceinline__ uint2 sel_waves(uint2 v, uint32_t (*s_two)[WAVES], uint2* total) {
   __syncthreads();
-  if (((int)threadIdx.x & 63) == 0) s_two[wave] = v;
-  __syncthreads();
-  uint2 before = make_uint2(0, 0), all = before;
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) {
-    const uint2 x = s_two[i];
-    if (i < wave) { before.x += x.x; before.y += x.y; }
-    all.x += x.x; all.y += x.y;
+  if (((int)threadIdx.x & 63) == 0) {
+    s_two[0][(int)threadIdx.x >> 6] = v.x;
+    s_two[1][(int)threadIdx.x >> 6] = v.y;
   }
-  *total = all;
+  __syncthreads();
+  uint2 before;
+  before.x = sel_before<WAVES>(s_two[0], &total->x);
+  before.y = sel_before<WAVES>(s_two[1], &total->y);
   return before;
 }
 
@@ -200,7 +210,7 @@ __global__ void __launch_bounds__(THREADS) evict_row_kernel(const EvictSelect a,
   constexpr int WAVES = THREADS / 64;
   __shared__ uint32_t s_bin[SEL_BINS];
   __shared__ uint32_t s_wave[WAVES], s_found[2];
-  __shared__ uint2 s_two[WAVES];
+  __shared__ uint32_t s_two[2][WAVES];
   __shared__ float2 s_mover[THREADS * J / 2];   // weight and position (as it is) of the n-th; no more than half of the slots move
   const int tid = (int)threadIdx.x, lane = tid & 63, base = (tid >> 6) * (each * 64);
   const EvictRow r(a, (int)blockIdx.x);
@@ -225,7 +235,10 @@ __global__ void __launch_bounds__(THREADS) evict_row_kernel(const EvictSelect a,
       for (int j = 0; j < J; ++j)
         sel_count(s_bin, base + j * 64 + lane < end && (pass == 0 || (k[j] >> (above & 31)) == (last >> (above & 31))), (k[j] >> low) & ((1u << sel_bits(pass)) - 1));
       __syncthreads();
-      sel_find<THREADS>(want, [&](int bin) { return s_bin[bin]; }, s_wave, s_found);
+      sel_find<THREADS>(want, [&](int bin, uint32_t* c) {
+#pragma unroll
+        for (int i = 0; i < SEL_BINS / THREADS; ++i) c[i] = s_bin[bin - i];
+      }, s_wave, s_found);
       last |= s_found[0] << low;
       want = s_found[1];
     }
@@ -296,7 +309,7 @@ template <int PASS>
 __global__ void __launch_bounds__(PART_THREADS) evict_part_kernel(const EvictSelect a, const EvictParts q) {
   __shared__ uint32_t s_bin[SEL_BINS];
   __shared__ uint32_t s_wave[PART_WAVES], s_found[2];
-  __shared__ uint2 s_two[PART_WAVES], s_part[PART_WAVES];
+  __shared__ uint32_t s_two[2][PART_WAVES], s_part[2][64], s_front[4];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int part = (int)(blockIdx.x % (unsigned)q.parts);
   const EvictRow r(a, (int)(blockIdx.x / (unsigned)q.parts));
@@ -323,11 +336,18 @@ __global__ void __launch_bounds__(PART_THREADS) evict_part_kernel(const EvictSel
       want = f[1];
     }
     const uint32_t* bins = q.bins + (((PASS - 1) * rows + r.row) * q.parts) * SEL_BINS;
-    sel_find<PART_THREADS>(want, [&](int bin) {
-      uint32_t n = 0;
-#pragma unroll 8
-      for (int p = 0; p < q.parts; ++p) n += bins[(int64_t)p * SEL_BINS + bin];
-      return n;
+    // (two neighbouring bins of sixteen parts on their way at a time)
+    sel_find<PART_THREADS>(want, [&](int bin, uint32_t* c) {
+      static_assert(SEL_BINS / PART_THREADS == 2, "two bins a thread");
+      c[0] = c[1] = 0;
+      for (int p0 = 0; p0 < q.parts; p0 += 16) {
+        uint2 x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = *(const uint2*)(bins + (int64_t)(p0 + i < q.parts ? p0 + i : 0) * SEL_BINS + bin - 1);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (p0 + i < q.parts) { c[0] += x[i].y; c[1] += x[i].x; }
+      }
     }, s_wave, s_found);
     const uint32_t digit = s_found[0];
     last |= digit << sel_low(PASS - 1);
@@ -367,39 +387,44 @@ __global__ void __launch_bounds__(PART_THREADS) evict_part_kernel(const EvictSel
     uint32_t* mine = q.bins + ((PASS * rows + r.row) * q.parts + part) * SEL_BINS;
     for (int i = tid; i < SEL_BINS; i += PART_THREADS) mine[i] = s_bin[i];
   } else {
-    // parts in slot order: keys that stay for sure and ties of each, sixteen parts at a time; what lies in front of this one
+    // Parts in slot order: keys that stay for sure and ties of each, a wavefront per part; then one wavefront, a lane per part, sums what lies in front of
+    // this part.  64 parts at a time.
     const uint32_t digit = last & ((1u << sel_bits(2)) - 1);
     const uint32_t* bins = q.bins + ((2 * rows + r.row) * q.parts) * SEL_BINS;
-    uint32_t ties = 0, ties_here = 0, holes = 0, movers = 0, all = 0;
-    for (int p0 = 0; p0 < q.parts; p0 += PART_WAVES) {
-      const int p = p0 + wave;
-      uint32_t n = 0, t = 0;
-      if (p < q.parts) {
+    uint32_t ties = 0, ties_all = 0, holes = 0, movers = 0, all = 0;
+    for (int p0 = 0; p0 < q.parts; p0 += 64) {
+      for (int p = p0 + wave; p < q.parts && p < p0 + 64; p += PART_WAVES) {
+        constexpr int U = (1 << sel_bits(2)) / 64;
+        uint32_t x[U], n = 0, t = 0;
 #pragma unroll
-        for (int u = 0; u < (1 << sel_bits(2)) / 64; ++u) {
-          const int i = u * 64 + lane;
-          const uint32_t c = bins[(int64_t)p * SEL_BINS + i];
-          n += i > (int)digit ? c : 0;
-          t += i == (int)digit ? c : 0;
+        for (int u = 0; u < U; ++u) x[u] = bins[(int64_t)p * SEL_BINS + u * 64 + lane];
+        const uint32_t larger = q.larger[r.row * q.parts + p];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          n += u * 64 + lane > (int)digit ? x[u] : 0;
+          t += u * 64 + lane == (int)digit ? x[u] : 0;
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) { n += __shfl_xor(n, o, 64); t += __shfl_xor(t, o, 64); }
-        n += q.larger[r.row * q.parts + p];
+        n = lane_of(lanes_scan(n), 63) + larger;
+        t = lane_of(lanes_scan(t), 63);
+        if (lane == 0) { s_part[0][p - p0] = n; s_part[1][p - p0] = t; }
       }
       __syncthreads();
-      if (lane == 0) s_part[wave] = make_uint2(n, t);
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < PART_WAVES; ++i) {
-        const uint2 x = s_part[i];              // (of parts that are not there: nothing)
-        const uint32_t kept = x.x + (want > ties_here ? (want - ties_here < x.y ? want - ties_here : x.y) : 0);
-        const bool front = p0 + i < part, low = p0 + i < q.below;
-        ties += front ? x.y : 0;
-        holes += front && low ? (uint32_t)(p0 + i + 1 < q.below ? PART : a.budget - (q.below - 1) * PART) - kept : 0;
-        movers += front && !low ? kept : 0;
-        all += low ? 0 : kept;
-        ties_here += x.y;
+      if (wave == 0) {
+        const int p = p0 + lane;
+        const uint32_t n = p < q.parts ? s_part[0][lane] : 0, t = p < q.parts ? s_part[1][lane] : 0;
+        const uint32_t upto = ties_all + lanes_scan(t), before = upto - t;
+        const uint32_t kept = n + (want > before ? (want - before < t ? want - before : t) : 0);
+        const bool low = p < q.below;
+        const uint32_t size = (uint32_t)(p + 1 < q.below ? PART : a.budget - (q.below - 1) * PART);
+        const uint32_t h = lanes_scan(low ? size - kept : 0), m = lanes_scan(low || p >= q.parts ? 0 : kept);
+        const int front = part - p0 < 0 ? 0 : (part - p0 < 64 ? part - p0 : 64);          // of these parts, in front of this one
+        if (lane == 0) { s_front[0] = s_front[1] = s_front[2] = 0; }
+        if (lane == front - 1) { s_front[0] = upto - ties_all; s_front[1] = h; s_front[2] = m; }
+        if (lane == 63) s_front[3] = m;
+        ties_all = lane_of(upto, 63);
       }
+      __syncthreads();
+      ties += s_front[0]; holes += s_front[1]; movers += s_front[2]; all += s_front[3];
     }
     uint32_t mine = 0;
 #pragma unroll
