@@ -58,7 +58,7 @@ def test_who_stays(gpu, L, budget, kind):
         check(w, pos, [L, max(0, L - 1)], budget, sinks=sinks, recent=recent)
 
 
-@pytest.mark.parametrize("L,budget", [(40000, 1000), (131072, 16384), (150001, 75000)])
+@pytest.mark.parametrize("L,budget", [(40000, 1000), (131072, 16384), (150001, 75000), (700001, 20000), (700001, 650000)])
 def test_long_rows(gpu, L, budget):
     for kind in ("sums", "ties", "close"):
         check(weights_of(1, 2, L, 1, kind), in_order(1, 2, L), [L - 3], budget, sinks=16, recent=100, out="inputs" if kind == "ties" else None)
