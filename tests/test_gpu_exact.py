@@ -39,6 +39,48 @@ def test_heads_per_kv_head(gpu, heads, H, dtype):
     check_decode(seqs, q, decode(seqs, q, w), 128 ** -0.5, before, w)
 
 
+# a bound on the lengths with which more than sixteen heads share their reads, however short the sequences are
+SHARED = 1 << 21
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", range(64, 577, 64))
+def test_heads_that_share_their_reads(gpu, d, dtype):
+    seqs = Sequences([0, 1, 15, 16, 17, 33, 150], 2, d, DTYPES[dtype], seed=d)
+    for heads in (34, 100):
+        q = seqs.query(7, heads, d)
+        before, w = start_weights(seqs, 150)
+        check_decode(seqs, q, decode(seqs, q, w, max_len=SHARED), d ** -0.5, before, w)
+    seqs = Sequences([2500, 31], 1, d, DTYPES[dtype], seed=d)
+    q = seqs.query(2, 70, d)
+    for splits in (1, 1024):                                       # one part, two
+        before, w = start_weights(seqs, 2500)
+        check_decode(seqs, q, decode(seqs, q, w, max_len=SHARED, n_split=splits), d ** -0.5, before, w)
+
+
+@pytest.mark.parametrize("layout", ["engine", "heads", "padded"])
+@pytest.mark.parametrize("dtype,d,heads", [("bf16", 128, 96), ("fp16", 256, 51), ("bf16", 512, 60), ("fp16", 576, 384)])
+def test_heads_that_share_their_reads_layouts_and_blocks(gpu, dtype, d, heads, layout):
+    seqs = Sequences([77, 300, 64], 3, d, DTYPES[dtype], layout=layout)
+    q = seqs.query(3, heads, d)
+    keep = [torch.ones(n, dtype=torch.bool) for n in seqs.lens]
+    for b, page, entry in ((1, 3, -1), (1, 18, seqs.blocks), (2, 0, 2 ** 31 - 1), (2, 1, -2 ** 31), (2, 2, seqs.blocks), (2, 3, -7)):
+        seqs.table[b, page] = entry
+        keep[b][page * PAGE: (page + 1) * PAGE] = False
+    before, w = start_weights(seqs, 300)
+    out = decode(seqs, q, w, scale=0.07, max_len=SHARED)
+    check_decode(seqs, q, out, 0.07, before, w, keep=keep)
+    assert not out[2].any()
+
+
+def test_many_heads_over_a_cache_of_some_length(gpu):
+    """Sizes at which the heads share their reads without being told, several parts to a sequence."""
+    seqs = Sequences([1400, 2, 900], 1, 576, torch.bfloat16)
+    q = seqs.query(3, 128, 576)
+    before, w = start_weights(seqs, 1400)
+    check_decode(seqs, q, decode(seqs, q, w), 576 ** -0.5, before, w)
+
+
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("n", [1, 2, 16, 31, 32, 33, 127, 128, 129, 511, 513, 1024, 1025, 4097])
 def test_lengths_and_splits(gpu, n, dtype):

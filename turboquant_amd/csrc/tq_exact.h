@@ -95,7 +95,7 @@ int exact_cache_init(ExactCache* c, const void* k, const void* v, int dtype, int
                      const int32_t* table, int bt_stride, const int32_t* lens);
 
 template <int DT> int launch_exact_decode(const ExactDecode& a, hipStream_t stream);
-template <int DT> int launch_exact_heads(const ExactDecode& a, int tile_waves, hipStream_t stream);
+template <int DT> int launch_exact_heads(const ExactDecode& a, hipStream_t stream);
 
 // a kernel may use more than 64 KB of LDS once it is told so, on every device for itself
 inline int exact_allow_lds(const void* kern, int bytes, std::atomic<uint64_t>& ready) {

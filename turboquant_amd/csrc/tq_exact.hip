@@ -175,7 +175,7 @@ static int64_t join_groups(int64_t rows, int n_split, int d) {
 
 // ---- how a call is split ----------------------------------------------------------------------------------------------------------------
 struct ExactPlan {
-  int tile_waves;                     // 0: the kernel of sixteen heads; else tiles of sixteen heads that a workgroup serves
+  bool shared;                        // the kernel of 64 heads, not that of sixteen
   int groups, n_split, chunk, block_tokens, score_pages, weight_tokens;
   size_t ml_at, acc_at, scores_at, bytes;
 };
@@ -190,11 +190,19 @@ static bool exact_plan(ExactPlan* p, int dtype, int B, int Hq, int Hkv, int d, i
   if (G > JOIN_MAX_SPLITS) return false;
   p->block_tokens = dtype == TQ_F32 ? 16 : 32;
   const int tiles = (G + EXACT_HEADS - 1) / EXACT_HEADS;
-  const bool shared = dtype != TQ_F32 && tiles > 1 && d <= 576;
-  p->tile_waves = !shared ? 0 : (tiles > 4 && d <= 256 ? 8 : (tiles > 2 ? 4 : 2));
-  p->groups = shared ? (tiles + p->tile_waves - 1) / p->tile_waves : tiles;
+  // More than sixteen heads share their reads where the passes over the cache that this saves outweigh a start that is 2-4 us longer: from 64 MB, all
+  // heads' passes together (bf16, sixteen / 64 heads a workgroup; one sequence of 16384, 32 heads: d 128 34 MB 9.9 / 12.1 us, d 448 59 MB 19.6 / 22.6, d 576
+  // 75 MB 26.6 / 23.1; 48 heads, 16 of 8192: d 128 201 MB 25.0 / 25.2, d 192 302 MB 41 / 32, d 576 906 MB 264 / 74).  d = 64 with 32 heads: 21.6 / 27.2 at
+  // 134 MB, never.
+  const int64_t passes = (int64_t)tiles * d * 4 * std::max<int64_t>(1, (int64_t)B * Hkv);
+  const bool shared = dtype != TQ_F32 && tiles > 1 && d <= 576 && (d > 64 || tiles > 2) && max_len > (int64_t(64) << 20) / passes;
+  p->shared = shared;
+  p->groups = shared ? (tiles + 3) / 4 : tiles;
   const int64_t pairs = std::max<int64_t>(1, (int64_t)B * Hkv * p->groups);
   const int64_t blocks = std::max<int64_t>(1, (max_len + p->block_tokens - 1) / p->block_tokens);
+  // As many workgroups as the card holds, and no split of more than 1024 tokens: sequences differ in length (64 of up to 4096, 32 / 8 heads of 128: one
+  // split 146 us, two 133, four 124, eight 124; all of 4096: 191.5, 190, 191, 197; four of 65536: 24 splits 213, 64 197).  The kernel of 64 heads fills the card
+  // once: its splits are dear to join.
   int64_t n = n_split;
   if (n == 0) {
     const int64_t resident = 256 * (shared ? (d > 256 ? 1 : 2) : (d <= 64 ? 4 : (d <= 128 ? 3 : (d <= 256 ? 2 : 1))));
@@ -265,8 +273,8 @@ extern "C" int tq_exact_decode(const void* q, int dtype, int B, int Hq, int Hkv,
   a.score_pages = p.score_pages;
   hipStream_t st = (hipStream_t)stream;
   int done;
-  if (p.tile_waves)
-    done = dtype == TQ_F16 ? launch_exact_heads<TQ_F16>(a, p.tile_waves, st) : launch_exact_heads<TQ_BF16>(a, p.tile_waves, st);
+  if (p.shared)
+    done = dtype == TQ_F16 ? launch_exact_heads<TQ_F16>(a, st) : launch_exact_heads<TQ_BF16>(a, st);
   else
     done = dtype == TQ_F32 ? launch_exact_decode<TQ_F32>(a, st)
                            : (dtype == TQ_F16 ? launch_exact_decode<TQ_F16>(a, st) : launch_exact_decode<TQ_BF16>(a, st));

@@ -2,13 +2,19 @@
 //
 // The mathematics and the operand layouts are those of tq_exact_impl.h; what differs is who reads.  There a workgroup reads keys and values for
 // sixteen heads, straight into registers: with 128 heads on one latent of 576 channels that is eight passes over the cache.  Here a workgroup
-// of TW wavefronts, one tile of sixteen heads each, shares a block of 32 tokens in LDS: the cache is read once for 16 TW heads.
+// of four wavefronts, one tile of sixteen heads each, shares a block of 32 tokens in LDS: the cache is read once for 64 heads, from memory for the first
+// 64 and from the die's cache for the others, which exact_place puts next to each other.
 //   * A wavefront owns its heads for the whole range of tokens - scores, softmax, accumulators -, so that nothing is exchanged or joined
-//     between wavefronts.  576 channels: 72 registers of queries, 144 of accumulators, two wavefronts per SIMD.
+//     between wavefronts.  576 channels: 72 registers of queries, 144 of accumulators and a chunk of values twice, one wavefront per SIMD (with two,
+//     of eight tiles in a workgroup, 256 registers each were not enough, and the spills' waits drained the loads ahead).
 //   * Blocks lie in LDS twice: while one is worked on, the next is filled by LDS-direct loads, which all wavefronts issue in turn.  One barrier per
 //     block: behind it everybody's part of this block has arrived and everybody is done with the other.
 //   * A row takes one 16-byte piece more than it has: rows then start 16 bytes apart in the banks, and the sixteen rows of a key operand are read
 //     without conflicts.
+// Bound at 576 channels by what a wavefront issues and its reads of LDS, not by memory: 64 sequences of 2048 tokens, 128 heads, bf16, 103 us for 302 MB
+// (2.9 TB/s) and 38.7 GFLOP x 2 (740 TFLOP/s of the 1127 that a large product reaches); a block's 108 matrix instructions take 1730 of its 4600 clocks.
+// Workgroups of two and eight tiles were slower or no faster (B x heads, bf16, lengths of 8192): 32 x 128 of 256: 175 us with two, 96 with four, 114 with
+// eight; 32 x 128 of 128: 109, 57, 57; 32 x 32 of 576, where half of four tiles are empty: 135, 126.
 #pragma once
 
 #include <type_traits>
@@ -16,6 +22,8 @@
 #include "tq_exact_impl.h"
 
 namespace tq {
+
+constexpr int HEADS_TILES = 4;                      // wavefronts of a workgroup, a tile of sixteen heads each
 
 // lane l's 16 bytes land at m0 + 16 l.  The compiler sees neither the load nor its write to LDS: ex_arrived() waits for it.
 __device__ __forceinline__ void ex_to_lds(const void* from, uint32_t m0) {
@@ -50,8 +58,9 @@ __device__ __forceinline__ int ex_anew(int x) {
   return x;
 }
 
-template <int DT, int D, int TW>
-__global__ void __launch_bounds__(TW * 64, TW == 8 || D <= 256 ? 2 : 1) exact_heads_kernel(const ExactDecode a) {
+template <int DT, int D>
+__global__ void __launch_bounds__(HEADS_TILES * 64, D <= 256 ? 2 : 1) exact_heads_kernel(const ExactDecode a) {
+  constexpr int TW = HEADS_TILES;
   using Lds = HeadsLds<D>;
   constexpr int KSTEPS = D / 32, TILES = D / 16, WIDE = Lds::WIDE, NARROW = (D - WIDE * 128) / 64;
   constexpr int KROW = Lds::KROW, VROW = Lds::VROW, LOADS = Lds::LOADS, TURN = Lds::KBYTES + Lds::VBYTES;
@@ -288,27 +297,21 @@ __global__ void __launch_bounds__(TW * 64, TW == 8 || D <= 256 ? 2 : 1) exact_he
 }
 
 template <int DT>
-int launch_exact_heads(const ExactDecode& a, int tw, hipStream_t stream) {
-  const dim3 grid((unsigned)exact_grid(a)), block(tw * 64);
-#define TQ_HEADS_TW(D, TW)                                                                                                  \
-  {                                                                                                                         \
-    const auto kern = exact_heads_kernel<DT, D, TW>;                                                                        \
-    static std::atomic<uint64_t> ready{0};                                                                                  \
-    if (const int rc = exact_allow_lds((const void*)kern, HeadsLds<D>::BYTES, ready)) return rc;                                  \
-    kern<<<grid, block, HeadsLds<D>::BYTES, stream>>>(a);                                                                         \
-    break;                                                                                                                  \
+int launch_exact_heads(const ExactDecode& a, hipStream_t stream) {
+  const dim3 grid((unsigned)exact_grid(a)), block(HEADS_TILES * 64);
+#define TQ_HEADS_D(D)                                                                                       \
+  case D: {                                                                                                 \
+    const auto kern = exact_heads_kernel<DT, D>;                                                            \
+    static std::atomic<uint64_t> ready{0};                                                                  \
+    if (const int rc = exact_allow_lds((const void*)kern, HeadsLds<D>::BYTES, ready)) return rc;            \
+    kern<<<grid, block, HeadsLds<D>::BYTES, stream>>>(a);                                                   \
+    break;                                                                                                  \
   }
-#define TQ_HEADS_D(D)                                                                 \
-  case D:                                                                             \
-    if constexpr (D <= 256) if (tw == 8) TQ_HEADS_TW(D, 8)                            \
-    if (tw == 4) TQ_HEADS_TW(D, 4)                                                    \
-    TQ_HEADS_TW(D, 2)
   switch (a.c.d) {
     TQ_HEADS_D(64) TQ_HEADS_D(128) TQ_HEADS_D(192) TQ_HEADS_D(256) TQ_HEADS_D(320) TQ_HEADS_D(384) TQ_HEADS_D(448) TQ_HEADS_D(512) TQ_HEADS_D(576)
     default: return TQ_EUNSUPPORTED;
   }
 #undef TQ_HEADS_D
-#undef TQ_HEADS_TW
   TQ_CHECK_LAUNCH();
   return TQ_OK;
 }
