@@ -250,7 +250,7 @@ def test_refusals(gpu):
     ok = lambda **kw: select_evictions(**{**dict(weights=w, positions=pos, seq_lens=lens, budget=20), **kw})
     e = ok()
     both = torch.zeros(2, 2, 80, device=gpu)
-    for bad, error in ((dict(budget=0), ValueError), (dict(sinks=-1), ValueError), (dict(recent=-1), ValueError), (dict(sinks=10, recent=11), ValueError),
+    for bad, error in ((dict(budget=0), ValueError), (dict(budget=2 ** 32 + 5), ValueError), (dict(sinks=-1), ValueError), (dict(recent=-1), ValueError), (dict(sinks=10, recent=11), ValueError),
                        (dict(weights=w.cpu()), RuntimeError), (dict(positions=pos.cpu()), RuntimeError), (dict(weights=w[0]), ValueError),
                        (dict(positions=pos[..., :39]), ValueError), (dict(weights=w.double()), TypeError), (dict(positions=pos.long()), TypeError),
                        (dict(seq_lens=lens[:1]), ValueError), (dict(seen=lens[:1]), ValueError), (dict(out=(w, pos[..., :39])), ValueError),
@@ -272,6 +272,10 @@ def test_refusals(gpu):
         cache.move_tokens(e, seqs.table.cpu())
     with pytest.raises(ValueError):
         ExactPagedCache.from_engine(seqs.kv[:, :, :, :1]).move_tokens(e, seqs.table)
+    for bad in (e._replace(src=e.src[..., :1]), e._replace(dst=e.dst.long()), e._replace(count=e.count[:1]),
+                e._replace(dst=e.dst[..., ::2], src=e.src[..., ::2])):
+        with pytest.raises(ValueError):
+            cache.move_tokens(bad, seqs.table)
     none = select_evictions(w[:0], pos[:0], lens[:0], 20)
     assert none.lens.shape == (0,)
     cache.move_tokens(none, seqs.table[:0])

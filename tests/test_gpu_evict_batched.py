@@ -123,6 +123,29 @@ def test_a_chunked_prompt_adds_up(gpu):
     assert torch.allclose(s.weights.sum(-1).cpu(), torch.tensor([13.0, 16.0, 16.0])[:, None].expand(3, 2) * 4, rtol=1e-4)
 
 
+def test_a_captured_step_adds_weights_and_ends_with_a_cut(gpu):
+    eager, captured = (runner(gpu, exact_layers=3, mode="full_tq") for _ in range(2))
+    for r in (eager, captured):
+        track_weights(r, 3, 192, window=16)
+        prompt(r, [50, 12, 90])
+    t = torch.tensor([1, 2, 3], device=gpu)
+    replay, first = captured.capture_decode_step(190, t)
+    assert near(first, eager.decode_step(t))
+    for step in range(3):
+        t = torch.tensor([step, 9, 40 * step], device=gpu)
+        assert near(replay(t), eager.decode_step(t)), step
+        assert captured.seq_lens == eager.seq_lens
+        for r in (eager, captured):
+            for s in r._tq_layer_states.values():
+                given = s.weights.sum(-1).cpu()               # every query so far gave 1 per head
+                assert torch.allclose(given, torch.tensor([18.0 + step, 14.0 + step, 18.0 + step])[:, None].expand(3, 2) * 4, rtol=1e-4)
+    captured.evict(48, sinks=4, recent=16)
+    with pytest.raises(RuntimeError, match="cut"):
+        replay(t)
+    with pytest.raises(RuntimeError, match="cut"):
+        captured.capture_decode_step(190, t)
+
+
 def test_refusals(gpu):
     with pytest.raises(ValueError):
         runner(gpu, exact_layers=1, no_alloc=True, mode="full_tq")

@@ -293,7 +293,8 @@ def test_refusals(gpu):
                        (dict(block_table=seqs.table[:1]), ValueError), (dict(block_table=seqs.table.cpu()), RuntimeError),
                        (dict(block_table=seqs.table[:, :0]), ValueError), (dict(seq_lens=seqs.seq_lens[:1]), ValueError),
                        (dict(n_split=-1), ValueError), (dict(n_split=1025), ValueError), (dict(max_len=-1), ValueError),
-                       (dict(out=q[:, :2]), ValueError), (dict(out=q.float()), ValueError),
+                       (dict(out=q[:, :2]), ValueError), (dict(out=q.float()), ValueError), (dict(out=torch._neg_view(q.clone())), ValueError),
+                       (dict(out=q.clone().requires_grad_()), RuntimeError),
                        (dict(weights=torch.zeros(2, 2, 40, device=gpu, dtype=torch.float64)), TypeError),
                        (dict(weights=torch.zeros(2, 3, 40, device=gpu)), ValueError), (dict(weights=torch.zeros(2, 2, 40)), RuntimeError),
                        (dict(weights=torch.zeros(2, 2, 80, device=gpu)[..., ::2]), ValueError),

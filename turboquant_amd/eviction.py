@@ -34,8 +34,11 @@ class Evictions(NamedTuple):
         if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] == 0:
             raise ValueError(f"block_table must be int32 ({B}, max_pages)")
         _ffi.require_gpu(block_table, "block_table")
-        if block_table.device != device or self.dst.device != device:
+        if block_table.device != device or any(t.device != device for t in (self.count, self.dst, self.src)):
             raise ValueError(f"the cache lives on {device}, the evictions on {self.dst.device}, block_table on {block_table.device}")
+        if self.src.shape != self.dst.shape or self.count.shape != (B, H) or any(
+                t.dtype != torch.int32 or not t.is_contiguous() or t.is_neg() for t in (self.count, self.dst, self.src)):
+            raise ValueError("count (B, H), dst and src (B, H, n) must be contiguous int32, as select_evictions gives them")
         table = block_table.contiguous().resolve_neg()
         return self.count, self.dst, self.src, table, table.shape[1]
 
@@ -61,7 +64,7 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
     """Cut every sequence to `budget` tokens, per KV head.
 
     weights (B, H, L) float32 and positions (B, H, L) int32 say of every slot how much weight its token has had and where in the
-    sequence it stood; seq_lens (B,) slots are in use, seen (B,) tokens the sequence has had in all (None: seq_lens, nothing
+    sequence it stood; seq_lens (B,) slots are in use (L of them at most), seen (B,) tokens the sequence has had in all (None: seq_lens, nothing
     was cut before).  The first `sinks` positions and the newest `recent` always stay (sinks + recent <= budget); of the others
     the heaviest, of two alike the one in the lower slot; a NaN counts as less than everything.  Sequences within the budget
     stay as they are.
@@ -85,8 +88,8 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
     if positions.device != dev:
         raise ValueError(f"weights live on {dev}, positions on {positions.device}")
     budget, sinks, recent = int(budget), int(sinks), int(recent)
-    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
-        raise ValueError(f"need 1 <= budget and sinks + recent <= budget, got budget {budget}, sinks {sinks}, recent {recent}")
+    if not 1 <= budget < 1 << 31 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError(f"need 1 <= budget < 2^31 and sinks + recent <= budget, got budget {budget}, sinks {sinks}, recent {recent}")
     for name, t in (("seq_lens", seq_lens), ("seen", seen)):
         if t is not None and t.shape != (B,):
             raise ValueError(f"{name} must have one entry for each of {B} sequences")

@@ -130,6 +130,10 @@ class ExactPagedCache:
         elif (out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or not out.is_contiguous() or
               out.data_ptr() % 16):
             raise ValueError("out must be like the query: contiguous, same shape, dtype and GPU")
+        elif out.is_neg():
+            raise ValueError("out is negated lazily: its memory does not hold its values")
+        else:
+            _require_plain(out, "out")
         w_ptr, w_b, w_h, w_len = None, 0, 0, 0
         if weights is not None:
             self._weights(weights, B)
@@ -150,6 +154,7 @@ class ExactPagedCache:
                 *self._strides[:3], self.num_blocks, table.data_ptr(), bt_stride, lens.data_ptr(), float(scale), int(max_len),
                 w_ptr, w_b, w_h, w_len, out.data_ptr(), workspace.data_ptr(), splits, _ffi.stream_ptr(self.device)),
                 "tq_exact_decode")
+        _ffi.changed(out)
         if weights is not None:
             _ffi.changed(weights)
         return out

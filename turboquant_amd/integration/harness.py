@@ -260,6 +260,8 @@ class MinimalRunner:
         state = {"steps": 1, "keep": (lens, meta, body)}
 
         def replay(new_tokens: torch.Tensor) -> torch.Tensor:
+            if any(self.evicted):
+                raise RuntimeError("the sequences have been cut since: the graph goes on with the lengths they had")
             tokens.copy_(new_tokens)
             graph.replay()
             state["steps"] += 1
