@@ -14,6 +14,12 @@
 //   softmax   one pass: running maximum and sum per head; a lane's accumulators all belong to its head, so a move of the maximum is a
 //             scalar of the lane.  Maximum, sum, scores and numerators are fp32; the weights are rounded to the cache's 16-bit type for the
 //             product (relative 2^-8 / 2^-11 at most, the size of the output's own rounding, and independent from token to token).
+// Bound by the memory system.  bf16, 16 sequences of 8192, 32 query on 8 KV heads of 128: 117 us for 546 MB, 4.7 TB/s where a large read reaches 5.4; one of
+// 131072, 16 on 2 heads of 256: 60 us, 4.5 TB/s; fp16, 96 of 61 .. 8190, 40 on 8 heads of 128: 145 - 155 us, 4.4 - 4.7 TB/s, the rest the ends of short
+// sequences; fp32, 8 of 1500 .. 2048, 16 heads of 64: 28 us, 4.2 TB/s.  One of 700 tokens: 5.4 us, a launch and four latencies one behind another (length,
+// table entry, keys and values, the join of the four wavefronts).
+// Registers before LDS: with the next block's keys and values on their way in registers a wavefront needs no barrier; with table entries read behind
+// a condition the compiler waited for them at once, and with them for the block on its way.
 // Tokens behind the length and those of a block number outside the cache have no weight; what lies in their slots is not used in any
 // product, so that NaN left there stays there.
 #pragma once
