@@ -122,22 +122,25 @@ __global__ void __launch_bounds__(WAVES * 64, window_waves_per_simd(DT, D, WAVES
       float mx[NT], sm[NT];                                  // first pass: maximum (unscaled) and sum; second: maximum (log2) and 1 / sum of the row
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int r = (tile0 + t) * 16 + col;
-        const bool live = r < n_rows;
-        const int w = live ? r / a.G : 0, g = r - w * a.G;
-        mx[t] = ADD ? 0.0f : -INFINITY;
+        // (a row behind the last is the last one over again, whose scores are hidden: behind a condition every load would be waited for by itself)
+        const int row = (tile0 + t) * 16 + col, r = row < n_rows ? row : n_rows - 1;
+        const int w = r / a.G, g = r - w * a.G;
+        mx[t] = -INFINITY;
         sm[t] = 0.0f;
-        if (ADD && live) {
+        if constexpr (ADD) {
           const float2 st = a.stat[row_at * padded + r];
           mx[t] = st.x;
           sm[t] = st.y;
         }
+        const char* from = (const char*)a.q + (((r1 - W + w) * a.Hq + h * a.G + g) * D) * SIZE + quarter * 16;
 #pragma unroll
-        for (int s = 0; s < KSTEPS; ++s) {
-          Q[t][s] = ex_u32x4{0, 0, 0, 0};
-          if (live) Q[t][s] = *(const ex_u32x4*)((const char*)a.q + (((r1 - W + w) * a.Hq + h * a.G + g) * D) * SIZE + s * 64 + quarter * 16);
-          Q[t][s] ^= a.flip;                                 // (a negative scale is the queries')
-        }
+        for (int s = 0; s < KSTEPS; ++s) Q[t][s] = *(const ex_u32x4*)(from + s * 64);
+      }
+      if (a.flip) {                                          // (a negative scale is the queries')
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int s = 0; s < KSTEPS; ++s) Q[t][s] ^= a.flip;
       }
       const bool full_tiles = (tile0 + NT) * 16 <= n_rows;
       for (int turn0 = sub, turn = 0; turn0 < sub_end; turn0 += token_waves, turn ^= 1) {
