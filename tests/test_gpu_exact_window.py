@@ -44,6 +44,15 @@ def test_rows_from_one_to_hundreds(gpu, heads, H, window, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("d,heads,H,window", [(64, 24, 1, 40), (128, 24, 1, 33), (192, 7, 1, 100), (256, 16, 2, 64), (256, 5, 1, 77), (256, 1, 1, 300), (320, 40, 1, 16)])
+def test_hundreds_of_rows_in_wide_workgroups(gpu, d, heads, H, window, dtype):
+    """Windows that some sequences fill, one has a part of, and one a single row of; a negative scale; hidden tokens in most blocks."""
+    seqs = Sequences([350, 90, 33, 1], H, d, DTYPES[dtype], seed=heads)
+    case(seqs, [310, 90, 1, 1], heads, window)
+    case(seqs, [350, 20, 33, 0], heads, window, scale=-0.2)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("n", [1, 16, 31, 32, 33, 129, 1023, 1024, 1025, 2100, 5000])
 def test_lengths(gpu, n, dtype):
     seqs = Sequences([n, max(0, n - 16)], 1, 64, DTYPES[dtype], seed=n)

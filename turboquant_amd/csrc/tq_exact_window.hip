@@ -97,6 +97,7 @@ extern "C" int tq_exact_window(const void* q, int dtype, int64_t rows, const int
   a.scale2 = std::max(std::fabs(sm_scale) * 1.4426950408889634f, 1.17549435e-38f);
   a.flip = std::signbit(sm_scale) ? (dtype == TQ_F32 ? 0x80000000u : 0x80008000u) : 0u;
   a.waves = p.waves;
+  a.per_head = (uint32_t)(((uint64_t)1 << 32) / (uint32_t)a.G + ((((uint64_t)1 << 32) % (uint32_t)a.G) != 0));
   a.ml = (float2*)((char*)workspace + p.ml_at);
   a.stat = (float2*)((char*)workspace + p.stat_at);
   a.weights = weights; a.w_b = w_b; a.w_h = w_h; a.L = (int)weight_len;

@@ -9,7 +9,7 @@
 // wavefronts of a workgroup stand side by side on the tiles, and, with few of those, on the tokens.  Keys lie in LDS twice, filled by LDS-direct loads
 // a turn ahead: read from memory as operands, they came from the L1 once for every wavefront, 16 lines of 64 bytes a load, and that was the bound.
 // Bound by reads of LDS, matrix instructions and the exponentials in turn: bf16, four sequences of 32768, 32 / 8 heads of 128, 32 queries: 66 us the first pass,
-// 5 the join, 68 the second; a pass is 268 MB (4.0 TB/s) and 34 GFLOP (520 TFLOP/s).  fp16, nine of 17 .. 4099, 16 / 2 heads of 256, 64 queries: 22 + 5 + 24 us
+// 5 the join, 68 the second; a pass is 268 MB (4.0 TB/s) and 34 GFLOP (520 TFLOP/s).  fp16, nine of 17 .. 4099, 16 / 2 heads of 256, 64 queries: 20 + 5 + 20 us
 // for 13 MB: the longest sequence's workgroups.  One of 1500: 7.1 + 3.5 + 8.4 us, three launches of latencies.
 // In the first pass a lane keeps maximum and sum of its own tokens (four of each sixteen) and joins them with the three other lanes of its
 // row at the end; in the second it sums its columns' weights of its tokens, over the tiles in registers, over lanes once per block.
@@ -122,25 +122,47 @@ __global__ void __launch_bounds__(WAVES * 64, window_waves_per_simd(DT, D, WAVES
       float mx[NT], sm[NT];                                  // first pass: maximum (unscaled) and sum; second: maximum (log2) and 1 / sum of the row
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        // (a row behind the last is the last one over again, whose scores are hidden: behind a condition every load would be waited for by itself)
-        const int row = (tile0 + t) * 16 + col, r = row < n_rows ? row : n_rows - 1;
-        const int w = r / a.G, g = r - w * a.G;
-        mx[t] = -INFINITY;
+        const int r = (tile0 + t) * 16 + col;
+        const bool live = r < n_rows;
+        mx[t] = ADD ? 0.0f : -INFINITY;
         sm[t] = 0.0f;
-        if constexpr (ADD) {
+        if (ADD && live) {
           const float2 st = a.stat[row_at * padded + r];
           mx[t] = st.x;
           sm[t] = st.y;
         }
-        const char* from = (const char*)a.q + (((r1 - W + w) * a.Hq + h * a.G + g) * D) * SIZE + quarter * 16;
+        if constexpr (window_staged(DT, D, WAVES)) {
+          if (a.tile_waves == a.waves) {
+            // A tile's rows by way of LDS, a wavefront for itself; offsets from the tile's first row.  (A row behind the last is the last one over again: its
+            // scores are hidden.)
+            const int row0 = (tile0 + t) * 16 < n_rows ? (tile0 + t) * 16 : n_rows - 1, w0 = row0 / a.G;
+            const char* base = (const char*)a.q + (((r1 - W + w0) * a.Hq + h * a.G + (row0 - w0 * a.G)) * D) * SIZE;
+            const uint32_t row_bytes = D * SIZE, turn_bytes = (uint32_t)(a.Hq - a.G) * row_bytes;
+            const uint32_t to = lds0 + (uint32_t)(2 * BLOCK + wave * 16 * D * SIZE);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // (the tile before has been read)
 #pragma unroll
-        for (int s = 0; s < KSTEPS; ++s) Q[t][s] = *(const ex_u32x4*)(from + s * 64);
-      }
-      if (a.flip) {                                          // (a negative scale is the queries')
+            for (int n = 0; n < PIECES / 4; ++n) {
+              const int piece = n * 64 + lane, in = piece / PIECES, at = piece - in * PIECES;
+              const int rr = row0 + in < n_rows ? row0 + in : n_rows - 1;
+              const uint32_t turns = (a.G == 1 ? (uint32_t)rr : __umulhi((uint32_t)rr, a.per_head)) - (uint32_t)w0;
+              ex_row_to_lds(base, (uint32_t)(rr - row0) * row_bytes + turns * turn_bytes + (uint32_t)window_place<PIECES>(at, in) * 16, to + n * 1024);
+            }
+            ex_arrived();
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+            for (int s = 0; s < KSTEPS; ++s)
+              Q[t][s] = *(const ex_u32x4*)(s_keys + 2 * BLOCK + wave * 16 * D * SIZE + (col * PIECES + window_place<PIECES>(s * 4 + quarter, col)) * 16) ^ a.flip;
+            continue;
+          }
+        }
+        const int w = live ? r / a.G : 0, g = r - w * a.G;
 #pragma unroll
-          for (int s = 0; s < KSTEPS; ++s) Q[t][s] ^= a.flip;
+        for (int s = 0; s < KSTEPS; ++s) {
+          Q[t][s] = ex_u32x4{0, 0, 0, 0};
+          if (live) Q[t][s] = *(const ex_u32x4*)((const char*)a.q + (((r1 - W + w) * a.Hq + h * a.G + g) * D) * SIZE + s * 64 + quarter * 16);
+          // (a negative scale is the queries'; and with something done to them they have arrived before the loop: where it waited for them, it waited for the keys
+          // on their way, 65 -> 90 us)
+          Q[t][s] ^= a.flip;
+        }
       }
       const bool full_tiles = (tile0 + NT) * 16 <= n_rows;
       for (int turn0 = sub, turn = 0; turn0 < sub_end; turn0 += token_waves, turn ^= 1) {
@@ -262,7 +284,8 @@ __global__ void __launch_bounds__(WAVES * 64, window_waves_per_simd(DT, D, WAVES
 template <int DT>
 int launch_exact_window(const ExactWindow& a, bool add, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.n_split * (add ? 1 : a.row_groups) * a.c.H * a.B)), block(a.waves * 64);
-  const int lds = 2 * a.waves / a.tile_waves * window_block_bytes(a.c.d);
+  const int lds = 2 * a.waves / a.tile_waves * window_block_bytes(a.c.d) +
+                  (a.tile_waves == a.waves && window_staged(DT, a.c.d, a.waves) ? a.waves * window_tile_bytes(DT, a.c.d) : 0);
 #define TQ_WINDOW(D, WAVES, ADD)                                                                                            \
   {                                                                                                                         \
     const auto kern = exact_window_kernel<DT, D, WAVES, ADD>;                                                               \
