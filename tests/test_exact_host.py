@@ -65,7 +65,7 @@ def window_args(**kw):
     (dict(q=None), -3), (dict(starts=None), -3), (dict(weights=None), -3), (dict(k=None), -3), (dict(lens=None), -3), (dict(workspace=None), -3),
     (dict(window=0), -1), (dict(window=1025), -1), (dict(rows=-1), -1), (dict(Hq=7), -1), (dict(d=65), -1), (dict(weight_len=0), -1),
     (dict(w_h=-1), -1), (dict(max_len=-1), -1), (dict(bt_stride=0), -1), (dict(workspace=P + 8), -1), (dict(q=P + 8), -2), (dict(k=P + 4), -2),
-    (dict(cs_t=100), -2), (dict(dtype=7), -1),
+    (dict(cs_t=100), -2), (dict(dtype=7), -1), (dict(Hq=1 << 20, Hkv=1 << 12), -1),
 ])
 def test_window_refuses(bad, rc):
     assert _ffi.lib().tq_exact_window(*window_args(**bad)) == rc

@@ -42,6 +42,7 @@ struct WindowPlan {
 static bool window_plan(WindowPlan* p, int dtype, int B, int Hq, int Hkv, int d, int W, int64_t max_len) {
   if (dtype < TQ_F32 || dtype > TQ_BF16 || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || d <= 0 || d % 64 || d > 768) return false;
   if (W <= 0 || W > 1024 || max_len < 0 || max_len > INT32_MAX - 64 || Hq / Hkv > 1024) return false;
+  if ((int64_t)Hq * d > 1 << 25) return false;               // (sixteen rows of queries lie within 32 bits of each other)
   const int G = Hq / Hkv, NT = window_tiles(dtype, d);
   p->block_tokens = dtype == TQ_F32 ? 16 : 32;
   p->row_tiles = (W * G + 15) / 16;
