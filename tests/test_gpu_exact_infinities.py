@@ -34,3 +34,13 @@ def test_in_any_part_of_a_sequence(gpu, dtype, splits):
     for at in (0, 300, 599):
         out = infinite(gpu, dtype, 64, 4, at, torch.full((64,), at), n_split=splits)
         assert (out == math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d,heads,bound", [(64, 4, 600), (128, 48, 1 << 21), (576, 100, 1 << 21)])
+def test_whatever_its_weight(gpu, dtype, d, heads, bound):
+    """A weight goes into the product as two 16-bit numbers: neither may be zero or negative, for weights that the type holds as for others."""
+    for seed in range(4):
+        where = torch.randint(0, 600, (d,), generator=torch.Generator().manual_seed(9 + seed))
+        where[0] = 0
+        assert (infinite(gpu, dtype, d, heads, seed, where, max_len=bound) == math.inf).all()

@@ -243,11 +243,16 @@ __global__ void __launch_bounds__(HEADS_TILES * 64, D <= 256 ? 2 : 1) exact_head
         pr[p][i] = __builtin_amdgcn_exp2f(pr[p][i] - ref);
         l += pr[p][i];
       }
-    ex_u32x4 P;
+    ex_u32x4 P, L;                                           // high and low halves
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) P[p * 2 + i] = ex_pack<DT>(pr[p][2 * i], pr[p][2 * i + 1]);
+      for (int i = 0; i < 2; ++i) {
+        uint32_t hi, lo;
+        ex_split<DT>(pr[p][2 * i], pr[p][2 * i + 1], &hi, &lo);
+        P[p * 2 + i] = hi;
+        L[p * 2 + i] = lo;
+      }
     // ---- values ----
     ex_u32x2 y[8];
 #pragma unroll
@@ -266,7 +271,7 @@ __global__ void __launch_bounds__(HEADS_TILES * 64, D <= 256 ? 2 : 1) exact_head
         ex_u32x4 f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = __builtin_amdgcn_perm(v[2 * j + 1][t >> 1], v[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
-        O[c * 8 + t] = ex_mfma<DT>(f, P, O[c * 8 + t]);
+        O[c * 8 + t] = ex_mfma<DT>(f, P, ex_mfma<DT>(f, L, O[c * 8 + t]));
         load_ahead(N + c * 8 + t);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -281,7 +286,7 @@ __global__ void __launch_bounds__(HEADS_TILES * 64, D <= 256 ? 2 : 1) exact_head
         ex_u32x4 f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = __builtin_amdgcn_perm(y[2 * j + 1][t >> 1], y[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
-        O[WIDE * 8 + t] = ex_mfma<DT>(f, P, O[WIDE * 8 + t]);
+        O[WIDE * 8 + t] = ex_mfma<DT>(f, P, ex_mfma<DT>(f, L, O[WIDE * 8 + t]));
         load_ahead(N + WIDE * 8 + t);
       }
     }

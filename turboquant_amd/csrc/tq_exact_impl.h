@@ -12,8 +12,8 @@
 //             permutes a block of 128 channels); row r of channel tile t is channel 8 r + t, so the tiles need no exchange between lanes.
 //             fp32: a lane's four channels of a token are the row operands of four instructions as they are.
 //   softmax   one pass: running maximum and sum per head; a lane's accumulators all belong to its head, so a move of the maximum is a
-//             scalar of the lane.  Maximum, sum, scores and numerators are fp32; the weights are rounded to the cache's 16-bit type for the
-//             product (relative 2^-8 / 2^-11 at most, the size of the output's own rounding, and independent from token to token).
+//             scalar of the lane.  Maximum, sum, scores and numerators are fp32.  The matrix instruction takes 16-bit weights: they go in as two
+//             numbers, a high and a low half (ex_split), so that what is rounded away is 2^-15 (fp16: 2^-21) of a weight.
 // Bound by the memory system.  bf16, 16 sequences of 8192, 32 query on 8 KV heads of 128: 117 us for 546 MB, 4.7 TB/s where a large read reaches 5.4; one of
 // 131072, 16 on 2 heads of 256: 60 us, 4.5 TB/s; fp16, 96 of 61 .. 8190, 40 on 8 heads of 128: 145 - 155 us, 4.4 - 4.7 TB/s, the rest the ends of short
 // sequences; fp32, 8 of 1500 .. 2048, 16 heads of 64: 28 us, 4.2 TB/s.  One of 700 tokens: 5.4 us, a launch and four latencies one behind another (length,
@@ -54,6 +54,23 @@ __device__ __forceinline__ uint32_t ex_pack(float lo, float hi) {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
     const h2 r = {(_Float16)lo, (_Float16)hi};
     return __builtin_bit_cast(uint32_t, r);
+  }
+}
+
+// Two weights as the sum of two numbers each of the cache's type.  The high one is cut, never rounded up, and always less than the weight, so that the low one
+// is positive where the weight is: with a low part of zero, or one below zero, an infinite value would give NaN (0 x inf, inf - inf) where it has to give
+// infinity.  fp16: less by 2^-24 at least, below which a low part would be rounded to nothing.
+template <int DT>
+__device__ __forceinline__ void ex_split(float a, float b, uint32_t* hi, uint32_t* lo) {
+  if constexpr (DT == TQ_BF16) {
+    const uint32_t ua = __builtin_elementwise_sub_sat(__float_as_uint(a), 1u), ub = __builtin_elementwise_sub_sat(__float_as_uint(b), 1u);
+    *hi = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+    *lo = ex_pack<DT>(a - __uint_as_float(ua & 0xffff0000u), b - __uint_as_float(ub & 0xffff0000u));
+  } else {
+    constexpr float LESS = 1.0f - 0x1p-22f;
+    const auto h = __builtin_amdgcn_cvt_pkrtz(fmaxf(fmaf(a, LESS, -0x1p-24f), 0.0f), fmaxf(fmaf(b, LESS, -0x1p-24f), 0.0f));
+    *hi = __builtin_bit_cast(uint32_t, h);
+    *lo = ex_pack<DT>(a - (float)h[0], b - (float)h[1]);
   }
 }
 
@@ -316,11 +333,16 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
           for (int t = 0; t < 4; ++t) O[c * 4 + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(VF[c][i][t], pr[0][i], O[c * 4 + t], 0, 0, 0);
       }
     } else {
-      ex_u32x4 P;
+      ex_u32x4 P, L;                                         // high and low halves
 #pragma unroll
       for (int p = 0; p < PAGES; ++p)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) P[p * 2 + i] = ex_pack<DT>(pr[p][2 * i], pr[p][2 * i + 1]);
+        for (int i = 0; i < 2; ++i) {
+          uint32_t hi, lo;
+          ex_split<DT>(pr[p][2 * i], pr[p][2 * i + 1], &hi, &lo);
+          P[p * 2 + i] = hi;
+          L[p * 2 + i] = lo;
+        }
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) {
         if constexpr (!AHEAD) load_chunk(now, c);
@@ -335,7 +357,7 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             f[j] = __builtin_amdgcn_perm(V[c][2 * j + 1][t >> 1], V[c][2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
-          O[c * 8 + t] = ex_mfma<DT>(f, P, O[c * 8 + t]);
+          O[c * 8 + t] = ex_mfma<DT>(f, P, ex_mfma<DT>(f, L, O[c * 8 + t]));
         }
       }
       if constexpr (NARROW > 0) {
@@ -351,7 +373,7 @@ __global__ void __launch_bounds__(256, (exact_waves_per_simd<DT, D>())) exact_de
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             f[j] = __builtin_amdgcn_perm(VN[2 * j + 1][t >> 1], VN[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
-          O[WIDE * 8 + t] = ex_mfma<DT>(f, P, O[WIDE * 8 + t]);
+          O[WIDE * 8 + t] = ex_mfma<DT>(f, P, ex_mfma<DT>(f, L, O[WIDE * 8 + t]));
         }
       }
     }
