@@ -431,7 +431,7 @@ int tq_exact_window(const void *q, int dtype, int64_t rows, const int32_t *query
  * where they are.  weights / positions: fp32 / int32 (B, H, L), element (b, h, slot) at base + b*.._b + h*.._h + slot; seq_lens and seen
  * (tokens that a sequence has had in all; NULL: seq_lens) are device int32 (B,); lengths above L are cut to L.  1 <= budget, sinks + recent <= budget.
  * Written: lens_out (B,) = min(length, budget); count (B, H) moves; dst / src (B, H, moves) slots, ascending, -1 from count on, moves at
- * least max(1, min(budget, L - budget)); weights_out / positions_out (B, H, L), which may be the inputs themselves (same address and strides):
+ * least max(1, min(budget, L - budget)); L and moves up to 2^30; weights_out / positions_out (B, H, L), which may be the inputs themselves (same address and strides):
  * those of the tokens that stay, then 0 and the positions that the next tokens will have.  workspace: tq_evict_select_bytes bytes, 16-byte
  * aligned (0 bytes: not looked at), of this call alone until it has run.
  * tq_move_tokens_exact, tq_move_tokens_pool: carry the moves out in an exact cache (all strides in elements) / in the compressed pages of

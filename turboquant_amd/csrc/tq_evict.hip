@@ -501,7 +501,7 @@ static EvictPlan evict_plan(int64_t rows, int L, int budget, int moves) {
   const int64_t front = std::min(L, budget);
   p.below = (int)((front + PART - 1) / PART);
   p.parts = p.below + (int)((L - front + PART - 1) / PART);
-  p.shares = (int)(((int64_t)L + FINISH_SHARE - 1) / FINISH_SHARE);
+  p.shares = (int)(((int64_t)std::max(L, moves) + FINISH_SHARE - 1) / FINISH_SHARE);
   size_t at = 0;
   const auto take = [&](size_t n) { const size_t here = at; at = (at + n + 255) & ~(size_t)255; return here; };
   p.bins_at = take((size_t)3 * rows * p.parts * SEL_BINS * 4);
@@ -672,7 +672,7 @@ extern "C" int tq_evict_select(const float* weights, int64_t w_b, int64_t w_h, c
   if (!weights || !positions || !seq_lens || !lens_out || !count || !dst || !src || !weights_out || !positions_out) return TQ_ENULL;
   if (B < 0 || H <= 0 || L <= 0 || budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget) return TQ_EINVAL;
   if (w_b < 0 || w_h < 0 || p_b < 0 || p_h < 0 || wo_b < 0 || wo_h < 0 || po_b < 0 || po_h < 0 || L > (1 << 30)) return TQ_EINVAL;
-  if (moves < std::max(1, std::min(budget, L - budget)) || (int64_t)B * H > INT32_MAX) return TQ_EINVAL;
+  if (moves < std::max(1, std::min(budget, L - budget)) || moves > (1 << 30) || (int64_t)B * H > INT32_MAX) return TQ_EINVAL;
   if (B == 0) return TQ_OK;
   const EvictSelect a{weights, w_b, w_h, positions, p_b, p_h, seq_lens, seen, B, H, L, budget, sinks, recent, moves, lens_out, count, dst, src,
                       weights_out, wo_b, wo_h, positions_out, po_b, po_h};
