@@ -73,6 +73,7 @@ class BatchedLayerState:
     weights: Optional[torch.Tensor] = None                     # (B, H_kv, tokens): what every slot's token has been given so far
     positions: Optional[torch.Tensor] = None                   # (B, H_kv, tokens): where in the sequence it stood
     window: int = 0
+    blocks_current: bool = True                                # the engine's blocks hold a step's tokens before its attention: do_kv_cache_update
 
     @property
     def supports_hybrid(self) -> bool:
@@ -264,21 +265,27 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
     """Hook every standard attention layer of `model_runner` with a compressed pool of `num_blocks`
     16-token pages (the engine's block count); returns {layer name: BatchedLayerState}.  Bit widths are
     assigned as by `install_hooks` (integration/vllm.py:333-359).  The first `exact_layers` of them get no pool: their
-    decode steps are answered from the engine's cache.  Latent-attention layers are left alone."""
+    decode steps are answered from the engine's cache.  Latent-attention layers are left alone.  A layer can stay exact
+    only if its backend has do_kv_cache_update."""
     if exact_layers and no_alloc:
         raise ValueError("exact layers are answered from the engine's cache, which no_alloc leaves out")
-    _single.set_mode(mode)
-    if initial_layers_key_bits is None:
-        initial_layers_key_bits = min(key_bits + 1, 4)
-    states: Dict[str, BatchedLayerState] = {}
-    device = torch.device(model_runner.device)
-    idx = 0
+    layers = []
     for name, module in model_runner.compilation_config.static_forward_context.items():
         impl = getattr(module, "impl", None)
         if impl is None or getattr(impl, "num_kv_heads", None) is None or not hasattr(impl, "head_size"):
             continue
         if _is_mla_impl(impl):
             continue
+        if len(layers) < exact_layers and not hasattr(impl, "do_kv_cache_update"):
+            raise ValueError(f"{name} cannot stay exact: its backend has no do_kv_cache_update, so that only its forward(), which a decode step does "
+                             "not reach, would write the engine's cache")
+        layers.append((name, module, impl))
+    _single.set_mode(mode)
+    if initial_layers_key_bits is None:
+        initial_layers_key_bits = min(key_bits + 1, 4)
+    states: Dict[str, BatchedLayerState] = {}
+    device = torch.device(model_runner.device)
+    for idx, (name, module, impl) in enumerate(layers):
         head_dim = int(impl.head_size)
         cfg = LayerConfig(head_dim=head_dim, num_kv_heads=int(impl.num_kv_heads),
                           num_query_heads=_query_heads_of(module, impl),
@@ -290,16 +297,15 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
             tq = TurboQuantProd(head_dim, bits=cfg.key_bits, device=device, seed=42 + 7 * idx)
             pool = PagedKVPool(tq, cfg.num_kv_heads, num_blocks, value_bits=value_bits,
                                value_group_size=cfg.value_group_size, dtype=dtype, device=device)
-        state = BatchedLayerState(config=cfg, quantizer=tq, pool=pool)
-        states[name] = state
         has_update = hasattr(impl, "do_kv_cache_update")
+        state = BatchedLayerState(config=cfg, quantizer=tq, pool=pool, blocks_current=has_update)
+        states[name] = state
         hooks = _BatchedLayerHooks(state, _unbound(impl.forward),
                                    _unbound(impl.do_kv_cache_update) if has_update else None, no_alloc)
         if has_update:
             impl.do_kv_cache_update = _bind(impl, hooks.kv_update)
         impl.forward = _bind(impl, hooks.forward)
         impl._tq_layer_state = state
-        idx += 1
     model_runner._tq_layer_states = states
     model_runner._tq_no_alloc = no_alloc
     logger.info("[TurboQuant] Batched hooks on %d layers (mode=%s, no_alloc=%s)", len(states), mode, no_alloc)
@@ -313,6 +319,10 @@ def track_weights(model_runner, batch: int, max_len: int, window: int = 32) -> N
         raise ValueError("weights are summed over the engine's cache, which no_alloc leaves out")
     if not 1 <= window <= 1024:
         raise ValueError(f"window must be 1 .. 1024, got {window}")
+    for name, state in model_runner._tq_layer_states.items():
+        if not state.blocks_current:
+            raise ValueError(f"weights are summed over the engine's cache before a step's attention: {name}, whose backend has no do_kv_cache_update, "
+                             "writes it too late")
     for state in model_runner._tq_layer_states.values():
         state.track(batch, max_len, window)
 
