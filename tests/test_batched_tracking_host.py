@@ -46,6 +46,11 @@ def test_exact_layers_of_a_backend_that_writes_its_cache_in_forward(which):
     assert "do_kv_cache_update" in refused(r, exact_layers=2)
 
 
+@pytest.mark.parametrize("head_dim", [32, 96, 832])
+def test_exact_layers_of_a_head_size_that_the_exact_cache_does_not_take(head_dim):
+    assert "head_dim" in refused(runner(head_dim), exact_layers=2)
+
+
 def test_exact_layers_that_are_taken():
     r = runner()
     assert len(install_batched_hooks(r, r.num_blocks, mode="hybrid", exact_layers=2)) == 2

@@ -46,7 +46,7 @@ import torch.nn.functional as F
 
 from .. import _ffi
 from ..eviction import select_evictions
-from ..exact import ExactPagedCache
+from ..exact import MAX_HEAD_DIM, ExactPagedCache
 from ..paged import APPEND, PAGE_TOKENS, PagedKVPool
 from ..quantizer import TurboQuantProd
 from . import vllm as _single
@@ -266,7 +266,7 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
     16-token pages (the engine's block count); returns {layer name: BatchedLayerState}.  Bit widths are
     assigned as by `install_hooks` (integration/vllm.py:333-359).  The first `exact_layers` of them get no pool: their
     decode steps are answered from the engine's cache.  Latent-attention layers are left alone.  A layer can stay exact
-    only if its backend has do_kv_cache_update."""
+    only if its backend has do_kv_cache_update and its head size is a multiple of 64 up to 768."""
     if exact_layers and no_alloc:
         raise ValueError("exact layers are answered from the engine's cache, which no_alloc leaves out")
     layers = []
@@ -279,6 +279,8 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
         if len(layers) < exact_layers and not hasattr(impl, "do_kv_cache_update"):
             raise ValueError(f"{name} cannot stay exact: its backend has no do_kv_cache_update, so that only its forward(), which a decode step does "
                              "not reach, would write the engine's cache")
+        if len(layers) < exact_layers and (int(impl.head_size) % 64 or not 0 < int(impl.head_size) <= MAX_HEAD_DIM):
+            raise ValueError(f"{name} cannot stay exact: its head_dim {int(impl.head_size)} is no multiple of 64 up to {MAX_HEAD_DIM}")
         layers.append((name, module, impl))
     _single.set_mode(mode)
     if initial_layers_key_bits is None:
