@@ -82,3 +82,45 @@ def test_a_backend_that_writes_its_cache_in_forward_is_not_tracked(gpu):
         track_weights(r, 3, 192)
     assert all(s.weights is None for s in states(r))
     decode(r, 1, 2, 3)
+
+
+@pytest.mark.parametrize("exact", [0, 1, 2])
+def test_a_cut_that_is_refused_leaves_everything_as_it_was(gpu, exact):
+    r = runner(gpu, exact_layers=exact, mode="hybrid")
+    prompt(r, [90, 12, 150])
+    decode(r, 1, 2, 3)
+    lens, table = torch.tensor(r.seq_lens, dtype=torch.int32, device=gpu), r.block_table
+    kept = everything(r)
+    for bad in (table.long(), table.cpu(), table[0], table[:2], table[:, :0]):
+        with pytest.raises((ValueError, RuntimeError)):
+            evict_batched(r, bad, lens, 40)
+        with pytest.raises((ValueError, RuntimeError)):
+            states(r)[0].evict(bad, lens, 40, kv_cache=r.kv_caches[0])
+    for bad in (dict(seq_lens=lens[:2]), dict(seen=lens[:2]), dict(budget=0), dict(sinks=30, recent=30)):
+        with pytest.raises(ValueError):
+            evict_batched(r, table, **{**dict(seq_lens=lens, budget=40), **bad})
+    last = r.layers[-1].attn                                  # (of all layers the one that would be cut last)
+    whole = last.kv_cache
+    for bad in ([torch.zeros(2, r.num_blocks, 8, 2, 64, dtype=torch.bfloat16, device=gpu)], [torch.zeros(2, 4, 16, 3, 64, dtype=torch.bfloat16, device=gpu)]):
+        last.kv_cache = bad
+        with pytest.raises(ValueError):
+            evict_batched(r, table, lens, 40)
+    assert same(kept, everything(r))
+    last.kv_cache = whole
+    r.evict(40)
+    assert r.seq_lens == [40, 13, 40]
+
+
+def test_an_exact_layer_without_its_cache_is_not_cut(gpu):
+    r = runner(gpu, exact_layers=2, mode="hybrid")
+    prompt(r, [90, 12, 150])
+    lens, kept = torch.tensor(r.seq_lens, dtype=torch.int32, device=gpu), everything(r)
+    with pytest.raises(ValueError, match="exact layer"):
+        states(r)[0].evict(r.block_table, lens, 40)
+    for bad in (None, [], [None], [r.kv_caches[-1][0]]):
+        r.layers[-1].attn.kv_cache = bad
+        with pytest.raises(ValueError, match="exact layer"):
+            evict_batched(r, r.block_table, lens, 40)
+    assert same(kept, everything(r))
+    r.layers[-1].attn.kv_cache = r.kv_caches[-1]              # the tensor itself, not in a list
+    assert evict_batched(r, r.block_table, lens, 40).tolist() == [40, 12, 40]

@@ -16,6 +16,15 @@ import torch
 from . import _ffi
 
 
+def check_table(block_table: torch.Tensor, batch: int, device: torch.device) -> None:
+    """What moves need of the block table of `batch` sequences whose cache lives on `device`."""
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or block_table.shape[1] == 0:
+        raise ValueError(f"block_table must be int32 ({batch}, max_pages)")
+    _ffi.require_gpu(block_table, "block_table")
+    if block_table.device != device:
+        raise ValueError(f"the cache lives on {device}, block_table on {block_table.device}")
+
+
 class Evictions(NamedTuple):
     """What `select_evictions` decided, for B sequences and H KV heads."""
     lens: torch.Tensor          # (B,) int32: tokens that each sequence holds from now on
@@ -31,11 +40,9 @@ class Evictions(NamedTuple):
         B, H, _ = self.dst.shape
         if H != num_kv_heads:
             raise ValueError(f"evictions of {H} KV heads for a cache of {num_kv_heads}")
-        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] == 0:
-            raise ValueError(f"block_table must be int32 ({B}, max_pages)")
-        _ffi.require_gpu(block_table, "block_table")
-        if block_table.device != device or any(t.device != device for t in (self.count, self.dst, self.src)):
-            raise ValueError(f"the cache lives on {device}, the evictions on {self.dst.device}, block_table on {block_table.device}")
+        check_table(block_table, B, device)
+        if any(t.device != device for t in (self.count, self.dst, self.src)):
+            raise ValueError(f"the cache lives on {device}, the evictions on {self.dst.device}")
         if self.src.shape != self.dst.shape or self.count.shape != (B, H) or any(
                 t.dtype != torch.int32 or not t.is_contiguous() or t.is_neg() for t in (self.count, self.dst, self.src)):
             raise ValueError("count (B, H), dst and src (B, H, n) must be contiguous int32, as select_evictions gives them")

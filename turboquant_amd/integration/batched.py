@@ -45,7 +45,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import _ffi
-from ..eviction import select_evictions
+from ..eviction import check_table, select_evictions
 from ..exact import MAX_HEAD_DIM, ExactPagedCache
 from ..paged import APPEND, PAGE_TOKENS, PagedKVPool
 from ..quantizer import TurboQuantProd
@@ -172,16 +172,32 @@ class BatchedLayerState:
         ExactPagedCache.from_engine(kv_cache).add_window_weights(query, meta.query_start_loc, meta.block_table, meta.seq_lens, self.weights,
                                                                  window=self.window, scale=scale, max_len=getattr(meta, "max_seq_len", None))
 
-    def evict(self, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int, seen: Optional[torch.Tensor] = None, sinks: int = 4,
-              recent: int = 0, kv_cache: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Cut every sequence to `budget` tokens (`select_evictions`), in the engine's cache (2, num_blocks, 16, H_kv, d), if there is one, and in
-        this layer's pages; returns the lengths that are left."""
+    def prepare_cut(self, block_table: torch.Tensor, kv_cache: Optional[torch.Tensor] = None) -> Optional[ExactPagedCache]:
+        """The cache that moves are carried out in, and every check of them: a cut that would fail halfway is not begun."""
         if self.weights is None:
             raise RuntimeError("nothing has been tracked: track_weights comes first")
+        check_table(block_table, self.weights.shape[0], self.weights.device)
+        if kv_cache is None:
+            if self.pool is None:
+                raise ValueError("an exact layer is cut in the engine's cache, (2, num_blocks, 16, H_kv, d): there is none")
+            return None
+        cache = ExactPagedCache.from_engine(kv_cache)
+        if cache.num_kv_heads != self.config.num_kv_heads or cache.device != self.weights.device:
+            raise ValueError(f"a cache of {cache.num_kv_heads} KV heads on {cache.device} for a layer of {self.config.num_kv_heads} on {self.weights.device}")
+        return cache
+
+    def evict(self, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int, seen: Optional[torch.Tensor] = None, sinks: int = 4,
+              recent: int = 0, kv_cache: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Cut every sequence to `budget` tokens (`select_evictions`), in the engine's cache (2, num_blocks, 16, H_kv, d), if there is one (an exact layer
+        has nothing else), and in this layer's pages; returns the lengths that are left."""
+        return self.cut(self.prepare_cut(block_table, kv_cache), block_table, seq_lens, budget, seen, sinks, recent)
+
+    def cut(self, cache: Optional[ExactPagedCache], block_table, seq_lens, budget, seen, sinks, recent) -> torch.Tensor:
+        """`evict` behind its `prepare_cut`."""
         e = select_evictions(self.weights, self.positions, seq_lens, budget, seen=seen, sinks=sinks, recent=recent,
                              out=(self.weights, self.positions))
-        if kv_cache is not None:
-            ExactPagedCache.from_engine(kv_cache).move_tokens(e, block_table)
+        if cache is not None:
+            cache.move_tokens(e, block_table)
         if self.pool is not None:
             self.pool.move_tokens(e, block_table)
         return e.lens
@@ -335,11 +351,14 @@ def evict_batched(model_runner, block_table: torch.Tensor, seq_lens: torch.Tenso
     now.  seq_lens (B,) tokens held, seen (B,) tokens had in all (None: nothing was cut before).  Blocks behind the new lengths are the
     engine's to give away.  A sequence's blocks must be its own (no prefix shared with another)."""
     ctx = model_runner.compilation_config.static_forward_context
+    states, caches = model_runner._tq_layer_states, {}
+    for name, state in states.items():                         # of all layers, before the first is cut
+        held = getattr(ctx[name], "kv_cache", None)
+        cache = held if torch.is_tensor(held) else held[0] if held else None
+        caches[name] = state.prepare_cut(block_table, cache if torch.is_tensor(cache) and cache.dim() == 5 else None)
     lens = seq_lens
-    for name, state in model_runner._tq_layer_states.items():
-        caches = getattr(ctx[name], "kv_cache", None)
-        cache = caches[0] if caches and torch.is_tensor(caches[0]) and caches[0].dim() == 5 else None
-        lens = state.evict(block_table, seq_lens, budget, seen=seen, sinks=sinks, recent=recent, kv_cache=cache)
+    for name, state in states.items():
+        lens = state.cut(caches[name], block_table, seq_lens, budget, seen, sinks, recent)
     return lens
 
 
