@@ -434,6 +434,8 @@ int tq_exact_window(const void *q, int dtype, int64_t rows, const int32_t *query
  * least max(1, min(budget, L - budget)); L and moves up to 2^30; weights_out / positions_out (B, H, L), which may be the inputs themselves (same address and strides):
  * those of the tokens that stay, then 0 and the positions that the next tokens will have.  workspace: tq_evict_select_bytes bytes, 16-byte
  * aligned (0 bytes: not looked at), of this call alone until it has run.
+ * tq_evict_begin: rows of weights / positions (B, H, L) whose sequence begins in this step - as many query rows, query_start_loc[b + 1] - query_start_loc[b]
+ * (device, B + 1 entries), as tokens, seq_lens[b], and one at least - are set to weights 0 and positions 0 .. L - 1; the others are left alone.
  * tq_move_tokens_exact, tq_move_tokens_pool: carry the moves out in an exact cache (all strides in elements) / in the compressed pages of
  * the same block numbers (`budget`: the one of the selection).  A sequence's pages must be its own: tokens are overwritten in place.  Moves that
  * touch a page outside the table row or the cache are left out.                                                                   */
@@ -442,6 +444,8 @@ int tq_evict_select(const float *weights, int64_t w_b, int64_t w_h, const int32_
                     const int32_t *seq_lens, const int32_t *seen, int B, int H, int L, int budget, int sinks, int recent,
                     int moves, int32_t *lens_out, int32_t *count, int32_t *dst, int32_t *src, float *weights_out, int64_t wo_b,
                     int64_t wo_h, int32_t *positions_out, int64_t po_b, int64_t po_h, void *workspace, void *stream);
+int tq_evict_begin(float *weights, int64_t w_b, int64_t w_h, int32_t *positions, int64_t p_b, int64_t p_h, const int32_t *seq_lens,
+                   const int32_t *query_start_loc, int B, int H, int L, void *stream);
 int tq_move_tokens_exact(void *k_cache, void *v_cache, int dtype, int d, int64_t cs_blk, int64_t cs_t, int64_t cs_h,
                          int64_t num_blocks, const int32_t *block_table, int bt_stride, const int32_t *count, const int32_t *dst,
                          const int32_t *src, int B, int H, int moves, void *stream);

@@ -61,6 +61,103 @@ def same(a, b):
     return all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
 
 
+# ---- rows -------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("exact", [0, 2])
+def test_a_row_that_takes_another_sequence_starts_anew(gpu, exact):
+    r, fresh = (runner(gpu, exact_layers=exact, mode="hybrid") for _ in range(2))
+    prompt(r, [90, 12, 150])
+    decode(r, 1, 2, 3)
+    r.evict(40, sinks=2, recent=10)
+    others = [(s.weights.clone(), s.positions.clone()) for s in states(r)]
+    r.seq_lens[2] = r.evicted[2] = 0                          # the engine gives the row away
+    prompt(r, [0, 0, 70], seed=3), prompt(fresh, [0, 0, 70], seed=3)
+    for s, f, (w, p) in zip(states(r), states(fresh), others):
+        assert torch.equal(s.weights[2], f.weights[2]) and torch.equal(s.positions[2], f.positions[2])
+        assert torch.equal(s.weights[:2], w[:2]) and torch.equal(s.positions[:2], p[:2])
+    held, seen = list(r.seq_lens), [n + e for n, e in zip(r.seq_lens, r.evicted)]
+    want = [evict64(s.weights.cpu(), s.positions.cpu(), held, seen, 30, 2, 10) for s in states(r)]
+    r.evict(30, sinks=2, recent=10)
+    for s, w in zip(states(r), want):
+        assert torch.equal(s.weights.cpu(), w[4]) and torch.equal(s.positions.cpu(), w[5])
+        for head in s.positions[2].cpu():
+            assert {0, 1} | set(range(60, 70)) <= set(head[:30].tolist())
+
+
+def test_a_sequence_of_one_token_starts_anew_in_a_decode_step(gpu):
+    r = runner(gpu, exact_layers=2, mode="hybrid")
+    prompt(r, [90, 12, 150])
+    r.evict(40, sinks=2, recent=10)
+    r.seq_lens[1] = r.evicted[1] = 0
+    decode(r, 7, 8, 9)
+    for s in states(r):
+        assert (s.weights[1, :, 0] == G).all() and not s.weights[1, :, 1:].any()
+        assert torch.equal(s.positions[1].cpu(), torch.arange(192, dtype=torch.int32).expand(2, 192))
+
+
+def test_a_captured_step_starts_a_row_anew_too(gpu):
+    r = runner(gpu, exact_layers=2, mode="full_tq")
+    prompt(r, [20, 12, 30])
+    for s in states(r):                                       # what an earlier sequence of the row would have left
+        s.weights[1] = 5.0
+        s.positions[1] = 99
+    r.seq_lens[1] = 0
+    replay, _ = r.capture_decode_step(190, torch.tensor([1, 2, 3], device=gpu))
+    for step in range(3):
+        replay(torch.tensor([4, step, 6], device=gpu))
+        for s, got in zip(states(r), given(r)):
+            assert torch.allclose(got, per_row(18 + step, 2 + step, 18 + step), rtol=1e-4)
+            assert torch.equal(s.positions[1].cpu(), torch.arange(192, dtype=torch.int32).expand(2, 192))
+
+
+def test_rows_in_another_order(gpu):
+    a, b = (runner(gpu, exact_layers=1, mode="hybrid") for _ in range(2))
+    for r in (a, b):
+        prompt(r, [90, 12, 150])
+        decode(r, 1, 2, 3)
+        r.evict(40, sinks=2, recent=10)
+        decode(r, 1, 2, 3)
+    order = [2, 0, 1]
+    batched.reorder_rows(b, order)
+    b.block_table = b.block_table[order].contiguous()
+    b.seq_lens, b.evicted = [b.seq_lens[i] for i in order], [b.evicted[i] for i in order]
+    for s, t in zip(states(a), states(b)):
+        assert torch.equal(s.weights[order], t.weights) and torch.equal(s.positions[order], t.positions)
+    for r in (a, b):
+        r.evict(30, sinks=2, recent=10)
+    assert [a.seq_lens[i] for i in order] == b.seq_lens
+    for s, t in zip(states(a), states(b)):
+        assert torch.equal(s.weights[order], t.weights) and torch.equal(s.positions[order], t.positions)
+    assert same(a.kv_caches, b.kv_caches) and same([s.pool.data for s in states(a)[1:]], [s.pool.data for s in states(b)[1:]])
+    batched.reorder_rows(b, [1, -1, -1])
+    for s, t in zip(states(a), states(b)):
+        assert torch.equal(s.weights[0], t.weights[0]) and not t.weights[1:].any()       # (row 1 of [2, 0, 1] is a's row 0)
+        assert torch.equal(t.positions[1].cpu(), torch.arange(192, dtype=torch.int32).expand(2, 192))
+    kept = everything(b)
+    for bad in ([0, 1], [0, 0, 1], [0, 1, 3], [0, 1, -2]):
+        with pytest.raises(ValueError):
+            batched.reorder_rows(b, bad)
+    assert same(kept, everything(b))
+
+
+def test_steps_of_fewer_rows_than_are_tracked_and_of_more(gpu):
+    r, wide = runner(gpu, exact_layers=1, mode="hybrid"), runner(gpu, exact_layers=1, mode="hybrid", batch=5)
+    for x in (r, wide):
+        prompt(x, [90, 12, 150])
+        decode(x, 1, 2, 3)
+        x.evict(40, sinks=2, recent=10)
+        decode(x, 1, 2, 3)
+    assert r.seq_lens == wide.seq_lens
+    for s, t in zip(states(r), states(wide)):
+        assert torch.equal(s.weights, t.weights[:3]) and torch.equal(s.positions, t.positions[:3]) and not t.weights[3:].any()
+    narrow = runner(gpu, exact_layers=1, mode="hybrid", batch=2)
+    with pytest.raises(ValueError, match="rows"):
+        prompt(narrow, [90, 12, 150])
+    assert states(narrow)[0].tokens_written == 0 and not any(s.weights.any() for s in states(narrow))
+    with pytest.raises(ValueError):
+        evict_batched(narrow, narrow.block_table, torch.tensor([1, 1, 1], dtype=torch.int32, device=gpu), 40)
+
+
 # ---- what is refused --------------------------------------------------------------------------------------------------------
 
 def test_a_backend_that_writes_its_cache_in_forward_is_not_tracked(gpu):

@@ -117,6 +117,7 @@ _SIGNATURES = {
                                   _vp, _vp]),
     "tq_evict_select": (C.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp,
                                   _i64, _i64, _vp, _vp]),
+    "tq_evict_begin": (C.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i, _i, _i, _vp]),
     "tq_evict_select_bytes": (C.c_size_t, [_i, _i, _i, _i, _i]),
     "tq_move_tokens_exact": (C.c_int, [_vp, _vp, _i, _i, _i64, _i64, _i64, _i64, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "tq_move_tokens_pool": (C.c_int, [_vp, _i64, C.POINTER(TqPageLayout), _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),

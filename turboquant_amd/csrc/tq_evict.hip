@@ -513,6 +513,29 @@ static EvictPlan evict_plan(int64_t rows, int L, int budget, int moves) {
   return p;
 }
 
+// ---- rows of sequences that begin ----
+// As many query rows in this step as tokens: nothing was there before it.  Weights 0, positions from 0 on, whatever an earlier sequence of the row has left.
+// One launch in every step; where nothing begins a workgroup reads three numbers and ends.
+constexpr int BEGIN_SHARE = 4096;
+struct EvictBegin {
+  float* w;  int64_t w_b, w_h;
+  int32_t* pos;  int64_t p_b, p_h;
+  const int32_t *lens, *starts;
+  int32_t H, L, shares;
+};
+__global__ void __launch_bounds__(256) evict_begin_kernel(const EvictBegin a) {
+  const int share = (int)(blockIdx.x % (unsigned)a.shares), row = (int)(blockIdx.x / (unsigned)a.shares), h = row % a.H, b = row / a.H;
+  const int64_t run = (int64_t)a.starts[b + 1] - a.starts[b];
+  if (run <= 0 || run != a.lens[b]) return;
+  float* w = a.w + b * a.w_b + h * a.w_h;
+  int32_t* pos = a.pos + b * a.p_b + h * a.p_h;
+  const int end = a.L - share * BEGIN_SHARE < BEGIN_SHARE ? a.L : (share + 1) * BEGIN_SHARE;
+  for (int i = share * BEGIN_SHARE + (int)threadIdx.x; i < end; i += 256) {
+    w[i] = 0.0f;
+    pos[i] = i;
+  }
+}
+
 // ---- the moves ----------------------------------------------------------------------------------------------------------------------------
 
 struct MoveList {
@@ -704,6 +727,20 @@ extern "C" int tq_evict_select(const float* weights, int64_t w_b, int64_t w_h, c
   evict_part_kernel<3><<<grid, block, 0, st>>>(a, q);
   TQ_CHECK_LAUNCH();
   evict_finish_kernel<<<dim3((unsigned)(rows * p.shares)), dim3(256), 0, st>>>(a, q, p.shares);
+  TQ_CHECK_LAUNCH();
+  return TQ_OK;
+}
+
+extern "C" int tq_evict_begin(float* weights, int64_t w_b, int64_t w_h, int32_t* positions, int64_t p_b, int64_t p_h, const int32_t* seq_lens,
+                              const int32_t* query_start_loc, int B, int H, int L, void* stream) {
+  using namespace tq;
+  if (!weights || !positions || !seq_lens || !query_start_loc) return TQ_ENULL;
+  if (B < 0 || H <= 0 || L <= 0 || L > (1 << 30) || w_b < 0 || w_h < 0 || p_b < 0 || p_h < 0) return TQ_EINVAL;
+  const int shares = (L + BEGIN_SHARE - 1) / BEGIN_SHARE;
+  if ((int64_t)B * H > INT32_MAX || (int64_t)B * H * shares > INT32_MAX) return TQ_EINVAL;
+  if (B == 0) return TQ_OK;
+  const EvictBegin a{weights, w_b, w_h, positions, p_b, p_h, seq_lens, query_start_loc, H, L, shares};
+  evict_begin_kernel<<<dim3((unsigned)((int64_t)B * H * shares)), dim3(256), 0, (hipStream_t)stream>>>(a);
   TQ_CHECK_LAUNCH();
   return TQ_OK;
 }

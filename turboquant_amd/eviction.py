@@ -144,3 +144,35 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
     if out is not None:
         _ffi.changed(new_w, new_p)
     return got
+
+
+def begin_rows(weights: torch.Tensor, positions: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor) -> None:
+    """Set the rows whose sequence begins in this step - as many query rows (query_start_loc[b + 1] - query_start_loc[b]) as tokens (seq_lens[b]) - to weights 0
+    and positions from 0 on, in place: a row of an engine's batch goes from one sequence to the next.  weights and positions (B, H, L) as in
+    `select_evictions`; decided on the GPU, so that a captured step does it too."""
+    _ffi.require_gpu(weights, "weights")
+    _ffi.require_gpu(positions, "positions")
+    if weights.dim() != 3 or weights.shape != positions.shape or 0 in weights.shape[1:]:
+        raise ValueError("weights and positions must both be (B, H, L)")
+    if weights.dtype != torch.float32 or positions.dtype != torch.int32:
+        raise TypeError("weights must be float32 and positions int32")
+    B, H, L = weights.shape
+    dev = weights.device
+    if positions.device != dev:
+        raise ValueError(f"weights live on {dev}, positions on {positions.device}")
+    for name, t in (("weights", weights), ("positions", positions)):
+        if (t.stride(2) != 1 and L > 1) or t.is_neg() or not own_rows(t):
+            raise ValueError(f"{name} need contiguous slots, memory of their own and their values in it")
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise RuntimeError(f"{name} requires a gradient")
+    if seq_lens.shape != (B,) or query_start_loc.shape != (B + 1,):
+        raise ValueError(f"seq_lens and query_start_loc must have {B} and {B + 1} entries")
+    if B == 0:
+        return
+    lens = seq_lens.to(device=dev, dtype=torch.int32).contiguous().resolve_neg()
+    starts = query_start_loc.to(device=dev, dtype=torch.int32).contiguous().resolve_neg()
+    with _ffi.on_device(dev):
+        _ffi.check(_ffi.lib().tq_evict_begin(
+            weights.data_ptr(), weights.stride(0), weights.stride(1), positions.data_ptr(), positions.stride(0), positions.stride(1), lens.data_ptr(),
+            starts.data_ptr(), B, H, L, _ffi.stream_ptr(dev)), "tq_evict_begin")
+    _ffi.changed(weights, positions)

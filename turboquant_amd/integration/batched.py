@@ -45,7 +45,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import _ffi
-from ..eviction import check_table, select_evictions
+from ..eviction import begin_rows, check_table, select_evictions
 from ..exact import MAX_HEAD_DIM, ExactPagedCache
 from ..paged import APPEND, PAGE_TOKENS, PagedKVPool
 from ..quantizer import TurboQuantProd
@@ -85,6 +85,7 @@ class BatchedLayerState:
         """Quantise this step's tokens (n, H_kv, d) into the pages their sequences own."""
         cfg = self.config
         n = int(meta.num_actual_tokens)
+        self.check_step(meta)
         if self.pool is None:                                  # the engine's own cache has them
             self.tokens_written += n
             return
@@ -141,7 +142,8 @@ class BatchedLayerState:
         self.decode_steps += 1
         cfg = self.config
         if self.pool is None:
-            return ExactPagedCache.from_engine(kv_cache).decode_attention(query, meta.block_table, meta.seq_lens, scale=scale, weights=self.weights,
+            weights = None if self.weights is None else self.weights[: query.shape[0]]
+            return ExactPagedCache.from_engine(kv_cache).decode_attention(query, meta.block_table, meta.seq_lens, scale=scale, weights=weights,
                                                                           max_len=getattr(meta, "max_seq_len", None))
         if (hybrid and cfg.ring_capacity > 0 and torch.is_tensor(kv_cache) and kv_cache.dim() == 5 and
                 kv_cache.shape[0] == 2 and tuple(kv_cache.shape[2:]) == (PAGE_TOKENS, cfg.num_kv_heads, cfg.head_dim) and
@@ -161,22 +163,46 @@ class BatchedLayerState:
 
     # ---- eviction ------------------------------------------------------------------
     def track(self, batch: int, max_len: int, window: int) -> None:
-        """Sum weights from now on, for `batch` sequences (rows of the step's block table) of up to max_len tokens."""
+        """Sum weights from now on, for up to `batch` sequences (rows of the step's block table) of up to max_len tokens."""
         shape = (batch, self.config.num_kv_heads, max_len)
         self.weights = torch.zeros(shape, dtype=torch.float32, device=self.config.device)
         self.positions = torch.arange(max_len, dtype=torch.int32, device=self.config.device).expand(shape).contiguous()
         self.window = window
 
+    def check_step(self, meta) -> None:
+        """Whether what is tracked has room for this step."""
+        if self.weights is None:
+            return
+        rows = meta.seq_lens.shape[0]
+        if rows > self.weights.shape[0]:
+            raise ValueError(f"a step of {rows} rows where {self.weights.shape[0]} are tracked")
+
+    def begin(self, meta) -> None:
+        """Rows whose sequence begins in this step have had nothing."""
+        rows = meta.seq_lens.shape[0]
+        begin_rows(self.weights[:rows], self.positions[:rows], meta.seq_lens, meta.query_start_loc)
+
+    def reorder(self, order: torch.Tensor) -> None:
+        """Row i goes on with what row order[i] has had; -1: with nothing."""
+        none = order < 0
+        at = order.clamp_min(0)
+        fresh = torch.arange(self.positions.shape[2], dtype=torch.int32, device=self.positions.device)
+        self.weights.copy_(self.weights[at].masked_fill_(none[:, None, None], 0))
+        self.positions.copy_(torch.where(none[:, None, None], fresh, self.positions[at]))
+
     def observe(self, query: torch.Tensor, meta, kv_cache: torch.Tensor, scale: Optional[float] = None) -> None:
         """Add the weights that the newest queries of every sequence in this step give; query (rows, H_q, d)."""
-        ExactPagedCache.from_engine(kv_cache).add_window_weights(query, meta.query_start_loc, meta.block_table, meta.seq_lens, self.weights,
-                                                                 window=self.window, scale=scale, max_len=getattr(meta, "max_seq_len", None))
+        ExactPagedCache.from_engine(kv_cache).add_window_weights(query, meta.query_start_loc, meta.block_table, meta.seq_lens,
+                                                                 self.weights[: meta.seq_lens.shape[0]], window=self.window, scale=scale, max_len=getattr(meta, "max_seq_len", None))
 
     def prepare_cut(self, block_table: torch.Tensor, kv_cache: Optional[torch.Tensor] = None) -> Optional[ExactPagedCache]:
         """The cache that moves are carried out in, and every check of them: a cut that would fail halfway is not begun."""
         if self.weights is None:
             raise RuntimeError("nothing has been tracked: track_weights comes first")
-        check_table(block_table, self.weights.shape[0], self.weights.device)
+        rows = block_table.shape[0] if block_table.dim() else 0
+        if rows > self.weights.shape[0]:
+            raise ValueError(f"a cut of {rows} rows where {self.weights.shape[0]} are tracked")
+        check_table(block_table, rows, self.weights.device)
         if kv_cache is None:
             if self.pool is None:
                 raise ValueError("an exact layer is cut in the engine's cache, (2, num_blocks, 16, H_kv, d): there is none")
@@ -194,8 +220,8 @@ class BatchedLayerState:
 
     def cut(self, cache: Optional[ExactPagedCache], block_table, seq_lens, budget, seen, sinks, recent) -> torch.Tensor:
         """`evict` behind its `prepare_cut`."""
-        e = select_evictions(self.weights, self.positions, seq_lens, budget, seen=seen, sinks=sinks, recent=recent,
-                             out=(self.weights, self.positions))
+        held = self.weights[: block_table.shape[0]], self.positions[: block_table.shape[0]]
+        e = select_evictions(*held, seq_lens, budget, seen=seen, sinks=sinks, recent=recent, out=held)
         if cache is not None:
             cache.move_tokens(e, block_table)
         if self.pool is not None:
@@ -257,6 +283,8 @@ class _BatchedLayerHooks:
             return passthrough()
         self.state.write(key, value, attn_metadata)
         n = int(attn_metadata.num_actual_tokens)
+        if self.state.weights is not None:
+            self.state.begin(attn_metadata)
         if self.state.weights is not None and int(attn_metadata.max_query_len) > 1:
             cfg = self.state.config
             self.state.observe(query[:n].reshape(n, cfg.num_query_heads, cfg.head_dim), attn_metadata, kv_cache, getattr(impl, "scale", None))
@@ -331,8 +359,12 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
 
 
 def track_weights(model_runner, batch: int, max_len: int, window: int = 32) -> None:
-    """Have every hooked layer sum the attention weight of its tokens from now on: `batch` rows of the block table, up to max_len tokens each.  A
-    prompt step adds what its newest `window` queries give, read from the engine's cache; a decode step adds its own in exact layers."""
+    """Have every hooked layer sum the attention weight of its tokens from now on: up to `batch` rows of the block table, up to max_len tokens each.  A
+    prompt step adds what its newest `window` queries give, read from the engine's cache; a decode step adds its own in exact layers.
+
+    What is summed belongs to a row.  A row whose sequence begins in a step (all of its tokens are that step's) starts anew; an engine that
+    gives rows of sequences that go on to others - a batch closed up, two rows swapped, a sequence that begins behind tokens it did not compute - says so
+    with `reorder_rows` before the next step."""
     if getattr(model_runner, "_tq_no_alloc", False):
         raise ValueError("weights are summed over the engine's cache, which no_alloc leaves out")
     if not 1 <= window <= 1024:
@@ -343,6 +375,20 @@ def track_weights(model_runner, batch: int, max_len: int, window: int = 32) -> N
                              "writes it too late")
     for state in model_runner._tq_layer_states.values():
         state.track(batch, max_len, window)
+
+
+def reorder_rows(model_runner, order) -> None:
+    """The rows of the batch have changed places: row i is now what row order[i] was, or, with -1, a sequence of which nothing has been summed.  order has
+    an entry for each tracked row, none of them twice."""
+    states = list(model_runner._tq_layer_states.values())
+    if not states or any(s.weights is None for s in states):
+        raise RuntimeError("nothing has been tracked: track_weights comes first")
+    order = [int(i) for i in order]
+    rows, taken = states[0].weights.shape[0], [i for i in order if i >= 0]
+    if len(order) != rows or any(not -1 <= i < rows for i in order) or len(set(taken)) != len(taken):
+        raise ValueError(f"order must name each of {rows} rows once at most, or -1, got {order}")
+    for s in states:
+        s.reorder(torch.tensor(order, device=s.weights.device))
 
 
 def evict_batched(model_runner, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int, seen: Optional[torch.Tensor] = None,
