@@ -158,6 +158,29 @@ def test_steps_of_fewer_rows_than_are_tracked_and_of_more(gpu):
         evict_batched(narrow, narrow.block_table, torch.tensor([1, 1, 1], dtype=torch.int32, device=gpu), 40)
 
 
+# ---- lengths ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("exact", [0, 2])
+def test_a_sequence_that_outgrows_what_is_tracked_is_refused(gpu, exact):
+    r = runner(gpu, track=64, exact_layers=exact, mode="hybrid")
+    with pytest.raises(ValueError, match="64"):
+        prompt(r, [10, 12, 65])
+    assert states(r)[0].tokens_written == 0 and not any(s.weights.any() for s in states(r))
+    prompt(r, [10, 12, 63])
+    decode(r, 1, 2, 3)
+    kept = [t.clone() for s in states(r) for t in (s.weights, s.positions)]
+    with pytest.raises(ValueError, match="64"):
+        decode(r, 1, 2, 3)
+    lens = torch.tensor([11, 13, 65], dtype=torch.int32)
+    for bad in (dict(seq_lens=lens), dict(seq_lens=lens.to(gpu), max_len=65)):
+        with pytest.raises(ValueError, match="64"):
+            evict_batched(r, r.block_table, budget=20, **bad)
+    assert all(torch.equal(a, b) for a, b in zip(kept, [t for s in states(r) for t in (s.weights, s.positions)]))
+    r.evict(20)
+    assert r.seq_lens == [11, 13, 20]
+    decode(r, 1, 2, 3)
+
+
 # ---- what is refused --------------------------------------------------------------------------------------------------------
 
 def test_a_backend_that_writes_its_cache_in_forward_is_not_tracked(gpu):

@@ -176,6 +176,15 @@ class BatchedLayerState:
         rows = meta.seq_lens.shape[0]
         if rows > self.weights.shape[0]:
             raise ValueError(f"a step of {rows} rows where {self.weights.shape[0]} are tracked")
+        longest = getattr(meta, "max_seq_len", None)
+        if longest is None:                                    # (what the lengths may be, without waiting for the GPU)
+            lens = getattr(meta, "seq_lens_cpu", None)
+            longest = meta.block_table.shape[-1] * PAGE_TOKENS if lens is None else max((int(n) for n in lens), default=0)
+        self.check_length(int(longest))
+
+    def check_length(self, longest: int) -> None:
+        if longest > self.weights.shape[2]:
+            raise ValueError(f"a sequence of up to {longest} tokens where {self.weights.shape[2]} are tracked: the newest would have no weight and no position")
 
     def begin(self, meta) -> None:
         """Rows whose sequence begins in this step have had nothing."""
@@ -195,7 +204,8 @@ class BatchedLayerState:
         ExactPagedCache.from_engine(kv_cache).add_window_weights(query, meta.query_start_loc, meta.block_table, meta.seq_lens,
                                                                  self.weights[: meta.seq_lens.shape[0]], window=self.window, scale=scale, max_len=getattr(meta, "max_seq_len", None))
 
-    def prepare_cut(self, block_table: torch.Tensor, kv_cache: Optional[torch.Tensor] = None) -> Optional[ExactPagedCache]:
+    def prepare_cut(self, block_table: torch.Tensor, seq_lens: torch.Tensor, kv_cache: Optional[torch.Tensor] = None,
+                    max_len: Optional[int] = None) -> Optional[ExactPagedCache]:
         """The cache that moves are carried out in, and every check of them: a cut that would fail halfway is not begun."""
         if self.weights is None:
             raise RuntimeError("nothing has been tracked: track_weights comes first")
@@ -203,6 +213,10 @@ class BatchedLayerState:
         if rows > self.weights.shape[0]:
             raise ValueError(f"a cut of {rows} rows where {self.weights.shape[0]} are tracked")
         check_table(block_table, rows, self.weights.device)
+        if max_len is None and not seq_lens.is_cuda:
+            max_len = int(seq_lens.max()) if seq_lens.numel() else 0
+        if max_len is not None:                                # (lengths on the GPU are those of steps, each of which was checked)
+            self.check_length(int(max_len))
         if kv_cache is None:
             if self.pool is None:
                 raise ValueError("an exact layer is cut in the engine's cache, (2, num_blocks, 16, H_kv, d): there is none")
@@ -213,10 +227,11 @@ class BatchedLayerState:
         return cache
 
     def evict(self, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int, seen: Optional[torch.Tensor] = None, sinks: int = 4,
-              recent: int = 0, kv_cache: Optional[torch.Tensor] = None) -> torch.Tensor:
+              recent: int = 0, kv_cache: Optional[torch.Tensor] = None, max_len: Optional[int] = None) -> torch.Tensor:
         """Cut every sequence to `budget` tokens (`select_evictions`), in the engine's cache (2, num_blocks, 16, H_kv, d), if there is one (an exact layer
-        has nothing else), and in this layer's pages; returns the lengths that are left."""
-        return self.cut(self.prepare_cut(block_table, kv_cache), block_table, seq_lens, budget, seen, sinks, recent)
+        has nothing else), and in this layer's pages; returns the lengths that are left.  max_len: a bound on seq_lens, checked against what is
+        tracked without waiting for the GPU."""
+        return self.cut(self.prepare_cut(block_table, seq_lens, kv_cache, max_len), block_table, seq_lens, budget, seen, sinks, recent)
 
     def cut(self, cache: Optional[ExactPagedCache], block_table, seq_lens, budget, seen, sinks, recent) -> torch.Tensor:
         """`evict` behind its `prepare_cut`."""
@@ -359,8 +374,9 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
 
 
 def track_weights(model_runner, batch: int, max_len: int, window: int = 32) -> None:
-    """Have every hooked layer sum the attention weight of its tokens from now on: up to `batch` rows of the block table, up to max_len tokens each.  A
-    prompt step adds what its newest `window` queries give, read from the engine's cache; a decode step adds its own in exact layers.
+    """Have every hooked layer sum the attention weight of its tokens from now on: up to `batch` rows of the block table, up to max_len tokens each
+    (a step that may hold longer sequences is refused).  A prompt step adds what its newest `window` queries give, read from the engine's cache; a
+    decode step adds its own in exact layers.
 
     What is summed belongs to a row.  A row whose sequence begins in a step (all of its tokens are that step's) starts anew; an engine that
     gives rows of sequences that go on to others - a batch closed up, two rows swapped, a sequence that begins behind tokens it did not compute - says so
@@ -392,16 +408,17 @@ def reorder_rows(model_runner, order) -> None:
 
 
 def evict_batched(model_runner, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int, seen: Optional[torch.Tensor] = None,
-                  sinks: int = 4, recent: int = 0) -> torch.Tensor:
+                  sinks: int = 4, recent: int = 0, max_len: Optional[int] = None) -> torch.Tensor:
     """Cut every sequence to `budget` tokens in every hooked layer, each KV head by its own weights; returns the lengths (B,) that all layers have
     now.  seq_lens (B,) tokens held, seen (B,) tokens had in all (None: nothing was cut before).  Blocks behind the new lengths are the
-    engine's to give away.  A sequence's blocks must be its own (no prefix shared with another)."""
+    engine's to give away.  A sequence's blocks must be its own (no prefix shared with another).  max_len: a bound on
+    seq_lens; one beyond what is tracked is refused (so are lengths on the host, and steps that would lead there)."""
     ctx = model_runner.compilation_config.static_forward_context
     states, caches = model_runner._tq_layer_states, {}
     for name, state in states.items():                         # of all layers, before the first is cut
         held = getattr(ctx[name], "kv_cache", None)
         cache = held if torch.is_tensor(held) else held[0] if held else None
-        caches[name] = state.prepare_cut(block_table, cache if torch.is_tensor(cache) and cache.dim() == 5 else None)
+        caches[name] = state.prepare_cut(block_table, seq_lens, cache if torch.is_tensor(cache) and cache.dim() == 5 else None, max_len)
     lens = seq_lens
     for name, state in states.items():
         lens = state.cut(caches[name], block_table, seq_lens, budget, seen, sinks, recent)

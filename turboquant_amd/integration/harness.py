@@ -216,7 +216,8 @@ class MinimalRunner:
         from .batched import evict_batched
         lens = torch.tensor(self.seq_lens, dtype=torch.int32)
         seen = lens + torch.tensor(self.evicted, dtype=torch.int32)
-        left = evict_batched(self, self.block_table, lens.to(self.device), budget, seen=seen.to(self.device), sinks=sinks, recent=recent)
+        left = evict_batched(self, self.block_table, lens.to(self.device), budget, seen=seen.to(self.device), sinks=sinks, recent=recent,
+                             max_len=max(self.seq_lens))
         now = left.tolist()
         self.evicted = [e + n - m for e, n, m in zip(self.evicted, self.seq_lens, now)]
         self.seq_lens = now
