@@ -61,6 +61,28 @@ def same(a, b):
     return all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
 
 
+# ---- steps ------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("mode", ["capture_only", "hybrid", "full_tq"])
+def test_an_exact_layer_counts_every_step_in_every_mode(gpu, mode):
+    r = runner(gpu, exact_layers=2, mode=mode)
+    prompt(r, [50, 12, 90])
+    for step in range(3):
+        decode(r, step, 9, 4)
+    for got in given(r):
+        assert torch.allclose(got, per_row(19, 15, 19), rtol=1e-4)
+
+
+def test_capture_only_and_hybrid_sum_the_same(gpu):
+    a, b = (runner(gpu, exact_layers=2, mode=mode) for mode in ("capture_only", "hybrid"))
+    for r, mode in ((a, "capture_only"), (b, "hybrid")):
+        single.set_mode(mode)
+        prompt(r, [50, 12, 90])
+        decode(r, 1, 9, 4)
+    for s, t in zip(states(a)[:1], states(b)[:1]):           # (the first layer: what it is given does not depend on the mode)
+        assert torch.allclose(s.weights, t.weights, rtol=1e-5, atol=1e-7)
+
+
 # ---- rows -------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("exact", [0, 2])

@@ -300,9 +300,10 @@ class _BatchedLayerHooks:
         n = int(attn_metadata.num_actual_tokens)
         if self.state.weights is not None:
             self.state.begin(attn_metadata)
-        if self.state.weights is not None and int(attn_metadata.max_query_len) > 1:
-            cfg = self.state.config
-            self.state.observe(query[:n].reshape(n, cfg.num_query_heads, cfg.head_dim), attn_metadata, kv_cache, getattr(impl, "scale", None))
+            # (an exact layer's decode step adds its weights where it is answered below, unless the backend answers it)
+            if int(attn_metadata.max_query_len) > 1 or (self.state.pool is None and mode == MODE_CAPTURE_ONLY):
+                cfg = self.state.config
+                self.state.observe(query[:n].reshape(n, cfg.num_query_heads, cfg.head_dim), attn_metadata, kv_cache, getattr(impl, "scale", None))
         if mode == MODE_CAPTURE_ONLY:
             return passthrough()
         if int(attn_metadata.max_query_len) > 1:               # prefill (or a mixed step): exact attention
