@@ -83,6 +83,23 @@ def test_capture_only_and_hybrid_sum_the_same(gpu):
         assert torch.allclose(s.weights, t.weights, rtol=1e-5, atol=1e-7)
 
 
+@pytest.mark.parametrize("exact", [0, 2])
+def test_what_a_sequence_is_given_does_not_depend_on_the_others_in_its_step(gpu, exact):
+    """A decoding sequence beside another's prompt: its token counts as in a step of its own - in exact layers, not in compressed ones."""
+    r = runner(gpu, exact_layers=exact, mode="hybrid")
+    prompt(r, [50, 12, 0])
+    before = [s.weights.clone() for s in states(r)]
+    prompt(r, [1, 1, 30], seed=1)
+    decoded = 1 if exact else 0
+    for got, s, w in zip(given(r), states(r), before):
+        assert torch.allclose(got, per_row(16 + decoded, 12 + decoded, 16), rtol=1e-4)
+        if not exact:
+            assert torch.equal(s.weights[:2], w[:2])
+    decode(r, 1, 2, 3)
+    for got in given(r):
+        assert torch.allclose(got, per_row(16 + 2 * decoded, 12 + 2 * decoded, 16 + decoded), rtol=1e-4)
+
+
 # ---- rows -------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("exact", [0, 2])

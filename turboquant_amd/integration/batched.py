@@ -29,8 +29,8 @@ prefill steps).  Modes are those of `integration.vllm`:
                 when the engine's cache was never allocated (`no_alloc`)
 
 The first `exact_layers` layers may stay uncompressed: their decode steps are answered from the engine's paged cache, all of it exactly
-(`ExactPagedCache`).  And a cache may be cut: `track_weights` has every layer sum the attention weight that its tokens get - the newest
-`window` queries of every prompt step, and in exact layers every decode step -, and `evict_batched` keeps the sinks, the newest and the heaviest
+(`ExactPagedCache`).  And a cache may be cut: `track_weights` has every layer sum the attention weight that its tokens get - from the newest
+`window` queries of a prompt's chunk in every step, and in exact layers from every decoded token, whoever else is in the step -, and `evict_batched` keeps the sinks, the newest and the heaviest
 of a sequence's tokens, in the engine's blocks and in the pages alike.  The engine goes on with the lengths that it returns.
 """
 
@@ -200,9 +200,16 @@ class BatchedLayerState:
         self.positions.copy_(torch.where(none[:, None, None], fresh, self.positions[at]))
 
     def observe(self, query: torch.Tensor, meta, kv_cache: torch.Tensor, scale: Optional[float] = None) -> None:
-        """Add the weights that the newest queries of every sequence in this step give; query (rows, H_q, d)."""
-        ExactPagedCache.from_engine(kv_cache).add_window_weights(query, meta.query_start_loc, meta.block_table, meta.seq_lens,
-                                                                 self.weights[: meta.seq_lens.shape[0]], window=self.window, scale=scale, max_len=getattr(meta, "max_seq_len", None))
+        """Add the weights that the newest queries of every sequence in this step give; query (rows, H_q, d).  Compressed layers: of every sequence with
+        more than one row in it."""
+        lens, starts = meta.seq_lens, meta.query_start_loc
+        if self.pool is not None:
+            # One row is a decode step's, which a compressed layer does not count: not beside another sequence's prompt either (a sequence without
+            # tokens gives nothing)
+            lens, starts = (t.to(self.weights.device) for t in (lens, starts))
+            lens = lens.masked_fill(starts[1:] - starts[:-1] == 1, 0)
+        ExactPagedCache.from_engine(kv_cache).add_window_weights(query, starts, meta.block_table, lens, self.weights[: lens.shape[0]], window=self.window,
+                                                                 scale=scale, max_len=getattr(meta, "max_seq_len", None))
 
     def prepare_cut(self, block_table: torch.Tensor, seq_lens: torch.Tensor, kv_cache: Optional[torch.Tensor] = None,
                     max_len: Optional[int] = None) -> Optional[ExactPagedCache]:
@@ -376,8 +383,9 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
 
 def track_weights(model_runner, batch: int, max_len: int, window: int = 32) -> None:
     """Have every hooked layer sum the attention weight of its tokens from now on: up to `batch` rows of the block table, up to max_len tokens each
-    (a step that may hold longer sequences is refused).  A prompt step adds what its newest `window` queries give, read from the engine's cache; a
-    decode step adds its own in exact layers.
+    (a step that may hold longer sequences is refused).  The newest `window` queries of every prompt, or of its chunk in a step, add what they give, read
+    from the engine's cache; a decoding sequence's query adds its own in exact layers, in compressed ones not: their generated tokens have only the
+    weight that later prompt chunks give them, so `recent` is what keeps them.
 
     What is summed belongs to a row.  A row whose sequence begins in a step (all of its tokens are that step's) starts anew; an engine that
     gives rows of sequences that go on to others - a batch closed up, two rows swapped, a sequence that begins behind tokens it did not compute - says so
