@@ -267,6 +267,21 @@ def ordinary(*tensors) -> bool:
     return True
 
 
+def require_constant(what: str, **tensors) -> None:
+    """Refuse a call that torch is recording, and arguments (None: not there) that it is differentiating: `what` has no derivative and would be a
+    constant of either."""
+    if _tracing():
+        raise RuntimeError(f"{what} cannot be traced: the trace would hold this call's result as a constant")
+    grad, dual = _grad_enabled(), _forward_ad._current_level >= 0
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if grad and t.requires_grad:
+            raise RuntimeError(f"{name} requires a gradient: {what} has none, call it under torch.no_grad()")
+        if dual and _forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has a tangent: {what} has no derivative")
+
+
 def changed(*tensors):
     """Tell autograd that a kernel wrote to these tensors in place."""
     for t in tensors:

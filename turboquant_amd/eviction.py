@@ -78,7 +78,8 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
 
     Tokens that stay and lie within the first `budget` slots do not move, those behind fill the holes in ascending order, so the slots are not
     in order of position afterwards (attention does not ask).  The inputs are left as they are; out=(weights, positions)
-    takes the new ones instead of new tensors, the inputs themselves included."""
+    takes the new ones instead of new tensors, the inputs themselves included.  The weights are numbers to choose by: neither
+    gradient nor tangent goes through this call."""
     fast = _ffi.native()
     if fast is not None and out is None:
         done = fast.evict_select(weights, positions, seq_lens, seen, budget, sinks, recent)
@@ -100,6 +101,7 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
     for name, t in (("seq_lens", seq_lens), ("seen", seen)):
         if t is not None and t.shape != (B,):
             raise ValueError(f"{name} must have one entry for each of {B} sequences")
+    _ffi.require_constant("select_evictions")
     weights, positions = weights.detach().resolve_neg(), positions.resolve_neg()
     if weights.stride(2) != 1 and L > 1:
         weights = weights.contiguous()
@@ -116,8 +118,7 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
                 raise ValueError(f"out must hold {name} (B, H, L) like the input's, slots contiguous")
             if new.is_neg():
                 raise ValueError(f"out {name} is negated lazily: its memory does not hold its values")
-            if torch.is_grad_enabled() and new.requires_grad:
-                raise RuntimeError(f"out {name} requires a gradient")
+            _ffi.require_constant("select_evictions", **{f"out {name}": new})
             if not own_rows(new):
                 raise ValueError(f"out {name} must not overlap itself")
             same = new.data_ptr() == old.data_ptr() and new.stride() == old.stride()
@@ -163,8 +164,7 @@ def begin_rows(weights: torch.Tensor, positions: torch.Tensor, seq_lens: torch.T
     for name, t in (("weights", weights), ("positions", positions)):
         if (t.stride(2) != 1 and L > 1) or t.is_neg() or not own_rows(t):
             raise ValueError(f"{name} need contiguous slots, memory of their own and their values in it")
-        if torch.is_grad_enabled() and t.requires_grad:
-            raise RuntimeError(f"{name} requires a gradient")
+        _ffi.require_constant("begin_rows", **{name: t})
     if seq_lens.shape != (B,) or query_start_loc.shape != (B + 1,):
         raise ValueError(f"seq_lens and query_start_loc must have {B} and {B + 1} entries")
     if B == 0:

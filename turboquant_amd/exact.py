@@ -22,11 +22,6 @@ MAX_HEAD_DIM = 768
 MAX_WINDOW = 1024
 
 
-def _require_plain(t: torch.Tensor, name: str) -> None:
-    if torch.is_grad_enabled() and t.requires_grad:
-        raise RuntimeError(f"{name} requires a gradient: the exact cache's operators have none, call them under torch.no_grad()")
-
-
 class ExactPagedCache:
     """An engine's key and value blocks, (num_blocks, 16, H_kv, d) each, equal strides, channels contiguous, rows on 16-byte
     boundaries; the object holds the two tensors and nothing else."""
@@ -91,7 +86,6 @@ class ExactPagedCache:
             raise ValueError("weights need contiguous tokens, and memory that holds their values")
         if not own_rows(weights):
             raise ValueError("weights must not overlap themselves")
-        _require_plain(weights, "weights")
 
     # ---- read ----------------------------------------------------------------------------------------------------------
     def decode_attention(self, query: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -118,7 +112,7 @@ class ExactPagedCache:
             raise ValueError(f"Incompatible GQA shapes: Q={Hq}, H_kv={self.num_kv_heads}, d={d}")
         if query.dtype != self.dtype or query.device != self.device:
             raise TypeError("the query must have the cache's dtype and live on its GPU")
-        _require_plain(query, "query")
+        _ffi.require_constant("decode_attention", query=query, weights=weights, out=out, key_cache=self.key_cache, value_cache=self.value_cache)
         table, bt_stride, lens = self._sequences(block_table, seq_lens, B)
         if scale is None:
             scale = 1.0 / math.sqrt(d)
@@ -132,8 +126,6 @@ class ExactPagedCache:
             raise ValueError("out must be like the query: contiguous, same shape, dtype and GPU")
         elif out.is_neg():
             raise ValueError("out is negated lazily: its memory does not hold its values")
-        else:
-            _require_plain(out, "out")
         w_ptr, w_b, w_h, w_len = None, 0, 0, 0
         if weights is not None:
             self._weights(weights, B)
@@ -191,7 +183,7 @@ class ExactPagedCache:
             raise ValueError(f"Incompatible GQA shapes: Q={Hq}, H_kv={self.num_kv_heads}, d={d}")
         if query.dtype != self.dtype or query.device != self.device:
             raise TypeError("the query must have the cache's dtype and live on its GPU")
-        _require_plain(query, "query")
+        _ffi.require_constant("add_window_weights", query=query, weights=weights, key_cache=self.key_cache)
         if query_start_loc.dim() != 1 or query_start_loc.shape[0] < 1:
             raise ValueError("query_start_loc must have one entry more than there are sequences")
         B = query_start_loc.shape[0] - 1
@@ -229,6 +221,7 @@ class ExactPagedCache:
         fast = _ffi.native()
         if fast is not None and fast.move_exact(self.key_cache, self.value_cache, block_table, evictions.count, evictions.dst, evictions.src):
             return
+        _ffi.require_constant("move_tokens", key_cache=self.key_cache, value_cache=self.value_cache)
         count, dst, src, table, bt_stride = evictions.for_cache(block_table, self.num_kv_heads, self.device)
         B, H, moves = dst.shape
         if B == 0:

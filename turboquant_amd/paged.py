@@ -456,6 +456,7 @@ class PagedKVPool:
     def move_tokens(self, evictions: Evictions, block_table: torch.Tensor) -> None:
         """Carry out the moves of `select_evictions` in the compressed pages of block_table (B, max_pages), in place: codes,
         norms and scales go along as they are.  The sequences' pages must be their own."""
+        _ffi.require_constant("move_tokens")
         count, dst, src, table, bt_stride = evictions.for_cache(block_table, self.num_kv_heads, self.device)
         B, H, moves = dst.shape
         if B == 0:
