@@ -32,6 +32,8 @@ The first `exact_layers` layers may stay uncompressed: their decode steps are an
 (`ExactPagedCache`).  And a cache may be cut: `track_weights` has every layer sum the attention weight that its tokens get - from the newest
 `window` queries of a prompt's chunk in every step, and in exact layers from every decoded token, whoever else is in the step -, and `evict_batched` keeps the sinks, the newest and the heaviest
 of a sequence's tokens, in the engine's blocks and in the pages alike.  The engine goes on with the lengths that it returns.
+A hybrid step's exact part are a sequence's last `ring_capacity` slots.  Tokens that stay fill the holes of those that go, so that right behind a cut
+the newest lie anywhere below the budget and most of them are read from the pages; they are the last slots again once `ring_capacity` more have come.
 """
 
 from __future__ import annotations
