@@ -60,7 +60,8 @@ def own_rows(t: torch.Tensor) -> bool:
     return True
 
 
-def _memory(t: torch.Tensor) -> Tuple[int, int]:
+def memory_of(t: torch.Tensor) -> Tuple[int, int]:
+    """The addresses from t's first element up to behind its last."""
     first = t.data_ptr()
     return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
 
@@ -123,10 +124,10 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
                 raise ValueError(f"out {name} must not overlap itself")
             same = new.data_ptr() == old.data_ptr() and new.stride() == old.stride()
             for other in (weights, positions):
-                a, b = _memory(new), _memory(other)
+                a, b = memory_of(new), memory_of(other)
                 if not (same and other is old) and a[0] < b[1] and b[0] < a[1]:
                     raise ValueError(f"out {name} must be the input itself or memory of its own")
-        a, b = _memory(new_w), _memory(new_p)
+        a, b = memory_of(new_w), memory_of(new_p)
         if a[0] < b[1] and b[0] < a[1]:
             raise ValueError("the two tensors of out must not overlap")
     moves = max(1, min(budget, L - budget))

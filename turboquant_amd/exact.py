@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _ffi
-from .eviction import Evictions, own_rows
+from .eviction import Evictions, memory_of, own_rows
 from .paged import PAGE_TOKENS
 
 MAX_HEAD_DIM = 768
@@ -97,7 +97,7 @@ class ExactPagedCache:
 
         weights (B, H_kv, L) float32, tokens contiguous: every token's softmax weight, summed over the query heads of its KV
         head, is added in place (tokens from L on have no place in it).  max_len bounds the lengths for the plan of the
-        splits: without it the width of the table does.  The `workspace` of a step (`workspace()`) belongs to it alone until
+        splits: without it the width of the table does.  out: memory of its own, or the query itself.  The `workspace` of a step (`workspace()`) belongs to it alone until
         it has run: graphs that may run at the same time need one each."""
         fast = _ffi.native()
         if fast is not None and n_split is None and workspace is None and out is None:
@@ -126,6 +126,14 @@ class ExactPagedCache:
             raise ValueError("out must be like the query: contiguous, same shape, dtype and GPU")
         elif out.is_neg():
             raise ValueError("out is negated lazily: its memory does not hold its values")
+        else:
+            first, end = memory_of(out)
+            for name, t in (("query", query), ("weights", weights), ("key_cache", self.key_cache), ("value_cache", self.value_cache)):
+                if t is None or t.numel() == 0 or out.numel() == 0 or (t is query and t.data_ptr() == first):
+                    continue                                     # (over the query itself: a row is read by those that write it, and before)
+                a, b = memory_of(t)
+                if first < b and a < end:
+                    raise ValueError(f"out must be memory of its own or the query itself, it overlaps {name}")
         w_ptr, w_b, w_h, w_len = None, 0, 0, 0
         if weights is not None:
             self._weights(weights, B)
