@@ -283,3 +283,17 @@ def test_an_exact_layer_without_its_cache_is_not_cut(gpu):
     assert same(kept, everything(r))
     r.layers[-1].attn.kv_cache = r.kv_caches[-1]              # the tensor itself, not in a list
     assert evict_batched(r, r.block_table, lens, 40).tolist() == [40, 12, 40]
+
+
+def test_a_decode_step_takes_memory_by_its_length_and_not_by_what_is_tracked(gpu):
+    """Scores of every head and token of the step, not of every place for one: 3 x 8 heads of 400000 places would be 38 MB."""
+    r = runner(gpu, track=400000, exact_layers=2, mode="hybrid")
+    prompt(r, [90, 12, 150])
+    s, q, meta = states(r)[0], torch.randn(3, 8, 64, device=gpu).bfloat16(), r.decode_metadata()
+    meta.block_table = torch.nn.functional.pad(meta.block_table, (0, 25000))             # (an engine's rows have room for its longest sequence)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    s.attend(q, meta, kv_cache=r.kv_caches[0])
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
+    assert torch.allclose(given(r)[0], per_row(17, 13, 17), rtol=1e-4)

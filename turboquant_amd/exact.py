@@ -96,7 +96,8 @@ class ExactPagedCache:
         seq_lens[b] tokens that block_table (B, max_pages) or (max_pages,) names; zeros for a sequence without tokens.
 
         weights (B, H_kv, L) float32, tokens contiguous: every token's softmax weight, summed over the query heads of its KV
-        head, is added in place (tokens from L on have no place in it).  max_len bounds the lengths for the plan of the
+        head, is added in place (tokens from L on have no place in it); meanwhile the step keeps 4 bytes for each of L places and query heads, so
+        that weights of a large capacity are best given as weights[..., :longest].  max_len bounds the lengths for the plan of the
         splits: without it the width of the table does.  out: memory of its own, or the query itself.  The `workspace` of a step (`workspace()`) belongs to it alone until
         it has run: graphs that may run at the same time need one each."""
         fast = _ffi.native()

@@ -144,9 +144,10 @@ class BatchedLayerState:
         self.decode_steps += 1
         cfg = self.config
         if self.pool is None:
-            weights = None if self.weights is None else self.weights[: query.shape[0]]
-            return ExactPagedCache.from_engine(kv_cache).decode_attention(query, meta.block_table, meta.seq_lens, scale=scale, weights=weights,
-                                                                          max_len=getattr(meta, "max_seq_len", None))
+            longest, weights = getattr(meta, "max_seq_len", None), self.weights
+            if weights is not None:                            # (the step keeps a score for every place; check_step has seen that there are no longer sequences)
+                weights = weights[: query.shape[0], :, : max(1, longest) if longest is not None else None]
+            return ExactPagedCache.from_engine(kv_cache).decode_attention(query, meta.block_table, meta.seq_lens, scale=scale, weights=weights, max_len=longest)
         if (hybrid and cfg.ring_capacity > 0 and torch.is_tensor(kv_cache) and kv_cache.dim() == 5 and
                 kv_cache.shape[0] == 2 and tuple(kv_cache.shape[2:]) == (PAGE_TOKENS, cfg.num_kv_heads, cfg.head_dim) and
                 kv_cache.dtype == query.dtype and cfg.ring_capacity <= 1024 and
