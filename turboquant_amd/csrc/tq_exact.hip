@@ -36,7 +36,7 @@ __device__ __forceinline__ void join_store(void* out, int64_t at, const float4& 
 template <int DT>
 __device__ __forceinline__ void exact_join_few(const ExactJoin& a, int row) {
   const int lane = (int)threadIdx.x & 63;
-  const int used = __builtin_amdgcn_readfirstlane(join_used(a, join_len(a, row / a.Hq)));
+  const int used = join_used(a, join_len(a, row / a.Hq));
   const float2 ml = lane < used ? a.ml[(int64_t)row * a.n_split + lane] : make_float2(-INFINITY, 0.0f);
   const float top = wave_max_fast(ml.x), ref = top == -INFINITY ? 0.0f : top;
   const float f = __builtin_amdgcn_exp2f(ml.x - ref), sum = wave_sum_fast(f * ml.y), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -50,9 +50,10 @@ __device__ __forceinline__ void exact_join_few(const ExactJoin& a, int row) {
       for (int i = 0; i < 8; ++i) x[i] = acc[(int64_t)(i0 + i < used ? i0 + i : used - 1) * quads];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (i0 + i >= used) break;                           // (not a factor of zero: an infinite numerator would give NaN)
-        const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (i0 + i) & 63));
-        o.x = fmaf(g, x[i].x, o.x); o.y = fmaf(g, x[i].y, o.y); o.z = fmaf(g, x[i].z, o.z); o.w = fmaf(g, x[i].w, o.w);
+        const bool in = i0 + i < used;                       // (where not, a numerator of zero: a factor of zero would make NaN of an infinite one)
+        const float g = in ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (i0 + i) & 63)) : 0.0f;
+        o.x = fmaf(g, in ? x[i].x : 0.0f, o.x); o.y = fmaf(g, in ? x[i].y : 0.0f, o.y);
+        o.z = fmaf(g, in ? x[i].z : 0.0f, o.z); o.w = fmaf(g, in ? x[i].w : 0.0f, o.w);
       }
     }
     join_store<DT>(a.out, (int64_t)row * a.d + q * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
