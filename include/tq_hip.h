@@ -418,7 +418,7 @@ int tq_exact_decode(const void *q, int dtype, int B, int Hq, int Hkv, int d, con
 /* What a prompt's newest queries make of the tokens of that cache: the softmax weights of the newest min(window, rows of the sequence, seq_lens[b])
  * queries of every sequence, causal among themselves, summed over them and the query heads of KV head h, are added to weights (as in
  * tq_exact_decode).  q (rows, Hq, d) contiguous, 16-byte aligned; sequence b's rows are query_start_loc[b] .. query_start_loc[b + 1] - 1 (device, B + 1
- * entries; what lies outside 0 .. rows is left out), the last of them at position seq_lens[b] - 1.  window up to 1024.  Values are not read. */
+ * entries; what lies outside 0 .. rows is left out), the last of them at position seq_lens[b] - 1.  window up to 1024, Hq * d up to 2^25.  Values are not read. */
 size_t tq_exact_window_bytes(int dtype, int B, int Hq, int Hkv, int d, int window, int64_t max_len);
 int tq_exact_window(const void *q, int dtype, int64_t rows, const int32_t *query_start_loc, int B, int Hq, int Hkv, int d,
                     int window, const void *k_cache, int64_t cs_blk, int64_t cs_t, int64_t cs_h, int64_t num_blocks,
@@ -426,7 +426,7 @@ int tq_exact_window(const void *q, int dtype, int64_t rows, const int32_t *query
                     float *weights, int64_t w_b, int64_t w_h, int64_t weight_len, void *workspace, void *stream);
 
 /* Which tokens stay when sequences of more than `budget` tokens are cut to it, per sequence and KV head: first those with a position below
- * `sinks` or from seen[b] - recent on, then by weight (NaN last, +inf as the largest number), of two alike the one in the lower slot.
+ * `sinks` or from seen[b] - recent on, then by weight (NaN as -inf, +inf as the largest number), of two alike the one in the lower slot.
  * A slot below the budget whose token goes is a hole; the k-th hole takes the k-th of the tokens that stay behind the budget, the others stay
  * where they are.  weights / positions: fp32 / int32 (B, H, L), element (b, h, slot) at base + b*.._b + h*.._h + slot; seq_lens and seen
  * (tokens that a sequence has had in all; NULL: seq_lens) are device int32 (B,); lengths above L are cut to L.  1 <= budget, sinks + recent <= budget.

@@ -194,9 +194,9 @@ static bool exact_plan(ExactPlan* p, int dtype, int B, int Hq, int Hkv, int d, i
   p->block_tokens = dtype == TQ_F32 ? 16 : 32;
   const int tiles = (G + EXACT_HEADS - 1) / EXACT_HEADS;
   // More than sixteen heads share their reads where the passes over the cache that this saves outweigh a start that is 2-4 us longer: from 64 MB, all
-  // heads' passes together (bf16, sixteen / 64 heads a workgroup; one sequence of 16384, 32 heads: d 128 34 MB 9.9 / 12.1 us, d 448 59 MB 19.6 / 22.6, d 576
-  // 75 MB 26.6 / 23.1; 48 heads, 16 of 8192: d 128 201 MB 25.0 / 25.2, d 192 302 MB 41 / 32, d 576 906 MB 264 / 74).  d = 64 with 32 heads: 21.6 / 27.2 at
-  // 134 MB, never.
+  // heads' passes together (bf16, one KV head, sixteen / 64 heads a workgroup; one sequence of 16384, 32 heads: d 128 17 MB 10.1 / 12.7 us, d 448 59 MB
+  // 20.5 / 24.1, d 576 75 MB 27.1 / 24.4; 16 of 8192: 32 heads of 128 134 MB 22.8 / 23.7, 48 heads of 128 201 MB 25.9 / 26.2, of 192 302 MB 45 / 36, of 576
+  // 906 MB 286 / 82).  d = 64 with 32 heads: 16.2 / 19.7 at 67 MB, never.
   const int64_t passes = (int64_t)tiles * d * 4 * std::max<int64_t>(1, (int64_t)B * Hkv);
   const bool shared = dtype != TQ_F32 && tiles > 1 && d <= 576 && (d > 64 || tiles > 2) && max_len > (int64_t(64) << 20) / passes;
   p->shared = shared;

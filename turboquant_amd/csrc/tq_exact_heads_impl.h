@@ -11,9 +11,9 @@
 //     block: behind it everybody's part of this block has arrived and everybody is done with the other.
 //   * A row takes one 16-byte piece more than it has: rows then start 16 bytes apart in the banks, and the sixteen rows of a key operand are read
 //     without conflicts.
-// Bound at 576 channels by what a wavefront issues and its reads of LDS, one wavefront per SIMD: 16 sequences of 8192 tokens, 128 heads, bf16, 104 us for
-// 302 MB (2.9 TB/s; as a plain read 56) and 38.7 GFLOP (370 TFLOP/s; as a large product 35 us).
-// Workgroups of two and eight tiles were slower or no faster (B x heads, bf16, lengths of 8192): 32 x 128 of 256: 175 us with two, 96 with four, 114 with
+// Bound at 576 channels by what a wavefront issues and its reads of LDS, one wavefront per SIMD: 16 sequences of 8192 tokens, 128 heads, bf16, 114 us for
+// 302 MB (2.6 TB/s; as a plain read 56) and 38.7 GFLOP (340 TFLOP/s; as a large product 35 us), the values' half of them done twice (104 us with weights in one number).
+// Workgroups of two and eight tiles were slower or no faster (B x heads, bf16, lengths of 8192, weights in one number): 32 x 128 of 256: 175 us with two, 96 with four, 114 with
 // eight; 32 x 128 of 128: 109, 57, 57; 32 x 32 of 576, where half of four tiles are empty: 135, 126.
 #pragma once
 

@@ -13,9 +13,11 @@
 //             fp32: a lane's four channels of a token are the row operands of four instructions as they are.
 //   softmax   one pass: running maximum and sum per head; a lane's accumulators all belong to its head, so a move of the maximum is a
 //             scalar of the lane.  Maximum, sum, scores and numerators are fp32.  The matrix instruction takes 16-bit weights: they go in as two
-//             numbers, a high and a low half (ex_split), so that what is rounded away is 2^-15 (fp16: 2^-21) of a weight.
+//             numbers, a high and a low half (ex_split), so that what is rounded away is 2^-15 (fp16: 2^-21) of a weight
+//             (rounded once, 2^-8 and 2^-11, outputs were a third and a fifth further from 64 bits than fp32 weights' are).  Twice the products of
+//             the values: nothing that shows at sixteen heads, 8 us of 114 with 128 heads on one of 576 channels.
 // Bound by the memory system.  bf16, 16 sequences of 8192, 32 query on 8 KV heads of 128: 117 us for 546 MB, 4.7 TB/s where a large read reaches 5.4; one of
-// 131072, 16 on 2 heads of 256: 60 us, 4.5 TB/s; fp16, 96 of 61 .. 8190, 40 on 8 heads of 128: 145 - 155 us, 4.4 - 4.7 TB/s, the rest the ends of short
+// 131072, 16 on 2 heads of 256: 62 us, 4.4 TB/s; fp16, 96 of 61 .. 8190, 40 on 8 heads of 128: 145 - 155 us, 4.4 - 4.7 TB/s, the rest the ends of short
 // sequences; fp32, 8 of 1500 .. 2048, 16 heads of 64: 28 us, 4.2 TB/s.  One of 700 tokens: 5.4 us, a launch and four latencies one behind another (length,
 // table entry, keys and values, the join of the four wavefronts).
 // Registers before LDS: with the next block's keys and values on their way in registers a wavefront needs no barrier; with table entries read behind

@@ -4,7 +4,8 @@
 //   first   m_r = max_t s_rt,  l_r = sum_t 2^(s_rt - m_r)          s_rt = scale log2 e  q_r . k_t  for t <= length - W' + w
 //   second  weights[t] += sum_r 2^(s_rt - m_r) / l_r
 //
-// The scores are computed twice rather than stored: at W = 32 and 32 heads of 128 a token's scores are 4 KB per KV head and its key 256 bytes.
+// The scores are computed twice rather than stored: at W = 32 and four heads of 128 on a KV head a token's scores are 512 bytes, which would be written and
+// read, and its key, which is read again, 256.
 // Tokens are rows of the matrix instruction, (query, head) rows its columns; those stay in registers, window_tiles() tiles of 16 per wavefront.  The
 // wavefronts of a workgroup stand side by side on the tiles, and, with few of those, on the tokens.  Keys lie in LDS twice, filled by LDS-direct loads
 // a turn ahead: read from memory as operands, they came from the L1 once for every wavefront, 16 lines of 64 bytes a load, and that was the bound.

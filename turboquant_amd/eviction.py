@@ -74,7 +74,7 @@ def select_evictions(weights: torch.Tensor, positions: torch.Tensor, seq_lens: t
     weights (B, H, L) float32 and positions (B, H, L) int32 say of every slot how much weight its token has had and where in the
     sequence it stood; seq_lens (B,) slots are in use (L of them at most), seen (B,) tokens the sequence has had in all (None: seq_lens, nothing
     was cut before).  The first `sinks` positions and the newest `recent` always stay (sinks + recent <= budget); of the others
-    the heaviest, of two alike the one in the lower slot; a NaN counts as less than everything.  Sequences within the budget
+    the heaviest, of two alike the one in the lower slot; a NaN counts as -inf.  Sequences within the budget
     stay as they are.
 
     Tokens that stay and lie within the first `budget` slots do not move, those behind fill the holes in ascending order, so the slots are not
