@@ -61,7 +61,8 @@ __device__ __forceinline__ uint32_t ex_pack(float lo, float hi) {
 
 // Two weights as the sum of two numbers each of the cache's type.  The high one is cut, never rounded up, and always less than the weight, so that the low one
 // is positive where the weight is: with a low part of zero, or one below zero, an infinite value would give NaN (0 x inf, inf - inf) where it has to give
-// infinity.  fp16: less by 2^-24 at least, below which a low part would be rounded to nothing.
+// infinity.  fp16: less by 2^-24 at least, below which a low part would be rounded to nothing; a weight below 2^-25 is nothing in either half, 2^-31 of the
+// largest and less.
 template <int DT>
 __device__ __forceinline__ void ex_split(float a, float b, uint32_t* hi, uint32_t* lo) {
   if constexpr (DT == TQ_BF16) {
