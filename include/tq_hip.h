@@ -40,7 +40,7 @@ extern "C" {
 
 #define TQ_ABI_VERSION 2
 
-enum { TQ_F32 = 0, TQ_F16 = 1, TQ_BF16 = 2 };
+enum { TQ_F32 = 0, TQ_F16 = 1, TQ_BF16 = 2, TQ_E4M3 = 3 /* elements of the 8-bit cache only */ };
 
 enum {
   TQ_OK = 0,
@@ -452,6 +452,52 @@ int tq_move_tokens_exact(void *k_cache, void *v_cache, int dtype, int d, int64_t
 int tq_move_tokens_pool(uint8_t *pool, int64_t num_pages, const tq_page_layout *layout, const int32_t *block_table, int bt_stride,
                         const int32_t *count, const int32_t *dst, const int32_t *src, int B, int H, int moves, int budget,
                         void *stream);
+
+/* ---- a step over a paged cache: rows of the exact cache or of one in 8 bits ---------------------------------------
+ * A step has `rows` rows; query_start_loc (device, B + 1 int32, ascending, the first 0) says whose: rows query_start_loc[b] .. [b + 1] - 1 are sequence b's
+ * newest, the last of them its token seq_lens[b] - 1.  Block tables as above.  (No counterpart in the reference, whose engine does this.)
+ *
+ * The 8-bit cache: k_cache / v_cache blocks of 16 tokens in e4m3, strides in elements (bytes) and multiples of 16, cs_t up to 2^24; k_scales / v_scales (num_blocks,
+ * Hkv) bytes: e + 127, every element of the block's KV head times 2^e; d 64, 128, 192 or 256.
+ *
+ * tq_fp8_write: the step's keys and values (rows, Hkv, d), element strides ks_t, ks_h, vs_t, vs_h, channels contiguous, rows on 16-byte boundaries, into the blocks of their
+ * tokens.  A block's e is the smallest that brings its largest finite value to 448 (-117 <= e <= 119, -117 for zeros); values are rounded to nearest even, infinite
+ * ones to 448 2^e, NaN stays.  Tokens that a block held before the step are rounded again where e grows; a block whose first slot is written
+ * starts anew.  Rows in front of token 0, behind the table's row or in blocks outside the cache are left out.  One table (bt_stride < 0) serves one sequence only.
+ *
+ * tq_fp8_read: the reverse: rows (rows, Hkv, d) contiguous, 16-byte aligned, `dtype`; a row without a token or with a block outside the cache is zeros.  fill: rows of
+ * no sequence become zeros, else they are left as they are.                                                                        */
+int tq_fp8_write(const void *k, const void *v, int dtype, int64_t rows, int64_t ks_t, int64_t ks_h, int64_t vs_t, int64_t vs_h,
+                 const int32_t *query_start_loc, int B, int Hkv, int d, void *k_cache, void *v_cache, uint8_t *k_scales, uint8_t *v_scales,
+                 int64_t cs_blk, int64_t cs_t, int64_t cs_h, int64_t num_blocks, const int32_t *block_table, int bt_stride,
+                 const int32_t *seq_lens, void *stream);
+int tq_fp8_read(void *k_out, void *v_out, int dtype, int64_t rows, const int32_t *query_start_loc, int B, int Hkv, int d, const void *k_cache,
+                const void *v_cache, const uint8_t *k_scales, const uint8_t *v_scales, int64_t cs_blk, int64_t cs_t, int64_t cs_h,
+                int64_t num_blocks, const int32_t *block_table, int bt_stride, const int32_t *seq_lens, int fill, void *stream);
+
+/* Attention of a step's rows over such a cache, causal: row i of a sequence with n rows stands at p = seq_lens[b] - n + i and sees token t if t <= p and
+ * (window <= 0 or t > p - window or t < sinks).  q, out (rows, Hq, d) contiguous, 16-byte aligned, `dtype` TQ_F16 or TQ_BF16; `cache`: the same (an exact cache, k_scales and v_scales
+ * unused) or TQ_E4M3; d 64, 128, 192 or 256; Hq / Hkv any whole number up to 1024.  A row that sees nothing is zeros; tokens without a block in the cache have no weight.
+ * query_start_loc null: a row per sequence (rows == B).  max_len bounds seq_lens and max_rows the rows of a sequence, for the plan: what exceeds them is right, too, and
+ * slower.  n_split: 0, or how many workgroups share a row's tokens, up to 1024.  fill as tq_fp8_read.  workspace: tq_attend_bytes bytes (starts: whether there is a
+ * query_start_loc), 16-byte aligned, of this call alone until it has run.  0: sizes out of range.                                   */
+size_t tq_attend_bytes(int dtype, int cache, int starts, int64_t rows, int B, int Hq, int Hkv, int d, int64_t max_len, int64_t max_rows,
+                       int64_t window, int sinks, int n_split);
+int tq_attend(const void *q, int dtype, int64_t rows, const int32_t *query_start_loc, int B, int Hq, int Hkv, int d, int cache,
+              const void *k_cache, const void *v_cache, const uint8_t *k_scales, const uint8_t *v_scales, int64_t cs_blk, int64_t cs_t,
+              int64_t cs_h, int64_t num_blocks, const int32_t *block_table, int bt_stride, const int32_t *seq_lens, float sm_scale,
+              int64_t max_len, int64_t max_rows, int64_t window, int sinks, void *out, int fill, void *workspace, int n_split, void *stream);
+
+/* The norm of every head of queries (rows, Hq, d) and keys (rows, Hkv, d) and their rotation by position, fp32 inside, rounded once:
+ *   y = x / sqrt(mean x^2 + eps) * weight (weight null: y = x);  pairs (i, i + rotary_dim / 2) of the first rotary_dim channels - interleaved: (2 i, 2 i + 1) - turn by
+ *   positions[row] * inv_freq[i].
+ * Element strides of tokens and heads, multiples of 4, channels contiguous, rows on 8-byte boundaries (fp32: 16); d a multiple of 8 up to 512, rotary_dim one up to d; positions
+ * int32, or int64 with wide_positions; inv_freq (rotary_dim / 2) double; weights (d) `dtype`.  The outputs may be the inputs.  Either of the two may have
+ * no heads.                                                                                                                     */
+int tq_rotate_heads(const void *q, const void *k, int dtype, int64_t rows, int Hq, int Hkv, int d, int64_t qs_t, int64_t qs_h, int64_t ks_t,
+                    int64_t ks_h, const void *positions, int wide_positions, const double *inv_freq, int rotary_dim, int interleaved,
+                    const void *q_weight, const void *k_weight, float eps, void *q_out, int64_t qo_t, int64_t qo_h, void *k_out, int64_t ko_t,
+                    int64_t ko_h, void *stream);
 
 /* Log-sum-exp merge of n_parts partial results per (b, query head):
  * parts (B*Hq, n_parts, d+2) fp32 = [running max, sum of exp, un-normalised acc];

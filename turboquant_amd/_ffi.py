@@ -18,7 +18,7 @@ import torch
 
 logger = logging.getLogger("turboquant.ffi")
 
-TQ_F32, TQ_F16, TQ_BF16 = 0, 1, 2
+TQ_F32, TQ_F16, TQ_BF16, TQ_E4M3 = 0, 1, 2, 3
 TQ_PAGE_TOKENS = 16
 TQ_MAX_TERMS = 15
 ABI_VERSION = 2
@@ -121,6 +121,13 @@ _SIGNATURES = {
     "tq_evict_select_bytes": (C.c_size_t, [_i, _i, _i, _i, _i]),
     "tq_move_tokens_exact": (C.c_int, [_vp, _vp, _i, _i, _i64, _i64, _i64, _i64, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "tq_move_tokens_pool": (C.c_int, [_vp, _i64, C.POINTER(TqPageLayout), _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "tq_fp8_write": (C.c_int, [_vp, _vp, _i, _i64, _i64, _i64, _i64, _i64, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i, _vp, _vp]),
+    "tq_fp8_read": (C.c_int, [_vp, _vp, _i, _i64, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i, _vp, _i, _vp]),
+    "tq_attend_bytes": (C.c_size_t, [_i, _i, _i, _i64, _i, _i, _i, _i, _i64, _i64, _i64, _i, _i]),
+    "tq_attend": (C.c_int, [_vp, _i, _i64, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i, _vp, _f, _i64, _i64, _i64, _i,
+                            _vp, _i, _vp, _i, _vp]),
+    "tq_rotate_heads": (C.c_int, [_vp, _vp, _i, _i64, _i, _i, _i, _i64, _i64, _i64, _i64, _vp, _i, _vp, _i, _i, _vp, _vp, _f, _vp, _i64, _i64, _vp,
+                                  _i64, _i64, _vp]),
     "tq_decode_merge": (C.c_int, [_vp, _i64, _i, _i, _i, _vp, _vp]),
     "tq_time_next_page_kernel": (None, [_vp, _vp]),
     "tq_time_next_key_kernel": (None, [_vp, _vp]),

@@ -1,0 +1,390 @@
+// Attention of few rows - one token of a sequence, or a few - over a paged cache (instantiated by one file per types).
+//
+// A unit is 16 NT rows of a KV head: the query heads of a token side by side, tokens one behind another; they are the columns of the matrix
+// instructions.  A workgroup's four wavefronts take 32 tokens each at a time, straight from memory into the operands, as the decode kernel of the exact
+// cache does it: no shared memory and no barrier in the loop, the next block's keys and values on their way in registers.
+//   scores    tokens are rows; a lane reads 16 bytes of ONE token's key.  8 bits: those are 16 channels, two steps of 32, and the queries lie in registers
+//             in that order; two numbers become 16-bit ones in an instruction (e4m3 is a subset of both), the block's scale multiplies the score.
+//   values    channels are rows; a lane reads its channels of its 8 tokens and turns them around in registers.  8 bits: half as many byte permutes, and the
+//             conversion to bf16 multiplies by the block's scale for nothing; bf16 for fp16 queries, too, whose range the scale might leave.
+//   softmax   one pass, running maximum and sum per row, all in 32 bits; weights go in as a high and a low half (ex_split).
+// Bound by the memory system.
+#pragma once
+
+#include "tq_attend.h"
+#include "tq_exact_impl.h"
+
+namespace tq {
+
+// two e4m3 numbers (the lower or the upper half of x) as 16-bit ones, times a power of two
+template <int QT, bool UPPER>
+__device__ __forceinline__ uint32_t f8_widen(uint32_t x, float scale) {
+  if constexpr (QT == TQ_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, UPPER));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, UPPER));
+}
+
+template <bool F8, int D, int NT>
+constexpr int attend_few_waves() {
+  if (NT == 1) return F8 ? (D <= 128 ? 4 : (D <= 192 ? 3 : 2)) : (D <= 64 ? 4 : (D <= 128 ? 3 : (D <= 192 ? 2 : 1)));
+  return F8 ? (D <= 64 ? 4 : (D <= 128 ? 2 : 1)) : (D <= 64 ? 3 : (D <= 128 ? 2 : 1));
+}
+
+template <int QT, bool F8, int D, int NT>
+__global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_few_kernel(const Attend a) {
+  constexpr int PT = F8 ? TQ_BF16 : QT;                      // of the value product
+  constexpr int SIZE = F8 ? 1 : 2, PAGES = 2, TB = 32;
+  constexpr int KLOADS = D * SIZE / 64, KSTEPS = D / 32;     // 16-byte pieces of a key that a lane reads; steps of 32 channels
+  constexpr int TILES = D / 16;
+  constexpr int WIDE = F8 ? 0 : D / 128, NARROW = F8 ? 0 : (D - WIDE * 128) / 64;
+  constexpr int VWORDS = D / 64;                             // 8 bits: words of a token that a lane reads
+  typedef uint32_t vword __attribute__((ext_vector_type(VWORDS == 3 ? 4 : VWORDS)));
+
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  const int col = lane & 15, quarter = lane >> 4;
+  const unsigned pairs = (unsigned)(a.units * a.H), split = blockIdx.x / pairs, pair = (blockIdx.x - split * pairs + split) % pairs;
+  const int h = (int)(pair % (unsigned)a.H);
+  int64_t number = pair / (unsigned)a.H;
+  AttendUnit u;
+  if (!attend_unit<16 * NT>(a, &number, &u)) {
+    // units behind the last: rows of no sequence, this KV head's part of them
+    if (split) return;
+    int64_t front;
+    const int64_t rest = step_rest(a.s, &front), others = a.units - (pair / (unsigned)a.H - number);
+    for (int64_t n = number; n < rest; n += others) {
+      const int64_t row = step_rest_row(a.s, front, rest, n) * a.Hq + h * a.G;
+      if (a.n_split > 1) {
+        for (int g = (int)threadIdx.x; g < a.G; g += 256) a.ml[(row + g) * a.n_split] = make_float2(-INFINITY, ATTEND_REST);
+      } else if (a.fill) {
+        for (int c = (int)threadIdx.x; c < a.G * D / 2; c += 256) ((uint32_t*)((uint16_t*)a.out + row * D))[c] = 0;
+      }
+    }
+    return;
+  }
+  const AttendBlocks<TB> list(a, u);
+  const int per = attend_per_split(list.count, a.n_split, a.chunk);
+  const int first = (int)split * per < list.count ? (int)split * per : list.count, last = first + per < list.count ? first + per : list.count;
+
+  // this lane's rows: one of each column tile
+  bool live[NT];
+  int64_t row[NT];                                           // (token row, head) of the step
+  int at_p[NT], behind[NT];                                  // what the row sees: t <= at_p and (t > behind or t < sinks)
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = n * 16 + col;
+    live[n] = r < u.rows;
+    const int x = u.first + (live[n] ? r : 0), i = x / a.G;
+    row[n] = (u.row + i) * a.Hq + h * a.G + (x - i * a.G);
+    at_p[n] = u.low + (i - u.first / a.G);
+    behind[n] = attend_behind(a, at_p[n]);
+  }
+  if (first >= last && a.n_split > 1) {
+    if (quarter == 0 && wave == 0) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        if (live[n]) a.ml[row[n] * a.n_split + split] = make_float2(-INFINITY, ATTEND_EMPTY);
+    }
+    return;
+  }
+  const int32_t* table = a.s.table + u.b * a.s.table_step;
+
+  ex_u32x4 Q[NT][KSTEPS];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) {
+      Q[n][s] = ex_u32x4{0, 0, 0, 0};
+      const int c = F8 ? (s >> 1) * 64 + quarter * 16 + (s & 1) * 8 : s * 32 + quarter * 8;
+      if (live[n]) Q[n][s] = *(const ex_u32x4*)((const uint16_t*)a.q + row[n] * D + c);
+    }
+  ex_f32x4 O[NT][TILES];
+  float m[NT], l[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) O[n][t] = ex_f32x4{0, 0, 0, 0};
+    m[n] = -INFINITY;
+    l[n] = 0.0f;
+  }
+
+  // a block's two pages: where they lie, their scales, how many of their tokens count
+  struct Pages {
+    int64_t at[PAGES];
+    uint32_t k_scale[PAGES], v_scale[PAGES];                 // (bytes as they are loaded: they are first looked at a block later)
+    int valid[PAGES], t0;
+    bool whole;
+  };
+  const int last_page = u.tokens > 0 ? (u.tokens - 1) / TQ_PAGE_TOKENS : 0;
+  const int low_behind = attend_behind(a, u.high);
+  const auto find = [&](Pages& x, int i) __attribute__((always_inline)) {
+    const int blk = list[i];
+    x.t0 = blk * TB;
+    x.whole = x.t0 + TB - 1 <= u.low && (x.t0 > low_behind || x.t0 + TB <= a.sinks);
+    int32_t entry[PAGES];
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p) {
+      const int page = blk * PAGES + p;
+      entry[p] = table[page < last_page ? page : last_page];
+    }
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p) {
+      const int left = u.tokens - (blk * PAGES + p) * TQ_PAGE_TOKENS;
+      x.valid[p] = left < 0 ? 0 : (left > TQ_PAGE_TOKENS ? TQ_PAGE_TOKENS : left);
+      int64_t page = entry[p];
+      if (page < 0 || page >= a.s.num_blocks) { page = 0; x.valid[p] = 0; }
+      x.whole &= x.valid[p] == TQ_PAGE_TOKENS;
+      x.at[p] = (page * a.s_blk + h * a.s_h) * SIZE;
+      if constexpr (F8) {
+        x.k_scale[p] = a.k_scales[page * a.H + h];
+        x.v_scale[p] = a.v_scales[page * a.H + h];
+      }
+    }
+  };
+  const auto scale_of = [](uint32_t byte) __attribute__((always_inline)) { return byte == 0 ? 0x1p-127f : __uint_as_float(byte << 23); };
+
+  const uint32_t step = (uint32_t)a.s_t * SIZE;
+  const uint32_t krow = (uint32_t)col * step + quarter * 16, vrow = (uint32_t)(quarter * 4) * step;
+  ex_u32x4 K[PAGES][KLOADS];
+  ex_u32x4 V[WIDE > 0 ? WIDE : 1][8];
+  ex_u32x2 VN[8];
+  vword VB[8];
+  const auto load_keys = [&](const Pages& x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+      for (int s = 0; s < KLOADS; ++s) K[p][s] = *(const ex_u32x4*)((const char*)a.k + x.at[p] + krow + s * 64);
+  };
+  const auto load_values = [&](const Pages& x) __attribute__((always_inline)) {
+    if constexpr (F8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint8_t* from = (const uint8_t*)a.v + x.at[i >> 2] + vrow + (i & 3) * step + col * (VWORDS * 4);
+        if constexpr (VWORDS == 3) {
+          typedef uint32_t three __attribute__((ext_vector_type(3), aligned(4)));
+          const three y = *(const three*)from;
+          VB[i] = vword{y[0], y[1], y[2], 0};
+        } else {
+          VB[i] = *(const vword*)from;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < WIDE; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) V[c][i] = *(const ex_u32x4*)((const char*)a.v + x.at[i >> 2] + vrow + (i & 3) * step + (c * 128 + col * 8) * 2);
+      if constexpr (NARROW > 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) VN[i] = *(const ex_u32x2*)((const char*)a.v + x.at[i >> 2] + vrow + (i & 3) * step + (WIDE * 128 + col * 4) * 2);
+      }
+    }
+  };
+
+  Pages now, next;
+  if (first + wave < last) {
+    find(now, first + wave);
+    load_keys(now);
+    load_values(now);
+  }
+  for (int blk = first + wave; blk < last; blk += 4) {
+    const bool more = blk + 4 < last;
+    if (more) find(next, blk + 4);
+    // ---- scores ----
+    ex_f32x4 S[NT][PAGES];
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) S[n][p] = ex_f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < KSTEPS; ++s) {
+        ex_u32x4 k;
+        if constexpr (F8) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t x = K[p][s >> 1][(s & 1) * 2 + w];
+            k[w * 2] = f8_widen<QT, false>(x, 1.0f);
+            k[w * 2 + 1] = f8_widen<QT, true>(x, 1.0f);
+          }
+        } else {
+          k = K[p][s];
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) S[n][p] = ex_mfma<QT>(k, Q[n][s], S[n][p]);
+      }
+    }
+    if (more) load_keys(next);
+    // ---- weights of this lane's rows: tokens quarter * 4 + i of each page ----
+    ex_u32x4 P[NT], L[NT];                                   // high and low halves
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float top = -INFINITY, pr[PAGES][4];
+#pragma unroll
+      for (int p = 0; p < PAGES; ++p) {
+        const float f = F8 ? a.scale2 * scale_of(now.k_scale[p]) : a.scale2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float s2 = S[n][p][i] * f;
+          const int in = quarter * 4 + i, t = now.t0 + p * TQ_PAGE_TOKENS + in;
+          const bool seen = now.whole || (in < now.valid[p] && t <= at_p[n] && (t > behind[n] || t < a.sinks));
+          pr[p][i] = seen ? s2 : -INFINITY;
+          top = fmaxf(top, pr[p][i]);
+        }
+      }
+      top = fmaxf(m[n], ex_quad_max(top));
+      if (__any(top > m[n] + EX_SLACK)) {
+        const float move = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[n] - top);
+        l[n] *= move;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) O[n][t] *= move;
+        m[n] = top;
+      }
+      const float ref = m[n] == -INFINITY ? 0.0f : m[n] - ex_lift<PT>();
+#pragma unroll
+      for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          pr[p][i] = __builtin_amdgcn_exp2f(pr[p][i] - ref);
+          l[n] += pr[p][i];
+        }
+#pragma unroll
+      for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t hi, lo;
+          ex_split<PT>(pr[p][2 * i], pr[p][2 * i + 1], &hi, &lo);
+          P[n][p * 2 + i] = hi;
+          L[n][p * 2 + i] = lo;
+        }
+    }
+    // ---- values; those of tokens that no row of the unit sees are put to zero, since NaN times nothing is NaN ----
+    bool none[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int in = quarter * 4 + (i & 3), t = now.t0 + (i >> 2) * TQ_PAGE_TOKENS + in;
+      none[i] = in >= now.valid[i >> 2] || !(t > attend_behind(a, u.low) || t < a.sinks);
+    }
+    if constexpr (F8) {
+      if (!now.whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (none[i]) VB[i] = vword{};
+      }
+      const float f0 = scale_of(now.v_scale[0]), f1 = scale_of(now.v_scale[1]);
+#pragma unroll
+      for (int w = 0; w < VWORDS; ++w)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          ex_u32x4 f[2];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t x = __builtin_amdgcn_perm(VB[2 * j + 1][w], VB[2 * j][w], half ? 0x07030602u : 0x05010400u);
+            f[0][j] = f8_widen<TQ_BF16, false>(x, j < 2 ? f0 : f1);
+            f[1][j] = f8_widen<TQ_BF16, true>(x, j < 2 ? f0 : f1);
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int t = w * 4 + half * 2 + k;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) O[n][t] = ex_mfma<PT>(f[k], P[n], ex_mfma<PT>(f[k], L[n], O[n][t]));
+          }
+        }
+    } else {
+#pragma unroll
+      for (int c = 0; c < WIDE; ++c) {
+        if (!now.whole) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (none[i]) V[c][i] = ex_u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          ex_u32x4 f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f[j] = __builtin_amdgcn_perm(V[c][2 * j + 1][t >> 1], V[c][2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) O[n][c * 8 + t] = ex_mfma<PT>(f, P[n], ex_mfma<PT>(f, L[n], O[n][c * 8 + t]));
+        }
+      }
+      if constexpr (NARROW > 0) {
+        if (!now.whole) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (none[i]) VN[i] = ex_u32x2{0, 0};
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          ex_u32x4 f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f[j] = __builtin_amdgcn_perm(VN[2 * j + 1][t >> 1], VN[2 * j][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) O[n][WIDE * 8 + t] = ex_mfma<PT>(f, P[n], ex_mfma<PT>(f, L[n], O[n][WIDE * 8 + t]));
+        }
+      }
+    }
+    if (more) load_values(next);
+    now = next;
+  }
+
+  // ---- the four wavefronts: to a common maximum, then summed pairwise (2, 3 -> 0, 1 -> 0) ----
+  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ __align__(16) ex_f32x4 s_acc[2][TILES][64];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (n) __syncthreads();
+    const float sum_lane = ex_quad_sum(l[n]);
+    if (quarter == 0) { s_m[wave][col] = m[n]; s_l[wave][col] = sum_lane; }
+    __syncthreads();
+    const float M = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
+    const float ref = M == -INFINITY ? 0.0f : M;
+    const float f = __builtin_amdgcn_exp2f(m[n] - ref);
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) sum += s_l[w][col] * __builtin_amdgcn_exp2f(s_m[w][col] - ref);
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) O[n][t] *= f;
+    if (wave >= 2)
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) s_acc[wave - 2][t][lane] = O[n][t];
+    __syncthreads();
+    if (wave < 2)
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) O[n][t] += s_acc[wave][t][lane];
+    __syncthreads();
+    if (wave == 1)
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) s_acc[0][t][lane] = O[n][t];
+    __syncthreads();
+    if (wave == 0 && live[n]) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) O[n][t] += s_acc[0][t][lane];
+      if (a.n_split > 1 && quarter == 0) a.ml[row[n] * a.n_split + split] = make_float2(M - ex_lift<PT>(), sum);
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      float* acc = a.acc + (row[n] * a.n_split + split) * D;
+#pragma unroll
+      for (int t = 0; t < TILES; t += 4)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = F8 ? (quarter * 4 + i) * TILES + t : ex_channel<WIDE>(t, quarter, i);      // and the three after it
+          const ex_f32x4 x = {O[n][t][i], O[n][t + 1][i], O[n][t + 2][i], O[n][t + 3][i]};
+          if (a.n_split > 1) *(ex_f32x4*)(acc + c) = x;
+          else *(ex_u32x2*)((uint16_t*)a.out + row[n] * D + c) = ex_u32x2{ex_pack<QT>(x[0] * inv, x[1] * inv), ex_pack<QT>(x[2] * inv, x[3] * inv)};
+        }
+    }
+  }
+}
+
+template <int QT, bool F8>
+int launch_attend_few(const Attend& a, int tiles, unsigned grid, hipStream_t stream) {
+#define TQ_ATTEND_D(D)                                                                                 \
+  case D:                                                                                              \
+    if (tiles == 1) attend_few_kernel<QT, F8, D, 1><<<dim3(grid), dim3(256), 0, stream>>>(a);          \
+    else attend_few_kernel<QT, F8, D, 2><<<dim3(grid), dim3(256), 0, stream>>>(a);                     \
+    break
+  switch (a.d) {
+    TQ_ATTEND_D(64); TQ_ATTEND_D(128); TQ_ATTEND_D(192); TQ_ATTEND_D(256);
+    default: return TQ_EUNSUPPORTED;
+  }
+#undef TQ_ATTEND_D
+  TQ_CHECK_LAUNCH();
+  return TQ_OK;
+}
+
+}  // namespace tq

@@ -1,5 +1,6 @@
 // Decode attention over a paged exact cache: entry points, and the launch that joins splits and adds weights.
 #include "tq_exact.h"
+#include "tq_join.h"
 
 #include <algorithm>
 
@@ -10,8 +11,6 @@ namespace tq {
 // Weights: weights[b, h, t] += sum over the heads of h of 2^(s_t - M) / sum, a thread per token, heads in order: no atomics, the same
 // result every time.  Both only need what the page kernel left, so that they share a launch.  Bound by the chain of length, maxima, sums and numerators:
 // 16 x 32 rows of four splits with the weights of 16 x 8 x 8192 tokens (25 MB) 8.2 us; 96 x 40 rows with those of 96 x 8 x 61 .. 8190 (44 MB) 18 - 20.
-constexpr int JOIN_MAX_SPLITS = 1024, JOIN_FEW = 16;
-
 __device__ __forceinline__ int join_len(const ExactJoin& a, int b) {
   const int64_t most = (int64_t)a.table_row * TQ_PAGE_TOKENS;
   const int n = a.lens[b];
@@ -20,91 +19,6 @@ __device__ __forceinline__ int join_len(const ExactJoin& a, int b) {
 __device__ __forceinline__ int join_used(const ExactJoin& a, int len) {
   return exact_splits_used((len + a.block_tokens - 1) / a.block_tokens, a.n_split, a.chunk);
 }
-template <int DT>
-__device__ __forceinline__ void join_store(void* out, int64_t at, const float4& x) {
-  if constexpr (DT == TQ_F32) {
-    *(float4*)((float*)out + at) = x;
-  } else {
-    Elem<DT>::store(out, at, x.x);
-    Elem<DT>::store(out, at + 1, x.y);
-    Elem<DT>::store(out, at + 2, x.z);
-    Elem<DT>::store(out, at + 3, x.w);
-  }
-}
-
-// Few splits: a wavefront per row, a lane knows the factor of its split.
-template <int DT>
-__device__ __forceinline__ void exact_join_few(const ExactJoin& a, int row) {
-  const int lane = (int)threadIdx.x & 63;
-  const int used = join_used(a, join_len(a, row / a.Hq));
-  const float2 ml = lane < used ? a.ml[(int64_t)row * a.n_split + lane] : make_float2(-INFINITY, 0.0f);
-  const float top = wave_max_fast(ml.x), ref = top == -INFINITY ? 0.0f : top;
-  const float f = __builtin_amdgcn_exp2f(ml.x - ref), sum = wave_sum_fast(f * ml.y), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int quads = a.d >> 2;
-  for (int q = lane; q < quads; q += 64) {
-    const float4* acc = (const float4*)(a.acc + (int64_t)row * a.n_split * a.d) + q;
-    float4 o = make_float4(0, 0, 0, 0);
-    for (int i0 = 0; i0 < used; i0 += 8) {                   // eight on their way at a time, the last one over again behind the end
-      float4 x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = acc[(int64_t)(i0 + i < used ? i0 + i : used - 1) * quads];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool in = i0 + i < used;                       // (where not, a numerator of zero: a factor of zero would make NaN of an infinite one)
-        const float g = in ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (i0 + i) & 63)) : 0.0f;
-        o.x = fmaf(g, in ? x[i].x : 0.0f, o.x); o.y = fmaf(g, in ? x[i].y : 0.0f, o.y);
-        o.z = fmaf(g, in ? x[i].z : 0.0f, o.z); o.w = fmaf(g, in ? x[i].w : 0.0f, o.w);
-      }
-    }
-    join_store<DT>(a.out, (int64_t)row * a.d + q * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-  }
-}
-
-// Many splits: a workgroup per row and 64 channels, sixteen lanes to a split, sixteen splits at a time.
-template <int DT>
-__device__ __forceinline__ void exact_join_many(const ExactJoin& a, int row, int slice, float* s_f, float* s_red, float4* s_o) {
-  const int tid = (int)threadIdx.x;
-  const int used = join_used(a, join_len(a, row / a.Hq));
-  const float2* ml = a.ml + (int64_t)row * a.n_split;
-  float top = -INFINITY;
-  for (int i = tid; i < used; i += 256) top = fmaxf(top, ml[i].x);
-  top = wave_max_fast(top);
-  if ((tid & 63) == 0) s_red[tid >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-  const float ref = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f;
-  for (int i = tid; i < used; i += 256) {
-    const float2 x = ml[i];
-    const float f = __builtin_amdgcn_exp2f(x.x - ref);
-    s_f[i] = f;
-    sum += f * x.y;
-  }
-  sum = wave_sum_fast(sum);
-  if ((tid & 63) == 0) s_red[4 + (tid >> 6)] = sum;
-  __syncthreads();
-  sum = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int quad = tid & 15, share = tid >> 4;
-  const float* acc = a.acc + (int64_t)row * a.n_split * a.d + slice * 64 + quad * 4;
-  float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-  for (int i = share; i < used; i += 16) {
-    const float4 x = *(const float4*)(acc + (int64_t)i * a.d);
-    const float f = s_f[i];
-    o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
-  }
-  s_o[tid] = o;
-  __syncthreads();
-  if (share != 0) return;
-#pragma unroll
-  for (int i = 1; i < 16; ++i) {
-    const float4 x = s_o[i * 16 + quad];
-    o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
-  }
-  join_store<DT>(a.out, (int64_t)row * a.d + slice * 64 + quad * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-}
-
 // A thread's four tokens are neighbours: sixteen bytes of each head's scores.
 __device__ __forceinline__ void exact_add_weights(const ExactJoin& a, int id, float2* s_head) {
   const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -158,10 +72,14 @@ __global__ void __launch_bounds__(256) exact_join_kernel(const ExactJoin a, int 
     exact_add_weights(a, id - row_groups, s_two);
   } else if (a.n_split <= JOIN_FEW) {
     id = id * 4 + ((int)threadIdx.x >> 6);
-    if (id < a.B * a.Hq) exact_join_few<DT>(a, id);
+    if (id < a.B * a.Hq) {
+      const int lane = (int)threadIdx.x & 63, used = join_used(a, join_len(a, id / a.Hq));
+      join_few<DT>(a.acc, a.n_split, a.d, a.out, id, used, lane < used ? a.ml[(int64_t)id * a.n_split + lane] : make_float2(-INFINITY, 0.0f));
+    }
   } else {
     const int slices = a.d >> 6;
-    exact_join_many<DT>(a, id / slices, id % slices, (float*)s_two, s_red, s_o);
+    const int row = id / slices;
+    join_many<DT>(a.ml, a.acc, a.n_split, a.d, a.out, row, join_used(a, join_len(a, row / a.Hq)), id % slices, (float*)s_two, s_red, s_o);
   }
 }
 
@@ -170,10 +88,6 @@ __global__ void __launch_bounds__(256) exact_join_kernel(const ExactJoin a, int 
 static int64_t join_tokens(int64_t pairs, int64_t len) {
   const int64_t groups = pairs * ((len + 1023) / 1024);
   return 1024 * std::max<int64_t>(1, std::min<int64_t>(groups / 2048, 64));
-}
-// workgroups that join rows
-static int64_t join_groups(int64_t rows, int n_split, int d) {
-  return n_split <= 1 ? 0 : (n_split <= JOIN_FEW ? (rows + 3) / 4 : rows * (d / 64));
 }
 
 // ---- how a call is split ----------------------------------------------------------------------------------------------------------------

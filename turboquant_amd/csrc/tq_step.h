@@ -1,0 +1,102 @@
+// A step of an engine over a paged cache: rows starts[b] .. starts[b + 1] - 1 of the step's tensors are sequence b's, the last of them its token
+// lens[b] - 1, whose block is table[b][token / 16].  All of it lies in device memory; the host knows the number of rows and of sequences only.
+#pragma once
+
+#include "tq_common.h"
+
+namespace tq {
+
+struct Step {
+  const int32_t* starts;   // B + 1; null: one row per sequence
+  const int32_t* lens;
+  const int32_t* table;
+  int64_t table_step;      // entries from one sequence's row to the next; 0: one row for all
+  int64_t num_blocks;
+  int32_t table_row;       // entries of a row
+  int32_t B;
+  int64_t rows;            // of the step's tensors
+};
+
+// Sequence b's rows: [row, row + run), the first of them token `token` (negative where a sequence has more rows than tokens).  What starts says is cut to
+// the rows that there are.
+struct StepRun {
+  int64_t row;
+  int32_t run, len;
+  __device__ __forceinline__ int32_t token() const { return len - run; }
+};
+__device__ __forceinline__ StepRun step_run(const Step& s, int b) {
+  StepRun r;
+  const int n = s.lens[b];
+  r.len = n < 0 ? 0 : (n > INT32_MAX - 64 ? INT32_MAX - 64 : n);      // (so that the next block's first token is a number, too)
+  if (!s.starts) { r.row = b; r.run = 1; return r; }
+  int64_t first = s.starts[b], end = s.starts[b + 1];
+  first = first < 0 ? 0 : first;
+  end = end > s.rows ? s.rows : end;
+  r.row = first;
+  r.run = end > first ? (int32_t)(end - first) : 0;
+  return r;
+}
+// tokens that the table has blocks for
+__device__ __forceinline__ int32_t step_cap(const Step& s) {
+  const int64_t most = (int64_t)s.table_row * TQ_PAGE_TOKENS;
+  return most > INT32_MAX ? INT32_MAX : (int32_t)most;
+}
+// Rows of no sequence: in front of the first one's and behind the last one's.  Their number, and the n-th of them.
+__device__ __forceinline__ int64_t step_rest(const Step& s, int64_t* front) {
+  *front = 0;
+  if (!s.starts) return 0;
+  int64_t a = s.starts[0], z = s.starts[s.B];
+  a = a < 0 ? 0 : (a > s.rows ? s.rows : a);
+  z = z < a ? a : (z > s.rows ? s.rows : z);
+  *front = a;
+  return a + s.rows - z;
+}
+__device__ __forceinline__ int64_t step_rest_row(const Step& s, int64_t front, int64_t rest, int64_t n) { return n < front ? n : n + s.rows - rest; }
+
+// Unit `u` of a step whose sequence b has count(b) of them: its sequence and which one of them it is; false (and u less all of them) if there are fewer.
+// A whole wavefront asks; u is the same in all lanes.  A lane adds up four sequences, so that up to 256 take one round of loads.
+template <class Count>
+__device__ __forceinline__ bool step_unit(const Step& s, int64_t* u, int* b, int64_t* j, Count count) {
+  const int lane = (int)threadIdx.x & 63;
+  for (int base = 0; base < s.B; base += 256) {
+    int64_t c[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = base + lane * 4 + i;
+      c[i] = at < s.B ? (int64_t)count(step_run(s, at)) : 0;
+      sum += c[i];
+    }
+    int64_t upto = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t below = __shfl_up((long long)upto, o, 64);
+      if (lane >= o) upto += below;
+    }
+    const int64_t all = __shfl((long long)upto, 63, 64);
+    if (*u < all) {
+      const int owner = __ffsll((unsigned long long)__ballot(upto > *u)) - 1;
+      int64_t left = *u - (upto - sum);
+      int which = 0;
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (which == i && left >= c[i]) { left -= c[i]; which = i + 1; }
+      *b = __builtin_amdgcn_readfirstlane(__shfl(base + lane * 4 + which, owner, 64));
+      *j = __shfl((long long)left, owner, 64);
+      return true;
+    }
+    *u -= all;
+  }
+  return false;
+}
+
+// what the entry points check of a step, and its description
+inline int step_init(Step* s, const int32_t* starts, int64_t rows, int B, const int32_t* lens, const int32_t* table, int bt_stride, int64_t num_blocks) {
+  if (!table || (!lens && B > 0)) return TQ_ENULL;
+  if (B < 0 || rows < 0 || rows > INT32_MAX || num_blocks <= 0 || bt_stride == 0 || bt_stride == INT32_MIN) return TQ_EINVAL;
+  s->starts = starts; s->lens = lens; s->table = table; s->rows = rows; s->B = B; s->num_blocks = num_blocks;
+  s->table_row = bt_stride < 0 ? -bt_stride : bt_stride;
+  s->table_step = bt_stride < 0 ? 0 : bt_stride;
+  return TQ_OK;
+}
+
+}  // namespace tq

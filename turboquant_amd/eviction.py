@@ -51,9 +51,9 @@ class Evictions(NamedTuple):
 
 
 def own_rows(t: torch.Tensor) -> bool:
-    """Whether no two elements of t (B, H, L), slots contiguous, lie in one place."""
-    reach = t.shape[2]
-    for stride, size in sorted((t.stride(i), t.shape[i]) for i in (0, 1) if t.shape[i] > 1):
+    """Whether no two elements of t, the last dimension's contiguous, lie in one place."""
+    reach = t.shape[-1]
+    for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(t.dim() - 1) if t.shape[i] > 1):
         if stride < reach:
             return False
         reach = stride * (size - 1) + reach

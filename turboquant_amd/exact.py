@@ -15,6 +15,7 @@ from typing import Optional
 import torch
 
 from . import _ffi
+from .attend import attend, check_workspace, plan_bytes, seen_by, sequences
 from .eviction import Evictions, memory_of, own_rows
 from .paged import PAGE_TOKENS
 
@@ -63,18 +64,7 @@ class ExactPagedCache:
     # ---- arguments that the calls share ------------------------------------------------------------------------------
     def _sequences(self, block_table: torch.Tensor, seq_lens: torch.Tensor, batch: int):
         """(table, its stride as the library takes it, lengths): int32 on this GPU, contiguous."""
-        if block_table.dtype != torch.int32 or block_table.dim() not in (1, 2) or block_table.shape[-1] == 0:
-            raise ValueError("block_table must be int32 (B, max_pages), or (max_pages,) for all sequences")
-        if block_table.dim() == 2 and block_table.shape[0] != batch:
-            raise ValueError(f"block_table has {block_table.shape[0]} rows for {batch} sequences")
-        if seq_lens.shape != (batch,):
-            raise ValueError(f"seq_lens must have one entry for each of {batch} sequences")
-        _ffi.require_gpu(block_table, "block_table")
-        if block_table.device != self.device:
-            raise ValueError(f"block_table lives on {block_table.device}, the cache on {self.device}")
-        table = block_table.contiguous().resolve_neg()
-        lens = seq_lens.to(device=self.device, dtype=torch.int32).contiguous().resolve_neg()
-        return table, (-table.shape[0] if table.dim() == 1 else table.shape[1]), lens
+        return sequences(self.device, block_table, seq_lens, batch)
 
     def _weights(self, weights: torch.Tensor, batch: int) -> None:
         _ffi.require_gpu(weights, "weights")
@@ -91,15 +81,21 @@ class ExactPagedCache:
     def decode_attention(self, query: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                          scale: Optional[float] = None, weights: Optional[torch.Tensor] = None,
                          n_split: Optional[int] = None, workspace: Optional[torch.Tensor] = None,
-                         out: Optional[torch.Tensor] = None, max_len: Optional[int] = None) -> torch.Tensor:
+                         out: Optional[torch.Tensor] = None, max_len: Optional[int] = None, window: Optional[int] = None,
+                         sinks: int = 0) -> torch.Tensor:
         """softmax(scale * q K^T) V for one query token per sequence, query (B, Hq, d) in the cache's dtype, over the
-        seq_lens[b] tokens that block_table (B, max_pages) or (max_pages,) names; zeros for a sequence without tokens.
+        seq_lens[b] tokens that block_table (B, max_pages) or (max_pages,) names; zeros for a sequence without tokens.  With a window over the last
+        `window` of them and the first `sinks` only, as `attention` takes it (no weights, and `out` is memory of its own).
 
         weights (B, H_kv, L) float32, tokens contiguous: every token's softmax weight, summed over the query heads of its KV
         head, is added in place (tokens from L on have no place in it); meanwhile the step keeps 4 bytes for each of L places and query heads, so
         that weights of a large capacity are best given as weights[..., :longest].  max_len bounds the lengths for the plan of the
         splits: without it the width of the table does.  out: memory of its own, or the query itself.  The `workspace` of a step (`workspace()`) belongs to it alone until
         it has run: graphs that may run at the same time need one each."""
+        if window is not None or sinks:
+            if weights is not None:
+                raise ValueError("weights are summed over whole sequences, not within a window")
+            return attend("decode_attention", self, query, None, block_table, seq_lens, scale, window, sinks, n_split, workspace, out, max_len, None)
         fast = _ffi.native()
         if fast is not None and n_split is None and workspace is None and out is None:
             done = fast.exact_decode(query, block_table, seq_lens, self.key_cache, self.value_cache, scale, max_len, weights)
@@ -148,7 +144,7 @@ class ExactPagedCache:
         if workspace is None:
             workspace = torch.empty(need // 4, dtype=torch.float32, device=self.device)
         else:
-            self._check_workspace(workspace, need)
+            check_workspace(workspace, need, self.device)
         with _ffi.on_device(self.device):
             _ffi.check(_ffi.lib().tq_exact_decode(
                 query.data_ptr(), self._tag, B, Hq, self.num_kv_heads, d, self.key_cache.data_ptr(), self.value_cache.data_ptr(),
@@ -167,6 +163,33 @@ class ExactPagedCache:
         if need == 0:
             raise ValueError(f"no plan for {B} x {Hq} query heads, max_len {max_len}, n_split {splits}")
         return need
+
+    def attention(self, query: torch.Tensor, query_start_loc: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                  scale: Optional[float] = None, window: Optional[int] = None, sinks: int = 0, n_split: Optional[int] = None,
+                  workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, max_len: Optional[int] = None,
+                  max_rows: Optional[int] = None) -> torch.Tensor:
+        """softmax(scale * q K^T) V for the rows of a step, query (rows, Hq, d) in the cache's dtype (fp16 or bf16; head_dim 64, 128, 192 or 256), whose keys and
+        values are in the blocks: row i of sequence b's n = query_start_loc[b + 1] - query_start_loc[b] stands at position p = seq_lens[b] - n + i and sees the
+        tokens up to its own; with a window only those behind p - window, and the first `sinks`.  A row that sees nothing is zeros.  Rows
+        behind the last sequence are zeros, or left as they are in a given `out`, which is memory of its own.
+
+        max_len and max_rows bound the lengths and a sequence's rows for the plan of the splits (without them the table's width and all rows
+        do).  The `workspace` of a step (`step_workspace()`) belongs to it alone until it has run: graphs that may run at the same time need one each."""
+        return attend("attention", self, query, query_start_loc, block_table, seq_lens, scale, window, sinks, n_split, workspace, out, max_len, max_rows)
+
+    def step_workspace(self, rows: int, Hq: int, max_len: int, B: Optional[int] = None, max_rows: Optional[int] = None, window: Optional[int] = None,
+                       sinks: int = 0, n_split: Optional[int] = None) -> torch.Tensor:
+        """A workspace for `attention` of this size over B sequences, or, without B, for `decode_attention` within a window."""
+        window, sinks = seen_by(window, sinks)
+        need = plan_bytes(self, self.dtype, B is not None, rows, rows if B is None else B, Hq, max_len, rows if max_rows is None else max_rows, window, sinks,
+                          n_split or 0)
+        return torch.empty(need // 4, dtype=torch.float32, device=self.device)
+
+    def tensors(self) -> dict:
+        return dict(key_cache=self.key_cache, value_cache=self.value_cache)
+
+    def _memory(self):
+        return self.key_cache.data_ptr(), self.value_cache.data_ptr(), None, None
 
     def workspace(self, B: int, Hq: int, max_len: int, n_split: Optional[int] = None, weight_len: int = 0) -> torch.Tensor:
         """A workspace for decode steps of this size; weight_len: the last dimension of `weights`, 0 without them."""
@@ -241,11 +264,3 @@ class ExactPagedCache:
                 table.data_ptr(), bt_stride, count.data_ptr(), dst.data_ptr(), src.data_ptr(), B, H, moves, _ffi.stream_ptr(self.device)),
                 "tq_move_tokens_exact")
         _ffi.changed(self.key_cache, self.value_cache)
-
-    def _check_workspace(self, workspace: torch.Tensor, need: int) -> None:
-        _ffi.require_gpu(workspace, "workspace")
-        have = workspace.numel() * workspace.element_size()
-        if have < need:
-            raise ValueError(f"the workspace holds {have} bytes, this step takes {need}")
-        if workspace.device != self.device or not workspace.is_contiguous() or workspace.data_ptr() % 16:
-            raise ValueError("the workspace must be contiguous, on a 16-byte boundary and on the cache's GPU")
