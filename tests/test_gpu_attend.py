@@ -110,6 +110,8 @@ def test_large_scores_and_scales(gpu, kind):
     """One token has all the weight; negative and zero scales."""
     s = make(kind, [300, 40], [1, 9], 1, 64)
     run(s, 2, size=30.0)
+    run(make(kind, [200, 90], [70, 3], 1, 64), 4, scale=-0.3)
+    run(make(kind, [200, 90], [70, 3], 1, 64), 4, scale=0.0)
     run(s, 2, scale=-0.2)
     run(s, 2, scale=0.0)
 

@@ -20,6 +20,7 @@ SOURCES = ["tq_decode_mfma_d128.hip", "tq_decode_mfma_d128_f16.hip", "tq_decode_
            "tq_quantize.hip", "tq_score.hip", "tq_decode.hip", "tq_decode_mfma.hip", "tq_exact_bf16.hip", "tq_exact_f16.hip",
            "tq_exact_f32.hip", "tq_exact_heads_bf16.hip", "tq_exact_heads_f16.hip", "tq_exact.hip", "tq_exact_window_bf16.hip", "tq_exact_window_f16.hip", "tq_exact_window_f32.hip",
            "tq_exact_window.hip", "tq_attend_few_bf16.hip", "tq_attend_few_f16.hip", "tq_attend_few_fp8_bf16.hip", "tq_attend_few_fp8_f16.hip",
+           "tq_attend_rows_bf16.hip", "tq_attend_rows_f16.hip", "tq_attend_rows_fp8_bf16.hip", "tq_attend_rows_fp8_f16.hip",
            "tq_attend.hip", "tq_fp8_store.hip", "tq_rotate.hip", "tq_evict.hip", "tq_probe.hip"]
 
 # packed-fp32 instructions stay off: some of their forms have produced wrong

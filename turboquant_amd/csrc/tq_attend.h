@@ -83,8 +83,21 @@ __device__ __forceinline__ bool attend_unit(const Attend& a, int64_t* u, AttendU
   return true;
 }
 
-// elements of a cache: TQ_F16, TQ_BF16, or
-constexpr int TQ_CACHE_E4M3 = TQ_E4M3;
+// Units behind the last sequence's, of which this is number `number` of `others`: rows of no sequence, KV head h's part of them
+template <int D>
+__device__ __forceinline__ void attend_rest(const Attend& a, int split, int h, int64_t number, int64_t others) {
+  if (split) return;
+  int64_t front;
+  const int64_t rest = step_rest(a.s, &front);
+  for (int64_t n = number; n < rest; n += others) {
+    const int64_t row = step_rest_row(a.s, front, rest, n) * a.Hq + h * a.G;
+    if (a.n_split > 1) {
+      for (int g = (int)threadIdx.x; g < a.G; g += 256) a.ml[(row + g) * a.n_split] = make_float2(-INFINITY, ATTEND_REST);
+    } else if (a.fill) {
+      for (int c = (int)threadIdx.x; c < a.G * D / 2; c += 256) ((uint32_t*)((uint16_t*)a.out + row * D))[c] = 0;
+    }
+  }
+}
 
 template <int QT, bool F8> int launch_attend_few(const Attend& a, int tiles, unsigned grid, hipStream_t stream);
 template <int QT, bool F8> int launch_attend_rows(const Attend& a, unsigned grid, hipStream_t stream);

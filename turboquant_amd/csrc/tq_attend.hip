@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendJoin a) {
 
 // ---- how a call is split ----------------------------------------------------------------------------------------------------------------
 struct AttendPlan {
-  int tiles;                          // column tiles of the kernel of few rows
+  int tiles;                          // column tiles of the kernel of few rows; 0: the kernel of many
   int64_t units, grid;
   int n_split, chunk;
   size_t ml_at, acc_at, bytes;
@@ -78,8 +78,8 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   const int G = Hq / Hkv;
   if (G > 1024) return false;
   max_rows = starts ? std::max<int64_t>(1, std::min(max_rows, rows)) : 1;
-  p->tiles = max_rows * G <= 16 ? 1 : 2;
-  const int M = 16 * p->tiles, TB = 32;
+  p->tiles = max_rows * G <= 16 ? 1 : (max_rows * G <= 32 ? 2 : 0);
+  const int M = p->tiles ? 16 * p->tiles : 128, TB = p->tiles ? 32 : 64;
   p->units = starts ? (rows * G + M - 1) / M + B + 1 : (int64_t)B * ((G + M - 1) / M);
   // (of these, up to B are not met, and most of a short row's are)
   const int64_t busy = starts ? std::max<int64_t>(std::min<int64_t>(B, rows), (rows * G + M - 1) / M) : p->units;
@@ -89,13 +89,14 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   const int64_t blocks = (tokens + TB - 1) / TB;
   int64_t n = n_split;
   if (n == 0) {
-    const int64_t resident = 256 * (p->tiles == 1 ? 3 : 2);
-    n = std::max((resident + pairs - 1) / pairs, (tokens + 1023) / 1024);
+    const int64_t resident = 256 * (p->tiles == 1 ? 3 : (p->tiles || d <= 128 ? 2 : 1));
+    n = (resident + pairs - 1) / pairs;
+    if (p->tiles) n = std::max(n, (tokens + 1023) / 1024);
     n = std::min<int64_t>(std::min<int64_t>(n, (blocks + 3) / 4), JOIN_MAX_SPLITS);
   }
   n = std::max<int64_t>(1, std::min(n, blocks));
   int64_t chunk = (blocks + n - 1) / n;
-  if (n_split == 0) chunk = (chunk + 3) & ~(int64_t)3;                             // (a block for each of the four wavefronts)
+  if (n_split == 0 && p->tiles) chunk = (chunk + 3) & ~(int64_t)3;                             // (a block for each of the four wavefronts)
   p->n_split = (int)std::max<int64_t>(1, (blocks + chunk - 1) / chunk);
   p->chunk = (int)chunk;
   const size_t all = (size_t)rows * Hq;
@@ -145,8 +146,14 @@ extern "C" int tq_attend(const void* q, int dtype, int64_t rows, const int32_t* 
   a.acc = (float*)((char*)workspace + p.acc_at);
   hipStream_t st = (hipStream_t)stream;
   int rc;
-  if (cache == TQ_E4M3) rc = dtype == TQ_F16 ? launch_attend_few<TQ_F16, true>(a, p.tiles, (unsigned)p.grid, st) : launch_attend_few<TQ_BF16, true>(a, p.tiles, (unsigned)p.grid, st);
-  else rc = dtype == TQ_F16 ? launch_attend_few<TQ_F16, false>(a, p.tiles, (unsigned)p.grid, st) : launch_attend_few<TQ_BF16, false>(a, p.tiles, (unsigned)p.grid, st);
+  const unsigned g = (unsigned)p.grid;
+  if (p.tiles) {
+    if (cache == TQ_E4M3) rc = dtype == TQ_F16 ? launch_attend_few<TQ_F16, true>(a, p.tiles, g, st) : launch_attend_few<TQ_BF16, true>(a, p.tiles, g, st);
+    else rc = dtype == TQ_F16 ? launch_attend_few<TQ_F16, false>(a, p.tiles, g, st) : launch_attend_few<TQ_BF16, false>(a, p.tiles, g, st);
+  } else {
+    if (cache == TQ_E4M3) rc = dtype == TQ_F16 ? launch_attend_rows<TQ_F16, true>(a, g, st) : launch_attend_rows<TQ_BF16, true>(a, g, st);
+    else rc = dtype == TQ_F16 ? launch_attend_rows<TQ_F16, false>(a, g, st) : launch_attend_rows<TQ_BF16, false>(a, g, st);
+  }
   if (rc || p.n_split == 1) return rc;
   const AttendJoin j{a.ml, a.acc, out, rows * Hq, p.n_split, d, fill};
   const dim3 grid((unsigned)join_groups(j.rows, p.n_split, d)), block(256);

@@ -46,18 +46,7 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
   int64_t number = pair / (unsigned)a.H;
   AttendUnit u;
   if (!attend_unit<16 * NT>(a, &number, &u)) {
-    // units behind the last: rows of no sequence, this KV head's part of them
-    if (split) return;
-    int64_t front;
-    const int64_t rest = step_rest(a.s, &front), others = a.units - (pair / (unsigned)a.H - number);
-    for (int64_t n = number; n < rest; n += others) {
-      const int64_t row = step_rest_row(a.s, front, rest, n) * a.Hq + h * a.G;
-      if (a.n_split > 1) {
-        for (int g = (int)threadIdx.x; g < a.G; g += 256) a.ml[(row + g) * a.n_split] = make_float2(-INFINITY, ATTEND_REST);
-      } else if (a.fill) {
-        for (int c = (int)threadIdx.x; c < a.G * D / 2; c += 256) ((uint32_t*)((uint16_t*)a.out + row * D))[c] = 0;
-      }
-    }
+    attend_rest<D>(a, (int)split, h, number, a.units - (pair / (unsigned)a.H - number));
     return;
   }
   const AttendBlocks<TB> list(a, u);

@@ -1,0 +1,369 @@
+// Attention of many rows - prompts, chunks of them, dozens of query heads on one KV head - over a paged cache (instantiated by one file per types).
+//
+// A unit is 128 RT rows of a KV head: the query heads of a token side by side, tokens one behind another.  A wavefront takes 32 RT of them, each a column of
+// its matrix instructions; the workgroup's keys and values go through LDS, 64 tokens at a time, in 16 bits whatever the cache holds, two buffers in turn:
+// the next tokens are on their way in registers while these are worked on, and a turn has one barrier.
+//   scores    S^T = K Q^T: tokens are rows.  A lane has 32 of the 64 scores of a row, its neighbour 32 lanes on the others.
+//   softmax   one pass, running maximum and sum per row in 32 bits; the reference moves by 2^8 at a time (EX_SLACK).
+//   values    O^T = V^T P^T: the contraction takes the tokens in the order in which a lane holds the weights already, so that no weight changes its lane;
+//             the transposing LDS read brings values in that order.
+// Weights are rounded once, to 16 bits, half a step of 2^-9 (fp16: 2^-12) that a sum over many averages out; a high and a low half, as the kernel of few
+// rows has them, would be half as many matrix instructions again.  8 bits for fp16 queries: bf16 values, whose range the block's scale
+// needs, and there the weights are two halves: one of bf16 would be eight times coarser than the output.
+// LDS: 16-byte pieces of a row change places by the row (rows_key_turn, rows_value_turn), so that neither reads nor writes meet in a bank.
+#pragma once
+
+#include "tq_attend.h"
+#include "tq_attend_few_impl.h"
+
+namespace tq {
+
+typedef float ro_f32x16 __attribute__((ext_vector_type(16)));
+typedef short ro_s16x4 __attribute__((ext_vector_type(4)));
+
+template <int DT>
+__device__ __forceinline__ ro_f32x16 rows_mfma(ex_u32x4 a, ex_u32x4 b, ro_f32x16 c) {
+  if constexpr (DT == TQ_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(ex_bf16x8, a), __builtin_bit_cast(ex_bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ex_f16x8, a), __builtin_bit_cast(ex_f16x8, b), c, 0, 0, 0);
+}
+
+constexpr int ROWS_TOKENS = 64;
+template <int D> constexpr int rows_lds() { return 2 * 2 * ROWS_TOKENS * D * 2; }
+
+// Where piece c (16 bytes, 8 channels) of a token's row lies.  Rows of 256 and 512 bytes begin in the same bank, of 128 and 384 in one of two.
+// Keys: 16 lanes read the same piece of 16 rows.  Values: 16 lanes read 32 bytes of 4 rows, the 16 beside them the next 32.
+template <int D> __device__ __forceinline__ int rows_key_turn(int t) { return D % 128 == 0 ? (t & 15) : ((t >> 1) & 7); }
+template <int D> __device__ __forceinline__ int rows_value_turn(int t) { return D % 128 == 0 ? (t & 3) << 2 : ((t >> 1) & 1) << 2; }
+
+template <int QT, bool F8, int D, int RT>
+__global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_rows_kernel(const Attend a) {
+  constexpr int PT = F8 ? TQ_BF16 : QT;                      // of the value product
+  constexpr bool HALVES = F8 && QT == TQ_F16;                // weights in two halves
+  constexpr bool FOLD = F8 && QT == TQ_BF16;                 // a key's scale goes into the key
+  constexpr int SIZE = F8 ? 1 : 2, ROW = D * 2;              // bytes of an element in the cache, of a row in LDS
+  constexpr int LANES = D * SIZE / 16, LOADS = ROWS_TOKENS * LANES / 256;
+  constexpr int KSTEPS = D / 16, TILES = D / 32, M = 128 * RT;
+  constexpr int HALF = ROWS_TOKENS * ROW;                    // keys or values of a turn
+  extern __shared__ __attribute__((aligned(16))) char s_rows[];
+
+  const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 31, half = lane >> 5;
+  // (the last units of a sequence have the most tokens: they begin first)
+  const unsigned pairs = (unsigned)(a.units * a.H), split = blockIdx.x / pairs, pair = (blockIdx.x - split * pairs + split) % pairs;
+  const int h = (int)(pair % (unsigned)a.H);
+  const int64_t unit = a.units - 1 - pair / (unsigned)a.H;
+  int64_t number = unit;
+  AttendUnit u;
+  if (!attend_unit<M>(a, &number, &u)) {
+    attend_rest<D>(a, (int)split, h, number, a.units - (unit - number));
+    return;
+  }
+  const AttendBlocks<ROWS_TOKENS> list(a, u);
+  const int per = attend_per_split(list.count, a.n_split, a.chunk);
+  const int first = (int)split * per < list.count ? (int)split * per : list.count, last = first + per < list.count ? first + per : list.count;
+
+  bool live[RT];
+  int64_t row[RT];
+  int at_p[RT], behind[RT];
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+    const int r = (wave * RT + n) * 32 + col;
+    live[n] = r < u.rows;
+    const int x = u.first + (live[n] ? r : 0), i = x / a.G;
+    row[n] = (u.row + i) * a.Hq + h * a.G + (x - i * a.G);
+    at_p[n] = u.low + (i - u.first / a.G);
+    behind[n] = attend_behind(a, at_p[n]);
+  }
+  if (first >= last && a.n_split > 1) {
+#pragma unroll
+    for (int n = 0; n < RT; ++n)
+      if (half == 0 && live[n]) a.ml[row[n] * a.n_split + split] = make_float2(-INFINITY, ATTEND_EMPTY);
+    return;
+  }
+  // the wavefront's first and last positions
+  const int r0 = wave * RT * 32, r1 = r0 + RT * 32 - 1;
+  const bool busy = r0 < u.rows;
+  const int w_low = u.low + (u.first + r0) / a.G - u.first / a.G, w_high = u.low + (u.first + (r1 < u.rows ? r1 : u.rows - 1)) / a.G - u.first / a.G;
+  const int w_behind_low = attend_behind(a, w_low), w_behind_high = attend_behind(a, w_high);
+  const int32_t* table = a.s.table + u.b * a.s.table_step;
+
+  // (a negative scale turns the queries and one of zero clears them, so that the scores' order is that of their products)
+  const float f = a.scale2 == 0.0f ? 1.0f : fabsf(a.scale2);
+  const uint32_t turn = a.scale2 < 0.0f ? 0x80008000u : 0u, keep = a.scale2 == 0.0f ? 0u : 0xffffffffu;
+  ex_u32x4 Q[RT][KSTEPS];
+#pragma unroll
+  for (int n = 0; n < RT; ++n)
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) {
+      Q[n][s] = ex_u32x4{0, 0, 0, 0};
+      if (live[n]) Q[n][s] = *(const ex_u32x4*)((const uint16_t*)a.q + row[n] * D + s * 16 + half * 8);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Q[n][s][i] = (Q[n][s][i] & keep) ^ turn;
+    }
+  ro_f32x16 O[RT][TILES];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) O[n][t][i] = 0.0f;
+    m[n] = -INFINITY;
+    l[n] = 0.0f;
+  }
+
+  // ---- a turn's tokens: table entries, loads into registers, registers into LDS ----
+  const int last_page = u.tokens > 0 ? (u.tokens - 1) / TQ_PAGE_TOKENS : 0;
+  struct Turn {
+    int32_t entry[4];
+    int t0;
+  };
+  const auto entries = [&](Turn& x, int i) __attribute__((always_inline)) {
+    const int at = i < last ? i : last - 1, blk = list[at < 0 ? 0 : at];      // (a unit without tokens: block 0, of which nothing is used)
+    x.t0 = blk * ROWS_TOKENS;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int page = blk * 4 + p;
+      x.entry[p] = table[page < last_page ? page : last_page];
+    }
+  };
+  ex_u32x4 KR[LOADS], VR[LOADS];
+  uint32_t ks[F8 ? LOADS : 1], vs[F8 ? LOADS : 1];
+  const auto token_of = [&](int i) __attribute__((always_inline)) { return (i * 256 + tid) / LANES; };
+  const auto good = [&](int32_t e) __attribute__((always_inline)) { return e >= 0 && e < a.s.num_blocks; };
+  const auto entry_of = [&](const Turn& x, int t) __attribute__((always_inline)) {
+    int p = t >> 4;
+    if constexpr (D != 192) p = __builtin_amdgcn_readfirstlane(p);      // (a wavefront's lanes are in one page)
+    return p == 0 ? x.entry[0] : (p == 1 ? x.entry[1] : (p == 2 ? x.entry[2] : x.entry[3]));
+  };
+  const auto load = [&](const Turn& x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int t = token_of(i), c = (i * 256 + tid) - t * LANES;
+      const int32_t e = entry_of(x, t);
+      const int64_t page = good(e) ? e : 0;
+      const int64_t at = (page * a.s_blk + h * a.s_h) * SIZE + (uint32_t)(t & 15) * (uint32_t)(a.s_t * SIZE) + c * 16;
+      KR[i] = *(const ex_u32x4*)((const char*)a.k + at);
+      VR[i] = *(const ex_u32x4*)((const char*)a.v + at);
+      if constexpr (F8) {
+        ks[i] = a.k_scales[page * a.H + h];
+        vs[i] = a.v_scales[page * a.H + h];
+      }
+    }
+  };
+  const auto scale_of = [](uint32_t byte) __attribute__((always_inline)) { return byte == 0 ? 0x1p-127f : __uint_as_float(byte << 23); };
+  const auto store = [&](const Turn& x, char* to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int t = token_of(i), c = (i * 256 + tid) - t * LANES;
+      // values of tokens that nobody sees are zeros: what lies in their slots may be NaN
+      const bool none = x.t0 + t >= u.tokens || !good(entry_of(x, t));
+      char *k = to + t * ROW, *v = to + HALF + t * ROW;
+      const int kt = rows_key_turn<D>(t), vt = rows_value_turn<D>(t);
+      if (none) VR[i] = ex_u32x4{0, 0, 0, 0};
+      if constexpr (F8) {
+        const float kf = FOLD ? scale_of(ks[i]) : 1.0f, vf = scale_of(vs[i]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          ex_u32x4 y, z;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            y[w * 2] = f8_widen<QT, false>(KR[i][j * 2 + w], kf);
+            y[w * 2 + 1] = f8_widen<QT, true>(KR[i][j * 2 + w], kf);
+            z[w * 2] = f8_widen<TQ_BF16, false>(VR[i][j * 2 + w], vf);
+            z[w * 2 + 1] = f8_widen<TQ_BF16, true>(VR[i][j * 2 + w], vf);
+          }
+          *(ex_u32x4*)(k + ((c * 2 + j) ^ kt) * 16) = y;
+          *(ex_u32x4*)(v + ((c * 2 + j) ^ vt) * 16) = z;
+        }
+      } else {
+        *(ex_u32x4*)(k + (c ^ kt) * 16) = KR[i];
+        *(ex_u32x4*)(v + (c ^ vt) * 16) = VR[i];
+      }
+    }
+  };
+  // ---- a lane's places in LDS ----
+  const int k_turn = rows_key_turn<D>(col);
+  const int j16 = lane & 15, v_turn = D % 128 == 0 ? j16 >> 2 : j16 >> 3;
+  const auto key_place = [&](int s) __attribute__((always_inline)) { return (uint32_t)(col * ROW + ((s * 2 + half) ^ k_turn) * 16); };
+  const auto value_place = [&](int ct) __attribute__((always_inline)) {
+    return (uint32_t)(HALF + (half * 4 + (j16 >> 2)) * ROW + ((ct ^ v_turn) * 4 + ((lane >> 4) & 1) * 2 + ((j16 & 3) >> 1)) * 16 + (j16 & 1) * 8);
+  };
+  constexpr int KPLACES = D % 128 == 0 ? 8 : 4, VPLACES = D % 128 == 0 ? 4 : 2;
+  uint32_t kp[KPLACES], vp[VPLACES];
+#pragma unroll
+  for (int s = 0; s < KPLACES; ++s) kp[s] = key_place(s);
+#pragma unroll
+  for (int t = 0; t < VPLACES; ++t) vp[t] = value_place(t);
+
+  Turn now, next;
+  entries(now, first);
+  if (first < last) {
+    load(now);
+    store(now, s_rows);
+  }
+  entries(next, first + 1);
+  __syncthreads();
+  for (int i = first; i < last; ++i) {
+    const bool more = i + 1 < last;
+    char* buffer = s_rows + ((i - first) & 1) * 2 * HALF;
+    char* other = s_rows + (((i - first) & 1) ^ 1) * 2 * HALF;
+    Turn after;
+    if (more) {
+      load(next);
+      entries(after, i + 2);
+    }
+    // what this wavefront's rows see of the turn: nothing, all of it, or some
+    const int t0 = now.t0, t1 = t0 + ROWS_TOKENS - 1;
+    const bool any = busy && t0 <= w_high && (t1 > w_behind_low || t0 < a.sinks);
+    if (any) {
+      bool whole = t1 <= w_low && t1 < u.tokens && (t0 > w_behind_high || t1 < a.sinks);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) whole = whole && good(now.entry[p]);
+      ro_f32x16 S[RT][2];
+#pragma unroll
+      for (int T = 0; T < 2; ++T) {
+#pragma unroll
+        for (int n = 0; n < RT; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) S[n][T][e] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KSTEPS; ++s) {
+          const ex_u32x4 k = *(const ex_u32x4*)(buffer + kp[s % KPLACES] + (s / KPLACES) * KPLACES * 32 + T * 32 * ROW);
+#pragma unroll
+          for (int n = 0; n < RT; ++n) S[n][T] = rows_mfma<QT>(k, Q[n][s], S[n][T]);
+        }
+      }
+      if constexpr (F8 && !FOLD) {
+        float g[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int64_t page = good(now.entry[p]) ? now.entry[p] : 0;
+          g[p] = scale_of(a.k_scales[page * a.H + h]);
+        }
+#pragma unroll
+        for (int n = 0; n < RT; ++n)
+#pragma unroll
+          for (int T = 0; T < 2; ++T)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) S[n][T][e] *= g[T * 2 + (e >> 3)];
+      }
+      ex_u32x4 P[RT][4], L[HALVES ? RT : 1][4];
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+        if (!whole) {
+#pragma unroll
+          for (int T = 0; T < 2; ++T)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int in = T * 32 + (e >> 2) * 8 + half * 4 + (e & 3), t = t0 + in;
+              const bool seen = t <= at_p[n] && t < u.tokens && (t > behind[n] || t < a.sinks) && good(now.entry[T * 2 + (e >> 3)]);
+              if (!seen) S[n][T][e] = -INFINITY;
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, S[n][T][e]);
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * f;
+        top = fmaxf(m[n], top);
+        if (__any(top > m[n] + EX_SLACK)) {
+          const float move = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[n] - top);
+          l[n] *= move;
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) O[n][t] *= move;
+          m[n] = top;
+        }
+        const float ref = m[n] == -INFINITY ? 0.0f : m[n] - ex_lift<PT>();
+        float sum = 0.0f;
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(S[n][T][e], f, -ref));
+            S[n][T][e] = p;
+            sum += p;
+          }
+        l[n] += sum;
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const int at = T * 2 + (e >> 3), w = (e & 7) >> 1;
+            if constexpr (HALVES) {
+              uint32_t hi, lo;
+              ex_split<PT>(S[n][T][e], S[n][T][e + 1], &hi, &lo);
+              P[n][at][w] = hi;
+              L[n][at][w] = lo;
+            } else {
+              P[n][at][w] = ex_pack<PT>(S[n][T][e], S[n][T][e + 1]);
+            }
+          }
+      }
+#pragma unroll
+      for (int at = 0; at < 4; ++at)
+#pragma unroll
+        for (int ct = 0; ct < TILES; ++ct) {
+          char* from = buffer + vp[ct % VPLACES] + (ct / VPLACES) * VPLACES * 64 + at * 16 * ROW;
+          typedef __attribute__((address_space(3))) ro_s16x4* lds4;
+          const ro_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)from);
+          const ro_s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(from + 8 * ROW));
+          const ex_u32x2 lo = __builtin_bit_cast(ex_u32x2, x), hi = __builtin_bit_cast(ex_u32x2, y);
+          const ex_u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+          for (int n = 0; n < RT; ++n) {
+            if constexpr (HALVES) O[n][ct] = rows_mfma<PT>(v, L[n][at], O[n][ct]);
+            O[n][ct] = rows_mfma<PT>(v, P[n][at], O[n][ct]);
+          }
+        }
+    }
+    if (more) store(next, other);
+    __syncthreads();
+    now = next;
+    next = after;
+  }
+
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l[n]), __float_as_uint(l[n]), false, false);
+    const float sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+    if (!live[n]) continue;
+    if (a.n_split > 1 && half == 0) a.ml[row[n] * a.n_split + split] = make_float2(m[n] - ex_lift<PT>(), sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float* acc = a.acc + (row[n] * a.n_split + split) * D;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int c = t * 32 + (e >> 2) * 8 + half * 4;       // and the three after it
+        const ex_f32x4 x = {O[n][t][e], O[n][t][e + 1], O[n][t][e + 2], O[n][t][e + 3]};
+        if (a.n_split > 1) *(ex_f32x4*)(acc + c) = x;
+        else *(ex_u32x2*)((uint16_t*)a.out + row[n] * D + c) = ex_u32x2{ex_pack<QT>(x[0] * inv, x[1] * inv), ex_pack<QT>(x[2] * inv, x[3] * inv)};
+      }
+  }
+}
+
+template <int QT, bool F8, int D>
+int launch_attend_rows_d(const Attend& a, unsigned grid, hipStream_t stream) {
+  static std::atomic<uint64_t> ready{0};
+  if (const int rc = exact_allow_lds((const void*)attend_rows_kernel<QT, F8, D, 1>, rows_lds<D>(), ready)) return rc;
+  attend_rows_kernel<QT, F8, D, 1><<<dim3(grid), dim3(256), rows_lds<D>(), stream>>>(a);
+  TQ_CHECK_LAUNCH();
+  return TQ_OK;
+}
+
+template <int QT, bool F8>
+int launch_attend_rows(const Attend& a, unsigned grid, hipStream_t stream) {
+  switch (a.d) {
+    case 64: return launch_attend_rows_d<QT, F8, 64>(a, grid, stream);
+    case 128: return launch_attend_rows_d<QT, F8, 128>(a, grid, stream);
+    case 192: return launch_attend_rows_d<QT, F8, 192>(a, grid, stream);
+    case 256: return launch_attend_rows_d<QT, F8, 256>(a, grid, stream);
+    default: return TQ_EUNSUPPORTED;
+  }
+}
+
+}  // namespace tq
