@@ -71,7 +71,13 @@ __device__ __forceinline__ bool attend_unit(const Attend& a, int64_t* u, AttendU
   } else if (!step_unit(a.s, u, &t->b, &j, [&](const StepRun& x) { return ((int64_t)x.run * a.G + M - 1) / M; })) {
     return false;
   }
+  // (all of it is the same for the whole wavefront, which only the scalar registers say to the compiler: its tables' entries are scalar loads then)
+  t->b = __builtin_amdgcn_readfirstlane(t->b);
+  j = step_uniform(j);
   r = step_run(a.s, t->b);
+  r.row = step_uniform(r.row);
+  r.run = __builtin_amdgcn_readfirstlane(r.run);
+  r.len = __builtin_amdgcn_readfirstlane(r.len);
   t->row = r.row;
   t->first = (int)(j * M);
   const int64_t left = (int64_t)r.run * a.G - j * M;

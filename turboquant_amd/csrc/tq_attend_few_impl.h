@@ -25,8 +25,8 @@ __device__ __forceinline__ uint32_t f8_widen(uint32_t x, float scale) {
 
 template <bool F8, int D, int NT>
 constexpr int attend_few_waves() {
-  if (NT == 1) return F8 ? (D <= 128 ? 4 : (D <= 192 ? 3 : 2)) : (D <= 64 ? 4 : (D <= 128 ? 3 : (D <= 192 ? 2 : 1)));
-  return F8 ? (D <= 64 ? 4 : (D <= 128 ? 2 : 1)) : (D <= 64 ? 3 : (D <= 128 ? 2 : 1));
+  if (NT == 1) return F8 ? (D <= 64 ? 4 : (D <= 128 ? 3 : 2)) : (D <= 64 ? 4 : (D <= 128 ? 3 : (D <= 192 ? 2 : 1)));
+  return F8 ? (D <= 64 ? 3 : (D <= 128 ? 2 : 1)) : (D <= 64 ? 3 : (D <= 128 ? 2 : 1));
 }
 
 template <int QT, bool F8, int D, int NT>
@@ -98,35 +98,39 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
   // a block's two pages: where they lie, their scales, how many of their tokens count
   struct Pages {
     int64_t at[PAGES];
-    uint32_t k_scale[PAGES], v_scale[PAGES];                 // (bytes as they are loaded: they are first looked at a block later)
+    uint32_t scales;                                         // lane l's: of page l & 1, of its keys or (l & 2) its values
     int valid[PAGES], t0;
     bool whole;
   };
+  struct Entries {
+    int32_t page[PAGES];
+    int blk;
+  };
   const int last_page = u.tokens > 0 ? (u.tokens - 1) / TQ_PAGE_TOKENS : 0;
-  const int low_behind = attend_behind(a, u.high);
-  const auto find = [&](Pages& x, int i) __attribute__((always_inline)) {
-    const int blk = list[i];
-    x.t0 = blk * TB;
+  const int low_behind = attend_behind(a, u.high), unit_behind = attend_behind(a, u.low);
+  // (table entries are read two blocks ahead, without a condition around them: those behind the last block are the last page's)
+  const auto entries = [&](Entries& x, int i) __attribute__((always_inline)) {
+    x.blk = list[i];
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p) {
+      const int page = x.blk * PAGES + p;
+      x.page[p] = step_entry(table, page < last_page ? page : last_page);
+    }
+  };
+  const auto find = [&](Pages& x, const Entries& e) __attribute__((always_inline)) {
+    x.t0 = e.blk * TB;
     x.whole = x.t0 + TB - 1 <= u.low && (x.t0 > low_behind || x.t0 + TB <= a.sinks);
-    int32_t entry[PAGES];
+    int64_t page[PAGES];
 #pragma unroll
     for (int p = 0; p < PAGES; ++p) {
-      const int page = blk * PAGES + p;
-      entry[p] = table[page < last_page ? page : last_page];
-    }
-#pragma unroll
-    for (int p = 0; p < PAGES; ++p) {
-      const int left = u.tokens - (blk * PAGES + p) * TQ_PAGE_TOKENS;
+      const int left = u.tokens - (e.blk * PAGES + p) * TQ_PAGE_TOKENS;
       x.valid[p] = left < 0 ? 0 : (left > TQ_PAGE_TOKENS ? TQ_PAGE_TOKENS : left);
-      int64_t page = entry[p];
-      if (page < 0 || page >= a.s.num_blocks) { page = 0; x.valid[p] = 0; }
+      page[p] = e.page[p];
+      if (page[p] < 0 || page[p] >= a.s.num_blocks) { page[p] = 0; x.valid[p] = 0; }
       x.whole &= x.valid[p] == TQ_PAGE_TOKENS;
-      x.at[p] = (page * a.s_blk + h * a.s_h) * SIZE;
-      if constexpr (F8) {
-        x.k_scale[p] = a.k_scales[page * a.H + h];
-        x.v_scale[p] = a.v_scales[page * a.H + h];
-      }
+      x.at[p] = (page[p] * a.s_blk + h * a.s_h) * SIZE;
     }
+    if constexpr (F8) x.scales = (lane & 2 ? a.v_scales : a.k_scales)[(lane & 1 ? page[1] : page[0]) * a.H + h];
   };
   const auto scale_of = [](uint32_t byte) __attribute__((always_inline)) { return byte == 0 ? 0x1p-127f : __uint_as_float(byte << 23); };
 
@@ -168,14 +172,26 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
   };
 
   Pages now, next;
+  Entries ahead;
   if (first + wave < last) {
-    find(now, first + wave);
+    entries(ahead, first + wave);
+    find(now, ahead);
     load_keys(now);
     load_values(now);
+    entries(ahead, first + wave + 4);
   }
   for (int blk = first + wave; blk < last; blk += 4) {
     const bool more = blk + 4 < last;
-    if (more) find(next, blk + 4);
+    if (more) find(next, ahead);
+    entries(ahead, blk + 8);
+    float k_scale[PAGES], v_scale[PAGES];
+    if constexpr (F8) {
+#pragma unroll
+      for (int p = 0; p < PAGES; ++p) {
+        k_scale[p] = a.scale2 * scale_of((uint32_t)__builtin_amdgcn_readlane((int)now.scales, p));
+        v_scale[p] = scale_of((uint32_t)__builtin_amdgcn_readlane((int)now.scales, 2 + p));
+      }
+    }
     // ---- scores ----
     ex_f32x4 S[NT][PAGES];
 #pragma unroll
@@ -207,16 +223,24 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
       float top = -INFINITY, pr[PAGES][4];
 #pragma unroll
       for (int p = 0; p < PAGES; ++p) {
-        const float f = F8 ? a.scale2 * scale_of(now.k_scale[p]) : a.scale2;
+        const float f = F8 ? k_scale[p] : a.scale2;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float s2 = S[n][p][i] * f;
-          const int in = quarter * 4 + i, t = now.t0 + p * TQ_PAGE_TOKENS + in;
-          const bool seen = now.whole || (in < now.valid[p] && t <= at_p[n] && (t > behind[n] || t < a.sinks));
-          pr[p][i] = seen ? s2 : -INFINITY;
-          top = fmaxf(top, pr[p][i]);
-        }
+        for (int i = 0; i < 4; ++i) pr[p][i] = S[n][p][i] * f;
       }
+      if (!now.whole) {
+#pragma unroll
+        for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int in = quarter * 4 + i, t = now.t0 + p * TQ_PAGE_TOKENS + in;
+            const bool seen = (in < now.valid[p]) & (t <= at_p[n]) & ((t > behind[n]) | (t < a.sinks));
+            pr[p][i] = seen ? pr[p][i] : -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int p = 0; p < PAGES; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, pr[p][i]);
       top = fmaxf(m[n], ex_quad_max(top));
       if (__any(top > m[n] + EX_SLACK)) {
         const float move = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[n] - top);
@@ -244,19 +268,18 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
         }
     }
     // ---- values; those of tokens that no row of the unit sees are put to zero, since NaN times nothing is NaN ----
-    bool none[8];
+    if (!now.whole) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int in = quarter * 4 + (i & 3), t = now.t0 + (i >> 2) * TQ_PAGE_TOKENS + in;
-      none[i] = in >= now.valid[i >> 2] || !(t > attend_behind(a, u.low) || t < a.sinks);
+      for (int i = 0; i < 8; ++i) {
+        const int in = quarter * 4 + (i & 3), t = now.t0 + (i >> 2) * TQ_PAGE_TOKENS + in;
+        const uint32_t keep = (in < now.valid[i >> 2]) & ((t > unit_behind) | (t < a.sinks)) ? 0xffffffffu : 0u;
+        if constexpr (F8) VB[i] &= keep;
+#pragma unroll
+        for (int c = 0; c < WIDE; ++c) V[c][i] &= keep;
+        if constexpr (NARROW > 0) VN[i] &= keep;
+      }
     }
     if constexpr (F8) {
-      if (!now.whole) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (none[i]) VB[i] = vword{};
-      }
-      const float f0 = scale_of(now.v_scale[0]), f1 = scale_of(now.v_scale[1]);
 #pragma unroll
       for (int w = 0; w < VWORDS; ++w)
 #pragma unroll
@@ -265,8 +288,8 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const uint32_t x = __builtin_amdgcn_perm(VB[2 * j + 1][w], VB[2 * j][w], half ? 0x07030602u : 0x05010400u);
-            f[0][j] = f8_widen<TQ_BF16, false>(x, j < 2 ? f0 : f1);
-            f[1][j] = f8_widen<TQ_BF16, true>(x, j < 2 ? f0 : f1);
+            f[0][j] = f8_widen<TQ_BF16, false>(x, v_scale[j >> 1]);
+            f[1][j] = f8_widen<TQ_BF16, true>(x, v_scale[j >> 1]);
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
@@ -278,11 +301,6 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
     } else {
 #pragma unroll
       for (int c = 0; c < WIDE; ++c) {
-        if (!now.whole) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (none[i]) V[c][i] = ex_u32x4{0, 0, 0, 0};
-        }
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
           ex_u32x4 f;
@@ -293,11 +311,6 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
         }
       }
       if constexpr (NARROW > 0) {
-        if (!now.whole) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (none[i]) VN[i] = ex_u32x2{0, 0};
-        }
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           ex_u32x4 f;

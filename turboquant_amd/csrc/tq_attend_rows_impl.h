@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       const int page = blk * 4 + p;
-      x.entry[p] = table[page < last_page ? page : last_page];
+      x.entry[p] = step_entry(table, page < last_page ? page : last_page);
     }
   };
   ex_u32x4 KR[LOADS], VR[LOADS];
@@ -258,8 +258,8 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const int in = T * 32 + (e >> 2) * 8 + half * 4 + (e & 3), t = t0 + in;
-              const bool seen = t <= at_p[n] && t < u.tokens && (t > behind[n] || t < a.sinks) && good(now.entry[T * 2 + (e >> 3)]);
-              if (!seen) S[n][T][e] = -INFINITY;
+              const bool seen = (t <= at_p[n]) & (t < u.tokens) & ((t > behind[n]) | (t < a.sinks)) & good(now.entry[T * 2 + (e >> 3)]);
+              S[n][T][e] = seen ? S[n][T][e] : -INFINITY;
             }
         }
         float top = -INFINITY;

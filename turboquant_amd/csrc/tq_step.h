@@ -53,6 +53,12 @@ __device__ __forceinline__ int64_t step_rest(const Step& s, int64_t* front) {
 }
 __device__ __forceinline__ int64_t step_rest_row(const Step& s, int64_t front, int64_t rest, int64_t n) { return n < front ? n : n + s.rows - rest; }
 
+// a number that is the same in all lanes, as a scalar
+__device__ __forceinline__ int64_t step_uniform(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)x >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // Unit `u` of a step whose sequence b has count(b) of them: its sequence and which one of them it is; false (and u less all of them) if there are fewer.
 // A whole wavefront asks; u is the same in all lanes.  A lane adds up four sequences, so that up to 256 take one round of loads.
 template <class Count>
@@ -72,7 +78,7 @@ __device__ __forceinline__ bool step_unit(const Step& s, int64_t* u, int* b, int
       const int64_t below = __shfl_up((long long)upto, o, 64);
       if (lane >= o) upto += below;
     }
-    const int64_t all = __shfl((long long)upto, 63, 64);
+    const int64_t all = step_uniform(__shfl((long long)upto, 63, 64));
     if (*u < all) {
       const int owner = __ffsll((unsigned long long)__ballot(upto > *u)) - 1;
       int64_t left = *u - (upto - sum);
@@ -81,12 +87,18 @@ __device__ __forceinline__ bool step_unit(const Step& s, int64_t* u, int* b, int
       for (int i = 0; i < 3; ++i)
         if (which == i && left >= c[i]) { left -= c[i]; which = i + 1; }
       *b = __builtin_amdgcn_readfirstlane(__shfl(base + lane * 4 + which, owner, 64));
-      *j = __shfl((long long)left, owner, 64);
+      *j = step_uniform(__shfl((long long)left, owner, 64));
       return true;
     }
     *u -= all;
   }
   return false;
+}
+
+// A table entry at a place that is the same for the whole wavefront: no launch writes its own table, so that this is a scalar load, which waits for no
+// vector load in front of it.
+__device__ __forceinline__ int32_t step_entry(const int32_t* table, int page) {
+  return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)table)[page];
 }
 
 // what the entry points check of a step, and its description
