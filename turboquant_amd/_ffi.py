@@ -166,10 +166,10 @@ _HOST_CALLS = ("tq_quantize_keys", "tq_dequant_keys", "tq_score", "tq_ring_write
                "tq_decode_attn_paged", "tq_decode_attn_paged_by_length", "tq_decode_attn_paged_ring", "tq_decode_attn_paged_ring_by_length",
                "tq_cache_append_bytes", "tq_cache_append", "tq_cache_scores_rows", "tq_cache_attend_bytes", "tq_cache_attend",
                "tq_exact_decode_bytes", "tq_exact_decode", "tq_exact_window_bytes", "tq_exact_window", "tq_evict_select_bytes", "tq_evict_select",
-               "tq_move_tokens_exact")
+               "tq_move_tokens_exact", "tq_fp8_write", "tq_fp8_read", "tq_attend_bytes", "tq_attend", "tq_rotate_heads")
 
 
-HOST_INTERFACE = 2                    # of csrc/tq_host.cpp: goes up with every change of a call's arguments or results
+HOST_INTERFACE = 3                    # of csrc/tq_host.cpp: goes up with every change of a call's arguments or results
 
 
 def host_stamp() -> str:

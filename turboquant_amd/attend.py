@@ -85,6 +85,11 @@ def attend(what: str, cache, query: torch.Tensor, query_start_loc: Optional[torc
            scale: Optional[float], window: Optional[int], sinks: int, n_split: Optional[int], workspace: Optional[torch.Tensor],
            out: Optional[torch.Tensor], max_len: Optional[int], max_rows: Optional[int]) -> torch.Tensor:
     """The calls `attention` and `decode_attention` (query_start_loc None) of both caches."""
+    fast = _ffi.native()
+    if fast is not None and n_split is None and workspace is None and out is None:
+        done = fast.attend(query, query_start_loc, block_table, seq_lens, *cache.operands(), scale, window, sinks, max_len, max_rows)
+        if done is not None:
+            return done
     _ffi.require_gpu(query, "query")
     if query.dim() != 3:
         raise ValueError("query must be (rows, Hq, d)" if query_start_loc is not None else "query must be (B, Hq, d)")

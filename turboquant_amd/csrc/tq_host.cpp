@@ -63,13 +63,19 @@ struct Library {
   decltype(&tq_evict_select_bytes) evict_select_bytes;
   decltype(&tq_evict_select) evict_select;
   decltype(&tq_move_tokens_exact) move_tokens_exact;
+  decltype(&tq_fp8_write) fp8_write;
+  decltype(&tq_fp8_read) fp8_read;
+  decltype(&tq_attend_bytes) attend_bytes;
+  decltype(&tq_attend) attend;
+  decltype(&tq_rotate_heads) rotate_heads;
 } g_lib{};
 constexpr const char* kNames[] = {"tq_quantize_keys", "tq_dequant_keys", "tq_score", "tq_ring_write", "tq_append_kv_paged",
                                   "tq_append_kv_newest", "tq_decode_workspace_bytes", "tq_decode_attn_paged", "tq_decode_attn_paged_by_length",
                                   "tq_decode_attn_paged_ring", "tq_decode_attn_paged_ring_by_length", "tq_cache_append_bytes",
                                   "tq_cache_append", "tq_cache_scores_rows", "tq_cache_attend_bytes", "tq_cache_attend",
                                   "tq_exact_decode_bytes", "tq_exact_decode", "tq_exact_window_bytes", "tq_exact_window",
-                                  "tq_evict_select_bytes", "tq_evict_select", "tq_move_tokens_exact"};
+                                  "tq_evict_select_bytes", "tq_evict_select", "tq_move_tokens_exact", "tq_fp8_write", "tq_fp8_read", "tq_attend_bytes", "tq_attend",
+                                  "tq_rotate_heads"};
 static_assert(sizeof(Library) == sizeof(kNames) / sizeof(kNames[0]) * sizeof(void*), "a pointer per name, in order");
 bool g_bound = false;
 
@@ -688,6 +694,186 @@ PyObject* move_exact(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   });
 }
 
+// ---- a step over a paged cache ---------------------------------------------------------------------------------------------------
+
+// Blocks and scales as Fp8PagedCache takes them
+struct Blocks8 {
+  at::Tensor k, v, ks, vs;
+  int64_t n = 0, H = 0, d = 0;
+  bool take(Plain& p, PyObject* const* a) {
+    k = p.take(a[0]); v = p.take(a[1]); ks = p.take(a[2]); vs = p.take(a[3]);
+    if (!p.ok || k.dim() != 4 || k.sizes() != v.sizes() || k.strides() != v.strides() || k.scalar_type() != at::kFloat8_e4m3fn ||
+        v.scalar_type() != at::kFloat8_e4m3fn || k.size(1) != TQ_PAGE_TOKENS || k.stride(3) != 1)
+      return false;
+    n = k.size(0); H = k.size(2); d = k.size(3);
+    if (n == 0 || H == 0 || H > INT_MAX || (d != 64 && d != 128 && d != 192 && d != 256)) return false;
+    for (const at::Tensor* t : {&ks, &vs})
+      if (!dense_as(*t, at::kByte) || t->dim() != 2 || t->size(0) != n || t->size(1) != H) return false;
+    return k.stride(0) % 16 == 0 && k.stride(1) % 16 == 0 && k.stride(2) % 16 == 0 && k.stride(1) <= 1 << 24 &&
+           (((uintptr_t)k.data_ptr() | (uintptr_t)v.data_ptr()) & 15) == 0;
+  }
+};
+// query_start_loc of a step, and with it its sequences
+struct Starts {
+  at::Tensor t;
+  int64_t B = 0;
+  bool take(Plain& p, PyObject* o) {
+    t = p.take(o);
+    if (!p.ok || !dense_as(t, at::kInt) || t.dim() != 1 || t.size(0) < 2 || t.size(0) > INT_MAX) return false;
+    B = t.size(0) - 1;
+    return true;
+  }
+  const int32_t* data() const { return (const int32_t*)t.data_ptr(); }
+};
+// whether the memory from a's first element to its last meets b's
+bool meet(const at::Tensor& a, const at::Tensor& b) {
+  const auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return (char*)t.data_ptr() + (last + 1) * (int64_t)t.element_size();
+  };
+  return a.numel() && b.numel() && (char*)a.data_ptr() < end(b) && (char*)b.data_ptr() < end(a);
+}
+// no two elements in one place; the last dimension's are neighbours
+bool own_places(const at::Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> by;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.size(i) > 1) by.emplace_back(t.stride(i), t.size(i));
+  std::sort(by.begin(), by.end());
+  int64_t reach = t.size(-1);
+  for (const auto& [stride, size] : by) {
+    if (stride < reach) return false;
+    reach = stride * (size - 1) + reach;
+  }
+  return true;
+}
+
+// fp8_cache(key blocks, value blocks, key scales, value scales) -> (blocks, H, d, three strides)
+PyObject* fp8_cache(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return entry<4>(args, n_args, [](PyObject* const* a) -> PyObject* {
+    Plain p;
+    Blocks8 c;
+    if (!c.take(p, a)) return nullptr;
+    return Py_BuildValue("LLL(LLLL)", (long long)c.n, (long long)c.H, (long long)c.d, (long long)c.k.stride(0), (long long)c.k.stride(1),
+                         (long long)c.k.stride(2), (long long)c.k.stride(3));
+  });
+}
+
+// fp8_write(key, value (rows, H, d), starts, block table, lengths, key blocks, value blocks, key scales, value scales) -> True
+PyObject* fp8_write(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return entry<9>(args, n_args, [](PyObject* const* a) -> PyObject* {
+    Plain p;
+    Blocks8 c;
+    Starts st;
+    Sequences s;
+    if (!c.take(p, a + 5) || !st.take(p, a[2]) || !s.take(p, a[3], a[4], st.B, st.B == 1) || !own_places(c.k)) return nullptr;
+    const at::Tensor k = p.take(a[0]), v = p.take(a[1]);
+    if (!p.ok || k.dim() != 3 || k.sizes() != v.sizes() || k.size(1) != c.H || k.size(2) != c.d || k.size(0) == 0 || v.scalar_type() != k.scalar_type()) return nullptr;
+    const int tag = dtype_tag(k.scalar_type());
+    if (tag < 0) return nullptr;
+    const int64_t piece = 16 / (int64_t)k.element_size();
+    for (const at::Tensor* t : {&k, &v}) {
+      if (t->stride(2) != 1 || t->stride(0) % piece || t->stride(1) % piece || ((uintptr_t)t->data_ptr() & 15)) return nullptr;
+      for (const at::Tensor* held : {&c.k, &c.v, &c.ks, &c.vs})
+        if (meet(*t, *held)) return nullptr;
+    }
+    if (unlocked(g_lib.fp8_write, k.data_ptr(), v.data_ptr(), tag, k.size(0), k.stride(0), k.stride(1), v.stride(0), v.stride(1), st.data(), (int)st.B, (int)c.H,
+                 (int)c.d, c.k.data_ptr(), c.v.data_ptr(), (uint8_t*)c.ks.data_ptr(), (uint8_t*)c.vs.data_ptr(), c.k.stride(0), c.k.stride(1), c.k.stride(2),
+                 c.n, s.entries(), (int)s.stride, s.lengths(), p.stream()) != TQ_OK)
+      return nullptr;
+    for (const at::Tensor* held : {&c.k, &c.v, &c.ks, &c.vs}) written(*held);
+    Py_RETURN_TRUE;
+  });
+}
+
+// fp8_read(starts, block table, lengths, rows, type's tag, key blocks, value blocks, key scales, value scales) -> (keys, values)
+PyObject* fp8_read(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return entry<9>(args, n_args, [](PyObject* const* a) -> PyObject* {
+    Plain p;
+    Blocks8 c;
+    Starts st;
+    Sequences s;
+    if (!c.take(p, a + 5) || !st.take(p, a[0]) || !s.take(p, a[1], a[2], st.B, true)) return nullptr;
+    const int64_t rows = int_arg(a[3]), tag = int_arg(a[4]);
+    if (PyErr_Occurred() || rows <= 0 || tag < TQ_F32 || tag > TQ_BF16) return nullptr;
+    const auto dt = tag == TQ_F32 ? at::kFloat : tag == TQ_F16 ? at::kHalf : at::kBFloat16;
+    const at::Tensor k = p.fresh({rows, c.H, c.d}, dt), v = p.fresh({rows, c.H, c.d}, dt);
+    if (unlocked(g_lib.fp8_read, k.data_ptr(), v.data_ptr(), (int)tag, rows, st.data(), (int)st.B, (int)c.H, (int)c.d, c.k.data_ptr(), c.v.data_ptr(),
+                 (const uint8_t*)c.ks.data_ptr(), (const uint8_t*)c.vs.data_ptr(), c.k.stride(0), c.k.stride(1), c.k.stride(2), c.n, s.entries(), (int)s.stride,
+                 s.lengths(), 1, p.stream()) != TQ_OK)
+      return nullptr;
+    return tuple({k, v});
+  });
+}
+
+// attend(query (rows, Hq, d), starts or None, block table, lengths, key blocks, value blocks, key scales or None, value scales or None, scale or None,
+//        window or None, sinks, longest or None, most rows or None) -> attention
+PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return entry<13>(args, n_args, [](PyObject* const* a) -> PyObject* {
+    Plain p;
+    Blocks c;
+    Blocks8 c8;
+    Starts st;
+    Sequences s;
+    const bool f8 = a[6] != Py_None, starts = a[1] != Py_None;
+    if (f8 ? !c8.take(p, a + 4) : !c.take(p, a[4], a[5])) return nullptr;
+    const at::Tensor &k = f8 ? c8.k : c.k, &v = f8 ? c8.v : c.v;
+    const int64_t n = f8 ? c8.n : c.n, H = f8 ? c8.H : c.H, d = f8 ? c8.d : c.d;
+    const at::Tensor q = p.take(a[0]);
+    if (!p.ok || q.dim() != 3 || q.size(2) != d || !q.is_contiguous() || ((uintptr_t)q.data_ptr() & 15)) return nullptr;
+    const int tag = dtype_tag(q.scalar_type()), cache = f8 ? TQ_E4M3 : c.tag;
+    const int64_t rows = q.size(0), Hq = q.size(1);
+    if (tag < 0 || rows == 0 || rows > INT_MAX || Hq == 0 || Hq > INT_MAX || Hq % H || (starts && !st.take(p, a[1]))) return nullptr;
+    const int64_t B = starts ? st.B : rows;
+    if (!s.take(p, a[2], a[3], B, true)) return nullptr;
+    const double scale = real_arg(a[8], 1.0 / std::sqrt((double)d));
+    const int64_t window = int_or(a[9], 0), sinks = int_arg(a[10]), table = s.row * TQ_PAGE_TOKENS;
+    const int64_t longest = std::min(int_or(a[11], table), table), most = int_or(a[12], rows);
+    if (PyErr_Occurred() || longest < 0 || most < 0 || sinks < 0 || sinks > INT_MAX || window > INT_MAX || (a[9] == Py_None ? sinks != 0 : window < 1)) return nullptr;
+    const size_t need = g_lib.attend_bytes(tag, cache, starts, rows, (int)B, (int)Hq, (int)H, (int)d, longest, most, window, (int)sinks, 0);
+    if (need == 0) return nullptr;
+    const at::Tensor ws = p.fresh({(int64_t)(need / 4)}, at::kFloat), out = p.fresh(q.sizes(), q.scalar_type());
+    if (unlocked(g_lib.attend, q.data_ptr(), tag, rows, starts ? st.data() : nullptr, (int)B, (int)Hq, (int)H, (int)d, cache, k.data_ptr(), v.data_ptr(),
+                 f8 ? (const uint8_t*)c8.ks.data_ptr() : nullptr, f8 ? (const uint8_t*)c8.vs.data_ptr() : nullptr, k.stride(0), k.stride(1), k.stride(2), n,
+                 s.entries(), (int)s.stride, s.lengths(), (float)scale, longest, most, window, (int)sinks, out.data_ptr(), 1, ws.data_ptr(), 0, p.stream()) != TQ_OK)
+      return nullptr;
+    return THPVariable_Wrap(out);
+  });
+}
+
+// rotate(query, key (rows, H, d), positions, frequencies, query weight or None, key weight or None, eps, interleaved) -> (query, key)
+PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return entry<8>(args, n_args, [](PyObject* const* a) -> PyObject* {
+    Plain p;
+    const at::Tensor q = p.take(a[0]), k = p.take(a[1]), pos = p.take(a[2]), f = p.take(a[3]);
+    if (!p.ok || q.dim() != 3 || k.dim() != 3 || q.size(0) != k.size(0) || q.size(2) != k.size(2) || k.scalar_type() != q.scalar_type()) return nullptr;
+    const int tag = dtype_tag(q.scalar_type());
+    const int64_t rows = q.size(0), d = q.size(2), r = f.dim() == 1 ? 2 * f.size(0) : -1, align = tag == TQ_F32 ? 16 : 8;
+    if (tag < 0 || rows == 0 || rows > INT_MAX || q.size(1) == 0 || k.size(1) == 0 || q.size(1) + k.size(1) > INT_MAX || d <= 0 || d % 8 || d > 512 || r <= 0 || r % 8 ||
+        r > d || !dense_as(f, at::kDouble) || !pos.is_contiguous() || pos.dim() != 1 || pos.size(0) != rows ||
+        (pos.scalar_type() != at::kLong && pos.scalar_type() != at::kInt))
+      return nullptr;
+    const auto fits = [&](const at::Tensor& t) { return t.stride(2) == 1 && t.stride(0) % 4 == 0 && t.stride(1) % 4 == 0 && (uintptr_t)t.data_ptr() % align == 0; };
+    if (!fits(q) || !fits(k)) return nullptr;
+    at::Tensor w[2];
+    for (int i = 0; i < 2; ++i) {
+      if (a[4 + i] == Py_None) continue;
+      w[i] = p.take(a[4 + i]);
+      if (!p.ok || !dense_as(w[i], q.scalar_type()) || w[i].dim() != 1 || w[i].size(0) != d || (uintptr_t)w[i].data_ptr() % align) return nullptr;
+    }
+    const double eps = real_arg(a[6], 0.0);
+    const int interleaved = PyObject_IsTrue(a[7]);
+    if (PyErr_Occurred() || interleaved < 0) return nullptr;
+    const at::Tensor qo = p.fresh(q.sizes(), q.scalar_type()), ko = p.fresh(k.sizes(), k.scalar_type());
+    if (unlocked(g_lib.rotate_heads, q.data_ptr(), k.data_ptr(), tag, rows, (int)q.size(1), (int)k.size(1), (int)d, q.stride(0), q.stride(1), k.stride(0),
+                 k.stride(1), pos.data_ptr(), (int)(pos.scalar_type() == at::kLong), (const double*)f.data_ptr(), (int)r, interleaved,
+                 w[0].defined() ? w[0].data_ptr() : nullptr, w[1].defined() ? w[1].data_ptr() : nullptr, (float)eps, qo.data_ptr(), qo.stride(0), qo.stride(1),
+                 ko.data_ptr(), ko.stride(0), ko.stride(1), p.stream()) != TQ_OK)
+      return nullptr;
+    return tuple({qo, ko});
+  });
+}
+
 // bind({name: address}): the library's functions
 PyObject* bind(PyObject*, PyObject* arg) {
   if (!PyDict_Check(arg)) { PyErr_SetString(PyExc_TypeError, "bind takes a dict of addresses"); return nullptr; }
@@ -711,6 +897,8 @@ PyMethodDef kMethods[] = {
     TQ_FAST(cache_scores, "scores of the cache object"), TQ_FAST(cache_attend, "weighted values of the cache object"),
     TQ_FAST(exact_cache, "an exact cache's blocks"), TQ_FAST(exact_decode, "a decode step over an exact cache"),
     TQ_FAST(exact_window, "a window's weights"), TQ_FAST(evict_select, "who stays"), TQ_FAST(move_exact, "moves in an exact cache"),
+    TQ_FAST(fp8_cache, "an 8-bit cache's blocks"), TQ_FAST(fp8_write, "a step's tokens into 8 bits"), TQ_FAST(fp8_read, "8 bits back"),
+    TQ_FAST(attend, "attention of a step's rows"), TQ_FAST(rotate, "heads' norms and rotation"),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tq_host", "host side of small calls", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

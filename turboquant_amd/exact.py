@@ -188,6 +188,9 @@ class ExactPagedCache:
     def tensors(self) -> dict:
         return dict(key_cache=self.key_cache, value_cache=self.value_cache)
 
+    def operands(self):
+        return self.key_cache, self.value_cache, None, None
+
     def _memory(self):
         return self.key_cache.data_ptr(), self.value_cache.data_ptr(), None, None
 

@@ -28,6 +28,12 @@ class Fp8PagedCache:
 
     def __init__(self, key_cache: torch.Tensor, value_cache: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor):
         self.key_cache, self.value_cache, self.key_scales, self.value_scales = key_cache, value_cache, key_scales, value_scales
+        fast = _ffi.native()
+        known = None if fast is None else fast.fp8_cache(key_cache, value_cache, key_scales, value_scales)
+        if known is not None:
+            self.num_blocks, self.num_kv_heads, self.head_dim, self._strides = known
+            self.device = key_cache.device
+            return
         for name, t in self.tensors().items():
             _ffi.require_gpu(t, name)
         if key_cache.dim() != 4 or key_cache.shape != value_cache.shape or key_cache.shape[1] != PAGE_TOKENS:
@@ -35,6 +41,8 @@ class Fp8PagedCache:
         self.device = key_cache.device
         if any(t.dtype != torch.float8_e4m3fn for t in (key_cache, value_cache)) or any(t.dtype != torch.uint8 for t in (key_scales, value_scales)):
             raise TypeError("key_cache and value_cache must be float8_e4m3fn, key_scales and value_scales uint8")
+        if any(t.is_neg() or t._is_zerotensor() for t in self.operands()):
+            raise ValueError("the cache must hold its values: a lazily negated tensor does not")
         if any(t.device != self.device for t in (value_cache, key_scales, value_scales)):
             raise TypeError("the cache and its scales must live on one GPU")
         self.num_blocks, _, self.num_kv_heads, self.head_dim = key_cache.shape
@@ -57,8 +65,11 @@ class Fp8PagedCache:
     def tensors(self) -> dict:
         return dict(key_cache=self.key_cache, value_cache=self.value_cache, key_scales=self.key_scales, value_scales=self.value_scales)
 
+    def operands(self):
+        return self.key_cache, self.value_cache, self.key_scales, self.value_scales
+
     def _memory(self):
-        return tuple(t.data_ptr() for t in (self.key_cache, self.value_cache, self.key_scales, self.value_scales))
+        return tuple(t.data_ptr() for t in self.operands())
 
     def memory_bytes(self) -> int:
         return sum(t.numel() for t in self.tensors().values())
@@ -72,6 +83,9 @@ class Fp8PagedCache:
         it holds, NaN stays.  Tokens that a block holds already are rounded again where a new one needs a larger scale; a block whose first slot is written
         starts anew.  A sequence's blocks must be its own while it writes to them; rows in front of token 0, behind the table or in blocks outside
         the cache are left out."""
+        fast = _ffi.native()
+        if fast is not None and fast.fp8_write(key, value, query_start_loc, block_table, seq_lens, *self.operands()):
+            return
         _ffi.require_gpu(key, "key")
         _ffi.require_gpu(value, "value")
         if key.dim() != 3 or key.shape != value.shape or tuple(key.shape[1:]) != (self.num_kv_heads, self.head_dim):
@@ -115,6 +129,11 @@ class Fp8PagedCache:
         """What is held of the tokens that `write` takes the same arguments for: keys and values (rows, H_kv, d), each rounded once to `dtype`.
         rows: query_start_loc's last entry, which the host does not know.  A row whose token is not in the cache is zeros, and so are
         rows behind the last sequence; with out=(keys, values), contiguous, those are left as they are."""
+        fast = _ffi.native()
+        if fast is not None and out is None and rows is not None:
+            done = fast.fp8_read(query_start_loc, block_table, seq_lens, rows, _ffi.dtype_tag(dtype), *self.operands())
+            if done is not None:
+                return done
         starts, B = step_starts(self.device, query_start_loc)
         table, bt_stride, lens = sequences(self.device, block_table, seq_lens, B)
         shape = (self.num_kv_heads, self.head_dim)

@@ -31,6 +31,11 @@ def rotate_heads(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
     as good at position 2^20 as at 1.  All of it in 32 bits, rounded once.  Views of a fused projection are read where they are.
 
     Returns new contiguous tensors, or out=(query, key), channels contiguous, which may be the inputs themselves."""
+    fast = _ffi.native()
+    if fast is not None and out is None:
+        done = fast.rotate(query, key, positions, inv_freq, q_weight, k_weight, eps, interleaved)
+        if done is not None:
+            return done
     _ffi.require_gpu(query, "query")
     _ffi.require_gpu(key, "key")
     if query.dim() != 3 or key.dim() != 3 or query.shape[0] != key.shape[0] or query.shape[2] != key.shape[2]:
