@@ -89,10 +89,25 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   const int64_t blocks = (tokens + TB - 1) / TB;
   int64_t n = n_split;
   if (n == 0) {
-    const int64_t resident = 256 * (p->tiles == 1 ? 3 : (p->tiles || d <= 128 ? 2 : 1));
-    n = (resident + pairs - 1) / pairs;
-    if (p->tiles) n = std::max(n, (tokens + 1023) / 1024);
-    n = std::min<int64_t>(std::min<int64_t>(n, (blocks + 3) / 4), JOIN_MAX_SPLITS);
+    if (p->tiles) {
+      // Workgroups enough for the bytes that have to be on their way: one for each compute unit where a turn of its four wavefronts is 64 KB, two where it
+      // is less (us; fp8, d 128, 8 heads, one sequence of 131072: 32 splits 67.7, 64 64.4, 128 65.4, 256 65.0; d 256, 2 heads: 64 47.6, 128 36.6, 256 38.5, 384 46.6;
+      // bf16, d 128, one of 65536: 16 75.7, 32 53.7, 64 58.5), no split of more than 2048 tokens (fp8, 32 of 8192: 1 138, 2 114.6, 4 106.4, 8 105.2), and of
+      // the next numbers of splits, while they leave 512 tokens, the first that leaves no compute unit without work in its last round (24 of 6000: 3 70.9, 4 62.9).
+      const int64_t turn = 4 * TB * 2 * d * (cache == TQ_E4M3 ? 1 : 2), target = turn >= 65536 ? 256 : 512;
+      n = std::max((target + pairs - 1) / pairs, (tokens + 2047) / 2048);
+      double best = 0;
+      for (int64_t i = n; i <= 2 * n && i <= std::max(n, tokens / 512); ++i) {
+        const double full = double(pairs * i) / (256 * ((pairs * i + 255) / 256));
+        if (full > best + 0.02) { best = full; n_split = (int)std::min<int64_t>(i, JOIN_MAX_SPLITS); }
+        if (best >= 0.95) break;
+      }
+      n = std::min<int64_t>(n_split, (blocks + 3) / 4);
+      n_split = 0;
+    } else {
+      n = (256 * (d <= 128 ? 2 : 1) + pairs - 1) / pairs;
+      n = std::min<int64_t>(std::min<int64_t>(n, (blocks + 3) / 4), JOIN_MAX_SPLITS);
+    }
   }
   n = std::max<int64_t>(1, std::min(n, blocks));
   int64_t chunk = (blocks + n - 1) / n;
