@@ -18,23 +18,30 @@ struct Attend {
   const void* q;                           // (rows, Hq, d)
   void* out;
   int32_t Hq, G, window, sinks;
-  int32_t n_split, chunk;                  // splits of a unit's tokens, blocks of a split (more where there are more tokens than planned for)
+  int32_t n_split, chunk;                  // splits of a unit's tokens at most, blocks of a split (more where there are more tokens than planned for)
+  int32_t target, cap;                     // where sequences differ: items of a head to share their blocks out to (0: as planned), splits of one of them at most
+  float share;                             // 1 / target
   int32_t fill;                            // rows of no sequence become zeros
   float scale2;                            // scale x log2 e: the softmax is one of powers of two
-  int64_t units;                           // rows' units that the grid has room for
-  float* acc;                              // (rows, Hq, n_split, d): numerators of a split; unused with one split
-  float2* ml;                              // (rows, Hq, n_split): its maximum (log2) and its sum; ATTEND_EMPTY, ATTEND_REST in the sum's place
+  int32_t units;                           // units that the plan has room for
+  int32_t items;                           // (unit, split) pairs that the grid has room for, for each KV head
+  // Partial results, where a row may have several: a workgroup's own (M rows), and of every row the first of its workgroups, how many there are, which of a
+  // workgroup's rows it is and how far they are apart.  0 of them: a row of no sequence; 1: it is in `out` already.
+  float* acc;                              // (workgroups, M, d): numerators
+  float2* ml;                              // (workgroups, M): maximum (log2) and sum
+  int2* shares;                            // (rows, Hq): first, number | row << 16 | planned << 24; null: all rows have one
 };
-constexpr float ATTEND_EMPTY = -1.0f;      // a split without tokens (these are the last ones of a row)
-constexpr float ATTEND_REST = -2.0f;       // of a row of no sequence, in its first split
 
-// The row with the lowest position that `unit rows` row .. row + n - 1 (of a sequence's run * G, heads of a token side by side) have, and what they see
+// What a workgroup works on: `rows` rows of a sequence's run * G (the heads of a token side by side), from `first` on, and a share of the tokens they see
 struct AttendUnit {
-  int b, h;
+  int b;
   int64_t row;             // of the sequence's first row in the step
-  int first, rows;         // unit rows: the first of them (token row * G + head), how many
+  int first, rows;
   int low, high;           // positions of the first and the last
   int tokens;              // up to the last's own token, as far as the table goes
+  int split, splits;       // which share, of how many (before it is known how many there are tokens for)
+  bool planned;            // shares as the host planned them
+  int apart;               // items from one share to the next
 };
 // Blocks of TB tokens that a unit sees any token of: `front` from token 0 on (sinks), then from `from` on
 template <int TB>
@@ -53,31 +60,9 @@ struct AttendBlocks {
 // the last position that row p does not see for its window (tokens up to it are seen only below `sinks`)
 __device__ __forceinline__ int attend_behind(const Attend& a, int p) { return p >= a.window ? p - a.window : -1; }
 
-__host__ __device__ __forceinline__ int attend_per_split(int blocks, int n_split, int chunk) {
-  const int least = (blocks + n_split - 1) / n_split;
-  return least > chunk ? least : chunk;
-}
-
-// Unit u of units of M rows: whose rows they are.  false: there are fewer; *u counts on from behind the last.
+// the j-th unit of M rows of a run
 template <int M>
-__device__ __forceinline__ bool attend_unit(const Attend& a, int64_t* u, AttendUnit* t) {
-  int64_t j = 0;
-  StepRun r;
-  if (!a.s.starts) {
-    const int per = (a.G + M - 1) / M;
-    if (*u >= (int64_t)a.s.B * per) { *u -= (int64_t)a.s.B * per; return false; }
-    t->b = (int)(*u / per);
-    j = *u - (int64_t)t->b * per;
-  } else if (!step_unit(a.s, u, &t->b, &j, [&](const StepRun& x) { return ((int64_t)x.run * a.G + M - 1) / M; })) {
-    return false;
-  }
-  // (all of it is the same for the whole wavefront, which only the scalar registers say to the compiler: its tables' entries are scalar loads then)
-  t->b = __builtin_amdgcn_readfirstlane(t->b);
-  j = step_uniform(j);
-  r = step_run(a.s, t->b);
-  r.row = step_uniform(r.row);
-  r.run = __builtin_amdgcn_readfirstlane(r.run);
-  r.len = __builtin_amdgcn_readfirstlane(r.len);
+__device__ __forceinline__ void attend_unit(const Attend& a, const StepRun& r, int64_t j, AttendUnit* t) {
   t->row = r.row;
   t->first = (int)(j * M);
   const int64_t left = (int64_t)r.run * a.G - j * M;
@@ -86,22 +71,136 @@ __device__ __forceinline__ bool attend_unit(const Attend& a, int64_t* u, AttendU
   t->high = r.token() + (t->first + t->rows - 1) / a.G;
   const int cap = step_cap(a.s);
   t->tokens = t->high < 0 ? 0 : (t->high + 1 < cap ? t->high + 1 : cap);
+}
+template <int M>
+__device__ __forceinline__ int attend_units(const Attend& a, const StepRun& r) { return (int)(((int64_t)r.run * a.G + M - 1) / M); }
+// Blocks that the last unit of a run, which sees the most, sees; with a window those of the rows that the unit may have at most.
+template <int M, int TB>
+__device__ __forceinline__ int attend_most(const Attend& a, const StepRun& r) {
+  AttendUnit t;
+  const int cap = step_cap(a.s), reach = (M - 1) / a.G + 1;
+  t.tokens = r.len < cap ? r.len : cap;
+  t.low = r.len - 1 - reach;
+  return r.run ? AttendBlocks<TB>(a, t).count : 0;
+}
+// ceil(blocks / chunk), 1 .. most.  (By a reciprocal: a division for each of four sequences a lane is half the time that looking them up takes.  One off
+// where numbers pass 24 bits is as good a share.)
+struct AttendSplits {
+  int chunk, most;
+  float inverse;
+  __device__ __forceinline__ AttendSplits(int chunk, int most) : chunk(chunk), most(most), inverse(__builtin_amdgcn_rcpf((float)chunk)) {}
+  __device__ __forceinline__ int operator()(int blocks) const {
+    int n = (int)((float)blocks * inverse);
+    n += n * chunk < blocks;
+    return n < 1 ? 1 : (n > most ? most : n);
+  }
+};
+
+// Item `n` of a step: whose rows, which share of their tokens.  false: there are fewer; it is then number *over of *others that are left over, if any.
+// Shares are planned by the longest sequence there may be, the first shares of all units in front of the second ones (with the shares of a unit next to
+// each other 32 sequences of 8192 took 120 us, so 106).  Where up to 256 sequences turn out to differ, their blocks are shared out anew, `target` items for each
+// KV head in all, so that no workgroup has much more to do than another, and none starts for nothing.
+template <int M, int TB>
+__device__ __forceinline__ bool attend_item(const Attend& a, int n, AttendUnit* t, int* over, int* others) {
+  int unit = 0;
+  StepRun run;
+  *over = *others = 0;
+  t->split = (unsigned)n / (unsigned)a.units;
+  int u = n - t->split * a.units;                            // of the units, as planned
+  t->planned = true;
+  t->splits = a.n_split;
+  t->apart = a.units;
+  if (!a.s.starts && a.target == 0) {
+    if (t->split >= a.n_split) return false;
+    const int per = (a.G + M - 1) / M;
+    t->b = (unsigned)u / (unsigned)per;
+    unit = u - t->b * per;
+    run = step_run(a.s, t->b);
+    run.len = __builtin_amdgcn_readfirstlane(run.len);
+  } else {
+    StepRun r[4];
+    int blocks[4];
+    bool found = false;
+    const int given = u;
+    for (int base = 0; base < a.s.B && !found; base += STEP_ROUND) {
+      step_runs(a.s, base, r);
+      int count[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) count[i] = base + i * 64 < a.s.B && r[i].run ? attend_units<M>(a, r[i]) : 0;
+      if (a.target > 0) {                                     // (a single round)
+        float total = 0.0f, longest = 0.0f, units = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          blocks[i] = 0;
+          if (base + i * 64 >= a.s.B) continue;
+          blocks[i] = attend_most<M, TB>(a, r[i]);
+          const float x = (float)count[i], y = (float)blocks[i];
+          total = fmaf(x, y, total);
+          units += x;
+          longest = fmaxf(longest, y);
+        }
+        total = wave_sum_fast(total);
+        if (wave_max_fast(longest) * wave_sum_fast(units) * 7 > total * 8) {       // (by more than an eighth)
+          const AttendSplits splits((int)fminf(ceilf(total * a.share), 1e9f), a.cap);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) count[i] *= splits(blocks[i]);
+          t->planned = false;
+          int j = n;
+          found = step_find(a.s, base, r, count, &j, &t->b, &unit, &run);
+          if (!found) {
+            *over = j;
+            *others = a.items - (n - j);
+            return false;
+          }
+          t->splits = __builtin_amdgcn_readfirstlane(splits(attend_most<M, TB>(a, run)));
+          t->apart = 1;
+          t->split = unit % t->splits;
+          unit = unit / t->splits;
+          break;
+        }
+      }
+      found = step_find(a.s, base, r, count, &u, &t->b, &unit, &run);
+    }
+    if (t->planned && t->split >= a.n_split) return false;
+    if (!found) {
+      if (t->split == 0) {
+        *over = u;
+        *others = a.units - (given - u);
+      }
+      return false;
+    }
+  }
+  // (all of it is the same for the whole wavefront, which only the scalar registers say to the compiler: its tables' entries are scalar loads then)
+  t->b = __builtin_amdgcn_readfirstlane(t->b);
+  t->split = __builtin_amdgcn_readfirstlane(t->split);
+  attend_unit<M>(a, run, __builtin_amdgcn_readfirstlane(unit), t);
   return true;
 }
 
-// Units behind the last sequence's, of which this is number `number` of `others`: rows of no sequence, KV head h's part of them
+// A unit's share of its blocks: [first, last) of the list, and how many shares there are blocks for (one at least)
+struct AttendShare {
+  int first, last, used;
+  __device__ __forceinline__ AttendShare(const Attend& a, const AttendUnit& u, int count) {
+    int per = (count + u.splits - 1) / u.splits;
+    if (u.planned && per < a.chunk) per = a.chunk;
+    per = per < 1 ? 1 : per;
+    used = count < 1 ? 1 : (count + per - 1) / per;
+    first = u.split * per < count ? u.split * per : count;
+    last = first + per < count ? first + per : count;
+  }
+};
+// Items behind the last sequence's, of which this is number `number` of `others`: rows of no sequence, KV head h's part of them
 template <int D>
-__device__ __forceinline__ void attend_rest(const Attend& a, int split, int h, int64_t number, int64_t others) {
-  if (split) return;
+__device__ __forceinline__ void attend_rest(const Attend& a, int h, int number, int64_t others) {
+  if (others <= 0) return;
   int64_t front;
   const int64_t rest = step_rest(a.s, &front);
   for (int64_t n = number; n < rest; n += others) {
     const int64_t row = step_rest_row(a.s, front, rest, n) * a.Hq + h * a.G;
-    if (a.n_split > 1) {
-      for (int g = (int)threadIdx.x; g < a.G; g += 256) a.ml[(row + g) * a.n_split] = make_float2(-INFINITY, ATTEND_REST);
-    } else if (a.fill) {
+    if (a.shares)
+      for (int g = (int)threadIdx.x; g < a.G; g += 256) a.shares[row + g] = make_int2(0, 0);
+    if (a.fill)
       for (int c = (int)threadIdx.x; c < a.G * D / 2; c += 256) ((uint32_t*)((uint16_t*)a.out + row * D))[c] = 0;
-    }
   }
 }
 

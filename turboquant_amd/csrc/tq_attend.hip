@@ -7,62 +7,46 @@
 namespace tq {
 
 struct AttendJoin {
+  const int2* shares;
   const float2* ml;
   const float* acc;
   void* out;
   int64_t rows;            // token rows x heads
-  int32_t n_split, d, fill;
+  int32_t M, H, d, few, units, grid, most;      // (units of the plan, workgroups, splits of a row)
 };
 
-// Splits that a row has (those without tokens are the last ones), -1 for a row of no sequence
-__device__ __forceinline__ int attend_used(const AttendJoin& a, int64_t row) {
-  const float2* ml = a.ml + row * a.n_split;
-  const int lane = (int)threadIdx.x & 63;
-  int used = 0;
-  for (int i0 = 0; i0 < a.n_split; i0 += 64) {
-    const float y = i0 + lane < a.n_split ? ml[i0 + lane].y : ATTEND_EMPTY;
-    if (i0 == 0 && __builtin_amdgcn_readfirstlane(__float_as_int(y)) == __float_as_int(ATTEND_REST)) return -1;
-    const int n = __popcll(__ballot(!(y < 0.0f)));
-    used += n;
-    if (n < 64) break;
-  }
-  return used;
-}
-
+// A wavefront per row, or a workgroup per row and 64 channels.
 template <int DT>
 __global__ void __launch_bounds__(256) attend_join_kernel(const AttendJoin a) {
   __shared__ float s_f[JOIN_MAX_SPLITS];
   __shared__ float s_red[8];
   __shared__ float4 s_o[256];
-  const int lane = (int)threadIdx.x & 63;
-  if (a.n_split <= JOIN_FEW) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
-    if (row >= a.rows) return;
-    const float2 none = make_float2(-INFINITY, 0.0f);
-    float2 ml = lane < a.n_split ? a.ml[row * a.n_split + lane] : make_float2(-INFINITY, ATTEND_EMPTY);
-    const bool rest = __builtin_amdgcn_readfirstlane(__float_as_int(ml.y)) == __float_as_int(ATTEND_REST);
-    if (rest && !a.fill) return;
-    const bool there = !rest && !(ml.y < 0.0f);              // (a sum may be NaN)
-    const int used = __popcll(__ballot(there));
-    join_few<DT>(a.acc, a.n_split, a.d, a.out, row, used, there ? ml : none);
+  const int slices = a.few ? 1 : a.d >> 6;
+  const int64_t row = a.few ? (int64_t)blockIdx.x * 4 + ((int)threadIdx.x >> 6) : blockIdx.x / (unsigned)slices;
+  if (row >= a.rows) return;
+  const int2 s = a.shares[row];
+  const int used = __builtin_amdgcn_readfirstlane(s.y & 0xffff), r = __builtin_amdgcn_readfirstlane(s.y >> 16 & 0xff);
+  const int from = __builtin_amdgcn_readfirstlane(s.x);
+  if (used < 2) return;                                      // (there already, or a row of no sequence)
+  // (rows whose starts do not ascend may have been nobody's work: what lies in their place is no share)
+  const int64_t between = (int64_t)(__builtin_amdgcn_readfirstlane(s.y >> 24) ? a.units : 1) * a.H;
+  if (used > a.most || r >= a.M || from < 0 || from + (used - 1) * between >= a.grid) return;
+  const int64_t first = (int64_t)from * a.M + r, apart = between * a.M;
+  if (a.few) {
+    const int lane = (int)threadIdx.x & 63;
+    const float2 ml = lane < used ? a.ml[first + lane * apart] : make_float2(-INFINITY, 0.0f);
+    join_few<DT, 16>(a.acc + first * a.d, apart * a.d, a.d, a.out, row, used, ml);
   } else {
-    const int slices = a.d >> 6;
-    const int64_t row = blockIdx.x / (unsigned)slices;
-    int used = attend_used(a, row);
-    if (used < 0) {
-      if (!a.fill) return;
-      used = 0;
-    }
-    join_many<DT>(a.ml, a.acc, a.n_split, a.d, a.out, row, used, (int)(blockIdx.x % (unsigned)slices), s_f, s_red, s_o);
+    join_many<DT>(a.ml + first, apart, a.acc + first * a.d, apart * a.d, a.d, a.out, row, used, (int)(blockIdx.x % (unsigned)slices), s_f, s_red, s_o);
   }
 }
 
 // ---- how a call is split ----------------------------------------------------------------------------------------------------------------
 struct AttendPlan {
   int tiles;                          // column tiles of the kernel of few rows; 0: the kernel of many
-  int64_t units, grid;
-  int n_split, chunk;
-  size_t ml_at, acc_at, bytes;
+  int64_t units, items, grid;
+  int M, n_split, chunk, target, cap, few;
+  size_t shares_at, ml_at, acc_at, bytes;
 };
 
 static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -80,13 +64,14 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   max_rows = starts ? std::max<int64_t>(1, std::min(max_rows, rows)) : 1;
   p->tiles = max_rows * G <= 16 ? 1 : (max_rows * G <= 32 ? 2 : 0);
   const int M = p->tiles ? 16 * p->tiles : 128, TB = p->tiles ? 32 : 64;
-  p->units = starts ? (rows * G + M - 1) / M + B + 1 : (int64_t)B * ((G + M - 1) / M);
+  const int64_t units = std::max<int64_t>(1, starts ? (rows * G + M - 1) / M + B + 1 : (int64_t)B * ((G + M - 1) / M));
   // (of these, up to B are not met, and most of a short row's are)
-  const int64_t busy = starts ? std::max<int64_t>(std::min<int64_t>(B, rows), (rows * G + M - 1) / M) : p->units;
+  const int64_t busy = starts ? std::max<int64_t>(std::min<int64_t>(B, rows), (rows * G + M - 1) / M) : units;
   const int64_t pairs = std::max<int64_t>(1, busy * Hkv);
   int64_t tokens = std::max<int64_t>(max_len, 1);
   if (window > 0 && window < tokens) tokens = std::min(tokens, window + max_rows + std::min<int64_t>(sinks, tokens) + TB);
   const int64_t blocks = (tokens + TB - 1) / TB;
+  const int given = n_split;
   int64_t n = n_split;
   if (n == 0) {
     if (p->tiles) {
@@ -103,7 +88,6 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
         if (best >= 0.95) break;
       }
       n = std::min<int64_t>(n_split, (blocks + 3) / 4);
-      n_split = 0;
     } else {
       n = (256 * (d <= 128 ? 2 : 1) + pairs - 1) / pairs;
       n = std::min<int64_t>(std::min<int64_t>(n, (blocks + 3) / 4), JOIN_MAX_SPLITS);
@@ -111,16 +95,32 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   }
   n = std::max<int64_t>(1, std::min(n, blocks));
   int64_t chunk = (blocks + n - 1) / n;
-  if (n_split == 0 && p->tiles) chunk = (chunk + 3) & ~(int64_t)3;                             // (a block for each of the four wavefronts)
+  if (!given && p->tiles) chunk = (chunk + 3) & ~(int64_t)3;                       // (a block for each of the four wavefronts)
+  p->M = M;
+  p->units = units;
   p->n_split = (int)std::max<int64_t>(1, (blocks + chunk - 1) / chunk);
   p->chunk = (int)chunk;
+  // Sequences that differ (to find out takes a workgroup 1 - 2 us: not where 2048 tokens are the most that one has to itself) have their blocks shared out anew: 1024
+  // items in all (us, as planned / shared out; fp8, 24 sequences of 61 .. 16000, 5 rows 75 / 54, one row 54 / 46; 96 of 61 .. 8190 86 / 81), and with many rows 512
+  // (exact, 64 of 100 .. 20000, 64 rows 694 / 448).  A row has up to 64 of them where that leaves the join a wavefront for each row (above, a workgroup
+  // for 64 channels of one).
+  const bool many = rows * Hq >= 512;
+  p->target = p->cap = 0;
+  if (!given && B > 1 && B <= STEP_ROUND && tokens > 2048) {
+    p->target = (int)(((p->tiles ? 1024 : 512) + Hkv - 1) / Hkv);
+    p->cap = (int)std::max<int64_t>(p->n_split, std::min<int64_t>((blocks + 3) / 4, many ? 64 : JOIN_MAX_SPLITS));
+  }
+  p->items = std::max<int64_t>(units * p->n_split, p->target ? p->target + units + 2 : 0);      // (2: total and its share are rounded)
+  const int most = std::max(p->n_split, p->cap);
+  p->few = most <= JOIN_FEW || (many && most <= 64);
   const size_t all = (size_t)rows * Hq;
+  p->grid = p->items * Hkv;
   size_t at = 0;
-  p->ml_at = at;      at = round256(at + all * p->n_split * sizeof(float2));
-  p->acc_at = at;     at = round256(at + (p->n_split > 1 ? all * p->n_split * d * sizeof(float) : 0));
+  p->shares_at = at;  at = round256(at + (most > 1 ? all * sizeof(int2) : 0));
+  p->ml_at = at;      at = round256(at + (most > 1 ? (size_t)p->grid * M * sizeof(float2) : 0));
+  p->acc_at = at;     at = round256(at + (most > 1 ? (size_t)p->grid * M * d * sizeof(float) : 0));
   p->bytes = std::max<size_t>(at, 256);
-  p->grid = p->units * Hkv * p->n_split;
-  return p->grid <= INT32_MAX && join_groups((int64_t)all, p->n_split, d) <= INT32_MAX;
+  return p->grid <= INT32_MAX && (int64_t)all * (d / 64) <= INT32_MAX;
 }
 
 }  // namespace tq
@@ -156,7 +156,9 @@ extern "C" int tq_attend(const void* q, int dtype, int64_t rows, const int32_t* 
   a.q = q; a.out = out; a.Hq = Hq; a.G = Hq / Hkv;
   a.window = window <= 0 || window > INT32_MAX ? ATTEND_ALL : (int32_t)window;
   a.sinks = sinks; a.n_split = p.n_split; a.chunk = p.chunk; a.fill = fill; a.scale2 = sm_scale * 1.4426950408889634f;
-  a.units = p.units;
+  a.target = p.target; a.cap = p.cap; a.units = (int32_t)p.units; a.items = (int32_t)p.items; a.share = p.target ? 1.0f / p.target : 0.0f;
+  const bool joined = std::max(p.n_split, p.cap) > 1;
+  a.shares = joined ? (int2*)((char*)workspace + p.shares_at) : nullptr;
   a.ml = (float2*)((char*)workspace + p.ml_at);
   a.acc = (float*)((char*)workspace + p.acc_at);
   hipStream_t st = (hipStream_t)stream;
@@ -169,9 +171,9 @@ extern "C" int tq_attend(const void* q, int dtype, int64_t rows, const int32_t* 
     if (cache == TQ_E4M3) rc = dtype == TQ_F16 ? launch_attend_rows<TQ_F16, true>(a, g, st) : launch_attend_rows<TQ_BF16, true>(a, g, st);
     else rc = dtype == TQ_F16 ? launch_attend_rows<TQ_F16, false>(a, g, st) : launch_attend_rows<TQ_BF16, false>(a, g, st);
   }
-  if (rc || p.n_split == 1) return rc;
-  const AttendJoin j{a.ml, a.acc, out, rows * Hq, p.n_split, d, fill};
-  const dim3 grid((unsigned)join_groups(j.rows, p.n_split, d)), block(256);
+  if (rc || !joined) return rc;
+  const AttendJoin j{a.shares, a.ml, a.acc, out, rows * Hq, p.M, Hkv, d, p.few, (int)p.units, (int)p.grid, std::max(p.n_split, p.cap)};
+  const dim3 grid((unsigned)(p.few ? (j.rows + 3) / 4 : j.rows * (d / 64))), block(256);
   if (dtype == TQ_F16) attend_join_kernel<TQ_F16><<<grid, block, 0, st>>>(j);
   else attend_join_kernel<TQ_BF16><<<grid, block, 0, st>>>(j);
   TQ_CHECK_LAUNCH();

@@ -41,17 +41,20 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int col = lane & 15, quarter = lane >> 4;
-  const unsigned pairs = (unsigned)(a.units * a.H), split = blockIdx.x / pairs, pair = (blockIdx.x - split * pairs + split) % pairs;
-  const int h = (int)(pair % (unsigned)a.H);
-  int64_t number = pair / (unsigned)a.H;
+  const int item = (int)(blockIdx.x / (unsigned)a.H), x = (int)(blockIdx.x - (unsigned)item * (unsigned)a.H);
   AttendUnit u;
-  if (!attend_unit<16 * NT>(a, &number, &u)) {
-    attend_rest<D>(a, (int)split, h, number, a.units - (pair / (unsigned)a.H - number));
+  int over, others;
+  if (!attend_item<16 * NT, TB>(a, item, &u, &over, &others)) {
+    attend_rest<D>(a, x, over, others);
     return;
   }
+  // Which KV head: not the same for all that a compute unit has at a time (as planned, shares of one unit), whose addresses would all be the same in the bits
+  // that tell heads apart.  32 sequences of 8192, 8 heads of 128, 8 bits: 122 us with head x, 119 with x + unit, 107 so.
+  const int h = (int)((unsigned)(x + (u.planned ? u.split : item)) % (unsigned)a.H), place = item * a.H + h;
   const AttendBlocks<TB> list(a, u);
-  const int per = attend_per_split(list.count, a.n_split, a.chunk);
-  const int first = (int)split * per < list.count ? (int)split * per : list.count, last = first + per < list.count ? first + per : list.count;
+  const AttendShare share(a, u, list.count);
+  if (u.split >= share.used) return;
+  const int first = share.first, last = share.last;
 
   // this lane's rows: one of each column tile
   bool live[NT];
@@ -66,13 +69,10 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
     at_p[n] = u.low + (i - u.first / a.G);
     behind[n] = attend_behind(a, at_p[n]);
   }
-  if (first >= last && a.n_split > 1) {
-    if (quarter == 0 && wave == 0) {
+  if (a.shares && u.split == 0 && wave == 0 && quarter == 0) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-        if (live[n]) a.ml[row[n] * a.n_split + split] = make_float2(-INFINITY, ATTEND_EMPTY);
-    }
-    return;
+    for (int n = 0; n < NT; ++n)
+      if (live[n]) a.shares[row[n]] = make_int2(place, share.used | (n * 16 + col) << 16 | (u.planned ? 1 << 24 : 0));
   }
   const int32_t* table = a.s.table + u.b * a.s.table_step;
 
@@ -357,16 +357,17 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
     if (wave == 0 && live[n]) {
 #pragma unroll
       for (int t = 0; t < TILES; ++t) O[n][t] += s_acc[0][t][lane];
-      if (a.n_split > 1 && quarter == 0) a.ml[row[n] * a.n_split + split] = make_float2(M - ex_lift<PT>(), sum);
+      const int64_t slot = (int64_t)place * (16 * NT) + n * 16 + col;
+      if (share.used > 1 && quarter == 0) a.ml[slot] = make_float2(M - ex_lift<PT>(), sum);
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      float* acc = a.acc + (row[n] * a.n_split + split) * D;
+      float* acc = a.acc + slot * D;
 #pragma unroll
       for (int t = 0; t < TILES; t += 4)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int c = F8 ? (quarter * 4 + i) * TILES + t : ex_channel<WIDE>(t, quarter, i);      // and the three after it
           const ex_f32x4 x = {O[n][t][i], O[n][t + 1][i], O[n][t + 2][i], O[n][t + 3][i]};
-          if (a.n_split > 1) *(ex_f32x4*)(acc + c) = x;
+          if (share.used > 1) *(ex_f32x4*)(acc + c) = x;
           else *(ex_u32x2*)((uint16_t*)a.out + row[n] * D + c) = ex_u32x2{ex_pack<QT>(x[0] * inv, x[1] * inv), ex_pack<QT>(x[2] * inv, x[3] * inv)};
         }
     }

@@ -50,18 +50,19 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
 
   const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 31, half = lane >> 5;
   // (the last units of a sequence have the most tokens: they begin first)
-  const unsigned pairs = (unsigned)(a.units * a.H), split = blockIdx.x / pairs, pair = (blockIdx.x - split * pairs + split) % pairs;
-  const int h = (int)(pair % (unsigned)a.H);
-  const int64_t unit = a.units - 1 - pair / (unsigned)a.H;
-  int64_t number = unit;
+  const unsigned turn_of = blockIdx.x / (unsigned)a.H;
+  const int h = (int)(blockIdx.x - turn_of * (unsigned)a.H);
+  const int item = a.items - 1 - (int)turn_of, place = item * a.H + h;
   AttendUnit u;
-  if (!attend_unit<M>(a, &number, &u)) {
-    attend_rest<D>(a, (int)split, h, number, a.units - (unit - number));
+  int over, others;
+  if (!attend_item<M, ROWS_TOKENS>(a, item, &u, &over, &others)) {
+    attend_rest<D>(a, h, over, others);
     return;
   }
   const AttendBlocks<ROWS_TOKENS> list(a, u);
-  const int per = attend_per_split(list.count, a.n_split, a.chunk);
-  const int first = (int)split * per < list.count ? (int)split * per : list.count, last = first + per < list.count ? first + per : list.count;
+  const AttendShare share(a, u, list.count);
+  if (u.split >= share.used) return;
+  const int first = share.first, last = share.last;
 
   bool live[RT];
   int64_t row[RT];
@@ -75,11 +76,10 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
     at_p[n] = u.low + (i - u.first / a.G);
     behind[n] = attend_behind(a, at_p[n]);
   }
-  if (first >= last && a.n_split > 1) {
+  if (a.shares && u.split == 0 && half == 0) {
 #pragma unroll
     for (int n = 0; n < RT; ++n)
-      if (half == 0 && live[n]) a.ml[row[n] * a.n_split + split] = make_float2(-INFINITY, ATTEND_EMPTY);
-    return;
+      if (live[n]) a.shares[row[n]] = make_int2(place, share.used | ((wave * RT + n) * 32 + col) << 16 | (u.planned ? 1 << 24 : 0));
   }
   // the wavefront's first and last positions
   const int r0 = wave * RT * 32, r1 = r0 + RT * 32 - 1;
@@ -331,16 +331,17 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
     const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l[n]), __float_as_uint(l[n]), false, false);
     const float sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
     if (!live[n]) continue;
-    if (a.n_split > 1 && half == 0) a.ml[row[n] * a.n_split + split] = make_float2(m[n] - ex_lift<PT>(), sum);
+    const int64_t slot = (int64_t)place * M + (wave * RT + n) * 32 + col;
+    if (share.used > 1 && half == 0) a.ml[slot] = make_float2(m[n] - ex_lift<PT>(), sum);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    float* acc = a.acc + (row[n] * a.n_split + split) * D;
+    float* acc = a.acc + slot * D;
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         const int c = t * 32 + (e >> 2) * 8 + half * 4;       // and the three after it
         const ex_f32x4 x = {O[n][t][e], O[n][t][e + 1], O[n][t][e + 2], O[n][t][e + 3]};
-        if (a.n_split > 1) *(ex_f32x4*)(acc + c) = x;
+        if (share.used > 1) *(ex_f32x4*)(acc + c) = x;
         else *(ex_u32x2*)((uint16_t*)a.out + row[n] * D + c) = ex_u32x2{ex_pack<QT>(x[0] * inv, x[1] * inv), ex_pack<QT>(x[2] * inv, x[3] * inv)};
       }
   }

@@ -74,12 +74,12 @@ __global__ void __launch_bounds__(256) exact_join_kernel(const ExactJoin a, int 
     id = id * 4 + ((int)threadIdx.x >> 6);
     if (id < a.B * a.Hq) {
       const int lane = (int)threadIdx.x & 63, used = join_used(a, join_len(a, id / a.Hq));
-      join_few<DT>(a.acc, a.n_split, a.d, a.out, id, used, lane < used ? a.ml[(int64_t)id * a.n_split + lane] : make_float2(-INFINITY, 0.0f));
+      join_few<DT>(a.acc + (int64_t)id * a.n_split * a.d, a.d, a.d, a.out, id, used, lane < used ? a.ml[(int64_t)id * a.n_split + lane] : make_float2(-INFINITY, 0.0f));
     }
   } else {
     const int slices = a.d >> 6;
     const int row = id / slices;
-    join_many<DT>(a.ml, a.acc, a.n_split, a.d, a.out, row, join_used(a, join_len(a, row / a.Hq)), id % slices, (float*)s_two, s_red, s_o);
+    join_many<DT>(a.ml + (int64_t)row * a.n_split, 1, a.acc + (int64_t)row * a.n_split * a.d, a.d, a.d, a.out, row, join_used(a, join_len(a, row / a.Hq)), id % slices, (float*)s_two, s_red, s_o);
   }
 }
 

@@ -31,13 +31,14 @@ struct Fp8Unit {
 __device__ __forceinline__ int store_blocks(const StepRun& r) {
   return r.run == 0 ? 0 : ((r.len - 1) >> 4) - (r.token() >> 4) + 1;
 }
-__device__ __forceinline__ bool store_unit(const Step& s, int64_t u, Fp8Unit* t, int64_t* rest_unit) {
-  int64_t j = 0;
+__device__ __forceinline__ bool store_unit(const Step& s, int u, Fp8Unit* t, int64_t* rest_unit) {
+  int j = 0;
+  StepRun r;
+  const bool found = step_unit(s, &u, &t->b, &j, &r, [](const StepRun& x) { return store_blocks(x); });
   *rest_unit = u;
-  if (!step_unit(s, rest_unit, &t->b, &j, [](const StepRun& r) { return store_blocks(r); })) return false;
-  const StepRun r = step_run(s, t->b);
+  if (!found) return false;
   const int first = r.token();
-  t->page = (first >> 4) + (int)j;
+  t->page = (first >> 4) + j;
   t->first = j == 0 ? first : t->page * TQ_PAGE_TOKENS;
   t->end = (t->page + 1) * TQ_PAGE_TOKENS < r.len ? (t->page + 1) * TQ_PAGE_TOKENS : r.len;
   t->row = r.row + (t->first - first);
@@ -90,7 +91,7 @@ __global__ void __launch_bounds__(256) fp8_write_kernel(const Fp8Store a) {
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   Fp8Unit t;
   int64_t rest;
-  if (!store_unit(a.s, blockIdx.x / a.parts, &t, &rest)) return;
+  if (!store_unit(a.s, (int)(blockIdx.x / a.parts), &t, &rest)) return;
   const int64_t block = store_block(a.s, t);
   if (block < 0) return;                                     // (rows in front of token 0 among them: their page has none)
   const int low = t.first - t.page * TQ_PAGE_TOKENS, high = t.end - t.page * TQ_PAGE_TOKENS;
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(256) fp8_read_kernel(const Fp8Store a) {
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   Fp8Unit t;
   int64_t rest, block = -1, front = 0, all = 0;
-  const bool mine = store_unit(a.s, blockIdx.x / a.parts, &t, &rest);
+  const bool mine = store_unit(a.s, (int)(blockIdx.x / a.parts), &t, &rest);
   int low = 0, high = 0;
   if (mine) {
     block = store_block(a.s, t);

@@ -19,22 +19,23 @@ __device__ __forceinline__ void join_store(void* out, int64_t at, const float4& 
   }
 }
 
-// Few splits: a wavefront per row, a lane knows the factor of its split (ml of lane < used; -inf, 0 behind them).
-template <int DT>
-__device__ __forceinline__ void join_few(const float* accs, int n_split, int d, void* out, int64_t row, int used, const float2& ml) {
+// Few splits, 64 at most: a wavefront per row, a lane knows the factor of its split (ml of lane < used; -inf, 0 behind them).  A split's numerators
+// lie `apart` floats behind the one's before it; AHEAD of them are on their way at a time.
+template <int DT, int AHEAD = 8>
+__device__ __forceinline__ void join_few(const float* accs, int64_t apart, int d, void* out, int64_t row, int used, const float2& ml) {
   const int lane = (int)threadIdx.x & 63;
   const float top = wave_max_fast(ml.x), ref = top == -INFINITY ? 0.0f : top;
   const float f = __builtin_amdgcn_exp2f(ml.x - ref), sum = wave_sum_fast(f * ml.y), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   const int quads = d >> 2;
   for (int q = lane; q < quads; q += 64) {
-    const float4* acc = (const float4*)(accs + row * n_split * d) + q;
+    const float* acc = accs + q * 4;
     float4 o = make_float4(0, 0, 0, 0);
-    for (int i0 = 0; i0 < used; i0 += 8) {                   // eight on their way at a time, the last one over again behind the end
-      float4 x[8];
+    for (int i0 = 0; i0 < used; i0 += AHEAD) {               // (the last one over again behind the end)
+      float4 x[AHEAD];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = acc[(int64_t)(i0 + i < used ? i0 + i : used - 1) * quads];
+      for (int i = 0; i < AHEAD; ++i) x[i] = *(const float4*)(acc + (i0 + i < used ? i0 + i : used - 1) * apart);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < AHEAD; ++i) {
         const bool in = i0 + i < used;                       // (where not, a numerator of zero: a factor of zero would make NaN of an infinite one)
         const float g = in ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (i0 + i) & 63)) : 0.0f;
         o.x = fmaf(g, in ? x[i].x : 0.0f, o.x); o.y = fmaf(g, in ? x[i].y : 0.0f, o.y);
@@ -47,12 +48,11 @@ __device__ __forceinline__ void join_few(const float* accs, int n_split, int d, 
 
 // Many splits: a workgroup per row and 64 channels, sixteen lanes to a split, sixteen splits at a time.
 template <int DT>
-__device__ __forceinline__ void join_many(const float2* mls, const float* accs, int n_split, int d, void* out, int64_t row, int used, int slice, float* s_f,
-                                          float* s_red, float4* s_o) {
+__device__ __forceinline__ void join_many(const float2* ml, int64_t ml_apart, const float* accs, int64_t apart, int d, void* out, int64_t row, int used, int slice,
+                                          float* s_f, float* s_red, float4* s_o) {
   const int tid = (int)threadIdx.x;
-  const float2* ml = mls + row * n_split;
   float top = -INFINITY;
-  for (int i = tid; i < used; i += 256) top = fmaxf(top, ml[i].x);
+  for (int i = tid; i < used; i += 256) top = fmaxf(top, ml[i * ml_apart].x);
   top = wave_max_fast(top);
   if ((tid & 63) == 0) s_red[tid >> 6] = top;
   __syncthreads();
@@ -60,7 +60,7 @@ __device__ __forceinline__ void join_many(const float2* mls, const float* accs, 
   const float ref = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f;
   for (int i = tid; i < used; i += 256) {
-    const float2 x = ml[i];
+    const float2 x = ml[i * ml_apart];
     const float f = __builtin_amdgcn_exp2f(x.x - ref);
     s_f[i] = f;
     sum += f * x.y;
@@ -71,11 +71,11 @@ __device__ __forceinline__ void join_many(const float2* mls, const float* accs, 
   sum = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   const int quad = tid & 15, share = tid >> 4;
-  const float* acc = accs + row * n_split * d + slice * 64 + quad * 4;
+  const float* acc = accs + slice * 64 + quad * 4;
   float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll 8
   for (int i = share; i < used; i += 16) {
-    const float4 x = *(const float4*)(acc + (int64_t)i * d);
+    const float4 x = *(const float4*)(acc + i * apart);
     const float f = s_f[i];
     o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
   }

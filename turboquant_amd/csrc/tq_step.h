@@ -59,38 +59,60 @@ __device__ __forceinline__ int64_t step_uniform(int64_t x) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// Unit `u` of a step whose sequence b has count(b) of them: its sequence and which one of them it is; false (and u less all of them) if there are fewer.
-// A whole wavefront asks; u is the same in all lanes.  A lane adds up four sequences, so that up to 256 take one round of loads.
-template <class Count>
-__device__ __forceinline__ bool step_unit(const Step& s, int64_t* u, int* b, int64_t* j, Count count) {
+// sums over the lanes up to each one, by row shifts and the two broadcasts of a row's last lane; the whole wavefront
+__device__ __forceinline__ int step_sums(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+// Sequences are looked at 256 at a time, four a lane and 64 apart, so that their loads are on their way together.
+constexpr int STEP_ROUND = 256;
+__device__ __forceinline__ void step_runs(const Step& s, int base, StepRun (&r)[4]) {
   const int lane = (int)threadIdx.x & 63;
-  for (int base = 0; base < s.B; base += 256) {
-    int64_t c[4], sum = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = base + lane * 4 + i;
-      c[i] = at < s.B ? (int64_t)count(step_run(s, at)) : 0;
-      sum += c[i];
-    }
-    int64_t upto = sum;
+  for (int i = 0; i < 4; ++i) {
+    const int at = base + i * 64 + lane;
+    r[i].run = r[i].len = 0;
+    r[i].row = 0;
+    if (base + i * 64 < s.B && at < s.B) r[i] = step_run(s, at);
+  }
+}
+// Of a round whose sequences have count[i] units each: which has unit *u (their sums fit 31 bits), which one of its units that is, and its rows.  false:
+// none of them, and *u is less by all of theirs.
+__device__ __forceinline__ bool step_find(const Step& s, int base, const StepRun (&r)[4], const int (&count)[4], int* u, int* b, int* j, StepRun* run) {
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t below = __shfl_up((long long)upto, o, 64);
-      if (lane >= o) upto += below;
-    }
-    const int64_t all = step_uniform(__shfl((long long)upto, 63, 64));
+  for (int i = 0; i < 4; ++i) {
+    if (base + i * 64 >= s.B) break;
+    const int upto = step_sums(count[i]), all = __builtin_amdgcn_readlane(upto, 63);
     if (*u < all) {
       const int owner = __ffsll((unsigned long long)__ballot(upto > *u)) - 1;
-      int64_t left = *u - (upto - sum);
-      int which = 0;
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (which == i && left >= c[i]) { left -= c[i]; which = i + 1; }
-      *b = __builtin_amdgcn_readfirstlane(__shfl(base + lane * 4 + which, owner, 64));
-      *j = step_uniform(__shfl((long long)left, owner, 64));
+      *b = base + i * 64 + owner;
+      *j = *u - (__builtin_amdgcn_readlane(upto, owner) - __builtin_amdgcn_readlane(count[i], owner));
+      run->row = __builtin_amdgcn_readlane((int)r[i].row, owner);      // (a step has less than 2^31 rows)
+      run->run = __builtin_amdgcn_readlane(r[i].run, owner);
+      run->len = __builtin_amdgcn_readlane(r[i].len, owner);
       return true;
     }
     *u -= all;
+  }
+  return false;
+}
+// Unit `u` of a step whose sequence b has count(b) of them: its sequence, which one of them it is and the sequence's rows; false (and u less all of them) if there are fewer.
+// A whole wavefront asks; u is the same in all lanes.
+template <class Count>
+__device__ __forceinline__ bool step_unit(const Step& s, int* u, int* b, int* j, StepRun* run, Count count) {
+  for (int base = 0; base < s.B; base += STEP_ROUND) {
+    StepRun r[4];
+    step_runs(s, base, r);
+    int c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = r[i].run ? count(r[i]) : 0;
+    if (step_find(s, base, r, c, u, b, j, run)) return true;
   }
   return false;
 }
