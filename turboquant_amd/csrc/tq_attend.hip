@@ -15,29 +15,46 @@ struct AttendJoin {
   int32_t M, H, d, few, units, grid, most;      // (units of the plan, workgroups, splits of a row)
 };
 
-// A wavefront per row, or a workgroup per row and 64 channels.
+// A row's shares, and where they lie.  (Rows whose starts do not ascend may have been nobody's work: what lies in their place is no share.)
+struct AttendRow {
+  int used;
+  int64_t first, apart;
+  __device__ __forceinline__ AttendRow(const AttendJoin& a, const int2& s) {
+    const int r = s.y >> 16 & 0xff;
+    const int64_t between = (int64_t)(s.y >> 24 ? a.units : 1) * a.H;
+    used = s.y & 0xffff;
+    if (used > a.most || r >= a.M || s.x < 0 || s.x + (used - 1) * between >= a.grid) used = 0;
+    first = (int64_t)s.x * a.M + r;
+    apart = between * a.M;
+  }
+};
+
+// A wavefront for each `few` rows, one after another; or (0) a workgroup per row and 64 channels.
 template <int DT>
 __global__ void __launch_bounds__(256) attend_join_kernel(const AttendJoin a) {
   __shared__ float s_f[JOIN_MAX_SPLITS];
   __shared__ float s_red[8];
   __shared__ float4 s_o[256];
-  const int slices = a.few ? 1 : a.d >> 6;
-  const int64_t row = a.few ? (int64_t)blockIdx.x * 4 + ((int)threadIdx.x >> 6) : blockIdx.x / (unsigned)slices;
-  if (row >= a.rows) return;
-  const int2 s = a.shares[row];
-  const int used = __builtin_amdgcn_readfirstlane(s.y & 0xffff), r = __builtin_amdgcn_readfirstlane(s.y >> 16 & 0xff);
-  const int from = __builtin_amdgcn_readfirstlane(s.x);
-  if (used < 2) return;                                      // (there already, or a row of no sequence)
-  // (rows whose starts do not ascend may have been nobody's work: what lies in their place is no share)
-  const int64_t between = (int64_t)(__builtin_amdgcn_readfirstlane(s.y >> 24) ? a.units : 1) * a.H;
-  if (used > a.most || r >= a.M || from < 0 || from + (used - 1) * between >= a.grid) return;
-  const int64_t first = (int64_t)from * a.M + r, apart = between * a.M;
+  const int lane = (int)threadIdx.x & 63;
   if (a.few) {
-    const int lane = (int)threadIdx.x & 63;
-    const float2 ml = lane < used ? a.ml[first + lane * apart] : make_float2(-INFINITY, 0.0f);
-    join_few<DT, 16>(a.acc + first * a.d, apart * a.d, a.d, a.out, row, used, ml);
+    const int64_t row0 = ((int64_t)blockIdx.x * 4 + ((int)threadIdx.x >> 6)) * a.few;
+    int2 mine = make_int2(0, 0);
+    if (lane < a.few && row0 + lane < a.rows) mine = a.shares[row0 + lane];
+    // (fewer than two: there already, or a row of no sequence)
+    for (uint64_t left = __ballot((mine.y & 0xffff) > 1); left; left &= left - 1) {
+      const int i = __ffsll((unsigned long long)left) - 1;
+      const AttendRow r(a, make_int2(__builtin_amdgcn_readlane(mine.x, i), __builtin_amdgcn_readlane(mine.y, i)));
+      if (r.used < 2) continue;
+      const float2 ml = lane < r.used ? a.ml[r.first + lane * r.apart] : make_float2(-INFINITY, 0.0f);
+      join_few<DT, 16>(a.acc + r.first * a.d, r.apart * a.d, a.d, a.out, row0 + i, r.used, ml);
+    }
   } else {
-    join_many<DT>(a.ml + first, apart, a.acc + first * a.d, apart * a.d, a.d, a.out, row, used, (int)(blockIdx.x % (unsigned)slices), s_f, s_red, s_o);
+    const int slices = a.d >> 6;
+    const int64_t row = blockIdx.x / (unsigned)slices;
+    const int2 s = a.shares[row];
+    const AttendRow r(a, make_int2(__builtin_amdgcn_readfirstlane(s.x), __builtin_amdgcn_readfirstlane(s.y)));
+    if (r.used < 2) return;
+    join_many<DT>(a.ml + r.first, r.apart, a.acc + r.first * a.d, r.apart * a.d, a.d, a.out, row, r.used, (int)(blockIdx.x % (unsigned)slices), s_f, s_red, s_o);
   }
 }
 
@@ -112,7 +129,8 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   }
   p->items = std::max<int64_t>(units * p->n_split, p->target ? p->target + units + 2 : 0);      // (2: total and its share are rounded)
   const int most = std::max(p->n_split, p->cap);
-  p->few = most <= JOIN_FEW || (many && most <= 64);
+  // (with many rows a sequence few are split: 131072 of which none is took 12 us with a wavefront each)
+  p->few = most <= JOIN_FEW || (many && most <= 64) ? (p->tiles ? 1 : 8) : 0;
   const size_t all = (size_t)rows * Hq;
   p->grid = p->items * Hkv;
   size_t at = 0;
@@ -173,7 +191,7 @@ extern "C" int tq_attend(const void* q, int dtype, int64_t rows, const int32_t* 
   }
   if (rc || !joined) return rc;
   const AttendJoin j{a.shares, a.ml, a.acc, out, rows * Hq, p.M, Hkv, d, p.few, (int)p.units, (int)p.grid, std::max(p.n_split, p.cap)};
-  const dim3 grid((unsigned)(p.few ? (j.rows + 3) / 4 : j.rows * (d / 64))), block(256);
+  const dim3 grid((unsigned)(p.few ? (j.rows + 4 * p.few - 1) / (4 * p.few) : j.rows * (d / 64))), block(256);
   if (dtype == TQ_F16) attend_join_kernel<TQ_F16><<<grid, block, 0, st>>>(j);
   else attend_join_kernel<TQ_BF16><<<grid, block, 0, st>>>(j);
   TQ_CHECK_LAUNCH();
