@@ -1,6 +1,6 @@
 // Attention of many rows - prompts, chunks of them, dozens of query heads on one KV head - over a paged cache (instantiated by one file per types).
 //
-// A unit is 128 RT rows of a KV head: the query heads of a token side by side, tokens one behind another.  A wavefront takes 32 RT of them, each a column of
+// A unit is 128 rows of a KV head: the query heads of a token side by side, tokens one behind another.  A wavefront takes 32 of them, each a column of
 // its matrix instructions; the workgroup's keys and values go through LDS, 64 tokens at a time, in 16 bits whatever the cache holds, two buffers in turn:
 // the next tokens are on their way in registers while these are worked on, and a turn has one barrier.
 //   scores    S^T = K Q^T: tokens are rows.  A lane has 32 of the 64 scores of a row, its neighbour 32 lanes on the others.
@@ -37,14 +37,14 @@ template <int D> constexpr int rows_lds() { return 2 * 2 * ROWS_TOKENS * D * 2; 
 template <int D> __device__ __forceinline__ int rows_key_turn(int t) { return D % 128 == 0 ? (t & 15) : ((t >> 1) & 7); }
 template <int D> __device__ __forceinline__ int rows_value_turn(int t) { return D % 128 == 0 ? (t & 3) << 2 : ((t >> 1) & 1) << 2; }
 
-template <int QT, bool F8, int D, int RT>
-__global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_rows_kernel(const Attend a) {
+template <int QT, bool F8, int D>
+__global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(const Attend a) {
   constexpr int PT = F8 ? TQ_BF16 : QT;                      // of the value product
   constexpr bool HALVES = F8 && QT == TQ_F16;                // weights in two halves
   constexpr bool FOLD = F8 && QT == TQ_BF16;                 // a key's scale goes into the key
   constexpr int SIZE = F8 ? 1 : 2, ROW = D * 2;              // bytes of an element in the cache, of a row in LDS
   constexpr int LANES = D * SIZE / 16, LOADS = ROWS_TOKENS * LANES / 256;
-  constexpr int KSTEPS = D / 16, TILES = D / 32, M = 128 * RT;
+  constexpr int KSTEPS = D / 16, TILES = D / 32, M = 128;
   constexpr int HALF = ROWS_TOKENS * ROW;                    // keys or values of a turn
   extern __shared__ __attribute__((aligned(16))) char s_rows[];
 
@@ -64,25 +64,14 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
   if (u.split >= share.used) return;
   const int first = share.first, last = share.last;
 
-  bool live[RT];
-  int64_t row[RT];
-  int at_p[RT], behind[RT];
-#pragma unroll
-  for (int n = 0; n < RT; ++n) {
-    const int r = (wave * RT + n) * 32 + col;
-    live[n] = r < u.rows;
-    const int x = u.first + (live[n] ? r : 0), i = x / a.G;
-    row[n] = (u.row + i) * a.Hq + h * a.G + (x - i * a.G);
-    at_p[n] = u.low + (i - u.first / a.G);
-    behind[n] = attend_behind(a, at_p[n]);
-  }
-  if (a.shares && u.split == 0 && half == 0) {
-#pragma unroll
-    for (int n = 0; n < RT; ++n)
-      if (live[n]) a.shares[row[n]] = make_int2(place, share.used | ((wave * RT + n) * 32 + col) << 16 | (u.planned ? 1 << 24 : 0));
-  }
+  // this lane's row
+  const int r = wave * 32 + col, x = u.first + (r < u.rows ? r : 0), token = x / a.G;
+  const bool live = r < u.rows;
+  const int64_t row = (u.row + token) * a.Hq + h * a.G + (x - token * a.G);
+  const int at_p = u.low + (token - u.first / a.G), behind = attend_behind(a, at_p);
+  if (a.shares && u.split == 0 && half == 0 && live) a.shares[row] = make_int2(place, share.used | r << 16 | (u.planned ? 1 << 24 : 0));
   // the wavefront's first and last positions
-  const int r0 = wave * RT * 32, r1 = r0 + RT * 32 - 1;
+  const int r0 = wave * 32, r1 = r0 + 31;
   const bool busy = r0 < u.rows;
   const int w_low = u.low + (u.first + r0) / a.G - u.first / a.G, w_high = u.low + (u.first + (r1 < u.rows ? r1 : u.rows - 1)) / a.G - u.first / a.G;
   const int w_behind_low = attend_behind(a, w_low), w_behind_high = attend_behind(a, w_high);
@@ -91,32 +80,25 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
   // (a negative scale turns the queries and one of zero clears them, so that the scores' order is that of their products)
   const float f = a.scale2 == 0.0f ? 1.0f : fabsf(a.scale2);
   const uint32_t turn = a.scale2 < 0.0f ? 0x80008000u : 0u, keep = a.scale2 == 0.0f ? 0u : 0xffffffffu;
-  ex_u32x4 Q[RT][KSTEPS];
+  ex_u32x4 Q[KSTEPS];
 #pragma unroll
-  for (int n = 0; n < RT; ++n)
+  for (int s = 0; s < KSTEPS; ++s) {
+    Q[s] = ex_u32x4{0, 0, 0, 0};
+    if (live) Q[s] = *(const ex_u32x4*)((const uint16_t*)a.q + row * D + s * 16 + half * 8);
 #pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) {
-      Q[n][s] = ex_u32x4{0, 0, 0, 0};
-      if (live[n]) Q[n][s] = *(const ex_u32x4*)((const uint16_t*)a.q + row[n] * D + s * 16 + half * 8);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) Q[n][s][i] = (Q[n][s][i] & keep) ^ turn;
-    }
-  ro_f32x16 O[RT][TILES];
-  float m[RT], l[RT];
-#pragma unroll
-  for (int n = 0; n < RT; ++n) {
-#pragma unroll
-    for (int t = 0; t < TILES; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) O[n][t][i] = 0.0f;
-    m[n] = -INFINITY;
-    l[n] = 0.0f;
+    for (int i = 0; i < 4; ++i) Q[s][i] = (Q[s][i] & keep) ^ turn;
   }
+  ro_f32x16 O[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) O[t][i] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
 
   // ---- a turn's tokens: table entries, loads into registers, registers into LDS ----
   const int last_page = u.tokens > 0 ? (u.tokens - 1) / TQ_PAGE_TOKENS : 0;
   struct Turn {
-    int32_t entry[4];
+    uint32_t entry[4];
     int t0;
   };
   const auto entries = [&](Turn& x, int i) __attribute__((always_inline)) {
@@ -125,43 +107,68 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       const int page = blk * 4 + p;
-      x.entry[p] = step_entry(table, page < last_page ? page : last_page);
+      x.entry[p] = (uint32_t)step_entry(table, page < last_page ? page : last_page);
+    }
+  };
+  // (scalar instructions are a wavefront's time as well: 64-bit products for each load were a fifth of it)
+  const uint32_t in_cache = a.s.num_blocks < 0x80000000ll ? (uint32_t)a.s.num_blocks : 0x80000000u;
+  const uint64_t block_bytes = (uint64_t)a.s_blk * SIZE, head_bytes = (uint64_t)h * a.s_h * SIZE;
+  const uint32_t step = (uint32_t)a.s_t * SIZE;
+  // all of a turn's tokens are the sequence's, in blocks of the cache
+  const auto complete = [&](const Turn& x) __attribute__((always_inline)) {
+    const uint32_t p = x.entry[0] > x.entry[1] ? x.entry[0] : x.entry[1], q = x.entry[2] > x.entry[3] ? x.entry[2] : x.entry[3];
+    return x.t0 + ROWS_TOKENS <= u.tokens && (p > q ? p : q) < in_cache;
+  };
+  // The i-th load of a lane: 16 bytes, piece piece_of of token token_of of the turn.  Rows of a power of two of pieces: the page is a wavefront's, and the
+  // lane's place in it always the same, but for 512 bytes of them, where it changes with odd i.  192 channels: lanes work their places out load by load.
+  constexpr bool EVEN = D != 192;
+  constexpr int APART = 256 / LANES, PER = F8 ? 2 : 1;       // tokens from a load to the next; pieces of 8 channels in one
+  const auto token_of = [&](int i) __attribute__((always_inline)) { return EVEN ? tid / LANES + i * APART : (i * 256 + tid) / LANES; };
+  const auto piece_of = [&](int i) __attribute__((always_inline)) { return EVEN ? tid % LANES : (i * 256 + tid) % LANES; };
+  const auto entry_of = [&](const Turn& x, int i) __attribute__((always_inline)) {
+    if constexpr (EVEN) {
+      constexpr int OWN = 64 / LANES;                        // tokens of a wavefront's load
+      if constexpr (OWN < 8) return x.entry[i * APART / 16];
+      else if constexpr (OWN < 16) return wave < 2 ? x.entry[i * APART / 16] : x.entry[i * APART / 16 + 1];
+      else return wave < 2 ? (wave < 1 ? x.entry[0] : x.entry[1]) : (wave < 3 ? x.entry[2] : x.entry[3]);
+    } else {
+      const int p = token_of(i) >> 4;
+      return p < 2 ? (p < 1 ? x.entry[0] : x.entry[1]) : (p < 3 ? x.entry[2] : x.entry[3]);
     }
   };
   ex_u32x4 KR[LOADS], VR[LOADS];
   uint32_t ks[F8 ? LOADS : 1], vs[F8 ? LOADS : 1];
-  const auto token_of = [&](int i) __attribute__((always_inline)) { return (i * 256 + tid) / LANES; };
-  const auto good = [&](int32_t e) __attribute__((always_inline)) { return e >= 0 && e < a.s.num_blocks; };
-  const auto entry_of = [&](const Turn& x, int t) __attribute__((always_inline)) {
-    int p = t >> 4;
-    if constexpr (D != 192) p = __builtin_amdgcn_readfirstlane(p);      // (a wavefront's lanes are in one page)
-    return p == 0 ? x.entry[0] : (p == 1 ? x.entry[1] : (p == 2 ? x.entry[2] : x.entry[3]));
-  };
+  const uint32_t here = EVEN ? (uint32_t)(tid / LANES % 16) * step + (uint32_t)(tid % LANES) * 16 : 0;
   const auto load = [&](const Turn& x) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int t = token_of(i), c = (i * 256 + tid) - t * LANES;
-      const int32_t e = entry_of(x, t);
-      const int64_t page = good(e) ? e : 0;
-      const int64_t at = (page * a.s_blk + h * a.s_h) * SIZE + (uint32_t)(t & 15) * (uint32_t)(a.s_t * SIZE) + c * 16;
-      KR[i] = *(const ex_u32x4*)((const char*)a.k + at);
-      VR[i] = *(const ex_u32x4*)((const char*)a.v + at);
+      const uint32_t e = entry_of(x, i), page = e < in_cache ? e : 0u;      // (a block that is there; its tokens are masked)
+      const uint64_t block = page * block_bytes + head_bytes;
+      uint32_t at = here + (APART < 16 ? (uint32_t)(i * APART % 16) * step : 0u);
+      if constexpr (!EVEN) at = (uint32_t)(token_of(i) & 15) * step + (uint32_t)piece_of(i) * 16;
+      KR[i] = *(const ex_u32x4*)((const char*)a.k + block + at);
+      VR[i] = *(const ex_u32x4*)((const char*)a.v + block + at);
       if constexpr (F8) {
-        ks[i] = a.k_scales[page * a.H + h];
-        vs[i] = a.v_scales[page * a.H + h];
+        ks[i] = a.k_scales[(uint64_t)page * a.H + h];
+        vs[i] = a.v_scales[(uint64_t)page * a.H + h];
       }
     }
   };
   const auto scale_of = [](uint32_t byte) __attribute__((always_inline)) { return byte == 0 ? 0x1p-127f : __uint_as_float(byte << 23); };
+  const int t_here = tid / LANES, c_here = tid % LANES * PER;
+  const uint32_t key_to = (uint32_t)(t_here * ROW + (c_here ^ rows_key_turn<D>(t_here)) * 16), value_to = (uint32_t)(t_here * ROW + (c_here ^ rows_value_turn<D>(t_here)) * 16);
   const auto store = [&](const Turn& x, char* to) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int t = token_of(i), c = (i * 256 + tid) - t * LANES;
+      uint32_t k = (key_to ^ (uint32_t)(rows_key_turn<D>(i * APART) * 16)) + (uint32_t)(i * APART * ROW), v = value_to + (uint32_t)(i * APART * ROW);
+      if constexpr (!EVEN) {
+        const int t = token_of(i), c = piece_of(i) * PER;
+        k = (uint32_t)(t * ROW + (c ^ rows_key_turn<D>(t)) * 16);
+        v = (uint32_t)(t * ROW + (c ^ rows_value_turn<D>(t)) * 16);
+      }
+      char *const kt = to, *const vt = to + HALF;
       // values of tokens that nobody sees are zeros: what lies in their slots may be NaN
-      const bool none = x.t0 + t >= u.tokens || !good(entry_of(x, t));
-      char *k = to + t * ROW, *v = to + HALF + t * ROW;
-      const int kt = rows_key_turn<D>(t), vt = rows_value_turn<D>(t);
-      if (none) VR[i] = ex_u32x4{0, 0, 0, 0};
+      if (!complete(x) && !(x.t0 + token_of(i) < u.tokens && entry_of(x, i) < in_cache)) VR[i] = ex_u32x4{0, 0, 0, 0};
       if constexpr (F8) {
         const float kf = FOLD ? scale_of(ks[i]) : 1.0f, vf = scale_of(vs[i]);
 #pragma unroll
@@ -174,28 +181,25 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
             z[w * 2] = f8_widen<TQ_BF16, false>(VR[i][j * 2 + w], vf);
             z[w * 2 + 1] = f8_widen<TQ_BF16, true>(VR[i][j * 2 + w], vf);
           }
-          *(ex_u32x4*)(k + ((c * 2 + j) ^ kt) * 16) = y;
-          *(ex_u32x4*)(v + ((c * 2 + j) ^ vt) * 16) = z;
+          *(ex_u32x4*)(kt + (k ^ (uint32_t)(j * 16))) = y;
+          *(ex_u32x4*)(vt + (v ^ (uint32_t)(j * 16))) = z;
         }
       } else {
-        *(ex_u32x4*)(k + (c ^ kt) * 16) = KR[i];
-        *(ex_u32x4*)(v + (c ^ vt) * 16) = VR[i];
+        *(ex_u32x4*)(kt + k) = KR[i];
+        *(ex_u32x4*)(vt + v) = VR[i];
       }
     }
   };
-  // ---- a lane's places in LDS ----
-  const int k_turn = rows_key_turn<D>(col);
-  const int j16 = lane & 15, v_turn = D % 128 == 0 ? j16 >> 2 : j16 >> 3;
-  const auto key_place = [&](int s) __attribute__((always_inline)) { return (uint32_t)(col * ROW + ((s * 2 + half) ^ k_turn) * 16); };
-  const auto value_place = [&](int ct) __attribute__((always_inline)) {
-    return (uint32_t)(HALF + (half * 4 + (j16 >> 2)) * ROW + ((ct ^ v_turn) * 4 + ((lane >> 4) & 1) * 2 + ((j16 & 3) >> 1)) * 16 + (j16 & 1) * 8);
-  };
+  // ---- a lane's places in LDS: the other steps and tiles lie where a few of the place's bits differ ----
+  const int j16 = lane & 15;
+  const uint32_t key_from = (uint32_t)(col * ROW + (half ^ rows_key_turn<D>(col)) * 16);
+  const uint32_t value_from = (uint32_t)(HALF + (half * 4 + (j16 >> 2)) * ROW + ((D % 128 == 0 ? j16 >> 2 : j16 >> 3) * 4 + ((lane >> 4) & 1) * 2 + ((j16 & 3) >> 1)) * 16 + (j16 & 1) * 8);
   constexpr int KPLACES = D % 128 == 0 ? 8 : 4, VPLACES = D % 128 == 0 ? 4 : 2;
   uint32_t kp[KPLACES], vp[VPLACES];
 #pragma unroll
-  for (int s = 0; s < KPLACES; ++s) kp[s] = key_place(s);
+  for (int s = 0; s < KPLACES; ++s) kp[s] = key_from ^ (uint32_t)(s * 32);
 #pragma unroll
-  for (int t = 0; t < VPLACES; ++t) vp[t] = value_place(t);
+  for (int t = 0; t < VPLACES; ++t) vp[t] = value_from ^ (uint32_t)(t * 64);
 
   Turn now, next;
   entries(now, first);
@@ -210,99 +214,81 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
     char* buffer = s_rows + ((i - first) & 1) * 2 * HALF;
     char* other = s_rows + (((i - first) & 1) ^ 1) * 2 * HALF;
     Turn after;
-    if (more) {
-      load(next);
-      entries(after, i + 2);
-    }
+    if (more) load(next);
+    entries(after, i + 2);
     // what this wavefront's rows see of the turn: nothing, all of it, or some
     const int t0 = now.t0, t1 = t0 + ROWS_TOKENS - 1;
     const bool any = busy && t0 <= w_high && (t1 > w_behind_low || t0 < a.sinks);
     if (any) {
-      bool whole = t1 <= w_low && t1 < u.tokens && (t0 > w_behind_high || t1 < a.sinks);
-#pragma unroll
-      for (int p = 0; p < 4; ++p) whole = whole && good(now.entry[p]);
-      ro_f32x16 S[RT][2];
+      const bool whole = t1 <= w_low && (t0 > w_behind_high || t1 < a.sinks) && complete(now);
+      ro_f32x16 S[2];
 #pragma unroll
       for (int T = 0; T < 2; ++T) {
 #pragma unroll
-        for (int n = 0; n < RT; ++n)
+        for (int e = 0; e < 16; ++e) S[T][e] = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) S[n][T][e] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < KSTEPS; ++s) {
-          const ex_u32x4 k = *(const ex_u32x4*)(buffer + kp[s % KPLACES] + (s / KPLACES) * KPLACES * 32 + T * 32 * ROW);
-#pragma unroll
-          for (int n = 0; n < RT; ++n) S[n][T] = rows_mfma<QT>(k, Q[n][s], S[n][T]);
-        }
+        for (int s = 0; s < KSTEPS; ++s)
+          S[T] = rows_mfma<QT>(*(const ex_u32x4*)(buffer + kp[s % KPLACES] + (s / KPLACES) * KPLACES * 32 + T * 32 * ROW), Q[s], S[T]);
       }
       if constexpr (F8 && !FOLD) {
-        float g[4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          const int64_t page = good(now.entry[p]) ? now.entry[p] : 0;
-          g[p] = scale_of(a.k_scales[page * a.H + h]);
+          const uint64_t page = now.entry[p] < in_cache ? now.entry[p] : 0u;
+          const float g = scale_of(a.k_scales[page * a.H + h]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) S[p >> 1][(p & 1) * 8 + e] *= g;
         }
-#pragma unroll
-        for (int n = 0; n < RT; ++n)
-#pragma unroll
-          for (int T = 0; T < 2; ++T)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) S[n][T][e] *= g[T * 2 + (e >> 3)];
       }
-      ex_u32x4 P[RT][4], L[HALVES ? RT : 1][4];
-#pragma unroll
-      for (int n = 0; n < RT; ++n) {
-        if (!whole) {
-#pragma unroll
-          for (int T = 0; T < 2; ++T)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int in = T * 32 + (e >> 2) * 8 + half * 4 + (e & 3), t = t0 + in;
-              const bool seen = (t <= at_p[n]) & (t < u.tokens) & ((t > behind[n]) | (t < a.sinks)) & good(now.entry[T * 2 + (e >> 3)]);
-              S[n][T][e] = seen ? S[n][T][e] : -INFINITY;
-            }
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int T = 0; T < 2; ++T)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) top = fmaxf(top, S[n][T][e]);
-        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * f;
-        top = fmaxf(m[n], top);
-        if (__any(top > m[n] + EX_SLACK)) {
-          const float move = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[n] - top);
-          l[n] *= move;
-#pragma unroll
-          for (int t = 0; t < TILES; ++t) O[n][t] *= move;
-          m[n] = top;
-        }
-        const float ref = m[n] == -INFINITY ? 0.0f : m[n] - ex_lift<PT>();
-        float sum = 0.0f;
+      if (!whole) {
 #pragma unroll
         for (int T = 0; T < 2; ++T)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(S[n][T][e], f, -ref));
-            S[n][T][e] = p;
-            sum += p;
-          }
-        l[n] += sum;
-#pragma unroll
-        for (int T = 0; T < 2; ++T)
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const int at = T * 2 + (e >> 3), w = (e & 7) >> 1;
-            if constexpr (HALVES) {
-              uint32_t hi, lo;
-              ex_split<PT>(S[n][T][e], S[n][T][e + 1], &hi, &lo);
-              P[n][at][w] = hi;
-              L[n][at][w] = lo;
-            } else {
-              P[n][at][w] = ex_pack<PT>(S[n][T][e], S[n][T][e + 1]);
-            }
+            const int t = t0 + T * 32 + (e >> 2) * 8 + half * 4 + (e & 3);
+            const bool seen = (t <= at_p) & (t < u.tokens) & ((t > behind) | (t < a.sinks)) & (now.entry[T * 2 + (e >> 3)] < in_cache);
+            S[T][e] = seen ? S[T][e] : -INFINITY;
           }
       }
+      float top = -INFINITY;
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, S[T][e]);
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(m, fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * f);
+      if (__any(top > m + EX_SLACK)) {
+        const float move = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+        l *= move;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) O[t] *= move;
+        m = top;
+      }
+      const float ref = m == -INFINITY ? 0.0f : m - ex_lift<PT>();
+      float sum = 0.0f;
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(S[T][e], f, -ref));
+          S[T][e] = p;
+          sum += p;
+        }
+      l += sum;
+      ex_u32x4 P[4], L[HALVES ? 4 : 1];
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const int at = T * 2 + (e >> 3), w = (e & 7) >> 1;
+          if constexpr (HALVES) {
+            uint32_t hi, lo;
+            ex_split<PT>(S[T][e], S[T][e + 1], &hi, &lo);
+            P[at][w] = hi;
+            L[at][w] = lo;
+          } else {
+            P[at][w] = ex_pack<PT>(S[T][e], S[T][e + 1]);
+          }
+        }
 #pragma unroll
       for (int at = 0; at < 4; ++at)
 #pragma unroll
@@ -313,11 +299,8 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
           const ro_s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(from + 8 * ROW));
           const ex_u32x2 lo = __builtin_bit_cast(ex_u32x2, x), hi = __builtin_bit_cast(ex_u32x2, y);
           const ex_u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-          for (int n = 0; n < RT; ++n) {
-            if constexpr (HALVES) O[n][ct] = rows_mfma<PT>(v, L[n][at], O[n][ct]);
-            O[n][ct] = rows_mfma<PT>(v, P[n][at], O[n][ct]);
-          }
+          if constexpr (HALVES) O[ct] = rows_mfma<PT>(v, L[at], O[ct]);
+          O[ct] = rows_mfma<PT>(v, P[at], O[ct]);
         }
     }
     if (more) store(next, other);
@@ -326,32 +309,29 @@ __global__ void __launch_bounds__(256, (D <= 128 && RT == 1 ? 2 : 1)) attend_row
     next = after;
   }
 
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+  const float sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+  if (!live) return;
+  const int64_t slot = (int64_t)place * M + r;
+  if (share.used > 1 && half == 0) a.ml[slot] = make_float2(m - ex_lift<PT>(), sum);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  float* acc = a.acc + slot * D;
 #pragma unroll
-  for (int n = 0; n < RT; ++n) {
-    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l[n]), __float_as_uint(l[n]), false, false);
-    const float sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-    if (!live[n]) continue;
-    const int64_t slot = (int64_t)place * M + (wave * RT + n) * 32 + col;
-    if (share.used > 1 && half == 0) a.ml[slot] = make_float2(m[n] - ex_lift<PT>(), sum);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    float* acc = a.acc + slot * D;
+  for (int t = 0; t < TILES; ++t)
 #pragma unroll
-    for (int t = 0; t < TILES; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int c = t * 32 + (e >> 2) * 8 + half * 4;       // and the three after it
-        const ex_f32x4 x = {O[n][t][e], O[n][t][e + 1], O[n][t][e + 2], O[n][t][e + 3]};
-        if (share.used > 1) *(ex_f32x4*)(acc + c) = x;
-        else *(ex_u32x2*)((uint16_t*)a.out + row[n] * D + c) = ex_u32x2{ex_pack<QT>(x[0] * inv, x[1] * inv), ex_pack<QT>(x[2] * inv, x[3] * inv)};
-      }
-  }
+    for (int e = 0; e < 16; e += 4) {
+      const int c = t * 32 + (e >> 2) * 8 + half * 4;         // and the three after it
+      const ex_f32x4 y = {O[t][e], O[t][e + 1], O[t][e + 2], O[t][e + 3]};
+      if (share.used > 1) *(ex_f32x4*)(acc + c) = y;
+      else *(ex_u32x2*)((uint16_t*)a.out + row * D + c) = ex_u32x2{ex_pack<QT>(y[0] * inv, y[1] * inv), ex_pack<QT>(y[2] * inv, y[3] * inv)};
+    }
 }
 
 template <int QT, bool F8, int D>
 int launch_attend_rows_d(const Attend& a, unsigned grid, hipStream_t stream) {
   static std::atomic<uint64_t> ready{0};
-  if (const int rc = exact_allow_lds((const void*)attend_rows_kernel<QT, F8, D, 1>, rows_lds<D>(), ready)) return rc;
-  attend_rows_kernel<QT, F8, D, 1><<<dim3(grid), dim3(256), rows_lds<D>(), stream>>>(a);
+  if (const int rc = exact_allow_lds((const void*)attend_rows_kernel<QT, F8, D>, rows_lds<D>(), ready)) return rc;
+  attend_rows_kernel<QT, F8, D><<<dim3(grid), dim3(256), rows_lds<D>(), stream>>>(a);
   TQ_CHECK_LAUNCH();
   return TQ_OK;
 }
