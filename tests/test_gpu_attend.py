@@ -174,3 +174,45 @@ def test_strided_queries_and_inference(gpu, kind):
     with torch.inference_mode():
         s.check(q, s.cache().attention(wide, s.starts.long(), s.table, s.seq_lens.cpu()), 0.125)
         s.check(q, s.cache().attention(torch._neg_view(-q.to(gpu)), s.starts, s.table, s.seq_lens), 0.125)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("G,runs", [(1, [1, 1]), (4, [3, 5]), (4, [60, 37]), (128, [2, 1]), (160, [3, 2])])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (21, 6)])
+def test_values_that_are_not_finite(gpu, kind, d, G, runs, window, sinks):
+    """Infinities and NaN among the values: in the channels of the rows that see them, and nowhere else."""
+    lens = [130, 90]
+    s = make(kind, lens, runs, 2, d)
+    q = s.query(2 * G).to(gpu)
+    kw = dict(window=window, sinks=sinks)
+    inf, nan = float("inf"), float("nan")
+    put = []                                                 # (sequence, token, head, channel, value)
+    for b, n in enumerate(lens):
+        edge = [n - 1, n - 2, n - runs[b], n - runs[b] + 1, n - runs[b] - 20, n - 22, n - 21, n - 20, 0, 5, 6, 33, 64]
+        for i, t in enumerate(e for e in edge if 0 <= e < n):
+            put.append((b, t, i % 2, (7 * i + b) % d, nan if kind.startswith("fp8") else (inf, -inf, nan)[i % 3]))
+            put.append((b, t, 1, d - 1, nan if kind.startswith("fp8") else inf))
+    odd = torch.zeros(2, max(lens), 2, d)
+    for b, t, h, c, x in put:
+        where = (int(s.table_cpu[b, t // 16]), t % 16, h, c)
+        s.q[1].view(torch.uint8 if kind.startswith("fp8") else s.q[1].dtype)[where] = 0
+        s.v64[where] = 0
+        odd[b, t, h, c] = x
+    clean = s.cache().attention(q, s.starts, s.table, s.seq_lens, **kw)
+    s.check(q.cpu(), clean, 1 / math.sqrt(d), window, sinks)
+    for b, t, h, c, x in put:
+        s.q[1].view(torch.uint8 if kind.startswith("fp8") else s.q[1].dtype)[int(s.table_cpu[b, t // 16]), t % 16, h, c] = 0x7f if kind.startswith("fp8") else x
+    for n_split in (None, 1, 3):
+        got = s.cache().attention(q, s.starts, s.table, s.seq_lens, **kw, **({} if n_split is None else {"n_split": n_split})).cpu()
+        at = 0
+        for b, run in enumerate(runs):
+            for i in range(run):
+                p = lens[b] - run + i
+                t = torch.arange(p + 1)
+                seen = (t > p - window) | (t < sinks) if window else torch.ones(p + 1, dtype=torch.bool)
+                add = odd[b, : p + 1][seen].sum(0).repeat_interleave(G, 0)
+                assert torch.equal(got[at + i].isfinite(), add.isfinite()), (b, i)
+            at += run
+        if n_split is None:
+            assert torch.equal(torch.where(got.isfinite(), got, clean.cpu()), clean.cpu())

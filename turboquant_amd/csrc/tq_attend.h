@@ -32,6 +32,29 @@ struct Attend {
   int2* shares;                            // (rows, Hq): first, number | row << 16 | planned << 24; null: all rows have one
 };
 
+// Infinities and NaN among the values.  A row's weights are 0 where it sees nothing, and 0 times them is NaN: where the rows of a unit see different tokens
+// (blocks at their own positions and at the window's edge), such values are put to zero before the product, and the rows that see them get them added
+// at the end, read once more.  A block that all rows see whole takes them as they are.
+//   16 or 8 bits each: the numbers of x that are finite
+template <int DT>
+__device__ __forceinline__ uint32_t attend_finite(uint32_t x) {
+  // (an exponent of all ones, in e4m3 all ones but the sign: a carry into the sign's place tells)
+  if constexpr (DT == TQ_E4M3) return x & ~(((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu);
+  else if constexpr (DT == TQ_BF16) return x & ~(((((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xffffu);
+  else return x & ~(((((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u) >> 15) * 0xffffu);
+}
+//   number i of x if it is not finite, else 0
+template <int DT>
+__device__ __forceinline__ float attend_not_finite(f8_u32x2 x, int i) {
+  if constexpr (DT == TQ_E4M3) {
+    return (x[0] >> i * 8 & 0x7f) == 0x7f ? NAN : 0.0f;
+  } else {
+    const uint32_t n = x[i >> 1] >> (i & 1) * 16 & 0xffff;
+    if constexpr (DT == TQ_BF16) return (n & 0x7f80) == 0x7f80 ? __uint_as_float(n << 16) : 0.0f;
+    else return (n & 0x7c00) == 0x7c00 ? __uint_as_float((n & 0x8000) << 16 | 0x7f800000u | (n & 0x3ff) << 13) : 0.0f;
+  }
+}
+
 // What a workgroup works on: `rows` rows of a sequence's run * G (the heads of a token side by side), from `first` on, and a share of the tokens they see
 struct AttendUnit {
   int b;

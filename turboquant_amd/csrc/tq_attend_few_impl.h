@@ -29,9 +29,11 @@ constexpr int attend_few_waves() {
   return F8 ? (D <= 64 ? 3 : (D <= 128 ? 2 : 1)) : (D <= 64 ? 3 : (D <= 128 ? 2 : 1));
 }
 
-template <int QT, bool F8, int D, int NT>
+// APART: rows of a unit may stand at different positions (not one token of each sequence)
+template <int QT, bool F8, int D, int NT, bool APART>
 __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_few_kernel(const Attend a) {
   constexpr int PT = F8 ? TQ_BF16 : QT;                      // of the value product
+  constexpr int VT = F8 ? TQ_E4M3 : QT;                      // of the cache
   constexpr int SIZE = F8 ? 1 : 2, PAGES = 2, TB = 32;
   constexpr int KLOADS = D * SIZE / 64, KSTEPS = D / 32;     // 16-byte pieces of a key that a lane reads; steps of 32 channels
   constexpr int TILES = D / 16;
@@ -171,6 +173,7 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
     }
   };
 
+  bool odd = false;                                          // values that are not finite have been put to zero
   Pages now, next;
   Entries ahead;
   if (first + wave < last) {
@@ -278,6 +281,28 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
         for (int c = 0; c < WIDE; ++c) V[c][i] &= keep;
         if constexpr (NARROW > 0) VN[i] &= keep;
       }
+      if (APART && u.low != u.high) {
+        uint32_t bad = 0;
+        const auto finite = [&](uint32_t x) __attribute__((always_inline)) {
+          const uint32_t y = attend_finite<VT>(x);
+          bad |= x ^ y;
+          return y;
+        };
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (F8)
+#pragma unroll
+            for (int w = 0; w < VWORDS; ++w) VB[i][w] = finite(VB[i][w]);
+#pragma unroll
+          for (int c = 0; c < WIDE; ++c)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) V[c][i][w] = finite(V[c][i][w]);
+          if constexpr (NARROW > 0)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) VN[i][w] = finite(VN[i][w]);
+        }
+        odd |= __any(bad != 0) != 0;
+      }
     }
     if constexpr (F8) {
 #pragma unroll
@@ -323,6 +348,31 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
     }
     if (more) load_values(next);
     now = next;
+  }
+  if (APART && odd) {
+    for (int blk = first + wave; blk < last; blk += 4) {
+      entries(ahead, blk);
+      find(now, ahead);
+      if (now.whole) continue;
+      for (int in = 0; in < TB; ++in) {
+        const int p = in / TQ_PAGE_TOKENS, t = now.t0 + in;
+        if ((in & (TQ_PAGE_TOKENS - 1)) >= (p ? now.valid[1] : now.valid[0])) continue;
+        const char* from = (const char*)a.v + (p ? now.at[1] : now.at[0]) + (uint32_t)(in & (TQ_PAGE_TOKENS - 1)) * step;
+#pragma unroll
+        for (int c = 0; c < TILES; c += 4)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            ex_u32x2 x;
+            if constexpr (F8) x[0] = x[1] = *(const uint32_t*)(from + (quarter * 4 + i) * TILES + c);
+            else x = *(const ex_u32x2*)(from + ex_channel<WIDE>(c, quarter, i) * 2);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              if ((t <= at_p[n]) & ((t > behind[n]) | (t < a.sinks)))
+#pragma unroll
+                for (int k = 0; k < 4; ++k) O[n][c + k][i] += attend_not_finite<VT>(x, k);
+          }
+      }
+    }
   }
 
   // ---- the four wavefronts: to a common maximum, then summed pairwise (2, 3 -> 0, 1 -> 0) ----
@@ -378,8 +428,13 @@ template <int QT, bool F8>
 int launch_attend_few(const Attend& a, int tiles, unsigned grid, hipStream_t stream) {
 #define TQ_ATTEND_D(D)                                                                                 \
   case D:                                                                                              \
-    if (tiles == 1) attend_few_kernel<QT, F8, D, 1><<<dim3(grid), dim3(256), 0, stream>>>(a);          \
-    else attend_few_kernel<QT, F8, D, 2><<<dim3(grid), dim3(256), 0, stream>>>(a);                     \
+    if (a.s.starts) {                                                                                  \
+      if (tiles == 1) attend_few_kernel<QT, F8, D, 1, true><<<dim3(grid), dim3(256), 0, stream>>>(a);  \
+      else attend_few_kernel<QT, F8, D, 2, true><<<dim3(grid), dim3(256), 0, stream>>>(a);             \
+    } else {                                                                                           \
+      if (tiles == 1) attend_few_kernel<QT, F8, D, 1, false><<<dim3(grid), dim3(256), 0, stream>>>(a); \
+      else attend_few_kernel<QT, F8, D, 2, false><<<dim3(grid), dim3(256), 0, stream>>>(a);            \
+    }                                                                                                  \
     break
   switch (a.d) {
     TQ_ATTEND_D(64); TQ_ATTEND_D(128); TQ_ATTEND_D(192); TQ_ATTEND_D(256);

@@ -42,6 +42,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
   constexpr int PT = F8 ? TQ_BF16 : QT;                      // of the value product
   constexpr bool HALVES = F8 && QT == TQ_F16;                // weights in two halves
   constexpr bool FOLD = F8 && QT == TQ_BF16;                 // a key's scale goes into the key
+  constexpr int VT = F8 ? TQ_E4M3 : QT;                      // of the cache
   constexpr int SIZE = F8 ? 1 : 2, ROW = D * 2;              // bytes of an element in the cache, of a row in LDS
   constexpr int LANES = D * SIZE / 16, LOADS = ROWS_TOKENS * LANES / 256;
   constexpr int KSTEPS = D / 16, TILES = D / 32, M = 128;
@@ -157,7 +158,33 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
   const auto scale_of = [](uint32_t byte) __attribute__((always_inline)) { return byte == 0 ? 0x1p-127f : __uint_as_float(byte << 23); };
   const int t_here = tid / LANES, c_here = tid % LANES * PER;
   const uint32_t key_to = (uint32_t)(t_here * ROW + (c_here ^ rows_key_turn<D>(t_here)) * 16), value_to = (uint32_t)(t_here * ROW + (c_here ^ rows_value_turn<D>(t_here)) * 16);
+  // all rows of the unit see all of a turn's tokens
+  const int behind_low = attend_behind(a, u.low), behind_high = attend_behind(a, u.high);
+  const auto seen_whole = [&](const Turn& x) __attribute__((always_inline)) {
+    return x.t0 + ROWS_TOKENS - 1 <= u.low && (x.t0 > behind_high || x.t0 + ROWS_TOKENS <= a.sinks) && complete(x);
+  };
+  bool odd = false;                                          // this wavefront has put values that are not finite to zero
   const auto store = [&](const Turn& x, char* to) __attribute__((always_inline)) {
+    if (!seen_whole(x)) {
+      // values of tokens that nobody sees are zeros: what lies in their slots may be NaN
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int t = x.t0 + token_of(i);
+        if (!((t < u.tokens) & (entry_of(x, i) < in_cache) & ((t > behind_low) | (t < a.sinks)))) VR[i] = ex_u32x4{0, 0, 0, 0};
+      }
+      if (u.low != u.high) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t y = attend_finite<VT>(VR[i][w]);
+            bad |= y ^ VR[i][w];
+            VR[i][w] = y;
+          }
+        odd |= __any(bad != 0) != 0;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       uint32_t k = (key_to ^ (uint32_t)(rows_key_turn<D>(i * APART) * 16)) + (uint32_t)(i * APART * ROW), v = value_to + (uint32_t)(i * APART * ROW);
@@ -167,8 +194,6 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
         v = (uint32_t)(t * ROW + (c ^ rows_value_turn<D>(t)) * 16);
       }
       char *const kt = to, *const vt = to + HALF;
-      // values of tokens that nobody sees are zeros: what lies in their slots may be NaN
-      if (!complete(x) && !(x.t0 + token_of(i) < u.tokens && entry_of(x, i) < in_cache)) VR[i] = ex_u32x4{0, 0, 0, 0};
       if constexpr (F8) {
         const float kf = FOLD ? scale_of(ks[i]) : 1.0f, vf = scale_of(vs[i]);
         // (eight lanes store together, every second piece of 256 bytes, so that half of the banks have two: to have four of the lanes begin with the other
@@ -309,6 +334,37 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
     __syncthreads();
     now = next;
     next = after;
+  }
+  if (u.low != u.high) {                                     // (all that remains of the buffers: whether any wavefront has)
+    if (tid == 0) *(uint32_t*)s_rows = 0;
+    __syncthreads();
+    if (odd) *(uint32_t*)s_rows = 1;
+    __syncthreads();
+    if (*(const uint32_t*)s_rows) {
+      for (int i = first; i < last; ++i) {
+        entries(now, i);
+        if (seen_whole(now)) continue;
+        for (int in = 0; in < ROWS_TOKENS && now.t0 + in < u.tokens; ++in) {
+          const int t = now.t0 + in;
+          const uint32_t page = (uint32_t)step_entry(table, t / TQ_PAGE_TOKENS);
+          if (page >= in_cache) continue;
+          const char* from = (const char*)a.v + page * block_bytes + head_bytes + (uint32_t)(in % TQ_PAGE_TOKENS) * step;
+          const bool sees = (t <= at_p) & ((t > behind) | (t < a.sinks));
+#pragma unroll
+          for (int c = 0; c < TILES; ++c)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const int at = (c * 32 + (e >> 2) * 8 + half * 4) * SIZE;
+              ex_u32x2 x;
+              if constexpr (F8) x[0] = x[1] = *(const uint32_t*)(from + at);
+              else x = *(const ex_u32x2*)(from + at);
+              if (sees)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) O[c][e + k] += attend_not_finite<VT>(x, k);
+            }
+        }
+      }
+    }
   }
 
   const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
