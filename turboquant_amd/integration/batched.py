@@ -29,7 +29,8 @@ prefill steps).  Modes are those of `integration.vllm`:
                 when the engine's cache was never allocated (`no_alloc`)
 
 The first `exact_layers` layers may stay uncompressed: their decode steps are answered from the engine's paged cache, all of it exactly
-(`ExactPagedCache`).  And a cache may be cut: `track_weights` has every layer sum the attention weight that its tokens get - from the newest
+(`ExactPagedCache`).  The next `fp8_layers` may keep 8 bits instead of two to four (`Fp8PagedCache`): their decode steps are answered from
+those in both modes, and with `no_alloc` their prompts, too, later chunks included.  Both honour the sliding window that a layer's backend names.  And a cache may be cut: `track_weights` has every layer sum the attention weight that its tokens get - from the newest
 `window` queries of a prompt's chunk in every step, and in exact layers from every decoded token, whoever else is in the step -, and `evict_batched` keeps the sinks, the newest and the heaviest
 of a sequence's tokens, in the engine's blocks and in the pages alike.  The engine goes on with the lengths that it returns.
 A hybrid step's exact part are a sequence's last `ring_capacity` slots.  Tokens that stay fill the holes of those that go, so that right behind a cut
@@ -41,14 +42,16 @@ from __future__ import annotations
 import logging
 import math
 from dataclasses import dataclass
-from typing import Dict, Optional
+from typing import Dict, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
 
 from .. import _ffi
+from ..attend import HEAD_DIMS, seen_by
 from ..eviction import begin_rows, check_table, select_evictions
 from ..exact import MAX_HEAD_DIM, ExactPagedCache
+from ..fp8 import Fp8PagedCache
 from ..paged import APPEND, PAGE_TOKENS, PagedKVPool
 from ..quantizer import TurboQuantProd
 from . import vllm as _single
@@ -64,9 +67,25 @@ def _host_list(meta, name):
     return [int(x) for x in t.tolist()]
 
 
+def _window_of(name: str, impl) -> Tuple[Optional[int], int]:
+    """(window, sinks) of a layer, as its backend names them: `sliding_window`, tokens that a query sees with its own among them, or flash attention's pair of
+    those on its left and right (-1: all), and `sink_tokens`, first tokens that stay visible."""
+    window = getattr(impl, "sliding_window", None)
+    if isinstance(window, (tuple, list)):
+        left, right = (int(x) for x in window)
+        if right > 0:
+            raise ValueError(f"{name} sees {right} tokens behind its own: not a causal layer")
+        window = left + 1 if left >= 0 else None
+    if window is None or int(window) <= 0:
+        return None, 0
+    window, sinks = int(window), int(getattr(impl, "sink_tokens", 0))
+    seen_by(window, sinks)
+    return window, sinks
+
+
 @dataclass
 class BatchedLayerState:
-    """One attention layer: its quantiser and the compressed pool that shadows the engine's blocks (None: the layer stays exact)."""
+    """One attention layer: its quantiser and the compressed pool that shadows the engine's blocks, or 8-bit blocks that do (neither: the layer stays exact)."""
     config: LayerConfig
     quantizer: Optional[TurboQuantProd]
     pool: Optional[PagedKVPool]
@@ -76,11 +95,13 @@ class BatchedLayerState:
     positions: Optional[torch.Tensor] = None                   # (B, H_kv, tokens): where in the sequence it stood
     window: int = 0
     blocks_current: bool = True                                # the engine's blocks hold a step's tokens before its attention: do_kv_cache_update
+    fp8: Optional[Fp8PagedCache] = None
+    sees: Tuple[Optional[int], int] = (None, 0)                # sliding window and sinks of an exact or 8-bit layer
 
     @property
     def supports_hybrid(self) -> bool:
         """Whether the engine's cache may be freed (an exact layer has nothing else)."""
-        return self.pool is not None
+        return self.pool is not None or self.fp8 is not None
 
     # ---- write -------------------------------------------------------------------
     def write(self, key: torch.Tensor, value: torch.Tensor, meta) -> None:
@@ -88,13 +109,15 @@ class BatchedLayerState:
         cfg = self.config
         n = int(meta.num_actual_tokens)
         self.check_step(meta)
-        if self.pool is None:                                  # the engine's own cache has them
+        if self.pool is None and self.fp8 is None:             # the engine's own cache has them
             self.tokens_written += n
             return
         k = key[:n].reshape(n, cfg.num_kv_heads, cfg.head_dim)
         v = value[:n].reshape(n, cfg.num_kv_heads, cfg.head_dim)
         table = meta.block_table
-        if int(meta.max_query_len) == 1:                       # one token per sequence: a single batched append
+        if self.fp8 is not None:
+            self.fp8.write(k, v, meta.query_start_loc, table, meta.seq_lens)
+        elif int(meta.max_query_len) == 1:                       # one token per sequence: a single batched append
             k, v, lens = k[:, None], v[:, None], meta.seq_lens
             if not (_ffi.as_defined(self.pool, APPEND) and self.pool._append_newest(k, v, table, lens)):
                 self.pool.append(k, v, table, start_pos=lens.to(torch.int32) - 1)
@@ -111,11 +134,25 @@ class BatchedLayerState:
         sequences of `block_table`: tokens [0, seq_lens[b]) of every sequence, read in place through the
         block table and written to the pages of the same numbers (the batch counterpart of
         capture.py:187-217, without the gather copy)."""
-        if self.pool is None:
+        if not self.supports_hybrid:
             raise RuntimeError("an exact layer has no pages to write to")
+        if self.fp8 is not None:
+            self._ingest_fp8(kv_cache, block_table, [int(n) for n in seq_lens.tolist()])
+            return
         self.pool.append_from_blocks(kv_cache[0], kv_cache[1], block_table, block_table, seq_lens,
                                      max_tokens=max_tokens)
         self.tokens_written += int(seq_lens.sum())
+
+    def _ingest_fp8(self, kv_cache, block_table, lens) -> None:
+        """Sequence by sequence, 4096 tokens at a time (whole blocks: none is rounded twice), gathered from their blocks."""
+        for b, length in enumerate(lens):
+            for first in range(0, length, 4096):
+                n = min(4096, length - first)
+                t = torch.arange(first, first + n, device=block_table.device)
+                block, slot = block_table[b].long()[t // PAGE_TOKENS], t % PAGE_TOKENS
+                step = torch.tensor([0, n, first + n], dtype=torch.int32).to(block_table.device)
+                self.fp8.write(kv_cache[0][block, slot], kv_cache[1][block, slot], step[:2], block_table[b: b + 1], step[2:])
+                self.tokens_written += n
 
     # ---- read --------------------------------------------------------------------
     def _exact_tail(self, kv_cache, meta):
@@ -143,8 +180,15 @@ class BatchedLayerState:
         """One query token per sequence, (B, H_q, d) -> (B, H_q, d)."""
         self.decode_steps += 1
         cfg = self.config
+        window, sinks = self.sees
+        if self.fp8 is not None:
+            return self.fp8.decode_attention(query, meta.block_table, meta.seq_lens, scale=scale, window=window, sinks=sinks,
+                                             max_len=getattr(meta, "max_seq_len", None))
         if self.pool is None:
             longest, weights = getattr(meta, "max_seq_len", None), self.weights
+            if window is not None:
+                return ExactPagedCache.from_engine(kv_cache).decode_attention(query, meta.block_table, meta.seq_lens, scale=scale, window=window, sinks=sinks,
+                                                                              max_len=longest)
             if weights is not None:                            # (the step keeps a score for every place; check_step has seen that there are no longer sequences)
                 weights = weights[: query.shape[0], :, : max(1, longest) if longest is not None else None]
             return ExactPagedCache.from_engine(kv_cache).decode_attention(query, meta.block_table, meta.seq_lens, scale=scale, weights=weights, max_len=longest)
@@ -163,6 +207,12 @@ class BatchedLayerState:
         rk, rv, rlen, hist = recent
         return self.pool.decode_attention(query, meta.block_table, hist, scale=scale, recent_k=rk, recent_v=rv,
                                           recent_len=rlen, max_len=getattr(meta, "max_seq_len", None))
+
+    def attend_rows(self, query: torch.Tensor, meta, scale: Optional[float] = None) -> torch.Tensor:
+        """The rows of a step, (n, H_q, d) -> (n, H_q, d), from the 8-bit blocks alone: prompts, chunks of them, single tokens beside them."""
+        window, sinks = self.sees
+        return self.fp8.attention(query, meta.query_start_loc, meta.block_table, meta.seq_lens, scale=scale, window=window, sinks=sinks,
+                                  max_len=getattr(meta, "max_seq_len", None), max_rows=int(meta.max_query_len))
 
     # ---- eviction ------------------------------------------------------------------
     def track(self, batch: int, max_len: int, window: int) -> None:
@@ -254,6 +304,8 @@ class BatchedLayerState:
         return e.lens
 
     def memory_bytes(self) -> int:
+        if self.fp8 is not None:
+            return self.fp8.memory_bytes()
         return 0 if self.pool is None else self.pool.data.numel()
 
 
@@ -281,6 +333,8 @@ class _BatchedLayerHooks:
         sequence only: there is no exact cache to read earlier tokens from)."""
         cfg = self.state.config
         q = query[:n].reshape(n, cfg.num_query_heads, cfg.head_dim)
+        if self.state.fp8 is not None:                         # (its blocks have the earlier tokens, and this step's are written)
+            return self.state.attend_rows(q, meta, getattr(impl, "scale", None))
         k = key[:n].reshape(n, cfg.num_kv_heads, cfg.head_dim)
         v = value[:n].reshape(n, cfg.num_kv_heads, cfg.head_dim)
         rep = cfg.num_query_heads // cfg.num_kv_heads
@@ -331,14 +385,22 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
                           value_group_size: int = 32, ring_capacity: int = 128, initial_layers_count: int = 4,
                           initial_layers_key_bits: Optional[int] = None, mode: str = MODE_CAPTURE_ONLY,
                           no_alloc: bool = False, dtype: torch.dtype = torch.bfloat16,
-                          exact_layers: int = 0) -> Dict[str, BatchedLayerState]:
+                          exact_layers: int = 0, fp8_layers: int = 0) -> Dict[str, BatchedLayerState]:
     """Hook every standard attention layer of `model_runner` with a compressed pool of `num_blocks`
     16-token pages (the engine's block count); returns {layer name: BatchedLayerState}.  Bit widths are
     assigned as by `install_hooks` (integration/vllm.py:333-359).  The first `exact_layers` of them get no pool: their
-    decode steps are answered from the engine's cache.  Latent-attention layers are left alone.  A layer can stay exact
-    only if its backend has do_kv_cache_update and its head size is a multiple of 64 up to 768."""
+    decode steps are answered from the engine's cache.  The next `fp8_layers` keep e4m3 blocks of the engine's numbers instead of pages, and have head sizes of
+    64, 128, 192 or 256.  Latent-attention layers are left alone.  A layer can stay exact
+    only if its backend has do_kv_cache_update and its head size is a multiple of 64 up to 768.
+
+    A backend's `sliding_window` (and `sink_tokens`) hold for exact and 8-bit layers (at those four head sizes); pages of two to four bits
+    are attended to as a whole."""
+    if exact_layers < 0 or fp8_layers < 0:
+        raise ValueError(f"exact_layers and fp8_layers must not be negative, got {exact_layers} and {fp8_layers}")
     if exact_layers and no_alloc:
         raise ValueError("exact layers are answered from the engine's cache, which no_alloc leaves out")
+    if fp8_layers and torch.device(model_runner.device).type != "cuda":
+        raise ValueError(f"8-bit layers need a GPU, the model runs on {model_runner.device}")
     layers = []
     for name, module in model_runner.compilation_config.static_forward_context.items():
         impl = getattr(module, "impl", None)
@@ -351,26 +413,33 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
                              "not reach, would write the engine's cache")
         if len(layers) < exact_layers and (int(impl.head_size) % 64 or not 0 < int(impl.head_size) <= MAX_HEAD_DIM):
             raise ValueError(f"{name} cannot stay exact: its head_dim {int(impl.head_size)} is no multiple of 64 up to {MAX_HEAD_DIM}")
-        layers.append((name, module, impl))
+        idx, sees = len(layers), (None, 0)
+        if idx < exact_layers + fp8_layers:
+            sees = _window_of(name, impl)
+            if int(impl.head_size) not in HEAD_DIMS and (idx >= exact_layers or sees[0] is not None):
+                raise ValueError(f"{name}: 8-bit layers and sliding windows take head sizes of {', '.join(map(str, HEAD_DIMS))}, got {int(impl.head_size)}")
+        layers.append((name, module, impl, sees))
     _single.set_mode(mode)
     if initial_layers_key_bits is None:
         initial_layers_key_bits = min(key_bits + 1, 4)
     states: Dict[str, BatchedLayerState] = {}
     device = torch.device(model_runner.device)
-    for idx, (name, module, impl) in enumerate(layers):
+    for idx, (name, module, impl, sees) in enumerate(layers):
         head_dim = int(impl.head_size)
         cfg = LayerConfig(head_dim=head_dim, num_kv_heads=int(impl.num_kv_heads),
                           num_query_heads=_query_heads_of(module, impl),
                           key_bits=initial_layers_key_bits if idx < initial_layers_count else key_bits,
                           value_bits=value_bits, value_group_size=min(value_group_size, head_dim),
                           ring_capacity=ring_capacity, layer_idx=idx, backend_kind="flash", device=device)
-        tq = pool = None
-        if idx >= exact_layers:
+        tq = pool = fp8 = None
+        if exact_layers <= idx < exact_layers + fp8_layers:
+            fp8 = Fp8PagedCache.allocate(num_blocks, cfg.num_kv_heads, head_dim, device)
+        elif idx >= exact_layers:
             tq = TurboQuantProd(head_dim, bits=cfg.key_bits, device=device, seed=42 + 7 * idx)
             pool = PagedKVPool(tq, cfg.num_kv_heads, num_blocks, value_bits=value_bits,
                                value_group_size=cfg.value_group_size, dtype=dtype, device=device)
         has_update = hasattr(impl, "do_kv_cache_update")
-        state = BatchedLayerState(config=cfg, quantizer=tq, pool=pool, blocks_current=has_update)
+        state = BatchedLayerState(config=cfg, quantizer=tq, pool=pool, blocks_current=has_update, fp8=fp8, sees=sees)
         states[name] = state
         hooks = _BatchedLayerHooks(state, _unbound(impl.forward),
                                    _unbound(impl.do_kv_cache_update) if has_update else None, no_alloc)
@@ -398,6 +467,10 @@ def track_weights(model_runner, batch: int, max_len: int, window: int = 32) -> N
     if not 1 <= window <= 1024:
         raise ValueError(f"window must be 1 .. 1024, got {window}")
     for name, state in model_runner._tq_layer_states.items():
+        if state.fp8 is not None:
+            raise ValueError(f"8-bit layers cannot be cut: the tokens of {name} would not move with the others")
+        if state.sees[0] is not None:
+            raise ValueError(f"layers with a sliding window cannot be cut: {name} tells by a token's slot how far behind it is")
         if not state.blocks_current:
             raise ValueError(f"weights are summed over the engine's cache before a step's attention: {name}, whose backend has no do_kv_cache_update, "
                              "writes it too late")

@@ -20,6 +20,8 @@ from typing import List, Optional, Sequence
 import torch
 import torch.nn.functional as F
 
+from ..rotary import inverse_frequencies, rotate_heads
+
 BLOCK = 16            # tokens per KV block of the runner = tokens per compressed page
 
 
@@ -41,8 +43,9 @@ class DenseBackend:
     """Exact attention over a paged cache (2, num_blocks, BLOCK, H_kv, d): the stand-in for the engine's
     own backend.  Sequence by sequence, causal inside the step's rows."""
 
-    def __init__(self, num_heads: int, num_kv_heads: int, head_size: int):
+    def __init__(self, num_heads: int, num_kv_heads: int, head_size: int, sliding_window: Optional[int] = None, sink_tokens: int = 0):
         self.num_heads, self.num_kv_heads, self.head_size = num_heads, num_kv_heads, head_size
+        self.sliding_window, self.sink_tokens = sliding_window, sink_tokens
         self.scale = 1.0 / math.sqrt(head_size)
 
     def do_kv_cache_update(self, layer, key, value, kv_cache, slot_mapping):
@@ -70,7 +73,10 @@ class DenseBackend:
             v = fv[slot].float().repeat_interleave(rep, 1)
             s = torch.einsum("thd,nhd->htn", q[r0:r1].float(), k) * self.scale
             t = r1 - r0
-            mask = pos[None, :] > (L - t + torch.arange(t, device=q.device))[:, None]
+            at = (L - t + torch.arange(t, device=q.device))[:, None]
+            mask = pos[None, :] > at
+            if self.sliding_window is not None:
+                mask = mask | ((pos[None, :] <= at - self.sliding_window) & (pos[None, :] >= self.sink_tokens))
             s = s.masked_fill(mask[None], float("-inf"))
             out[r0:r1] = torch.einsum("htn,nhd->thd", s.softmax(-1), v).to(q.dtype)
         res = out if query.dim() == 3 else out.reshape(n, -1)
@@ -107,11 +113,13 @@ class MinimalRunner:
 
     `num_blocks` blocks of 16 tokens are shared by all sequences; sequence b owns the blocks
     block_table[b].  With `exact_cache=False` no exact KV cache is allocated (the compressed pool is
-    then the only KV storage and the hooks must run in `full_tq` mode with `no_alloc=True`)."""
+    then the only KV storage and the hooks must run in `full_tq` mode with `no_alloc=True`).
+    qk_norm: heads of queries and keys are normed before they are rotated, both by `rotate_heads` (needs a GPU).
+    sliding_window, sink_tokens: what every layer's backend names (`DenseBackend`)."""
 
     def __init__(self, n_layers: int, hidden: int, num_heads: int, num_kv_heads: int, head_dim: int, ffn: int,
                  vocab: int, batch: int, max_seq_len: int, device, exact_cache: bool = True, seed: int = 0,
-                 dtype: torch.dtype = torch.bfloat16):
+                 dtype: torch.dtype = torch.bfloat16, qk_norm: bool = False, sliding_window: Optional[int] = None, sink_tokens: int = 0):
         self.device = torch.device(device)
         self.n_layers, self.hidden, self.hq, self.hkv, self.d, self.vocab = n_layers, hidden, num_heads, num_kv_heads, head_dim, vocab
         self.batch, self.dtype = batch, dtype
@@ -126,7 +134,7 @@ class MinimalRunner:
         ctx = {}
         self.kv_caches: List[torch.Tensor] = []
         for i in range(n_layers):
-            impl = DenseBackend(num_heads, num_kv_heads, head_dim)
+            impl = DenseBackend(num_heads, num_kv_heads, head_dim, sliding_window, sink_tokens)
             cache = (torch.zeros(2, self.num_blocks, BLOCK, num_kv_heads, head_dim, dtype=dtype, device=self.device)
                      if exact_cache else None)
             mod = AttentionModule(impl, cache)
@@ -138,6 +146,11 @@ class MinimalRunner:
                 ln2=torch.ones(hidden, dtype=dtype, device=self.device),
                 wqkv=w(hidden, (num_heads + 2 * num_kv_heads) * head_dim), wo=w(num_heads * head_dim, hidden),
                 w_gate_up=w(hidden, 2 * ffn), w_down=w(ffn, hidden)))
+        self.inv_freq = None
+        if qk_norm:
+            self.inv_freq = inverse_frequencies(head_dim, device=self.device)
+            for lay in self.layers:
+                lay.q_norm, lay.k_norm = (1 + w(head_dim) for _ in range(2))
         self.compilation_config = types.SimpleNamespace(static_forward_context=ctx)
         # sequence b owns a shuffled set of blocks, as a block allocator would hand them out
         perm = torch.randperm(self.num_blocks, generator=torch.Generator().manual_seed(seed + 1))
@@ -186,8 +199,12 @@ class MinimalRunner:
             h = _rms(x, lay.ln1)
             qkv = h @ lay.wqkv
             q, k, v = qkv.split([hq * d, hkv * d, hkv * d], dim=-1)
-            q = _rope(q.view(T, hq, d), positions).reshape(T, hq * d)
-            k = _rope(k.view(T, hkv, d), positions)
+            q, k = q.view(T, hq, d), k.view(T, hkv, d)
+            if self.inv_freq is None:
+                q, k = _rope(q, positions), _rope(k, positions)
+            else:
+                q, k = rotate_heads(q, k, positions, self.inv_freq, lay.q_norm, lay.k_norm)
+            q = q.reshape(T, hq * d)
             v = v.view(T, hkv, d).contiguous()
             impl, cache = lay.attn.impl, lay.attn.kv_cache[0]
             if hasattr(impl, "do_kv_cache_update"):
