@@ -46,6 +46,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
   constexpr int SIZE = F8 ? 1 : 2, ROW = D * 2;              // bytes of an element in the cache, of a row in LDS
   constexpr int LANES = D * SIZE / 16, LOADS = ROWS_TOKENS * LANES / 256;
   constexpr int KSTEPS = D / 16, TILES = D / 32, M = 128;
+  constexpr int KAHEAD = 6;                                  // reads of keys that are on their way at a time
   constexpr int HALF = ROWS_TOKENS * ROW;                    // keys or values of a turn
   extern __shared__ __attribute__((aligned(16))) char s_rows[];
 
@@ -250,13 +251,21 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
       const bool whole = t1 <= w_low && (t0 > w_behind_high || t1 < a.sinks) && complete(now);
       ro_f32x16 S[2];
 #pragma unroll
-      for (int T = 0; T < 2; ++T) {
+      for (int T = 0; T < 2; ++T)
 #pragma unroll
         for (int e = 0; e < 16; ++e) S[T][e] = 0.0f;
 #pragma unroll
-        for (int s = 0; s < KSTEPS; ++s)
+      for (int s = 0; s < KSTEPS; ++s)
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
           S[T] = rows_mfma<QT>(*(const ex_u32x4*)(buffer + kp[s % KPLACES] + (s / KPLACES) * KPLACES * 32 + T * 32 * ROW), Q[s], S[T]);
+      __builtin_amdgcn_sched_group_barrier(0x100, KAHEAD, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * KSTEPS - KAHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
+      __builtin_amdgcn_sched_group_barrier(0x008, KAHEAD, 0);
       if constexpr (F8 && !FOLD) {
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
@@ -291,33 +300,25 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
         m = top;
       }
       const float ref = m == -INFINITY ? 0.0f : m - ex_lift<PT>();
-      float sum = 0.0f;
+      // Sixteen tokens at a time: the weights and values of the next while the matrix instructions of these run.
+      ex_u32x4 P[2], L[2], V[2][TILES];
+      const auto weights = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
-      for (int T = 0; T < 2; ++T)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(S[T][e], f, -ref));
-          S[T][e] = p;
-          sum += p;
-        }
-      l += sum;
-      ex_u32x4 P[4], L[HALVES ? 4 : 1];
-#pragma unroll
-      for (int T = 0; T < 2; ++T)
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const int at = T * 2 + (e >> 3), w = (e & 7) >> 1;
+        for (int i = 0; i < 8; i += 2) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(S[at >> 1][(at & 1) * 8 + i], f, -ref)), y = __builtin_amdgcn_exp2f(fmaf(S[at >> 1][(at & 1) * 8 + i + 1], f, -ref));
+          l += x;
+          l += y;
           if constexpr (HALVES) {
             uint32_t hi, lo;
-            ex_split<PT>(S[T][e], S[T][e + 1], &hi, &lo);
-            P[at][w] = hi;
-            L[at][w] = lo;
+            ex_split<PT>(x, y, &hi, &lo);
+            P[at & 1][i >> 1] = hi;
+            L[at & 1][i >> 1] = lo;
           } else {
-            P[at][w] = ex_pack<PT>(S[T][e], S[T][e + 1]);
+            P[at & 1][i >> 1] = ex_pack<PT>(x, y);
           }
         }
-#pragma unroll
-      for (int at = 0; at < 4; ++at)
+      };
+      const auto values = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
         for (int ct = 0; ct < TILES; ++ct) {
           char* from = buffer + vp[ct % VPLACES] + (ct / VPLACES) * VPLACES * 64 + at * 16 * ROW;
@@ -325,10 +326,33 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
           const ro_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)from);
           const ro_s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(from + 8 * ROW));
           const ex_u32x2 lo = __builtin_bit_cast(ex_u32x2, x), hi = __builtin_bit_cast(ex_u32x2, y);
-          const ex_u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
-          if constexpr (HALVES) O[ct] = rows_mfma<PT>(v, L[at], O[ct]);
-          O[ct] = rows_mfma<PT>(v, P[at], O[ct]);
+          V[at & 1][ct] = ex_u32x4{lo[0], lo[1], hi[0], hi[1]};
         }
+      };
+      values(0);
+      weights(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int at = 0; at < 4; ++at) {
+        if (at < 3) {
+          values(at + 1);
+          weights(at + 1);
+        }
+#pragma unroll
+        for (int ct = 0; ct < TILES; ++ct) {
+          if constexpr (HALVES) O[ct] = rows_mfma<PT>(V[at & 1][ct], L[at & 1], O[ct]);
+          O[ct] = rows_mfma<PT>(V[at & 1][ct], P[at & 1], O[ct]);
+        }
+        if (at < 3) {
+#pragma unroll
+          for (int ct = 0; ct < TILES; ++ct) {
+            __builtin_amdgcn_sched_group_barrier(0x008, HALVES ? 2 : 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x402, (28 + TILES - 1) / TILES, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     if (more) store(next, other);
     __syncthreads();
