@@ -16,6 +16,8 @@
 #include "tq_attend.h"
 #include "tq_attend_few_impl.h"
 
+#include <type_traits>
+
 namespace tq {
 
 typedef float ro_f32x16 __attribute__((ext_vector_type(16)));
@@ -81,14 +83,14 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
 
   // (a negative scale turns the queries and one of zero clears them, so that the scores' order is that of their products)
   const float f = a.scale2 == 0.0f ? 1.0f : fabsf(a.scale2);
-  const uint32_t turn = a.scale2 < 0.0f ? 0x80008000u : 0u, keep = a.scale2 == 0.0f ? 0u : 0xffffffffu;
+  const uint32_t sign = a.scale2 < 0.0f ? 0x80008000u : 0u, keep = a.scale2 == 0.0f ? 0u : 0xffffffffu;
   ex_u32x4 Q[KSTEPS];
 #pragma unroll
   for (int s = 0; s < KSTEPS; ++s) {
     Q[s] = ex_u32x4{0, 0, 0, 0};
     if (live) Q[s] = *(const ex_u32x4*)((const uint16_t*)a.q + row * D + s * 16 + half * 8);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) Q[s][i] = (Q[s][i] & keep) ^ turn;
+    for (int i = 0; i < 4; ++i) Q[s][i] = (Q[s][i] & keep) ^ sign;
   }
   ro_f32x16 O[TILES];
 #pragma unroll
@@ -106,10 +108,14 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
   const auto entries = [&](Turn& x, int i) __attribute__((always_inline)) {
     const int at = i < last ? i : last - 1, blk = list[at < 0 ? 0 : at];      // (a unit without tokens: block 0, of which nothing is used)
     x.t0 = blk * ROWS_TOKENS;
+    if (blk * 4 + 3 <= last_page) {
+      x.entry = step_entries(table, blk * 4);
+    } else {
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const int page = blk * 4 + p;
-      x.entry[p] = (uint32_t)step_entry(table, page < last_page ? page : last_page);
+      for (int p = 0; p < 4; ++p) {
+        const int page = blk * 4 + p;
+        x.entry[p] = (uint32_t)step_entry(table, page < last_page ? page : last_page);
+      }
     }
   };
   // (scalar instructions are a wavefront's time as well: 64-bit products for each load were a fifth of it)
@@ -121,8 +127,10 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
     const uint32_t p = x.entry[0] > x.entry[1] ? x.entry[0] : x.entry[1], q = x.entry[2] > x.entry[3] ? x.entry[2] : x.entry[3];
     return x.t0 + ROWS_TOKENS <= u.tokens && (p > q ? p : q) < in_cache;
   };
-  // The i-th load of a lane: 16 bytes, piece piece_of of token token_of of the turn.  Rows of a power of two of pieces: the page is a wavefront's, and the
-  // lane's place in it always the same, but for 512 bytes of them, where it changes with odd i.  192 channels: lanes work their places out load by load.
+  // The i-th load of a lane: 16 bytes of token token_of of the turn.  16 bits: they go to LDS directly, a wavefront's 1 KB to 1 KB of it, and a lane reads
+  // the piece that belongs where its bytes land; a wavefront's tokens are one page's.  Lanes' places in a page repeat with every load, with 512 bytes a row every
+  // two and with 192 channels every three.
+  // 8 bits go through registers: rows of a power of two of pieces have one place in all pages, with 192 channels lanes work it out load by load.
   constexpr bool EVEN = D != 192;
   constexpr int APART = 256 / LANES, PER = F8 ? 2 : 1;       // tokens from a load to the next; pieces of 8 channels in one
   const auto token_of = [&](int i) __attribute__((always_inline)) { return EVEN ? tid / LANES + i * APART : (i * 256 + tid) / LANES; };
@@ -134,29 +142,52 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
       else if constexpr (OWN < 16) return wave < 2 ? x.entry[i * APART / 16] : x.entry[i * APART / 16 + 1];
       else return wave < 2 ? (wave < 1 ? x.entry[0] : x.entry[1]) : (wave < 3 ? x.entry[2] : x.entry[3]);
     } else {
-      const int p = token_of(i) >> 4;
+      const int p = F8 ? token_of(i) >> 4 : (i * 4 + wave) / 6;
       return p < 2 ? (p < 1 ? x.entry[0] : x.entry[1]) : (p < 3 ? x.entry[2] : x.entry[3]);
     }
   };
-  ex_u32x4 KR[LOADS], VR[LOADS];
-  uint32_t ks[F8 ? LOADS : 1], vs[F8 ? LOADS : 1];
+  const auto scale_of = [](uint32_t byte) __attribute__((always_inline)) { return byte == 0 ? 0x1p-127f : __uint_as_float(byte << 23); };
+  // 16 bits
+  constexpr int PLACES = D == 192 ? 3 : (D == 256 ? 2 : 1);
+  uint32_t key_at[PLACES], value_at[PLACES];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)s_rows;
+  // 8 bits
+  constexpr int HELD = F8 ? LOADS : 1;
+  ex_u32x4 KR[HELD], VR[HELD];
+  uint32_t ks[HELD], vs[HELD];
+  uint32_t next_g[4];                                        // fp16 queries: the scales of the next turn's keys, and of these
+  float g[4];
   const uint32_t here = EVEN ? (uint32_t)(tid / LANES % 16) * step + (uint32_t)(tid % LANES) * 16 : 0;
-  const auto load = [&](const Turn& x) __attribute__((always_inline)) {
+  if constexpr (!F8) {
+#pragma unroll
+    for (int i = 0; i < PLACES; ++i) {
+      const int t = (i * 256 + tid) / LANES, piece = (i * 256 + tid) % LANES;
+      key_at[i] = (uint32_t)(t & 15) * step + (uint32_t)(piece ^ rows_key_turn<D>(t)) * 16;
+      value_at[i] = (uint32_t)(t & 15) * step + (uint32_t)(piece ^ rows_value_turn<D>(t)) * 16;
+    }
+  }
+  const auto load = [&](const Turn& x, uint32_t to) __attribute__((always_inline)) {
+    if constexpr (F8 && !FOLD)
+#pragma unroll
+      for (int p = 0; p < 4; ++p) next_g[p] = a.k_scales[(uint64_t)(x.entry[p] < in_cache ? x.entry[p] : 0u) * a.H + h];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const uint32_t e = entry_of(x, i), page = e < in_cache ? e : 0u;      // (a block that is there; its tokens are masked)
       const uint64_t block = page * block_bytes + head_bytes;
-      uint32_t at = here + (APART < 16 ? (uint32_t)(i * APART % 16) * step : 0u);
-      if constexpr (!EVEN) at = (uint32_t)(token_of(i) & 15) * step + (uint32_t)piece_of(i) * 16;
-      KR[i] = *(const ex_u32x4*)((const char*)a.k + block + at);
-      VR[i] = *(const ex_u32x4*)((const char*)a.v + block + at);
       if constexpr (F8) {
+        uint32_t at = here + (APART < 16 ? (uint32_t)(i * APART % 16) * step : 0u);
+        if constexpr (!EVEN) at = (uint32_t)(token_of(i) & 15) * step + (uint32_t)piece_of(i) * 16;
+        KR[i] = *(const ex_u32x4*)((const char*)a.k + block + at);
+        VR[i] = *(const ex_u32x4*)((const char*)a.v + block + at);
         ks[i] = a.k_scales[(uint64_t)page * a.H + h];
         vs[i] = a.v_scales[(uint64_t)page * a.H + h];
+      } else {
+        const uint32_t m0 = lds0 + to + (uint32_t)(i * 256 + wave * 64) * 16;
+        ex_row_to_lds((const char*)a.k + block, key_at[i % PLACES], m0);
+        ex_row_to_lds((const char*)a.v + block, value_at[i % PLACES], m0 + HALF);
       }
     }
   };
-  const auto scale_of = [](uint32_t byte) __attribute__((always_inline)) { return byte == 0 ? 0x1p-127f : __uint_as_float(byte << 23); };
   const int t_here = tid / LANES, c_here = tid % LANES * PER;
   const uint32_t key_to = (uint32_t)(t_here * ROW + (c_here ^ rows_key_turn<D>(t_here)) * 16), value_to = (uint32_t)(t_here * ROW + (c_here ^ rows_value_turn<D>(t_here)) * 16);
   // all rows of the unit see all of a turn's tokens
@@ -165,37 +196,47 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
     return x.t0 + ROWS_TOKENS - 1 <= u.low && (x.t0 > behind_high || x.t0 + ROWS_TOKENS <= a.sinks) && complete(x);
   };
   bool odd = false;                                          // this wavefront has put values that are not finite to zero
-  const auto store = [&](const Turn& x, char* to) __attribute__((always_inline)) {
-    if (!seen_whole(x)) {
-      // values of tokens that nobody sees are zeros: what lies in their slots may be NaN
+  // where all rows do not: values of tokens that nobody sees are zeros - what lies in their slots may be NaN -, and so are those that are not finite
+  const auto sanitise = [&](const Turn& x, int i, ex_u32x4 v) __attribute__((always_inline)) {
+    const int t = x.t0 + token_of(i);
+    if (!((t < u.tokens) & (entry_of(x, i) < in_cache) & ((t > behind_low) | (t < a.sinks)))) v = ex_u32x4{0, 0, 0, 0};
+    if (u.low != u.high) {
+      ex_u32x4 y;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) y[w] = attend_finite<VT>(v[w]);
+      odd |= __any(((y[0] ^ v[0]) | (y[1] ^ v[1]) | (y[2] ^ v[2]) | (y[3] ^ v[3])) != 0) != 0;
+      v = y;
+    }
+    return v;
+  };
+  const auto store = [&](int i, bool whole, char* to) __attribute__((always_inline)) {
+    if constexpr (!F8) {
+      ex_arrived();
+      if (!whole) {
+        Turn x;
+        entries(x, i);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          ex_u32x4* const v = (ex_u32x4*)(to + HALF + (i * 256 + tid) * 16);
+          *v = sanitise(x, i, *v);
+        }
+      }
+    } else {
+      if (!whole) {
+        Turn x;
+        entries(x, i);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) VR[i] = sanitise(x, i, VR[i]);
+      }
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int t = x.t0 + token_of(i);
-        if (!((t < u.tokens) & (entry_of(x, i) < in_cache) & ((t > behind_low) | (t < a.sinks)))) VR[i] = ex_u32x4{0, 0, 0, 0};
-      }
-      if (u.low != u.high) {
-        uint32_t bad = 0;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t y = attend_finite<VT>(VR[i][w]);
-            bad |= y ^ VR[i][w];
-            VR[i][w] = y;
-          }
-        odd |= __any(bad != 0) != 0;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      uint32_t k = (key_to ^ (uint32_t)(rows_key_turn<D>(i * APART) * 16)) + (uint32_t)(i * APART * ROW), v = value_to + (uint32_t)(i * APART * ROW);
-      if constexpr (!EVEN) {
-        const int t = token_of(i), c = piece_of(i) * PER;
-        k = (uint32_t)(t * ROW + (c ^ rows_key_turn<D>(t)) * 16);
-        v = (uint32_t)(t * ROW + (c ^ rows_value_turn<D>(t)) * 16);
-      }
-      char *const kt = to, *const vt = to + HALF;
-      if constexpr (F8) {
+        uint32_t k = (key_to ^ (uint32_t)(rows_key_turn<D>(i * APART) * 16)) + (uint32_t)(i * APART * ROW), v = value_to + (uint32_t)(i * APART * ROW);
+        if constexpr (!EVEN) {
+          const int t = token_of(i), c = piece_of(i) * PER;
+          k = (uint32_t)(t * ROW + (c ^ rows_key_turn<D>(t)) * 16);
+          v = (uint32_t)(t * ROW + (c ^ rows_value_turn<D>(t)) * 16);
+        }
+        char *const kt = to, *const vt = to + HALF;
         const float kf = FOLD ? scale_of(ks[i]) : 1.0f, vf = scale_of(vs[i]);
         // (eight lanes store together, every second piece of 256 bytes, so that half of the banks have two: to have four of the lanes begin with the other
         // piece leaves no conflict and takes longer, 536 us for 522)
@@ -212,9 +253,6 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
           *(ex_u32x4*)(kt + (k ^ (uint32_t)(j * 16))) = y;
           *(ex_u32x4*)(vt + (v ^ (uint32_t)(j * 16))) = z;
         }
-      } else {
-        *(ex_u32x4*)(kt + k) = KR[i];
-        *(ex_u32x4*)(vt + v) = VR[i];
       }
     }
   };
@@ -229,26 +267,40 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
 #pragma unroll
   for (int t = 0; t < VPLACES; ++t) vp[t] = value_from ^ (uint32_t)(t * 64);
 
-  Turn now, next;
-  entries(now, first);
+  Turn ahead;                                                // table entries of the turn behind the one that is worked on
+  entries(ahead, first);
+  int t0 = ahead.t0;
+  bool whole = seen_whole(ahead);
   if (first < last) {
-    load(now);
-    store(now, s_rows);
+    load(ahead, 0);
+    store(first, whole, s_rows);
+    if constexpr (F8 && !FOLD)
+#pragma unroll
+      for (int p = 0; p < 4; ++p) g[p] = scale_of(next_g[p]);
   }
-  entries(next, first + 1);
+  entries(ahead, first + 1);
   __syncthreads();
-  for (int i = first; i < last; ++i) {
+  const auto turn = [&](int i, auto which) __attribute__((always_inline)) {
+    char* const buffer = s_rows + decltype(which)::value * 2 * HALF;
+    char* const other = s_rows + (decltype(which)::value ^ 1) * 2 * HALF;
     const bool more = i + 1 < last;
-    char* buffer = s_rows + ((i - first) & 1) * 2 * HALF;
-    char* other = s_rows + (((i - first) & 1) ^ 1) * 2 * HALF;
+    // (first of all, since scalar loads and reads of LDS have one counter: the keys would wait for them)
     Turn after;
-    if (more) load(next);
     entries(after, i + 2);
+    if (more) load(ahead, (decltype(which)::value ^ 1) * 2 * HALF);
+    const int next_t0 = ahead.t0;
+    const bool next_whole = seen_whole(ahead);
+    ahead = after;
     // what this wavefront's rows see of the turn: nothing, all of it, or some
-    const int t0 = now.t0, t1 = t0 + ROWS_TOKENS - 1;
+    const int t1 = t0 + ROWS_TOKENS - 1;
     const bool any = busy && t0 <= w_high && (t1 > w_behind_low || t0 < a.sinks);
     if (any) {
-      const bool whole = t1 <= w_low && (t0 > w_behind_high || t1 < a.sinks) && complete(now);
+      bool clear = whole;
+      if (!whole && t1 <= w_low && (t0 > w_behind_high || t1 < a.sinks)) {
+        Turn now;
+        entries(now, i);
+        clear = complete(now);
+      }
       ro_f32x16 S[2];
 #pragma unroll
       for (int T = 0; T < 2; ++T)
@@ -266,16 +318,14 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
       __builtin_amdgcn_sched_group_barrier(0x008, KAHEAD, 0);
-      if constexpr (F8 && !FOLD) {
+      if constexpr (F8 && !FOLD)
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const uint64_t page = now.entry[p] < in_cache ? now.entry[p] : 0u;
-          const float g = scale_of(a.k_scales[page * a.H + h]);
+        for (int p = 0; p < 4; ++p)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) S[p >> 1][(p & 1) * 8 + e] *= g;
-        }
-      }
-      if (!whole) {
+          for (int e = 0; e < 8; ++e) S[p >> 1][(p & 1) * 8 + e] *= g[p];
+      if (!clear) {
+        Turn now;
+        entries(now, i);
 #pragma unroll
         for (int T = 0; T < 2; ++T)
 #pragma unroll
@@ -354,10 +404,17 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (more) store(next, other);
+    if (more) store(i + 1, next_whole, other);
+    if constexpr (F8 && !FOLD)
+#pragma unroll
+      for (int p = 0; p < 4; ++p) g[p] = scale_of(next_g[p]);
     __syncthreads();
-    now = next;
-    next = after;
+    t0 = next_t0;
+    whole = next_whole;
+  };
+  for (int i = first; i < last; i += 2) {
+    turn(i, std::integral_constant<int, 0>());
+    if (i + 1 < last) turn(i + 1, std::integral_constant<int, 1>());
   }
   if (u.low != u.high) {                                     // (all that remains of the buffers: whether any wavefront has)
     if (tid == 0) *(uint32_t*)s_rows = 0;
@@ -366,6 +423,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
     __syncthreads();
     if (*(const uint32_t*)s_rows) {
       for (int i = first; i < last; ++i) {
+        Turn now;
         entries(now, i);
         if (seen_whole(now)) continue;
         for (int in = 0; in < ROWS_TOKENS && now.t0 + in < u.tokens; ++in) {

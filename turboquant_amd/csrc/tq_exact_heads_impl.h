@@ -25,15 +25,6 @@ namespace tq {
 
 constexpr int HEADS_TILES = 4;                      // wavefronts of a workgroup, a tile of sixteen heads each
 
-// lane l's 16 bytes land at m0 + 16 l.  The compiler sees neither the load nor its write to LDS: ex_arrived() waits for it.
-__device__ __forceinline__ void ex_to_lds(const void* from, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(m0) : "memory", "m0");
-}
-__device__ __forceinline__ void ex_row_to_lds(const void* base, uint32_t off, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(m0) : "memory", "m0");
-}
-__device__ __forceinline__ void ex_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 // Where a block's rows lie in LDS, in 16-byte pieces.  Up to 448 channels they follow one another, and a load takes 64 pieces wherever a row ends.  512 and
 // 576 channels: a load takes the first 64 pieces of ONE row, whose address is the wavefront's (a scalar and the lane's constant; with divisions by
 // the length of a row the loads were 250 of a block's 815 vector instructions), and with 576 another takes the last 8 of eight rows.

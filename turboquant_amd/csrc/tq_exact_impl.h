@@ -30,6 +30,15 @@
 
 namespace tq {
 
+// lane l's 16 bytes land at m0 + 16 l.  The compiler sees neither the load nor its write to LDS: ex_arrived() waits for it.
+__device__ __forceinline__ void ex_to_lds(const void* from, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(m0) : "memory", "m0");
+}
+__device__ __forceinline__ void ex_row_to_lds(const void* base, uint32_t off, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(m0) : "memory", "m0");
+}
+__device__ __forceinline__ void ex_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 typedef float ex_f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t ex_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t ex_u32x2 __attribute__((ext_vector_type(2)));

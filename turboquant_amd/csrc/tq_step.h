@@ -122,6 +122,11 @@ __device__ __forceinline__ bool step_unit(const Step& s, int* u, int* b, int* j,
 __device__ __forceinline__ int32_t step_entry(const int32_t* table, int page) {
   return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)table)[page];
 }
+// four of them, one behind another
+__device__ __forceinline__ uint32_t __attribute__((ext_vector_type(4))) step_entries(const int32_t* table, int page) {
+  typedef uint32_t four __attribute__((ext_vector_type(4), aligned(4)));
+  return *(const __attribute__((address_space(4))) four*)(uintptr_t)(table + page);
+}
 
 // what the entry points check of a step, and its description
 inline int step_init(Step* s, const int32_t* starts, int64_t rows, int B, const int32_t* lens, const int32_t* table, int bt_stride, int64_t num_blocks) {
