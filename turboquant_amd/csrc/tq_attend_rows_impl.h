@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
   constexpr int SIZE = F8 ? 1 : 2, ROW = D * 2;              // bytes of an element in the cache, of a row in LDS
   constexpr int LANES = D * SIZE / 16, LOADS = ROWS_TOKENS * LANES / 256;
   constexpr int KSTEPS = D / 16, TILES = D / 32, M = 128;
-  constexpr int KAHEAD = 6;                                  // reads of keys that are on their way at a time
+    constexpr int KAHEAD = 4;                                  // reads of keys that are on their way at a time
   constexpr int HALF = ROWS_TOKENS * ROW;                    // keys or values of a turn
   extern __shared__ __attribute__((aligned(16))) char s_rows[];
 
@@ -318,6 +318,19 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
       __builtin_amdgcn_sched_group_barrier(0x008, KAHEAD, 0);
+      ex_u32x4 V[2][TILES];
+      const auto values = [&](int at) __attribute__((always_inline)) {
+#pragma unroll
+        for (int ct = 0; ct < TILES; ++ct) {
+          char* from = buffer + vp[ct % VPLACES] + (ct / VPLACES) * VPLACES * 64 + at * 16 * ROW;
+          typedef __attribute__((address_space(3))) ro_s16x4* lds4;
+          const ro_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)from);
+          const ro_s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(from + 8 * ROW));
+          const ex_u32x2 lo = __builtin_bit_cast(ex_u32x2, x), hi = __builtin_bit_cast(ex_u32x2, y);
+          V[at & 1][ct] = ex_u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+      };
+      values(0);
       if constexpr (F8 && !FOLD)
 #pragma unroll
         for (int p = 0; p < 4; ++p)
@@ -351,7 +364,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
       }
       const float ref = m == -INFINITY ? 0.0f : m - ex_lift<PT>();
       // Sixteen tokens at a time: the weights and values of the next while the matrix instructions of these run.
-      ex_u32x4 P[2], L[2], V[2][TILES];
+      ex_u32x4 P[2], L[2];
       const auto weights = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
@@ -368,18 +381,6 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
           }
         }
       };
-      const auto values = [&](int at) __attribute__((always_inline)) {
-#pragma unroll
-        for (int ct = 0; ct < TILES; ++ct) {
-          char* from = buffer + vp[ct % VPLACES] + (ct / VPLACES) * VPLACES * 64 + at * 16 * ROW;
-          typedef __attribute__((address_space(3))) ro_s16x4* lds4;
-          const ro_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)from);
-          const ro_s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(from + 8 * ROW));
-          const ex_u32x2 lo = __builtin_bit_cast(ex_u32x2, x), hi = __builtin_bit_cast(ex_u32x2, y);
-          V[at & 1][ct] = ex_u32x4{lo[0], lo[1], hi[0], hi[1]};
-        }
-      };
-      values(0);
       weights(0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
