@@ -213,6 +213,7 @@ def test_values_that_are_not_finite(gpu, kind, d, G, runs, window, sinks):
                 seen = (t > p - window) | (t < sinks) if window else torch.ones(p + 1, dtype=torch.bool)
                 add = odd[b, : p + 1][seen].sum(0).repeat_interleave(G, 0)
                 assert torch.equal(got[at + i].isfinite(), add.isfinite()), (b, i)
+                assert torch.equal(got[at + i].isposinf(), add.isposinf()) and torch.equal(got[at + i].isneginf(), add.isneginf()), (b, i)
             at += run
         if n_split is None:
             assert torch.equal(torch.where(got.isfinite(), got, clean.cpu()), clean.cpu())

@@ -8,7 +8,12 @@
 //   values    channels are rows; a lane reads its channels of its 8 tokens and turns them around in registers.  8 bits: half as many byte permutes, and the
 //             conversion to bf16 multiplies by the block's scale for nothing; bf16 for fp16 queries, too, whose range the scale might leave.
 //   softmax   one pass, running maximum and sum per row, all in 32 bits; weights go in as a high and a low half (ex_split).
-// Bound by the memory system.
+//
+// Bound by the memory system, whose 5.5 TB/s (a large read) it comes near where there is enough of it: one token of 32 sequences of 8192, 32 query heads on
+// 8 of 128, 8 bits: 538 MB in 107 us with the join's 5 (5.0 TB/s); bf16 blocks, the last 4096 of 32 sequences of 32768: as many bytes, 103 us.
+// One sequence of 131072, 16 query heads on 2 of 256, 8 bits: 134 MB in 36 us, of which the first loads and the join are 9.  One of 700: 10 us, the chain of length,
+// table, keys, values and the join's launch.  Several rows on 8 bits are bound by instructions: 24 sequences of 61 .. 16000, 5 rows, 20 columns of the 32, fp16 queries, 154 MB
+// in 54 us, where 32 tokens of a wavefront are 48 matrix instructions and 300 of the vector unit's (64 conversions, 24 permutes, the weights' halves).
 #pragma once
 
 #include "tq_attend.h"

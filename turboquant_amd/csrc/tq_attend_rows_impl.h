@@ -2,7 +2,8 @@
 //
 // A unit is 128 rows of a KV head: the query heads of a token side by side, tokens one behind another.  A wavefront takes 32 of them, each a column of
 // its matrix instructions; the workgroup's keys and values go through LDS, 64 tokens at a time, in 16 bits whatever the cache holds, two buffers in turn:
-// the next tokens are on their way in registers while these are worked on, and a turn has one barrier.
+// the next tokens are on their way while these are worked on - 16 bits straight to LDS (through registers 64 channels take 338 us for 285, 128 509 for 469, 256 1264
+// for 1107; two sequences of 8192, 2048 rows, 32 query heads on 8), 8 bits in registers to be converted -, and a turn has one barrier.
 //   scores    S^T = K Q^T: tokens are rows.  A lane has 32 of the 64 scores of a row, its neighbour 32 lanes on the others.
 //   softmax   one pass, running maximum and sum per row in 32 bits; the reference moves by 2^8 at a time (EX_SLACK).
 //   values    O^T = V^T P^T: the contraction takes the tokens in the order in which a lane holds the weights already, so that no weight changes its lane;
@@ -10,6 +11,14 @@
 // Weights are rounded once, to 16 bits, half a step of 2^-9 (fp16: 2^-12) that a sum over many averages out; a high and a low half, as the kernel of few
 // rows has them, would be half as many matrix instructions again.  8 bits for fp16 queries: bf16 values, whose range the block's scale
 // needs, and there the weights are two halves: one of bf16 would be eight times coarser than the output.
+// Instructions of a wavefront follow one another: those of the vector unit stand between the matrix instructions (weights and values of the next sixteen tokens
+// beside the product of these; 256 channels 1541 -> 1331 us), keys are read four ahead, and turns come in pairs, so that buffers are constants in addresses
+// (64 channels 354 -> 345 us).
+// Bound by both kinds of instructions of two wavefronts on a SIMD (192 and 256 channels: one): a turn of 128 channels is 1024 cycles of matrix instructions and 160 vector ones, 32 of
+// them exponentials.  bf16, 128 channels: 481 GFLOP in 469 us, 1.03 PFLOP/s, where a large product of the library reaches 1.40; with a window of 4096, one prompt of 8192, 413 in
+// 419; 64 channels 0.84, 192 0.79, 256 0.87 PFLOP/s; 8 bits, 128 channels 0.95 (fp16 queries with their two halves 0.69).
+// With 32 tokens a turn and three wavefronts on a SIMD 128 channels take 413 us for 419 with the window and 511 for 467 without (512 workgroups at a time become 768, of 1024); the
+// next turn's scores computed ahead of this one's products take 41 - 264 registers more than there are.
 // LDS: 16-byte pieces of a row change places by the row (rows_key_turn, rows_value_turn), so that neither reads nor writes meet in a bank.
 #pragma once
 
