@@ -232,3 +232,30 @@ def test_rotation_refuses(gpu):
     for out in ((q, q), (q, torch.empty_like(q)), (q[:5], k), (q.clone(), k.double()), (k, k), (torch.empty(1, 4, 64, device=gpu).expand(6, -1, -1), k.clone())):
         with pytest.raises(ValueError):
             rotate_heads(q, k, pos, f, out=out)
+
+
+@pytest.mark.parametrize("kind", ["fp8", "fp8 fp16"])
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("runs", [[1, 1], [5, 2], [60, 20]])
+def test_scales_of_blocks_that_hold_nothing(gpu, kind, d, runs):
+    """A cache that was never cleared: bytes of NaN and scales of 2^128 wherever no sequence's token is, block 0 among them; entries outside the cache."""
+    s = Step([100, 90], runs, 2, d, "fp8", torch.float16 if kind == "fp8 fp16" else torch.bfloat16, spare=40, seed=1)
+    used = s.table_cpu[s.table_cpu >= 0].long()
+    assert 0 not in used
+    empty = torch.ones(s.blocks, dtype=torch.bool)
+    empty[used] = False
+    for scales in s.scales:
+        scales[empty.to(gpu)] = 255
+    for bad in (-1, s.blocks, 2 ** 31 - 1):
+        s.table_cpu[0, 2], s.table_cpu[1, 0] = bad, bad
+        s.table = s.table_cpu.to(gpu)
+        q = s.query(8)
+        for window, sinks in ((None, 0), (40, 3)):
+            s.check(q, s.cache().attention(q.to(gpu), s.starts, s.table, s.seq_lens, window=window, sinks=sinks), 1 / math.sqrt(d), window, sinks)
+
+
+def test_frequencies_that_want_gradients(gpu):
+    q, k = torch.randn(3, 2, 64, device=gpu), torch.randn(3, 1, 64, device=gpu)
+    f = inverse_frequencies(64, device=gpu).requires_grad_()
+    with pytest.raises(RuntimeError):
+        rotate_heads(q, k, torch.arange(3, device=gpu), f)

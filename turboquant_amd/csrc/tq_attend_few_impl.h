@@ -139,7 +139,6 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
     }
     if constexpr (F8) x.scales = (lane & 2 ? a.v_scales : a.k_scales)[(lane & 1 ? page[1] : page[0]) * a.H + h];
   };
-  const auto scale_of = [](uint32_t byte) __attribute__((always_inline)) { return byte == 0 ? 0x1p-127f : __uint_as_float(byte << 23); };
 
   const uint32_t step = (uint32_t)a.s_t * SIZE;
   const uint32_t krow = (uint32_t)col * step + quarter * 16, vrow = (uint32_t)(quarter * 4) * step;
@@ -196,8 +195,8 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
     if constexpr (F8) {
 #pragma unroll
       for (int p = 0; p < PAGES; ++p) {
-        k_scale[p] = a.scale2 * scale_of((uint32_t)__builtin_amdgcn_readlane((int)now.scales, p));
-        v_scale[p] = scale_of((uint32_t)__builtin_amdgcn_readlane((int)now.scales, 2 + p));
+        k_scale[p] = a.scale2 * f8_scale((uint32_t)__builtin_amdgcn_readlane((int)now.scales, p));
+        v_scale[p] = f8_scale((uint32_t)__builtin_amdgcn_readlane((int)now.scales, 2 + p));
       }
     }
     // ---- scores ----

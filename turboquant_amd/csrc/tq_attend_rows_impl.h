@@ -155,7 +155,6 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
       return p < 2 ? (p < 1 ? x.entry[0] : x.entry[1]) : (p < 3 ? x.entry[2] : x.entry[3]);
     }
   };
-  const auto scale_of = [](uint32_t byte) __attribute__((always_inline)) { return byte == 0 ? 0x1p-127f : __uint_as_float(byte << 23); };
   // 16 bits
   constexpr int PLACES = D == 192 ? 3 : (D == 256 ? 2 : 1);
   uint32_t key_at[PLACES], value_at[PLACES];
@@ -246,7 +245,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
           v = (uint32_t)(t * ROW + (c ^ rows_value_turn<D>(t)) * 16);
         }
         char *const kt = to, *const vt = to + HALF;
-        const float kf = FOLD ? scale_of(ks[i]) : 1.0f, vf = scale_of(vs[i]);
+        const float kf = FOLD ? f8_scale(ks[i]) : 1.0f, vf = f8_scale(vs[i]);
         // (eight lanes store together, every second piece of 256 bytes, so that half of the banks have two: to have four of the lanes begin with the other
         // piece leaves no conflict and takes longer, 536 us for 522)
 #pragma unroll
@@ -285,7 +284,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
     store(first, whole, s_rows);
     if constexpr (F8 && !FOLD)
 #pragma unroll
-      for (int p = 0; p < 4; ++p) g[p] = scale_of(next_g[p]);
+      for (int p = 0; p < 4; ++p) g[p] = f8_scale(next_g[p]);
   }
   entries(ahead, first + 1);
   __syncthreads();
@@ -417,7 +416,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
     if (more) store(i + 1, next_whole, other);
     if constexpr (F8 && !FOLD)
 #pragma unroll
-      for (int p = 0; p < 4; ++p) g[p] = scale_of(next_g[p]);
+      for (int p = 0; p < 4; ++p) g[p] = f8_scale(next_g[p]);
     __syncthreads();
     t0 = next_t0;
     whole = next_whole;

@@ -31,9 +31,9 @@ __device__ __forceinline__ int f8_exponent(float largest) {
   return e < F8_LOWEST ? F8_LOWEST : (e > F8_HIGHEST ? F8_HIGHEST : e);
 }
 __device__ __forceinline__ float f8_power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
-__device__ __forceinline__ float f8_scale(uint8_t byte) {     // (no such scale as 2^-127 is written; a cache that is all zeros has it)
-  return byte == 0 ? 0x1p-127f : __uint_as_float((uint32_t)byte << 23);
-}
+// The scale that a byte says.  2^-127 and 2^127 are never written: a cache that is all zeros has the one, and the other is what a byte that nobody wrote says at most, so that
+// zeros in place of its block's values stay zeros (2^128 is infinite).
+__device__ __forceinline__ float f8_scale(uint32_t byte) { return byte == 0 ? 0x1p-127f : __uint_as_float((byte < 254u ? byte : 254u) << 23); }
 // what has no e4m3 number of its size becomes the largest; NaN stays
 __device__ __forceinline__ float f8_clamp(float x) { return x > 448.0f ? 448.0f : (x < -448.0f ? -448.0f : x); }
 __device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d) {

@@ -58,7 +58,7 @@ def rotate_heads(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None and (w.shape != (d,) or w.dtype != query.dtype or w.device != dev):
             raise ValueError(f"{name} must be ({d},) like the query: same dtype and GPU")
-    _ffi.require_constant("rotate_heads", query=query, key=key, q_weight=q_weight, k_weight=k_weight)
+    _ffi.require_constant("rotate_heads", query=query, key=key, q_weight=q_weight, k_weight=k_weight, inv_freq=inv_freq)
     align = 16 if query.dtype == torch.float32 else 8
     fits = lambda t: t.stride(2) == 1 and all(s >= 0 and s % 4 == 0 for s in t.stride()[:2]) and t.data_ptr() % align == 0
     given = query, key
