@@ -15,8 +15,9 @@
 // beside the product of these; 256 channels 1541 -> 1331 us), keys are read four ahead, and turns come in pairs, so that buffers are constants in addresses
 // (64 channels 354 -> 345 us).
 // Bound by both kinds of instructions of two wavefronts on a SIMD (192 and 256 channels: one): a turn of 128 channels is 1024 cycles of matrix instructions and 160 vector ones, 32 of
-// them exponentials.  bf16, 128 channels: 481 GFLOP in 469 us, 1.03 PFLOP/s, where a large product of the library reaches 1.40; with a window of 4096, one prompt of 8192, 413 in
-// 419; 64 channels 0.84, 192 0.79, 256 0.87 PFLOP/s; 8 bits, 128 channels 0.95 (fp16 queries with their two halves 0.69).
+// them exponentials.  bf16, 128 channels: 481 GFLOP in 460 us, 1.05 PFLOP/s, where a large product of the library reaches 1.40; with a window of 4096, one prompt of 8192, 413 in
+// 424; 64 channels 0.87, 192 0.79, 256 0.87 PFLOP/s; 8 bits, 128 channels 0.98 (fp16 queries with their two halves 0.71).  Eight wavefronts to a workgroup, which would load half as
+// often, 460 us, too.
 // With 32 tokens a turn and three wavefronts on a SIMD 128 channels take 413 us for 419 with the window and 511 for 467 without (512 workgroups at a time become 768, of 1024); the
 // next turn's scores computed ahead of this one's products take 41 - 264 registers more than there are.
 // LDS: 16-byte pieces of a row change places by the row (rows_key_turn, rows_value_turn), so that neither reads nor writes meet in a bank.
@@ -288,6 +289,11 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
   }
   entries(ahead, first + 1);
   __syncthreads();
+  // A wavefront that is further in its turn goes first: 64 channels 292 -> 275 us, 128 476 -> 460, 256 1106 -> 1098, 8 bits 128 508 -> 490; but 64 channels of 8 bits, whose
+  // turn is conversions for the most part, 327 -> 360.
+  const auto priority = [](auto p) __attribute__((always_inline)) {
+    if constexpr (!F8 || D > 64) __builtin_amdgcn_s_setprio(decltype(p)::value);
+  };
   const auto turn = [&](int i, auto which) __attribute__((always_inline)) {
     char* const buffer = s_rows + decltype(which)::value * 2 * HALF;
     char* const other = s_rows + (decltype(which)::value ^ 1) * 2 * HALF;
@@ -309,6 +315,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
         entries(now, i);
         clear = complete(now);
       }
+      priority(std::integral_constant<int, 1>());
       ro_f32x16 S[2];
 #pragma unroll
       for (int T = 0; T < 2; ++T)
@@ -356,6 +363,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
             S[T][e] = seen ? S[T][e] : -INFINITY;
           }
       }
+      priority(std::integral_constant<int, 2>());
       float top = -INFINITY;
 #pragma unroll
       for (int T = 0; T < 2; ++T)
@@ -390,6 +398,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
         }
       };
       weights(0);
+      priority(std::integral_constant<int, 3>());
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int at = 0; at < 4; ++at) {
@@ -413,6 +422,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    priority(std::integral_constant<int, 0>());
     if (more) store(i + 1, next_whole, other);
     if constexpr (F8 && !FOLD)
 #pragma unroll
