@@ -69,6 +69,27 @@ struct AttendPlan {
 static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // starts: whether the rows are the sequences' as starts say, up to max_rows of one (else one row each).  n_split 0: chosen here.
+// Splits of the tokens of units of 128 rows: the least of what the model says they take, in us.  A turn is 1.15 (128 channels, a workgroup on a compute unit; up to the
+// other half of them 1.35, since some get two; two on all of them 2.05, so that the second gains little; 192 and 256 channels have one, 1.2), and a join is a launch and the
+// partial results' way out and back, 5 and 1 for 2 MB.  No split has less than four turns of 128 channels.  Measured (us; bf16, 32 query heads on 8 of 128, one sequence, 1 / 2 / 4 / 8 / 16 splits): 512
+// tokens, 512 rows 20 / 26 / 31 / 39; 1024, 1024 30 / 41 / 54 / 64; 4096, 64 rows 82 / 50 / 32 / 24 / 23, 512 rows 82 / 71 / 58 / 64 / 89; 16384, 64 rows
+// 309 / 165 / 90 / 54 / 42, 512 rows 305 / 199 / 152 / 158 / 175, 2048 rows 483 / 541 / 553 / 587 / 674.
+static int64_t attend_rows_splits(int64_t pairs, int64_t blocks, int64_t rows, int d) {
+  const int64_t most = std::min<int64_t>(blocks * 128 / (4 * std::max(d, 128)), JOIN_MAX_SPLITS);
+  const double channels = d / 128.0, mb = (double)rows * d * 4e-6;
+  int64_t best = 1;
+  double least = 0;
+  for (int64_t n = 1; n <= std::max<int64_t>(most, 1); ++n) {
+    const int64_t groups = pairs * n, turns = (blocks + n - 1) / n;
+    double turn = groups <= 128 ? 1.15 : (groups <= 256 ? 1.35 : 2.05 * (double)((groups + 511) / 512));
+    if (d > 128) turn = 1.2 * (double)((groups + 255) / 256);
+    const double us = (double)turns * turn * channels + (n > 1 ? 5 + 0.5 * mb * (double)n : 0);
+    if (n == 1 || us < least) { best = n; least = us; }
+    if (groups > 512) break;                                 // (behind two on all compute units more of them are more rounds)
+  }
+  return best;
+}
+
 static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_t rows, int B, int Hq, int Hkv, int d, int64_t max_len, int64_t max_rows,
                         int64_t window, int sinks, int n_split) {
   if ((dtype != TQ_F16 && dtype != TQ_BF16) || (cache != dtype && cache != TQ_E4M3) || rows < 0 || rows > INT32_MAX || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv)
@@ -106,8 +127,7 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
       }
       n = std::min<int64_t>(n_split, (blocks + 3) / 4);
     } else {
-      n = (256 * (d <= 128 ? 2 : 1) + pairs - 1) / pairs;
-      n = std::min<int64_t>(std::min<int64_t>(n, (blocks + 3) / 4), JOIN_MAX_SPLITS);
+      n = attend_rows_splits(pairs, blocks, rows * Hq, d);
     }
   }
   n = std::max<int64_t>(1, std::min(n, blocks));
@@ -130,7 +150,7 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   p->items = std::max<int64_t>(units * p->n_split, p->target ? p->target + units + 2 : 0);      // (2: total and its share are rounded)
   const int most = std::max(p->n_split, p->cap);
   // (with many rows a sequence few are split: 131072 of which none is took 12 us with a wavefront each)
-  p->few = most <= JOIN_FEW || (many && most <= 64) ? (p->tiles ? 1 : 8) : 0;
+  p->few = most <= JOIN_FEW || (many && most <= 64) ? (p->tiles || p->n_split > 1 ? 1 : 8) : 0;
   const size_t all = (size_t)rows * Hq;
   p->grid = p->items * Hkv;
   size_t at = 0;
