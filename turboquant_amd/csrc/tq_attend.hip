@@ -140,12 +140,13 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   // Sequences that differ (to find out takes a workgroup 1 - 2 us: not where 2048 tokens are the most that one has to itself) have their blocks shared out anew: 1024
   // items in all (us, as planned / shared out; fp8, 24 sequences of 61 .. 16000, 5 rows 75 / 54, one row 54 / 46; 96 of 61 .. 8190 86 / 81), and with many rows 512
   // (exact, 64 of 100 .. 20000, 64 rows 694 / 448).  A row has up to 64 of them where that leaves the join a wavefront for each row (above, a workgroup
-  // for 64 channels of one).
+  // for 64 channels of one), and of few rows up to 96, none of less than 512 tokens (without these bounds / with: 40 of 50 .. 6000, 16 heads on 2 of 256 36.5 / 25.2; 4 of
+  // 1000 .. 100000, 32 on 4 41.9 / 38.0; 8 of 5000 .. 60000, 16 on 2 of 256 58.0 / 60.3).
   const bool many = rows * Hq >= 512;
   p->target = p->cap = 0;
   if (!given && B > 1 && B <= STEP_ROUND && tokens > 2048) {
     p->target = (int)(((p->tiles ? 1024 : 512) + Hkv - 1) / Hkv);
-    p->cap = (int)std::max<int64_t>(p->n_split, std::min<int64_t>((blocks + 3) / 4, many ? 64 : JOIN_MAX_SPLITS));
+    p->cap = (int)std::max<int64_t>(p->n_split, std::min<int64_t>((blocks + 3) / 4, many ? 64 : (p->tiles ? 96 : JOIN_MAX_SPLITS)));
   }
   p->items = std::max<int64_t>(units * p->n_split, p->target ? p->target + units + 2 : 0);      // (2: total and its share are rounded)
   const int most = std::max(p->n_split, p->cap);
