@@ -216,3 +216,45 @@ def test_what_cannot_be_cut_is_refused(gpu):
     with pytest.raises(ValueError, match="sliding window"):
         track_weights(r, 3, 100)
     assert all(s.weights is None for s in r._tq_layer_states.values())
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (24, 4)])
+def test_a_captured_layer_is_replayed(gpu, window, sinks):
+    """Rotation, write and attention in one graph: every replay is another step (chunks, single tokens, rows of no sequence), the program's own work in between."""
+    Hq, H, d, B, rows = 16, 2, 64, 3, 90
+    g = torch.Generator().manual_seed(8)
+    inv = inverse_frequencies(d, device=gpu)
+    table = torch.randperm(B * 20, generator=g).to(torch.int32).view(B, 20).to(gpu)
+    caches = [Fp8PagedCache.allocate(B * 20, H, d, gpu) for _ in range(2)]
+    qkv = torch.zeros(rows, (Hq + 2 * H) * d, dtype=torch.bfloat16, device=gpu)
+    positions, starts, lens = (torch.zeros(n, dtype=torch.int32, device=gpu) for n in (rows, B + 1, B))
+    workspace = caches[0].workspace(rows, Hq, 320, B=B, max_rows=rows, window=window, sinks=sinks)
+
+    def layer(cache, **kw):
+        q, k, v = (x.view(rows, -1, d) for x in qkv.split([Hq * d, H * d, H * d], -1))
+        q, k = rotate_heads(q, k, positions, inv)
+        cache.write(k, v, starts, table, lens)
+        return q, cache.attention(q, starts, table, lens, window=window, sinks=sinks, max_len=320, max_rows=rows, **kw)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(caches[0], workspace=workspace)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q, out = layer(caches[0], workspace=workspace)
+    now = [0] * B
+    for runs in ([40, 17, 33], [1, 1, 1], [5, 0, 80], [60, 1, 2], [1, 1, 1]):
+        now = [n + r for n, r in zip(now, runs)]
+        qkv.copy_(torch.randn(qkv.shape, generator=g))
+        starts.copy_(torch.tensor([0] + runs).cumsum(0))
+        lens.copy_(torch.tensor(now))
+        positions.copy_(torch.cat([torch.arange(n - r, n) for n, r in zip(now, runs)] + [torch.zeros(rows - sum(runs), dtype=torch.long)]))
+        graph.replay()
+        torch.cuda.synchronize()
+        _, eager = layer(caches[1])
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and (out[sum(runs):] == 0).all()
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(caches[0].operands(), caches[1].operands()))
+        check_rows(q[: sum(runs)], out[: sum(runs)], held_by(caches[0], table, now), now, runs, 1 / math.sqrt(d), window, sinks)
