@@ -165,8 +165,9 @@ __device__ __forceinline__ bool attend_item(const Attend& a, int n, AttendUnit* 
         total = wave_sum_fast(total);
         longest = wave_max_fast(longest);
         if (longest * wave_sum_fast(units) * 7 > total * 8) {  // (by more than an eighth)
-          // (few rows: not less than 512 tokens, of which a wavefront has four turns, nor so little that the longest sequence would have more shares than it may)
-          const float least = M > 32 ? 1.0f : fmaxf(16.0f, ceilf(longest * (1.0f / (float)a.cap)));
+          // (few rows: not less than 512 tokens, of which a wavefront has four turns, nor so little that the longest sequence would have more shares than it may; many: not less
+          // than 2048 tokens, 32 turns, since the join of many rows takes its time)
+          const float least = M > 32 ? 32.0f : fmaxf(16.0f, ceilf(longest * (1.0f / (float)a.cap)));
           const AttendSplits splits((int)fminf(fmaxf(ceilf(total * a.share), least), 1e9f), a.cap);
 #pragma unroll
           for (int i = 0; i < 4; ++i) count[i] *= splits(blocks[i]);

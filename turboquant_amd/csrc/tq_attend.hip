@@ -141,7 +141,8 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   // items in all (us, as planned / shared out; fp8, 24 sequences of 61 .. 16000, 5 rows 75 / 54, one row 54 / 46; 96 of 61 .. 8190 86 / 81), and with many rows 512
   // (exact, 64 of 100 .. 20000, 64 rows 694 / 448).  A row has up to 64 of them where that leaves the join a wavefront for each row (above, a workgroup
   // for 64 channels of one), and of few rows up to 96, none of less than 512 tokens (without these bounds / with: 40 of 50 .. 6000, 16 heads on 2 of 256 36.5 / 25.2; 4 of
-  // 1000 .. 100000, 32 on 4 41.9 / 38.0; 8 of 5000 .. 60000, 16 on 2 of 256 58.0 / 60.3).
+  // 1000 .. 100000, 32 on 4 41.9 / 38.0; 8 of 5000 .. 60000, 16 on 2 of 256 58.0 / 60.3).  Of many rows none has less than 2048 tokens (one turn at least / so; exact, 32 heads on 8
+  // of 128: 24 of 300 .. 16000, 16 rows 116 / 101; 16 of 300 .. 5000, 64 rows 85 / 73; 3 of 300 .. 30000, 64 rows 57 / 62).
   const bool many = rows * Hq >= 512;
   p->target = p->cap = 0;
   if (!given && B > 1 && B <= STEP_ROUND && tokens > 2048) {
@@ -150,8 +151,9 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   }
   p->items = std::max<int64_t>(units * p->n_split, p->target ? p->target + units + 2 : 0);      // (2: total and its share are rounded)
   const int most = std::max(p->n_split, p->cap);
-  // (with many rows a sequence few are split: 131072 of which none is took 12 us with a wavefront each)
-  p->few = most <= JOIN_FEW || (many && most <= 64) ? (p->tiles || p->n_split > 1 ? 1 : 8) : 0;
+  // (with many rows a sequence few are split: 131072 of which none is took 12 us with a wavefront each; 8 sequences of 300 .. 4000, 300 rows, 9600 rows of 32 heads, with eight rows each 105, with
+  // four 99)
+  p->few = most <= JOIN_FEW || (many && most <= 64) ? (p->tiles || p->n_split > 1 ? 1 : (int)std::min<int64_t>(8, std::max<int64_t>(1, rows * Hq / 16384))) : 0;
   const size_t all = (size_t)rows * Hq;
   p->grid = p->items * Hkv;
   size_t at = 0;

@@ -4,7 +4,7 @@
 // 16-bit input, 8 of the cache), which is all of it, so that the largest value is a reduction over the wavefront and the block is read once.
 // Tokens that a block held before the step keep their bytes unless the block's exponent grows: then they are rounded again from what they stand for.
 // No two wavefronts write to one block of a head: a block belongs to one sequence.
-// Bound by the memory system where there are prompts (32768 rows, 8 heads of 128, bf16: write 51 us, 201 MB in and out, read 35 us, a launch each: 403 MB in 89 us, 4.5 TB/s; a
+// Bound by the memory system where there are prompts (32768 rows, 8 heads of 128, bf16: write 44 us, 201 MB in and out, read 38, a launch each: 403 MB in 84 us, 4.8 TB/s; a
 // large copy reaches 5.1), by the chain of starts, lengths, table entry and rows where there are tokens (64 tokens: 4.6 and 5.2 us, of which a launch that does nothing is 2).
 #include "tq_fp8.h"
 
