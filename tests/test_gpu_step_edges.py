@@ -259,3 +259,36 @@ def test_frequencies_that_want_gradients(gpu):
     f = inverse_frequencies(64, device=gpu).requires_grad_()
     with pytest.raises(RuntimeError):
         rotate_heads(q, k, torch.arange(3, device=gpu), f)
+
+
+def test_keys_and_values_in_one_place(gpu):
+    """Written to, a cache's four tensors are memory of their own; values in the gaps between keys are."""
+    H, d, n = 2, 64, 4
+    bytes_ = lambda *shape: torch.zeros(*shape, dtype=torch.uint8, device=gpu)
+    scales = [bytes_(n, H) for _ in range(2)]
+    k, v = (torch.randn(20, H, d, device=gpu, generator=torch.Generator(gpu).manual_seed(i)) for i in range(2))
+    step = [torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([0, 20], [[2, 1]], [20])]
+    one = bytes_(n, PAGE, H, d).view(F8)
+    for bad in ((one, one, *scales), (one[:-1], one[1:], *(s[:-1] for s in scales)), (one, bytes_(n, PAGE, H, d).view(F8), scales[0], scales[0]),
+                (one, bytes_(n, PAGE, H, d).view(F8), scales[0], one.view(torch.uint8).flatten()[: n * H].view(n, H))):
+        cache = Fp8PagedCache(*bad)
+        with pytest.raises(ValueError, match="overlaps itself"):
+            cache.write(k, v, *step)
+        cache.read(*step, rows=20)
+    apart = Fp8PagedCache.allocate(n, H, d, gpu)
+    apart.write(k, v, *step)
+    want = apart.read(*step, rows=20)
+    blocks = bytes_(n, 2, PAGE, H, d).view(F8)
+    sides = bytes_(n, PAGE, H, 2 * d).view(F8)
+    rows = bytes_(n, PAGE, 2, H, d).view(F8)
+    for a, b in ((blocks[:, 0], blocks[:, 1]), (blocks[:, 1], blocks[:, 0]), (sides[..., :d], sides[..., d:]), (rows[:, :, 0], rows[:, :, 1])):
+        cache = Fp8PagedCache(a, b, bytes_(n, H), bytes_(n, H))
+        cache.write(k, v, *step)
+        assert all(torch.equal(x, y) for x, y in zip(cache.read(*step, rows=20), want))
+
+
+def test_rotation_over_what_it_reads(gpu):
+    room = torch.zeros(4, 64, dtype=torch.float64, device=gpu)
+    q, k, f = torch.randn(4, 1, 64, device=gpu), torch.randn(4, 1, 64, device=gpu), room[0, :32]
+    with pytest.raises(ValueError, match="inv_freq"):
+        rotate_heads(q, k, torch.arange(4, device=gpu), f, out=(room.view(torch.float32)[:, None, :64], k.clone()))

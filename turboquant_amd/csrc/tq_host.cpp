@@ -734,9 +734,9 @@ bool meet(const at::Tensor& a, const at::Tensor& b) {
   };
   return a.numel() && b.numel() && (char*)a.data_ptr() < end(b) && (char*)b.data_ptr() < end(a);
 }
-// no two elements in one place; the last dimension's are neighbours
-bool own_places(const at::Tensor& t) {
-  std::vector<std::pair<int64_t, int64_t>> by;
+// no two elements of t and its twin of the same strides in one place; the last dimension's are neighbours, an element is a byte
+bool own_places(const at::Tensor& t, const at::Tensor& twin) {
+  std::vector<std::pair<int64_t, int64_t>> by{{std::abs((char*)twin.data_ptr() - (char*)t.data_ptr()), 2}};
   for (int64_t i = 0; i + 1 < t.dim(); ++i)
     if (t.size(i) > 1) by.emplace_back(t.stride(i), t.size(i));
   std::sort(by.begin(), by.end());
@@ -766,7 +766,9 @@ PyObject* fp8_write(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     Blocks8 c;
     Starts st;
     Sequences s;
-    if (!c.take(p, a + 5) || !st.take(p, a[2]) || !s.take(p, a[3], a[4], st.B, st.B == 1) || !own_places(c.k)) return nullptr;
+    if (!c.take(p, a + 5) || !st.take(p, a[2]) || !s.take(p, a[3], a[4], st.B, st.B == 1) || !own_places(c.k, c.v) || meet(c.ks, c.vs) ||
+        meet(c.k, c.ks) || meet(c.k, c.vs) || meet(c.v, c.ks) || meet(c.v, c.vs))
+      return nullptr;
     const at::Tensor k = p.take(a[0]), v = p.take(a[1]);
     if (!p.ok || k.dim() != 3 || k.sizes() != v.sizes() || k.size(1) != c.H || k.size(2) != c.d || k.size(0) == 0 || v.scalar_type() != k.scalar_type()) return nullptr;
     const int tag = dtype_tag(k.scalar_type());

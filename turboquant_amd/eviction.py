@@ -50,10 +50,17 @@ class Evictions(NamedTuple):
         return self.count, self.dst, self.src, table, table.shape[1]
 
 
-def own_rows(t: torch.Tensor) -> bool:
-    """Whether no two elements of t, the last dimension's contiguous, lie in one place."""
+def own_rows(t: torch.Tensor, twin: Optional[torch.Tensor] = None) -> bool:
+    """Whether no two elements of t, the last dimension's contiguous, lie in one place; with a twin of the same strides, of both of them (one may lie in gaps that the
+    other leaves)."""
     reach = t.shape[-1]
-    for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(t.dim() - 1) if t.shape[i] > 1):
+    places = [(t.stride(i), t.shape[i]) for i in range(t.dim() - 1) if t.shape[i] > 1]
+    if twin is not None:
+        apart = abs(twin.data_ptr() - t.data_ptr())
+        if apart % t.element_size():
+            return False
+        places.append((apart // t.element_size(), 2))
+    for stride, size in sorted(places):
         if stride < reach:
             return False
         reach = stride * (size - 1) + reach

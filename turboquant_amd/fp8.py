@@ -96,7 +96,8 @@ class Fp8PagedCache:
         _ffi.require_constant("write", key=key, value=value, **self.tensors())
         if any(overlaps(t, held) for t in (key, value) for held in self.tensors().values()):
             raise ValueError("key and value must not lie in the cache's own memory")
-        if not own_rows(self.key_cache):
+        k, v, k_scales, v_scales = self.operands()
+        if not own_rows(k, v) or overlaps(k_scales, v_scales) or any(overlaps(x, y) for x in (k, v) for y in (k_scales, v_scales)):
             raise ValueError("a cache that overlaps itself cannot be written to")
         starts, B = step_starts(self.device, query_start_loc)
         table, bt_stride, lens = sequences(self.device, block_table, seq_lens, B)

@@ -80,6 +80,9 @@ def rotate_heads(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
                 if overlaps(t, other) and not (other.data_ptr() == t.data_ptr() and other.stride() == t.stride() and other.shape == t.shape) and \
                         not _beside(t, other):
                     raise ValueError(f"out {name} must be the input itself or memory of its own")
+            for what, other in (("positions", positions), ("inv_freq", inv_freq), ("q_weight", q_weight), ("k_weight", k_weight)):
+                if other is not None and overlaps(t, other):
+                    raise ValueError(f"out {name} overlaps {what}")
         if overlaps(*new) and not _beside(*new):
             raise ValueError("the two tensors of out must not overlap")
     q_weight, k_weight = (None if w is None else _weight(w, align) for w in (q_weight, k_weight))
