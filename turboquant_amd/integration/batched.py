@@ -68,7 +68,7 @@ def _host_list(meta, name):
 
 
 def _window_of(name: str, impl) -> Tuple[Optional[int], int]:
-    """(window, sinks) of a layer, as its backend names them: `sliding_window`, tokens that a query sees with its own among them, or flash attention's pair of
+    """(window, sinks) of a layer, as its backend names them: `sliding_window`, tokens that a query sees with its own among them, or the pair of
     those on its left and right (-1: all), and `sink_tokens`, first tokens that stay visible."""
     window = getattr(impl, "sliding_window", None)
     if isinstance(window, (tuple, list)):
