@@ -11,7 +11,7 @@
 //
 // Bound by the memory system, whose 5.5 TB/s (a large read) it comes near where there is enough of it: one token of 32 sequences of 8192, 32 query heads on
 // 8 of 128, 8 bits: 538 MB in 107 us with the join's 5 (5.0 TB/s); bf16 blocks, the last 4096 of 32 sequences of 32768: as many bytes, 103 us.
-// One sequence of 131072, 16 query heads on 2 of 256, 8 bits: 134 MB in 36 us, of which the first loads and the join are 9.  One of 700: 10 us, the chain of length,
+// One sequence of 131072, 16 query heads on 2 of 256, 8 bits: 134 MB in 35 us, of which the first loads and the join are 8.  One of 700: 10 us, the chain of length,
 // table, keys, values and the join's launch.  Several rows on 8 bits are bound by instructions: 24 sequences of 61 .. 16000, 5 rows, 20 columns of the 32, fp16 queries, 154 MB
 // in 54 us, where 32 tokens of a wavefront are 48 matrix instructions and 300 of the vector unit's (64 conversions, 24 permutes, the weights' halves).
 #pragma once
@@ -48,7 +48,16 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int col = lane & 15, quarter = lane >> 4;
-  const int item = (int)(blockIdx.x / (unsigned)a.H), x = (int)(blockIdx.x - (unsigned)item * (unsigned)a.H);
+  // Two heads' rows share a line of 128 bytes where a row is 64 or 192: they go to one of the eight dies, whose L2 the line is in then, eight workgroups apart (sixteen of
+  // them are eight pairs, and so are those behind the last sixteen).  8 bits, 32 sequences of 8192, 32 heads on 8: of 64 92 -> 63 us, of 192 175 -> 170; 16 sequences, 32 on 32 of 64 173 -> 118.
+  constexpr bool PAIRS = F8 && (D == 64 || D == 192);
+  const bool paired = PAIRS && a.H % 2 == 0;
+  unsigned at = blockIdx.x;
+  if (paired) {
+    const unsigned from = at & ~15u, r = at - from, half = (gridDim.x - from < 16u ? gridDim.x - from : 16u) / 2u;
+    at = from + (r < half ? 2u * r : 2u * (r - half) + 1u);
+  }
+  const int item = (int)(at / (unsigned)a.H), x = (int)(at - (unsigned)item * (unsigned)a.H);
   AttendUnit u;
   int over, others;
   if (!attend_item<16 * NT, TB>(a, item, &u, &over, &others)) {
@@ -57,7 +66,7 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_f
   }
   // Which KV head: not the same for all that a compute unit has at a time (as planned, shares of one unit), whose addresses would all be the same in the bits
   // that tell heads apart.  32 sequences of 8192, 8 heads of 128, 8 bits: 122 us with head x, 119 with x + unit, 107 so.
-  const int h = (int)((unsigned)(x + (u.planned ? u.split : item)) % (unsigned)a.H), place = item * a.H + h;
+  const int h = (int)((unsigned)(x + (u.planned ? u.split : item) * (paired ? 2 : 1)) % (unsigned)a.H), place = item * a.H + h;
   const AttendBlocks<TB> list(a, u);
   const AttendShare share(a, u, list.count);
   if (u.split >= share.used) return;
