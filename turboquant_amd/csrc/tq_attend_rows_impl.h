@@ -65,6 +65,8 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
 
   const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 31, half = lane >> 5;
   // (the last units of a sequence have the most tokens: they begin first)
+  // (units of a KV head follow one another on a die, whose L2 has its blocks: with two heads that share lines on each, as few rows have them, 8 bits of 64 channels 320 -> 345 us,
+  // of 192 1031 -> 1228)
   const unsigned turn_of = blockIdx.x / (unsigned)a.H;
   const int h = (int)(blockIdx.x - turn_of * (unsigned)a.H);
   const int item = a.items - 1 - (int)turn_of, place = item * a.H + h;
