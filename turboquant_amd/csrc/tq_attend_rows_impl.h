@@ -16,7 +16,8 @@
 // (64 channels 354 -> 345 us).
 // Bound by both kinds of instructions of two wavefronts on a SIMD (192 and 256 channels: one): a turn of 128 channels is 1024 cycles of matrix instructions and 160 vector ones, 32 of
 // them exponentials.  bf16, 128 channels: 481 GFLOP in 460 us, 1.05 PFLOP/s, where a large product of the library reaches 1.40; with a window of 4096, one prompt of 8192, 413 in
-// 424; 64 channels 0.87, 192 0.79, 256 0.87 PFLOP/s; 8 bits, 128 channels 0.98 (fp16 queries with their two halves 0.71).  Eight wavefronts to a workgroup, which would load half as
+// 424; 64 channels 0.87, 192 0.79, 256 0.87 PFLOP/s; 8 bits, 128 channels 0.98 (fp16 queries with their two halves 0.71).  The clock falls as they are busier: with 16 bits straight to LDS a launch takes a fifth
+// fewer cycles and a tenth less time.  Eight wavefronts to a workgroup, which would load half as
 // often, 460 us, too; two tiles of rows to a wavefront, which would read LDS half as often, 64 channels 274, 128 627 (at one wavefront on a SIMD half of its registers are the
 // accumulators', and scores are copied out of them).  Without its reads of LDS a turn of 128 channels would take 0.78 of its time, without its loads 0.87, without exponentials 0.91.
 // With 32 tokens a turn and three wavefronts on a SIMD 128 channels take 413 us for 419 with the window and 511 for 467 without (512 workgroups at a time become 768, of 1024); the
