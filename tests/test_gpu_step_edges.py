@@ -292,3 +292,23 @@ def test_rotation_over_what_it_reads(gpu):
     q, k, f = torch.randn(4, 1, 64, device=gpu), torch.randn(4, 1, 64, device=gpu), room[0, :32]
     with pytest.raises(ValueError, match="inv_freq"):
         rotate_heads(q, k, torch.arange(4, device=gpu), f, out=(room.view(torch.float32)[:, None, :64], k.clone()))
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("G", [1, 4, 16, 64])
+@pytest.mark.parametrize("runs", [[1], [3], [1, 0, 2], [16], [33, 1]])
+@pytest.mark.parametrize("extra", [1, 2, 40])
+def test_rows_of_no_sequence_behind_full_units(gpu, kind, G, runs, extra):
+    """The units of a step may be as many as there can be: rows of no sequence are zeros all the same, or as they were."""
+    s = Step([300 + 7 * i for i in range(len(runs))], runs, 2, 64, *KINDS[kind], extra=extra)
+    q = s.query(2 * G).to(gpu)
+    for kw in (dict(), dict(n_split=1), dict(n_split=5), dict(max_len=16), dict(window=50, sinks=2)):
+        got = s.cache().attention(q, s.starts, s.table, s.seq_lens, **kw)
+        assert (got[sum(runs):] == 0).all()
+        out = torch.full_like(got, 3.0)
+        s.cache().attention(q, s.starts, s.table, s.seq_lens, out=out, **kw)
+        assert (out[sum(runs):] == 3).all() and torch.equal(out[: sum(runs)], got[: sum(runs)])
+    late = s.starts + extra                                  # rows in front of the first sequence
+    moved = torch.cat([q[sum(runs):], q[: sum(runs)]])
+    got2 = s.cache().attention(moved, late, s.table, s.seq_lens, window=50, sinks=2)
+    assert (got2[:extra] == 0).all() and torch.equal(got2[extra:], got[: sum(runs)])

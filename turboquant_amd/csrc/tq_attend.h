@@ -144,6 +144,9 @@ __device__ __forceinline__ bool attend_item(const Attend& a, int n, AttendUnit* 
     StepRun r[4];
     int blocks[4];
     bool found = false;
+    // (behind the last share there is an item for rows of no sequence, if there are no units left over: as many units as there may be are then all met)
+    const bool rest = n == a.units * a.n_split;
+    if (rest) u = a.units;
     const int given = u;
     for (int base = 0; base < a.s.B && !found; base += STEP_ROUND) {
       step_runs(a.s, base, r);
@@ -188,14 +191,15 @@ __device__ __forceinline__ bool attend_item(const Attend& a, int n, AttendUnit* 
       }
       found = step_find(a.s, base, r, count, &u, &t->b, &unit, &run);
     }
-    if (t->planned && t->split >= a.n_split) return false;
+    if (t->planned && t->split >= a.n_split && !rest) return false;
     if (!found) {
-      if (t->split == 0) {
+      if (t->split == 0 || rest) {
         *over = u;
-        *others = a.units - (given - u);
+        *others = a.units + 1 - (given - u);
       }
       return false;
     }
+    if (t->planned && rest) return false;                    // (more units than there may be: starts that do not ascend)
   }
   // (all of it is the same for the whole wavefront, which only the scalar registers say to the compiler: its tables' entries are scalar loads then)
   t->b = __builtin_amdgcn_readfirstlane(t->b);

@@ -102,7 +102,8 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   max_rows = starts ? std::max<int64_t>(1, std::min(max_rows, rows)) : 1;
   p->tiles = max_rows * G <= 16 ? 1 : (max_rows * G <= 32 ? 2 : 0);
   const int M = p->tiles ? 16 * p->tiles : 128, TB = p->tiles ? 32 : 64;
-  const int64_t units = std::max<int64_t>(1, starts ? (rows * G + M - 1) / M + B + 1 : (int64_t)B * ((G + M - 1) / M));
+  // (every sequence with rows may have a last unit that is not full)
+  const int64_t units = std::max<int64_t>(1, starts ? (rows * G + std::min<int64_t>(B, rows) * (M - 1)) / M : (int64_t)B * ((G + M - 1) / M));
   // (of these, up to B are not met, and most of a short row's are)
   const int64_t busy = starts ? std::max<int64_t>(std::min<int64_t>(B, rows), (rows * G + M - 1) / M) : units;
   const int64_t pairs = std::max<int64_t>(1, busy * Hkv);
@@ -149,7 +150,8 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
     p->target = (int)(((p->tiles ? 1024 : 512) + Hkv - 1) / Hkv);
     p->cap = (int)std::max<int64_t>(p->n_split, std::min<int64_t>((blocks + 3) / 4, many ? 64 : (p->tiles ? 96 : JOIN_MAX_SPLITS)));
   }
-  p->items = std::max<int64_t>(units * p->n_split, p->target ? p->target + units + 2 : 0);      // (2: total and its share are rounded)
+  // (one for rows of no sequence; 2: total and its share are rounded)
+  p->items = std::max<int64_t>(units * p->n_split + (starts ? 1 : 0), p->target ? p->target + units + 3 : 0);
   const int most = std::max(p->n_split, p->cap);
   // (with many rows a sequence few are split: 131072 of which none is took 12 us with a wavefront each; 8 sequences of 300 .. 4000, 300 rows, 9600 rows of 32 heads, with eight rows each 105, with
   // four 99)

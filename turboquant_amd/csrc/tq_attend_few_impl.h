@@ -28,15 +28,18 @@ __device__ __forceinline__ uint32_t f8_widen(uint32_t x, float scale) {
   else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, UPPER));
 }
 
-template <bool F8, int D, int NT>
+// Wavefronts on a SIMD.  (16 bits, 128 channels, rows at different positions: at three 8 registers are spilled, 2 rows of 24 sequences of 61 .. 16000 78 us, at two 71; 4 rows of 32 of
+// 8192 214 / 199)
+template <bool F8, int D, int NT, bool APART>
 constexpr int attend_few_waves() {
+  if (!F8 && D == 128 && NT == 1 && APART) return 2;
   if (NT == 1) return F8 ? (D <= 64 ? 4 : (D <= 128 ? 3 : 2)) : (D <= 64 ? 4 : (D <= 128 ? 3 : (D <= 192 ? 2 : 1)));
   return F8 ? (D <= 64 ? 3 : (D <= 128 ? 2 : 1)) : (D <= 64 ? 3 : (D <= 128 ? 2 : 1));
 }
 
 // APART: rows of a unit may stand at different positions (not one token of each sequence)
 template <int QT, bool F8, int D, int NT, bool APART>
-__global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT>())) attend_few_kernel(const Attend a) {
+__global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT, APART>())) attend_few_kernel(const Attend a) {
   constexpr int PT = F8 ? TQ_BF16 : QT;                      // of the value product
   constexpr int VT = F8 ? TQ_E4M3 : QT;                      // of the cache
   constexpr int SIZE = F8 ? 1 : 2, PAGES = 2, TB = 32;
