@@ -492,8 +492,8 @@ int tq_attend(const void *q, int dtype, int64_t rows, const int32_t *query_start
  *   y = x / sqrt(mean x^2 + eps) * weight (weight null: y = x);  pairs (i, i + rotary_dim / 2) of the first rotary_dim channels - interleaved: (2 i, 2 i + 1) - turn by
  *   positions[row] * inv_freq[i].
  * Element strides of tokens and heads, multiples of 4, channels contiguous, rows on 8-byte boundaries (fp32: 16); d a multiple of 8 up to 512, rotary_dim one up to d; positions
- * int32, or int64 with wide_positions; inv_freq (rotary_dim / 2) double; weights (d) `dtype`.  The outputs may be the inputs.  Either of the two may have
- * no heads.                                                                                                                     */
+ * int32, or int64 with wide_positions; inv_freq (rotary_dim / 2) double; weights (d) `dtype`.  q_out may be q and k_out k, with its strides; neither may lie over
+ * what else the call reads, the other input among it.  Either of the two may have no heads.                                      */
 int tq_rotate_heads(const void *q, const void *k, int dtype, int64_t rows, int Hq, int Hkv, int d, int64_t qs_t, int64_t qs_h, int64_t ks_t,
                     int64_t ks_h, const void *positions, int wide_positions, const double *inv_freq, int rotary_dim, int interleaved,
                     const void *q_weight, const void *k_weight, float eps, void *q_out, int64_t qo_t, int64_t qo_h, void *k_out, int64_t ko_t,

@@ -30,7 +30,8 @@ def rotate_heads(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
     r = 2 len(inv_freq) channels, or (2 i, 2 i + 1) if interleaved, turn by the angle position * inv_freq[i] (float64, `inverse_frequencies`), which is
     as good at position 2^20 as at 1.  All of it in 32 bits, rounded once.  Views of a fused projection are read where they are.
 
-    Returns new contiguous tensors, or out=(query, key), channels contiguous, which may be the inputs themselves."""
+    Returns new contiguous tensors, or out=(query, key), channels contiguous: each may be its own input (not the other, nor memory that the
+    other shares)."""
     fast = _ffi.native()
     if fast is not None and out is None:
         done = fast.rotate(query, key, positions, inv_freq, q_weight, k_weight, eps, interleaved)
@@ -70,18 +71,18 @@ def rotate_heads(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
         new = tuple(out)
         if len(new) != 2:
             raise ValueError("out must be two tensors, for query and key")
-        for t, old, name in zip(new, given, ("query", "key")):
+        for t, old, other, name in zip(new, given, given[::-1], ("query", "key")):
             if t.shape != old.shape or t.dtype != old.dtype or t.device != dev or not fits(t) or t.is_neg():
                 raise ValueError(f"out {name} must be like it: same shape, dtype and GPU, channels contiguous, rows on {align}-byte boundaries")
             _ffi.require_constant("rotate_heads", **{f"out {name}": t})
             if not own_rows(t):
                 raise ValueError(f"out {name} must not overlap itself")
-            for other in (query, key):
-                if overlaps(t, other) and not (other.data_ptr() == t.data_ptr() and other.stride() == t.stride() and other.shape == t.shape) and \
-                        not _beside(t, other):
-                    raise ValueError(f"out {name} must be the input itself or memory of its own")
-            for what, other in (("positions", positions), ("inv_freq", inv_freq), ("q_weight", q_weight), ("k_weight", k_weight)):
-                if other is not None and overlaps(t, other):
+            # (a head is read by the lanes that write it: over its own input only, and the other input's heads are read at other times)
+            itself = t.data_ptr() == old.data_ptr() and t.stride() == old.stride()
+            if any(overlaps(t, x) and not _beside(t, x) for x in ((other,) if itself else (old, other))):
+                raise ValueError(f"out {name} must be {name} itself or memory of its own")
+            for what, x in (("positions", positions), ("inv_freq", inv_freq), ("q_weight", q_weight), ("k_weight", k_weight)):
+                if x is not None and overlaps(t, x):
                     raise ValueError(f"out {name} overlaps {what}")
         if overlaps(*new) and not _beside(*new):
             raise ValueError("the two tensors of out must not overlap")
