@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from turboquant_amd import _ffi
+from turboquant_amd.fp8 import Fp8PagedCache
 from turboquant_amd.rotary import inverse_frequencies, rotate_heads
 
 
@@ -78,3 +79,33 @@ def test_outputs_beside_inputs_of_one_projection(calls):
         with pytest.raises(ValueError):
             rotate(q, k, out)
     assert len(calls) == 4
+
+
+# ---- rows and heads that are alone ------------------------------------------------------------------------------------------------
+
+def cache8(blocks=4, H=2, d=64):
+    k = torch.zeros(blocks, 16, H, d, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    s = torch.zeros(blocks, H, dtype=torch.uint8)
+    return Fp8PagedCache(k, k.clone(), s, s.clone())
+
+
+def step(*runs):
+    starts = torch.tensor([0, *runs]).cumsum(0).to(torch.int32)
+    return starts, torch.arange(4, dtype=torch.int32).expand(len(runs), 4).contiguous(), torch.tensor([max(1, r) for r in runs], dtype=torch.int32)
+
+
+@pytest.mark.parametrize("shape,strides", [((1, 2, 64), (1001, 64, 1)), ((3, 1, 64), (64, 7, 1)), ((1, 1, 64), (3, 5, 1))])
+def test_a_step_between_rows_that_nobody_takes(calls, shape, strides):
+    """torch calls a tensor contiguous whatever the stride of a dimension of one element: the library is not given it."""
+    x = torch.zeros(2048).as_strided(shape, strides)
+    cache = cache8(H=shape[1])
+    cache.write(x, x, *step(shape[0]))
+    rotate_heads(x, x, torch.arange(shape[0]), inverse_frequencies(64))
+    y, z = (torch.zeros(2048).as_strided(shape, strides) for _ in range(2))
+    got = rotate_heads(x, x.clone(), torch.arange(shape[0]), inverse_frequencies(64), out=(y, z))
+    assert got[0] is y and got[1] is z
+    rotate_heads(y, z, torch.arange(shape[0]), inverse_frequencies(64), out=(y, z))
+    at = {"tq_fp8_write": (4, 5, 6, 7), "tq_rotate_heads": (7, 8, 9, 10, 20, 21, 23, 24)}
+    for name, a in calls:
+        assert all(a[i] >= 0 and a[i] % 4 == 0 for i in at[name]), (name, [a[i] for i in at[name]])
+    assert len(calls) == 4 and calls[0][1][0] == x.data_ptr() and calls[2][1][0] == x.data_ptr()      # (read where it lies)

@@ -59,6 +59,11 @@ def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     return x[0] < y[1] and y[0] < x[1]
 
 
+def row_strides(t: torch.Tensor) -> tuple:
+    """Strides of tokens and heads (rows, H, d) as the library takes them: of a dimension of one element torch leaves any number, which nothing goes by."""
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:2], t.shape[:2]))
+
+
 def seen_by(window: Optional[int], sinks: int):
     """(window as the library takes it, sinks) of a call, checked."""
     if window is None:

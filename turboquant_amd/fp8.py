@@ -13,7 +13,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _ffi
-from .attend import HEAD_DIMS, attend, overlaps, plan_bytes, seen_by, sequences, step_starts
+from .attend import HEAD_DIMS, attend, overlaps, plan_bytes, row_strides, seen_by, sequences, step_starts
 from .eviction import own_rows
 from .paged import PAGE_TOKENS
 
@@ -109,7 +109,7 @@ class Fp8PagedCache:
         key, value = (self._rows_of(t) for t in (key, value))
         with _ffi.on_device(self.device):
             _ffi.check(_ffi.lib().tq_fp8_write(
-                key.data_ptr(), value.data_ptr(), tag, rows, *key.stride()[:2], *value.stride()[:2], starts.data_ptr(), B, self.num_kv_heads,
+                key.data_ptr(), value.data_ptr(), tag, rows, *row_strides(key), *row_strides(value), starts.data_ptr(), B, self.num_kv_heads,
                 self.head_dim, *self._memory(), *self._strides[:3], self.num_blocks, table.data_ptr(), bt_stride, lens.data_ptr(),
                 _ffi.stream_ptr(self.device)), "tq_fp8_write")
         _ffi.changed(*self.tensors().values())
@@ -119,7 +119,7 @@ class Fp8PagedCache:
         """Rows as the library reads them: channels contiguous, on 16-byte boundaries."""
         t = t.resolve_neg()
         piece = 16 // t.element_size()
-        if t.stride(2) != 1 or any(s < 0 or s % piece for s in t.stride()[:2]) or t.data_ptr() % 16:
+        if t.stride(2) != 1 or any(s % piece for s in row_strides(t)) or t.data_ptr() % 16:
             t = t.contiguous()
             if t.data_ptr() % 16:
                 t = t.clone()

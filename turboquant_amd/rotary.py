@@ -10,7 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _ffi
-from .attend import overlaps
+from .attend import overlaps, row_strides
 from .eviction import own_rows
 
 MAX_HEAD_DIM = 512
@@ -61,7 +61,7 @@ def rotate_heads(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
             raise ValueError(f"{name} must be ({d},) like the query: same dtype and GPU")
     _ffi.require_constant("rotate_heads", query=query, key=key, q_weight=q_weight, k_weight=k_weight, inv_freq=inv_freq)
     align = 16 if query.dtype == torch.float32 else 8
-    fits = lambda t: t.stride(2) == 1 and all(s >= 0 and s % 4 == 0 for s in t.stride()[:2]) and t.data_ptr() % align == 0
+    fits = lambda t: t.stride(2) == 1 and all(s % 4 == 0 for s in row_strides(t)) and t.data_ptr() % align == 0
     given = query, key
     query, key = (t if fits(t) else t.contiguous() for t in (query.resolve_neg(), key.resolve_neg()))
     query, key = (t if fits(t) else t.clone() for t in (query, key))
@@ -78,7 +78,7 @@ def rotate_heads(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
             if not own_rows(t):
                 raise ValueError(f"out {name} must not overlap itself")
             # (a head is read by the lanes that write it: over its own input only, and the other input's heads are read at other times)
-            itself = t.data_ptr() == old.data_ptr() and t.stride() == old.stride()
+            itself = t.data_ptr() == old.data_ptr() and row_strides(t) == row_strides(old)
             if any(overlaps(t, x) and not _beside(t, x) for x in ((other,) if itself else (old, other))):
                 raise ValueError(f"out {name} must be {name} itself or memory of its own")
             for what, x in (("positions", positions), ("inv_freq", inv_freq), ("q_weight", q_weight), ("k_weight", k_weight)):
@@ -92,9 +92,9 @@ def rotate_heads(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
         return new
     with _ffi.on_device(dev):
         _ffi.check(_ffi.lib().tq_rotate_heads(
-            query.data_ptr(), key.data_ptr(), tag, rows, Hq, H, d, *query.stride()[:2], *key.stride()[:2], positions.data_ptr(),
+            query.data_ptr(), key.data_ptr(), tag, rows, Hq, H, d, *row_strides(query), *row_strides(key), positions.data_ptr(),
             int(positions.dtype == torch.int64), inv_freq.data_ptr(), r, int(bool(interleaved)), _ffi.ptr(q_weight), _ffi.ptr(k_weight), float(eps),
-            new[0].data_ptr(), *new[0].stride()[:2], new[1].data_ptr(), *new[1].stride()[:2], _ffi.stream_ptr(dev)), "tq_rotate_heads")
+            new[0].data_ptr(), *row_strides(new[0]), new[1].data_ptr(), *row_strides(new[1]), _ffi.stream_ptr(dev)), "tq_rotate_heads")
     if out is not None:
         _ffi.changed(*new)
     return new
