@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from turboquant_amd import _ffi
+from turboquant_amd.exact import ExactPagedCache
 from turboquant_amd.fp8 import Fp8PagedCache
 from turboquant_amd.rotary import inverse_frequencies, rotate_heads
 
@@ -109,3 +110,72 @@ def test_a_step_between_rows_that_nobody_takes(calls, shape, strides):
     for name, a in calls:
         assert all(a[i] >= 0 and a[i] % 4 == 0 for i in at[name]), (name, [a[i] for i in at[name]])
     assert len(calls) == 4 and calls[0][1][0] == x.data_ptr() and calls[2][1][0] == x.data_ptr()      # (read where it lies)
+
+
+# ---- memory that a call writes and what it goes by ----------------------------------------------------------------------------------
+
+def over(t, like):
+    """A tensor like `like` in the memory of t."""
+    return t.view(-1).view(torch.uint8)[: like.numel() * like.element_size()].view(like.dtype).view(like.shape)
+
+
+def wide_step(ints=1 << 15):
+    """A step of two rows whose starts, table and lengths have memory enough behind them for an output or a workspace."""
+    starts, table, lens = (torch.zeros(ints, dtype=torch.int32) for _ in range(3))
+    return dict(query_start_loc=starts, block_table=table, seq_lens=lens), (starts[:3], table[:8].view(2, 4), lens[:2])
+
+
+@pytest.mark.parametrize("what", ["query_start_loc", "block_table", "seq_lens"])
+def test_attention_does_not_write_what_it_goes_by(calls, what):
+    held, args = wide_step()
+    cache, q = cache8(), torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    work = cache.workspace(2, 4, 64, B=2)
+    for call in (lambda **kw: cache.attention(q, *args, **kw), lambda **kw: cache.decode_attention(q, *args[1:], **kw)):
+        if what == "query_start_loc" and call(out=torch.zeros_like(q)) is not None and calls[-1][1][3] is None:
+            continue                                          # (a decode step has no starts)
+        for kw in (dict(out=over(held[what], q)), dict(workspace=over(held[what], work))):
+            n = len(calls)
+            with pytest.raises(ValueError):
+                call(**kw)
+            assert len(calls) == n
+        call(out=torch.zeros_like(q), workspace=work)
+        assert calls[-1][0] == "tq_attend"
+
+
+@pytest.mark.parametrize("what", ["query_start_loc", "block_table", "seq_lens"])
+def test_read_does_not_write_what_it_goes_by(calls, what):
+    held, args = wide_step()
+    cache, k = cache8(), torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    for out in ((over(held[what], k), k), (k, over(held[what], k))):
+        with pytest.raises(ValueError):
+            cache.read(*args, out=out)
+    assert not calls
+    cache.read(*args, out=(k, k.clone()))
+    assert calls[-1][0] == "tq_fp8_read"
+
+
+@pytest.mark.parametrize("what", [0, 1, 2])
+@pytest.mark.parametrize("part", ["key_cache", "value_scales"])
+def test_write_does_not_write_what_it_goes_by(calls, what, part):
+    cache = cache8()
+    starts, table, lens = step(1)
+    k = torch.zeros(1, 2, 64)
+    args = [starts, table[:, :2].contiguous(), lens]
+    args[what] = over(cache.tensors()[part], args[what])
+    with pytest.raises(ValueError):
+        cache.write(k, k, *args)
+    assert not calls
+
+
+@pytest.mark.parametrize("what", ["block_table", "seq_lens"])
+def test_exact_decode_does_not_write_what_it_goes_by(calls, what):
+    held, args = wide_step()
+    k = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    cache, q = ExactPagedCache(k, k.clone()), torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    work = cache.workspace(2, 4, 64)
+    for kw in (dict(out=over(held[what], q)), dict(workspace=over(held[what], work))):
+        with pytest.raises(ValueError):
+            cache.decode_attention(q, *args[1:], **kw)
+    assert not calls
+    cache.decode_attention(q, *args[1:], out=q, workspace=work)
+    assert calls[-1][0] == "tq_exact_decode"

@@ -115,6 +115,9 @@ def attend(what: str, cache, query: torch.Tensor, query_start_loc: Optional[torc
     if query_start_loc is not None:
         starts, B = step_starts(device, query_start_loc)
     table, bt_stride, lens = sequences(device, block_table, seq_lens, B)
+    goes_by = dict(block_table=table, seq_lens=lens)
+    if starts is not None:
+        goes_by["query_start_loc"] = starts
     if scale is None:
         scale = 1.0 / math.sqrt(d)
     query = query.contiguous().resolve_neg()
@@ -128,7 +131,7 @@ def attend(what: str, cache, query: torch.Tensor, query_start_loc: Optional[torc
     elif out.is_neg():
         raise ValueError("out is negated lazily: its memory does not hold its values")
     else:
-        for name, t in dict(query=query, **held).items():
+        for name, t in dict(query=query, **held, **goes_by).items():
             if overlaps(out, t):
                 raise ValueError(f"out must be memory of its own, it overlaps {name}")
     longest = table.shape[-1] * PAGE_TOKENS
@@ -142,7 +145,7 @@ def attend(what: str, cache, query: torch.Tensor, query_start_loc: Optional[torc
         workspace = torch.empty(need // 4, dtype=torch.float32, device=device)
     else:
         check_workspace(workspace, need, device)
-        for name, t in dict(query=query, out=out, **held).items():
+        for name, t in dict(query=query, out=out, **held, **goes_by).items():
             if overlaps(workspace, t):
                 raise ValueError(f"the workspace overlaps {name}")
     k, v, k_scales, v_scales = cache._memory()

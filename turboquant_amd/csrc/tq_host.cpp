@@ -779,6 +779,9 @@ PyObject* fp8_write(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
       for (const at::Tensor* held : {&c.k, &c.v, &c.ks, &c.vs})
         if (meet(*t, *held)) return nullptr;
     }
+    for (const at::Tensor* t : {&st.t, &s.table, &s.lens})
+      for (const at::Tensor* held : {&c.k, &c.v, &c.ks, &c.vs})
+        if (meet(*t, *held)) return nullptr;
     if (unlocked(g_lib.fp8_write, k.data_ptr(), v.data_ptr(), tag, k.size(0), k.stride(0), k.stride(1), v.stride(0), v.stride(1), st.data(), (int)st.B, (int)c.H,
                  (int)c.d, c.k.data_ptr(), c.v.data_ptr(), (uint8_t*)c.ks.data_ptr(), (uint8_t*)c.vs.data_ptr(), c.k.stride(0), c.k.stride(1), c.k.stride(2),
                  c.n, s.entries(), (int)s.stride, s.lengths(), p.stream()) != TQ_OK)

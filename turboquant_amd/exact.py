@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _ffi
-from .attend import attend, check_workspace, plan_bytes, seen_by, sequences
+from .attend import attend, check_workspace, overlaps, plan_bytes, seen_by, sequences
 from .eviction import Evictions, memory_of, own_rows
 from .paged import PAGE_TOKENS
 
@@ -125,7 +125,8 @@ class ExactPagedCache:
             raise ValueError("out is negated lazily: its memory does not hold its values")
         else:
             first, end = memory_of(out)
-            for name, t in (("query", query), ("weights", weights), ("key_cache", self.key_cache), ("value_cache", self.value_cache)):
+            for name, t in (("query", query), ("weights", weights), ("key_cache", self.key_cache), ("value_cache", self.value_cache), ("block_table", table),
+                            ("seq_lens", lens)):
                 if t is None or t.numel() == 0 or out.numel() == 0 or (t is query and t.data_ptr() == first):
                     continue                                     # (over the query itself: a row is read by those that write it, and before)
                 a, b = memory_of(t)
@@ -145,6 +146,9 @@ class ExactPagedCache:
             workspace = torch.empty(need // 4, dtype=torch.float32, device=self.device)
         else:
             check_workspace(workspace, need, self.device)
+            for name, t in dict(query=query, out=out, weights=weights, block_table=table, seq_lens=lens, **self.tensors()).items():
+                if t is not None and overlaps(workspace, t):
+                    raise ValueError(f"the workspace overlaps {name}")
         with _ffi.on_device(self.device):
             _ffi.check(_ffi.lib().tq_exact_decode(
                 query.data_ptr(), self._tag, B, Hq, self.num_kv_heads, d, self.key_cache.data_ptr(), self.value_cache.data_ptr(),

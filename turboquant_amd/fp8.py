@@ -103,6 +103,8 @@ class Fp8PagedCache:
         table, bt_stride, lens = sequences(self.device, block_table, seq_lens, B)
         if bt_stride < 0 and B > 1:
             raise ValueError(f"one table for {B} sequences: they would write to the same blocks")
+        if any(overlaps(t, held) for t in (starts, table, lens) for held in self.tensors().values()):
+            raise ValueError("query_start_loc, block_table and seq_lens must not lie in the cache's own memory")
         rows = key.shape[0]
         if rows == 0 or B == 0:
             return
@@ -151,6 +153,8 @@ class Fp8PagedCache:
                     raise ValueError(f"out must be two contiguous tensors ({'rows' if rows is None else rows}, {shape[0]}, {shape[1]}) of one dtype on the cache's GPU")
                 if any(overlaps(t, o) for o in self.tensors().values()):
                     raise ValueError("out must not lie in the cache's own memory")
+            if any(overlaps(t, o) for t in out for o in (starts, table, lens)):
+                raise ValueError("out must not lie over query_start_loc, block_table or seq_lens")
             if overlaps(keys, values):
                 raise ValueError("the two tensors of out must not overlap")
         _ffi.require_constant("read", keys=keys, values=values, **self.tensors())
