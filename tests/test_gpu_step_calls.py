@@ -1,0 +1,72 @@
+"""Calls of a step's operators that the documentation allows and that are easy to get wrong: no sequences, outputs in place, factors and blocks of no
+size, workspaces with old contents."""
+
+import math
+
+import pytest
+import torch
+
+from tests.step_helpers import DTYPES, Step
+from turboquant_amd import _ffi
+from turboquant_amd.rotary import inverse_frequencies, rotate_heads
+
+pytestmark = pytest.mark.gpu
+KINDS = {"bf16": (torch.bfloat16, torch.bfloat16), "fp16": (torch.float16, torch.float16), "fp8": ("fp8", torch.bfloat16), "fp8 fp16": ("fp8", torch.float16)}
+
+
+@pytest.fixture(params=["native", "python"])
+def side(request, monkeypatch):
+    if request.param == "python":
+        monkeypatch.setattr(_ffi, "native", lambda: None)
+    return request.param
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_a_step_of_no_sequence(gpu, side, kind):
+    """Rows of nobody: zeros, or left as they are in a given output; nothing is written."""
+    s = Step([20], [3], 2, 64, *KINDS[kind])
+    cache, q = s.cache(), s.query(4).to(gpu)
+    starts, table, lens = s.starts[:1], s.table[:0], s.seq_lens[:0]
+    for n_split in (None, 3):
+        kw = {} if n_split is None else dict(n_split=n_split, max_len=4000)
+        assert (cache.attention(q, starts, table, lens, **kw) == 0).all()
+        out = torch.full_like(q, 5)
+        assert (cache.attention(q, starts, table, lens, out=out, **kw) == 5).all()
+    if kind.startswith("fp8"):
+        k, v = cache.read(starts, table, lens, rows=3)
+        assert k.shape == (3, 2, 64) and (k == 0).all() and (v == 0).all()
+        held = [t.clone().view(torch.uint8) for t in cache.operands()]
+        cache.write(k, v, starts, table, lens)
+        assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(held, cache.operands()))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_rotation_in_place_with_as_many_heads(gpu, side, dtype):
+    """Each output over its own input, several rounds of heads a workgroup; the other way about is refused (tests/test_step_calls_host.py)."""
+    rows, H, d = 1030, 40, 128
+    g = torch.Generator().manual_seed(1)
+    q, k = (torch.randn(rows, H, d, generator=g).to(DTYPES[dtype]).to(gpu) for _ in range(2))
+    pos, f = torch.arange(rows, device=gpu), inverse_frequencies(d, device=gpu)
+    want = rotate_heads(q, k, pos, f)
+    for out in ((q.clone(), k.clone()), (torch.empty_like(q), k.clone())):
+        src = (out[0] if torch.equal(out[0], q) else q, out[1])
+        got = rotate_heads(*src, pos, f, out=out)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(ValueError):
+        rotate_heads(q, k, pos, f, out=(k, q))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_one_row_of_any_stride(gpu, side, dtype):
+    from turboquant_amd.fp8 import Fp8PagedCache
+    x = torch.randn(4096, generator=torch.Generator().manual_seed(2)).to(DTYPES[dtype]).to(gpu)
+    odd, even = x.as_strided((1, 2, 64), (1001, 64, 1)), x[:128].view(1, 2, 64).clone()
+    pos, f = torch.tensor([12345], device=gpu), inverse_frequencies(64, device=gpu)
+    assert all(torch.equal(a, b) for a, b in zip(rotate_heads(odd, odd, pos, f), rotate_heads(even, even, pos, f)))
+    starts, table, lens = (torch.tensor(t, dtype=torch.int32, device=gpu) for t in ([0, 1], [[1]], [7]))
+    held = []
+    for t in (odd, even):
+        cache = Fp8PagedCache.allocate(2, 2, 64, gpu)
+        cache.write(t, t, starts, table, lens)
+        held.append(cache)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(held[0].operands(), held[1].operands())) and held[0].key_scales.any()

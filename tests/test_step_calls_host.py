@@ -179,3 +179,15 @@ def test_exact_decode_does_not_write_what_it_goes_by(calls, what):
     assert not calls
     cache.decode_attention(q, *args[1:], out=q, workspace=work)
     assert calls[-1][0] == "tq_exact_decode"
+
+
+# ---- a step of no sequence ------------------------------------------------------------------------------------------------------------
+
+def test_a_step_of_no_sequence_has_no_table():
+    """Its table has no rows, so no memory: the rows are nobody's and become zeros.  (Refusals that come after the table's, so that nothing is launched.)"""
+    from tests.test_step_host import attend_args, read_args, write_args
+    lib = _ffi.lib()
+    none = dict(B=0, table=None, lens=None)
+    assert lib.tq_attend(*attend_args(**none, kc=1 << 20 | 8)) == -2 and lib.tq_fp8_read(*read_args(**none, kc=1 << 20 | 8)) == -2
+    assert lib.tq_fp8_write(*write_args(**none, kc=1 << 20 | 8)) == -2
+    assert lib.tq_attend(*attend_args(**none, rows=0)) == 0 and lib.tq_fp8_read(*read_args(**none, rows=0)) == 0

@@ -130,7 +130,7 @@ __device__ __forceinline__ uint32_t __attribute__((ext_vector_type(4))) step_ent
 
 // what the entry points check of a step, and its description
 inline int step_init(Step* s, const int32_t* starts, int64_t rows, int B, const int32_t* lens, const int32_t* table, int bt_stride, int64_t num_blocks) {
-  if (!table || (!lens && B > 0)) return TQ_ENULL;
+  if ((!table || !lens) && B > 0) return TQ_ENULL;           // (no sequence: nobody looks at either)
   if (B < 0 || rows < 0 || rows > INT32_MAX || num_blocks <= 0 || bt_stride == 0 || bt_stride == INT32_MIN) return TQ_EINVAL;
   s->starts = starts; s->lens = lens; s->table = table; s->rows = rows; s->B = B; s->num_blocks = num_blocks;
   s->table_row = bt_stride < 0 ? -bt_stride : bt_stride;
