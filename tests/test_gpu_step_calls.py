@@ -70,3 +70,22 @@ def test_one_row_of_any_stride(gpu, side, dtype):
         cache.write(t, t, starts, table, lens)
         held.append(cache)
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(held[0].operands(), held[1].operands())) and held[0].key_scales.any()
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("G,runs", [(4, [1, 1]), (4, [3, 2]), (16, [2, 1]), (8, [40, 5])])
+@pytest.mark.parametrize("scale", [1e-12, -1e-12, 1e-30, 1e-38])
+def test_factors_of_no_size(gpu, kind, d, G, runs, scale):
+    """Keys of zeros, whose 8-bit scales are the smallest there are, times a factor so small that the two are nothing together: all visible tokens
+    have the same weight, and those behind the rows none."""
+    s = Step([37, 70], runs, 2, d, *KINDS[kind])
+    for b, n in enumerate(s.lens):
+        blocks = s.table_cpu[b, : (n + 15) // 16].long()
+        s.q[0].view(torch.uint8)[blocks.to(gpu)] = 0
+        s.k64[blocks] = 0
+        if kind.startswith("fp8"):
+            s.scales[0][blocks.to(gpu)] = 10 if b else 0
+    q = s.query(2 * G)
+    s.check(q, s.cache().attention(q.to(gpu), s.starts, s.table, s.seq_lens, scale=scale), scale)
+    s.check(q, s.cache().attention(q.to(gpu), s.starts, s.table, s.seq_lens, scale=scale, window=20, sinks=3), scale, 20, 3)

@@ -218,6 +218,7 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT, APART>())) a
 #pragma unroll
       for (int p = 0; p < PAGES; ++p) {
         k_scale[p] = scale * f8_scale((uint32_t)__builtin_amdgcn_readlane((int)now.scales, p));
+        if constexpr (LATER) k_scale[p] = fmaxf(k_scale[p], 0x1p-149f);      // (two small ones may be nothing together, and nothing times a masked score's -inf is NaN)
         v_scale[p] = f8_scale((uint32_t)__builtin_amdgcn_readlane((int)now.scales, 2 + p));
       }
     }
