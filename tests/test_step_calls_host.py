@@ -191,3 +191,31 @@ def test_a_step_of_no_sequence_has_no_table():
     assert lib.tq_attend(*attend_args(**none, kc=1 << 20 | 8)) == -2 and lib.tq_fp8_read(*read_args(**none, kc=1 << 20 | 8)) == -2
     assert lib.tq_fp8_write(*write_args(**none, kc=1 << 20 | 8)) == -2
     assert lib.tq_attend(*attend_args(**none, rows=0)) == 0 and lib.tq_fp8_read(*read_args(**none, rows=0)) == 0
+
+
+# ---- workspaces -----------------------------------------------------------------------------------------------------------------------------
+
+MIB = 1 << 20
+
+
+@pytest.mark.parametrize("call,most", [
+    # single tokens of 256 sequences in a wide table: 0.27 GB are four splits of 256 x 32 rows of 128 channels 16 times over
+    (dict(cache=3, starts=0, rows=256, B=256, Hq=32, Hkv=32, d=128, max_len=131072), 80), (dict(cache=2, starts=0, rows=256, B=256, Hq=16, Hkv=16, d=256, max_len=131072), 80),
+    (dict(cache=3, starts=0, rows=256, B=256, Hq=32, Hkv=8, d=128, max_len=131072), 80), (dict(cache=3, starts=0, rows=300, B=300, Hq=32, Hkv=32, d=128, max_len=1 << 20), 80),
+    # three drafted rows each
+    (dict(cache=3, rows=768, B=256, Hq=16, Hkv=16, d=256, max_len=131072, max_rows=3), 160), (dict(cache=2, rows=768, B=256, Hq=64, Hkv=8, d=256, max_len=131072, max_rows=3), 400),
+    # prompts: what is shared out anew is bounded whatever the number of rows, and a large part of the output only where that is small
+    (dict(cache=3, rows=4096, B=2, Hq=32, Hkv=8, d=128, max_len=8192, max_rows=2048), 80), (dict(cache=2, rows=64 * 2048, B=64, Hq=32, Hkv=8, d=128, max_len=6144, max_rows=2048), 120),
+    (dict(cache=2, rows=64 * 2048, B=64, Hq=32, Hkv=8, d=256, max_len=1 << 20, max_rows=2048), 200),
+    # nothing to share
+    (dict(cache=2, rows=8192, B=1, Hq=32, Hkv=8, d=128, max_len=8192, max_rows=8192), 1), (dict(cache=3, starts=0, rows=256, B=256, Hq=32, Hkv=8, d=128, max_len=300), 1)])
+def test_workspaces_are_bounded(call, most):
+    """By the rows of the step times their splits, and by what is shared out anew: less than 2 x 1024 workgroups' rows (many rows: 2 x 512 of 128)."""
+    a = {**dict(dtype=2, cache=2, starts=1, rows=0, B=0, Hq=0, Hkv=0, d=0, max_len=0, max_rows=1, window=0, sinks=0, n_split=0), **call}
+    assert 0 < _ffi.lib().tq_attend_bytes(*a.values()) <= most * MIB, _ffi.lib().tq_attend_bytes(*a.values()) / MIB
+
+
+def test_a_wider_table_takes_no_more_for_ever():
+    """A workspace does not grow with the bound of the lengths once there are workgroups enough."""
+    need = lambda B, n: _ffi.lib().tq_attend_bytes(2, 3, 0, B, B, 32, 8, 128, n, 1, 0, 0, 0)
+    assert need(64, 1 << 17) == need(64, 1 << 20) and need(300, 1 << 15) == need(300, 1 << 24)

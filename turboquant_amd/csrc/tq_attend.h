@@ -25,11 +25,13 @@ struct Attend {
   float scale2;                            // scale x log2 e: the softmax is one of powers of two
   int32_t units;                           // units that the plan has room for
   int32_t items;                           // (unit, split) pairs that the grid has room for, for each KV head
-  // Partial results, where a row may have several: a workgroup's own (M rows), and of every row the first of its workgroups, how many there are, which of a
-  // workgroup's rows it is and how far they are apart.  0 of them: a row of no sequence; 1: it is in `out` already.
-  float* acc;                              // (workgroups, M, d): numerators
-  float2* ml;                              // (workgroups, M): maximum (log2) and sum
-  int2* shares;                            // (rows, Hq): first, number | row << 16 | planned << 24; null: all rows have one
+  // Partial results, where a row may have several, and of every row how many: 0 where it is no sequence's, 1 where it is in `out` already.  As planned, a row has n_split
+  // places of its own.  Shared out anew, a workgroup has `part` places, if its unit is split at all: for a KV head there are less than 2 target such shares, since a unit is
+  // split only if it has more blocks than a share, of which all units have `target`.
+  float* acc;                              // (places, d): numerators
+  float2* ml;                              // (places): maximum (log2) and sum
+  int2* shares;                            // (rows, Hq): shared out anew the first of its workgroups; number | row in the unit << 16 | planned << 24; null: all rows have one
+  int32_t part, parts;                     // rows that a unit has at most; workgroups of split units that there is room for, for each KV head
 };
 
 // Infinities and NaN among the values.  A row's weights are 0 where it sees nothing, and 0 times them is NaN: where the rows of a unit see different tokens
@@ -64,7 +66,7 @@ struct AttendUnit {
   int tokens;              // up to the last's own token, as far as the table goes
   int split, splits;       // which share, of how many (before it is known how many there are tokens for)
   bool planned;            // shares as the host planned them
-  int apart;               // items from one share to the next
+  int place;               // shared out anew: which of the shares of split units it is
 };
 // Blocks of TB tokens that a unit sees any token of: `front` from token 0 on (sinks), then from `from` on
 template <int TB>
@@ -132,7 +134,7 @@ __device__ __forceinline__ bool attend_item(const Attend& a, int n, AttendUnit* 
   int u = n - t->split * a.units;                            // of the units, as planned
   t->planned = true;
   t->splits = a.n_split;
-  t->apart = a.units;
+  t->place = 0;
   if (!a.s.starts && a.target == 0) {
     if (t->split >= a.n_split) return false;
     const int per = (a.G + M - 1) / M;
@@ -183,8 +185,14 @@ __device__ __forceinline__ bool attend_item(const Attend& a, int n, AttendUnit* 
             return false;
           }
           t->splits = __builtin_amdgcn_readfirstlane(splits(attend_most<M, TB>(a, run)));
-          t->apart = 1;
           t->split = unit % t->splits;
+          if (t->splits > 1) {
+            int split[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) split[i] = splits(blocks[i]) > 1 ? count[i] : 0;
+            t->place = __builtin_amdgcn_readfirstlane(step_before(a.s, split, t->b) + unit);
+            if (t->place - t->split + t->splits > a.parts) return false;      // (starts that do not ascend: more than there may be)
+          }
           unit = unit / t->splits;
           break;
         }
@@ -220,6 +228,13 @@ struct AttendShare {
     last = first + per < count ? first + per : count;
   }
 };
+// Where the partial result of a unit's row r lies, `row` of the step's rows x heads; and what the join is told of a row
+__device__ __forceinline__ int64_t attend_place(const Attend& a, const AttendUnit& u, int h, int r, int64_t row) {
+  return u.planned ? row * a.n_split + u.split : ((int64_t)u.place * a.H + h) * a.part + r;
+}
+__device__ __forceinline__ int2 attend_told(const Attend& a, const AttendUnit& u, int h, int r, int used) {
+  return make_int2(u.place * a.H + h, used | r << 16 | (u.planned ? 1 << 24 : 0));
+}
 // Items behind the last sequence's, of which this is number `number` of `others`: rows of no sequence, KV head h's part of them
 template <int D>
 __device__ __forceinline__ void attend_rest(const Attend& a, int h, int number, int64_t others) {

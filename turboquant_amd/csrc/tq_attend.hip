@@ -12,20 +12,25 @@ struct AttendJoin {
   const float* acc;
   void* out;
   int64_t rows;            // token rows x heads
-  int32_t M, H, d, few, units, grid, most;      // (units of the plan, workgroups, splits of a row)
+  int32_t H, d, few, n_split, part, parts, cap;
 };
 
 // A row's shares, and where they lie.  (Rows whose starts do not ascend may have been nobody's work: what lies in their place is no share.)
 struct AttendRow {
   int used;
   int64_t first, apart;
-  __device__ __forceinline__ AttendRow(const AttendJoin& a, const int2& s) {
-    const int r = s.y >> 16 & 0xff;
-    const int64_t between = (int64_t)(s.y >> 24 ? a.units : 1) * a.H;
+  __device__ __forceinline__ AttendRow(const AttendJoin& a, const int2& s, int64_t row) {
     used = s.y & 0xffff;
-    if (used > a.most || r >= a.M || s.x < 0 || s.x + (used - 1) * between >= a.grid) used = 0;
-    first = (int64_t)s.x * a.M + r;
-    apart = between * a.M;
+    if (s.y >> 24) {
+      if (used > a.n_split) used = 0;
+      first = row * a.n_split;
+      apart = 1;
+    } else {
+      const int r = s.y >> 16 & 0xff;
+      if (used > a.cap || r >= a.part || s.x < 0 || s.x + (int64_t)(used - 1) * a.H >= (int64_t)a.parts * a.H) used = 0;
+      first = (int64_t)s.x * a.part + r;
+      apart = (int64_t)a.H * a.part;
+    }
   }
 };
 
@@ -43,7 +48,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendJoin a) {
     // (fewer than two: there already, or a row of no sequence)
     for (uint64_t left = __ballot((mine.y & 0xffff) > 1); left; left &= left - 1) {
       const int i = __ffsll((unsigned long long)left) - 1;
-      const AttendRow r(a, make_int2(__builtin_amdgcn_readlane(mine.x, i), __builtin_amdgcn_readlane(mine.y, i)));
+      const AttendRow r(a, make_int2(__builtin_amdgcn_readlane(mine.x, i), __builtin_amdgcn_readlane(mine.y, i)), row0 + i);
       if (r.used < 2) continue;
       const float2 ml = lane < r.used ? a.ml[r.first + lane * r.apart] : make_float2(-INFINITY, 0.0f);
       join_few<DT, 16>(a.acc + r.first * a.d, r.apart * a.d, a.d, a.out, row0 + i, r.used, ml);
@@ -52,7 +57,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendJoin a) {
     const int slices = a.d >> 6;
     const int64_t row = blockIdx.x / (unsigned)slices;
     const int2 s = a.shares[row];
-    const AttendRow r(a, make_int2(__builtin_amdgcn_readfirstlane(s.x), __builtin_amdgcn_readfirstlane(s.y)));
+    const AttendRow r(a, make_int2(__builtin_amdgcn_readfirstlane(s.x), __builtin_amdgcn_readfirstlane(s.y)), row);
     if (r.used < 2) return;
     join_many<DT>(a.ml + r.first, r.apart, a.acc + r.first * a.d, r.apart * a.d, a.d, a.out, row, r.used, (int)(blockIdx.x % (unsigned)slices), s_f, s_red, s_o);
   }
@@ -62,7 +67,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendJoin a) {
 struct AttendPlan {
   int tiles;                          // column tiles of the kernel of few rows; 0: the kernel of many
   int64_t units, items, grid;
-  int M, n_split, chunk, target, cap, few;
+  int n_split, chunk, target, cap, few, part, parts;
   size_t shares_at, ml_at, acc_at, bytes;
 };
 
@@ -116,10 +121,11 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
     if (p->tiles) {
       // Workgroups enough for the bytes that have to be on their way: one for each compute unit where a turn of its four wavefronts is 64 KB, two where it
       // is less (us; fp8, d 128, 8 heads, one sequence of 131072: 32 splits 67.7, 64 64.4, 128 65.4, 256 65.0; d 256, 2 heads: 64 47.6, 128 36.6, 256 38.5, 384 46.6;
-      // bf16, d 128, one of 65536: 16 75.7, 32 53.7, 64 58.5), no split of more than 2048 tokens (fp8, 32 of 8192: 1 138, 2 114.6, 4 106.4, 8 105.2), and of
-      // the next numbers of splits, while they leave 512 tokens, the first that leaves no compute unit without work in its last round (24 of 6000: 3 70.9, 4 62.9).
+      // bf16, d 128, one of 65536: 16 75.7, 32 53.7, 64 58.5), no split of more than 2048 tokens (fp8, 32 of 8192: 1 138, 2 114.6, 4 106.4, 8 105.2) as long as that makes no more
+      // than 4096 workgroups or four splits (d 128, splits of 2048 / so: fp8, 8 heads, 32 of 65536 752 / 737, 64 of 65536 1504 / 1449, 128 of 32768 1558 / 1481; 16 heads, 256 of 4096, one split 860, two 780,
+      // four 742), and of the next numbers of splits, while they leave 512 tokens, the first that leaves no compute unit without work in its last round (24 of 6000: 3 70.9, 4 62.9).
       const int64_t turn = 4 * TB * 2 * d * (cache == TQ_E4M3 ? 1 : 2), target = turn >= 65536 ? 256 : 512;
-      n = std::max((target + pairs - 1) / pairs, (tokens + 2047) / 2048);
+      n = std::max((target + pairs - 1) / pairs, std::min((tokens + 2047) / 2048, std::max<int64_t>(4, 4096 / pairs)));
       double best = 0;
       for (int64_t i = n; i <= 2 * n && i <= std::max(n, tokens / 512); ++i) {
         const double full = double(pairs * i) / (256 * ((pairs * i + 255) / 256));
@@ -134,7 +140,6 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   n = std::max<int64_t>(1, std::min(n, blocks));
   int64_t chunk = (blocks + n - 1) / n;
   if (!given && p->tiles) chunk = (chunk + 3) & ~(int64_t)3;                       // (a block for each of the four wavefronts)
-  p->M = M;
   p->units = units;
   p->n_split = (int)std::max<int64_t>(1, (blocks + chunk - 1) / chunk);
   p->chunk = (int)chunk;
@@ -158,10 +163,15 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   p->few = most <= JOIN_FEW || (many && most <= 64) ? (p->tiles || p->n_split > 1 ? 1 : (int)std::min<int64_t>(8, std::max<int64_t>(1, rows * Hq / 16384))) : 0;
   const size_t all = (size_t)rows * Hq;
   p->grid = p->items * Hkv;
+  // Partial results: as planned, each row's splits; shared out anew, those of split units (Attend), of which there are 2 target at most, and no more than all units have.
+  // (4: total and its share are rounded.)
+  p->part = (int)std::min<int64_t>(M, starts ? rows * G : G);
+  p->parts = p->target ? (int)std::min<int64_t>(2 * p->target + 4, units * p->cap) : 0;
+  const size_t places = most > 1 ? std::max(p->n_split > 1 ? all * p->n_split : 0, (size_t)p->parts * Hkv * p->part) : 0;
   size_t at = 0;
   p->shares_at = at;  at = round256(at + (most > 1 ? all * sizeof(int2) : 0));
-  p->ml_at = at;      at = round256(at + (most > 1 ? (size_t)p->grid * M * sizeof(float2) : 0));
-  p->acc_at = at;     at = round256(at + (most > 1 ? (size_t)p->grid * M * d * sizeof(float) : 0));
+  p->ml_at = at;      at = round256(at + places * sizeof(float2));
+  p->acc_at = at;     at = round256(at + places * d * sizeof(float));
   p->bytes = std::max<size_t>(at, 256);
   return p->grid <= INT32_MAX && (int64_t)all * (d / 64) <= INT32_MAX;
 }
@@ -202,6 +212,7 @@ extern "C" int tq_attend(const void* q, int dtype, int64_t rows, const int32_t* 
   a.target = p.target; a.cap = p.cap; a.units = (int32_t)p.units; a.items = (int32_t)p.items; a.share = p.target ? 1.0f / p.target : 0.0f;
   const bool joined = std::max(p.n_split, p.cap) > 1;
   a.shares = joined ? (int2*)((char*)workspace + p.shares_at) : nullptr;
+  a.part = p.part; a.parts = p.parts;
   a.ml = (float2*)((char*)workspace + p.ml_at);
   a.acc = (float*)((char*)workspace + p.acc_at);
   hipStream_t st = (hipStream_t)stream;
@@ -215,7 +226,7 @@ extern "C" int tq_attend(const void* q, int dtype, int64_t rows, const int32_t* 
     else rc = dtype == TQ_F16 ? launch_attend_rows<TQ_F16, false>(a, g, st) : launch_attend_rows<TQ_BF16, false>(a, g, st);
   }
   if (rc || !joined) return rc;
-  const AttendJoin j{a.shares, a.ml, a.acc, out, rows * Hq, p.M, Hkv, d, p.few, (int)p.units, (int)p.grid, std::max(p.n_split, p.cap)};
+  const AttendJoin j{a.shares, a.ml, a.acc, out, rows * Hq, Hkv, d, p.few, p.n_split, p.part, p.parts, p.cap};
   const dim3 grid((unsigned)(p.few ? (j.rows + 4 * p.few - 1) / (4 * p.few) : j.rows * (d / 64))), block(256);
   if (dtype == TQ_F16) attend_join_kernel<TQ_F16><<<grid, block, 0, st>>>(j);
   else attend_join_kernel<TQ_BF16><<<grid, block, 0, st>>>(j);

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT, APART>())) a
   }
   // Which KV head: not the same for all that a compute unit has at a time (as planned, shares of one unit), whose addresses would all be the same in the bits
   // that tell heads apart.  32 sequences of 8192, 8 heads of 128, 8 bits: 122 us with head x, 119 with x + unit, 107 so.
-  const int h = (int)((unsigned)(x + (u.planned ? u.split : item) * (paired ? 2 : 1)) % (unsigned)a.H), place = item * a.H + h;
+  const int h = (int)((unsigned)(x + (u.planned ? u.split : item) * (paired ? 2 : 1)) % (unsigned)a.H);
   const AttendBlocks<TB> list(a, u);
   const AttendShare share(a, u, list.count);
   if (u.split >= share.used) return;
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT, APART>())) a
   if (a.shares && u.split == 0 && wave == 0 && quarter == 0) {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
-      if (live[n]) a.shares[row[n]] = make_int2(place, share.used | (n * 16 + col) << 16 | (u.planned ? 1 << 24 : 0));
+      if (live[n]) a.shares[row[n]] = attend_told(a, u, h, n * 16 + col, share.used);
   }
   const int32_t* table = a.s.table + u.b * a.s.table_step;
 
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(256, (attend_few_waves<F8, D, NT, APART>())) a
     if (wave == 0 && live[n]) {
 #pragma unroll
       for (int t = 0; t < TILES; ++t) O[n][t] += s_acc[0][t][lane];
-      const int64_t slot = (int64_t)place * (16 * NT) + n * 16 + col;
+      const int64_t slot = attend_place(a, u, h, n * 16 + col, row[n]);
       if (share.used > 1 && quarter == 0) a.ml[slot] = make_float2(M - ex_lift<PT>(), sum);
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       float* acc = a.acc + slot * D;

@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
   // of 192 1031 -> 1228)
   const unsigned turn_of = blockIdx.x / (unsigned)a.H;
   const int h = (int)(blockIdx.x - turn_of * (unsigned)a.H);
-  const int item = a.items - 1 - (int)turn_of, place = item * a.H + h;
+  const int item = a.items - 1 - (int)turn_of;
   AttendUnit u;
   int over, others;
   if (!attend_item<M, ROWS_TOKENS>(a, item, &u, &over, &others)) {
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
   const bool live = r < u.rows;
   const int64_t row = (u.row + token) * a.Hq + h * a.G + (x - token * a.G);
   const int at_p = u.low + (token - u.first / a.G), behind = attend_behind(a, at_p);
-  if (a.shares && u.split == 0 && half == 0 && live) a.shares[row] = make_int2(place, share.used | r << 16 | (u.planned ? 1 << 24 : 0));
+  if (a.shares && u.split == 0 && half == 0 && live) a.shares[row] = attend_told(a, u, h, r, share.used);
   // the wavefront's first and last positions
   const int r0 = wave * 32, r1 = r0 + 31;
   const bool busy = r0 < u.rows;
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
   const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
   const float sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
   if (!live) return;
-  const int64_t slot = (int64_t)place * M + r;
+  const int64_t slot = attend_place(a, u, h, r, row);
   if (share.used > 1 && half == 0) a.ml[slot] = make_float2(m - ex_lift<PT>(), sum);
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   float* acc = a.acc + slot * D;

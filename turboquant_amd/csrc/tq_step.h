@@ -102,6 +102,17 @@ __device__ __forceinline__ bool step_find(const Step& s, int base, const StepRun
   }
   return false;
 }
+// How many units the sequences in front of sequence b have, of a step's first round.
+__device__ __forceinline__ int step_before(const Step& s, const int (&count)[4], int b) {
+  int before = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i * 64 > b) break;
+    const int upto = step_sums(count[i]), in = b - i * 64 < 64 ? b - i * 64 : 63;
+    before += __builtin_amdgcn_readlane(upto, in) - (b - i * 64 < 64 ? __builtin_amdgcn_readlane(count[i], in) : 0);
+  }
+  return before;
+}
 // Unit `u` of a step whose sequence b has count(b) of them: its sequence, which one of them it is and the sequence's rows; false (and u less all of them) if there are fewer.
 // A whole wavefront asks; u is the same in all lanes.
 template <class Count>
