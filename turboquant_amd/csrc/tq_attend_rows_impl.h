@@ -9,7 +9,8 @@
 //   values    O^T = V^T P^T: the contraction takes the tokens in the order in which a lane holds the weights already, so that no weight changes its lane;
 //             the transposing LDS read brings values in that order.
 // Weights are rounded once, to 16 bits, half a step of 2^-9 (fp16: 2^-12) that a sum over many averages out; a high and a low half, as the kernel of few
-// rows has them, would be half as many matrix instructions again.  8 bits for fp16 queries: bf16 values, whose range the block's scale
+// rows has them, would be half as many matrix instructions again.  Numerators and sum are of the same rounded weights, so that what all tokens' values have in common
+// comes out as it is (sums of the weights as they were before: 64 channels 288 -> 299 us, 256 1058 -> 1069, 128 and 192 the same).  8 bits for fp16 queries: bf16 values, whose range the block's scale
 // needs, and there the weights are two halves: one of bf16 would be eight times coarser than the output.
 // Instructions of a wavefront follow one another: those of the vector unit stand between the matrix instructions (weights and values of the next sixteen tokens
 // beside the product of these; 256 channels 1541 -> 1331 us), keys are read four ahead, and turns come in pairs, so that buffers are constants in addresses
@@ -41,6 +42,18 @@ __device__ __forceinline__ ro_f32x16 rows_mfma(ex_u32x4 a, ex_u32x4 b, ro_f32x16
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(ex_bf16x8, a), __builtin_bit_cast(ex_bf16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ex_f16x8, a), __builtin_bit_cast(ex_f16x8, b), c, 0, 0, 0);
+}
+
+// sum + both of two 16-bit numbers (fp16's small ones count)
+template <int DT>
+__device__ __forceinline__ float rows_add(uint32_t x, float sum) {
+  if constexpr (DT == TQ_BF16) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, x), b2{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, x), h2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+  }
 }
 
 constexpr int ROWS_TOKENS = 64;
@@ -389,9 +402,9 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
           const float x = __builtin_amdgcn_exp2f(fmaf(S[at >> 1][(at & 1) * 8 + i], f, -ref)), y = __builtin_amdgcn_exp2f(fmaf(S[at >> 1][(at & 1) * 8 + i + 1], f, -ref));
-          l += x;
-          l += y;
           if constexpr (HALVES) {
+            l += x;
+            l += y;
             uint32_t hi, lo;
             ex_split<PT>(x, y, &hi, &lo);
             P[at & 1][i >> 1] = hi;
@@ -410,6 +423,9 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
           values(at + 1);
           weights(at + 1);
         }
+        if constexpr (!HALVES)                               // (behind the next weights: right behind their own rounding 256 channels take 1081 us for 1069)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) l = rows_add<PT>(P[at & 1][i], l);
 #pragma unroll
         for (int ct = 0; ct < TILES; ++ct) {
           if constexpr (HALVES) O[ct] = rows_mfma<PT>(V[at & 1][ct], L[at & 1], O[ct]);
@@ -420,7 +436,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
           for (int ct = 0; ct < TILES; ++ct) {
             __builtin_amdgcn_sched_group_barrier(0x008, HALVES ? 2 : 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-            __builtin_amdgcn_sched_group_barrier(0x402, (28 + TILES - 1) / TILES, 0);
+            __builtin_amdgcn_sched_group_barrier(0x402, ((HALVES ? 28 : 20) + TILES - 1) / TILES, 0);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
