@@ -44,3 +44,15 @@ def test_values_that_are_all_the_same(gpu, kind, d, G, runs):
         assert torch.equal(got, want), f"off by {float(((got.double() - want.double()) / want.double()).abs().max()) * 2 ** 8:.3g} steps of bf16"
     got = s.cache().decode_attention(q[:3], s.table, s.seq_lens, window=1000).cpu()
     assert torch.equal(got, c.to(got.dtype).repeat_interleave(G, 0).expand_as(got))
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("G", [1, 16, 32, 33, 64, 128, 160])
+def test_decode_steps_lose_nothing_by_their_heads(gpu, kind, d, G):
+    """A decode step's weights are two halves whatever the number of heads on one."""
+    s = Step([1, 70, 333, 0], [1] * 4, 1, d, *KINDS[kind])
+    q = s.query(G)
+    for window, sinks in ((20, 3), (1000, 0)):
+        got = s.cache().decode_attention(q.to(gpu), s.table, s.seq_lens, window=window, sinks=sinks)
+        s.check(q, got, 1 / math.sqrt(d), window, sinks, weight_step=2.0 ** -21 if kind == "fp16" else 2.0 ** -15)

@@ -64,10 +64,10 @@ template <int D> constexpr int rows_lds() { return 2 * 2 * ROWS_TOKENS * D * 2; 
 template <int D> __device__ __forceinline__ int rows_key_turn(int t) { return D % 128 == 0 ? (t & 15) : ((t >> 1) & 7); }
 template <int D> __device__ __forceinline__ int rows_value_turn(int t) { return D % 128 == 0 ? (t & 3) << 2 : ((t >> 1) & 1) << 2; }
 
-template <int QT, bool F8, int D>
+// HALVES: weights go into the product as a high and a low half
+template <int QT, bool F8, int D, bool HALVES>
 __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(const Attend a) {
   constexpr int PT = F8 ? TQ_BF16 : QT;                      // of the value product
-  constexpr bool HALVES = F8 && QT == TQ_F16;                // weights in two halves
   constexpr bool FOLD = F8 && QT == TQ_BF16;                 // a key's scale goes into the key
   constexpr int VT = F8 ? TQ_E4M3 : QT;                      // of the cache
   constexpr int SIZE = F8 ? 1 : 2, ROW = D * 2;              // bytes of an element in the cache, of a row in LDS
@@ -506,13 +506,20 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
     }
 }
 
-template <int QT, bool F8, int D>
-int launch_attend_rows_d(const Attend& a, unsigned grid, hipStream_t stream) {
+template <int QT, bool F8, int D, bool HALVES>
+int launch_attend_rows_h(const Attend& a, unsigned grid, hipStream_t stream) {
   static std::atomic<uint64_t> ready{0};
-  if (const int rc = exact_allow_lds((const void*)attend_rows_kernel<QT, F8, D>, rows_lds<D>(), ready)) return rc;
-  attend_rows_kernel<QT, F8, D><<<dim3(grid), dim3(256), rows_lds<D>(), stream>>>(a);
+  if (const int rc = exact_allow_lds((const void*)attend_rows_kernel<QT, F8, D, HALVES>, rows_lds<D>(), ready)) return rc;
+  attend_rows_kernel<QT, F8, D, HALVES><<<dim3(grid), dim3(256), rows_lds<D>(), stream>>>(a);
   TQ_CHECK_LAUNCH();
   return TQ_OK;
+}
+// Two halves for fp16 queries over 8 bits, and for a decode step's, so that its results are as good with dozens of heads on one as with a few (bf16, 32 sequences of 8192, 64 heads on one of
+// 128 33.1 -> 34.6 us, 128 heads 43.7 -> 52.1; 16 of 8192, 128 on 2 of 256 59.8 -> 70.3).
+template <int QT, bool F8, int D>
+int launch_attend_rows_d(const Attend& a, unsigned grid, hipStream_t stream) {
+  if ((F8 && QT == TQ_F16) || !a.s.starts) return launch_attend_rows_h<QT, F8, D, true>(a, grid, stream);
+  return launch_attend_rows_h<QT, F8, D, F8 && QT == TQ_F16>(a, grid, stream);
 }
 
 template <int QT, bool F8>
