@@ -219,3 +219,25 @@ def test_a_wider_table_takes_no_more_for_ever():
     """A workspace does not grow with the bound of the lengths once there are workgroups enough."""
     need = lambda B, n: _ffi.lib().tq_attend_bytes(2, 3, 0, B, B, 32, 8, 128, n, 1, 0, 0, 0)
     assert need(64, 1 << 17) == need(64, 1 << 20) and need(300, 1 << 15) == need(300, 1 << 24)
+
+
+# ---- hooks --------------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("window,hooks,warned", [(8, {}, [0, 1, 2]), (None, {}, []), (8, dict(exact_layers=1), [1, 2]), (8, dict(exact_layers=3), []), (0, {}, []), ((7, 0), {}, [0, 1, 2]),
+                                                 ((-1, -1), {}, []), ((-1, 3), {}, [0, 1, 2]), ("half", {}, [0, 1, 2])])
+def test_a_window_that_pages_do_not_honour_is_said(monkeypatch, caplog, window, hooks, warned):
+    from turboquant_amd.integration import batched, vllm as single
+    from turboquant_amd.integration.harness import MinimalRunner
+    monkeypatch.setattr(batched, "TurboQuantProd", lambda *a, **k: None)
+    monkeypatch.setattr(batched, "PagedKVPool", lambda *a, **k: None)
+    r = MinimalRunner(n_layers=3, hidden=32, num_heads=4, num_kv_heads=2, head_dim=64, ffn=32, vocab=10, batch=2, max_seq_len=32, device="cpu")
+    for lay in r.layers:
+        lay.attn.impl.sliding_window = window
+    before = single.get_mode()
+    try:
+        with caplog.at_level("WARNING"):
+            states = batched.install_batched_hooks(r, r.num_blocks, mode="hybrid", **hooks)
+    finally:
+        single.set_mode(before)
+    said = [m.getMessage() for m in caplog.records if "sliding window" in m.getMessage()]
+    assert len(said) == bool(warned) and all((name in said[0]) == (i in warned) for i, name in enumerate(states) if warned)

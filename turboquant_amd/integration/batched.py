@@ -83,6 +83,17 @@ def _window_of(name: str, impl) -> Tuple[Optional[int], int]:
     return window, sinks
 
 
+def _names_a_window(impl) -> bool:
+    """Whether a layer's backend has its queries see part of the tokens only, in whatever form it says so."""
+    window = getattr(impl, "sliding_window", None)
+    try:
+        if isinstance(window, (tuple, list)):
+            return any(int(x) >= 0 for x in window)
+        return window is not None and int(window) > 0
+    except (TypeError, ValueError, OverflowError):
+        return True
+
+
 @dataclass
 class BatchedLayerState:
     """One attention layer: its quantiser and the compressed pool that shadows the engine's blocks, or 8-bit blocks that do (neither: the layer stays exact)."""
@@ -394,14 +405,14 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
     only if its backend has do_kv_cache_update and its head size is a multiple of 64 up to 768.
 
     A backend's `sliding_window` (and `sink_tokens`) hold for exact and 8-bit layers (at those four head sizes); pages of two to four bits
-    are attended to as a whole."""
+    are attended to as a whole, which a warning says of layers whose backend names a window: their decode steps see more tokens in `hybrid` and `full_tq` than the backend's."""
     if exact_layers < 0 or fp8_layers < 0:
         raise ValueError(f"exact_layers and fp8_layers must not be negative, got {exact_layers} and {fp8_layers}")
     if exact_layers and no_alloc:
         raise ValueError("exact layers are answered from the engine's cache, which no_alloc leaves out")
     if fp8_layers and torch.device(model_runner.device).type != "cuda":
         raise ValueError(f"8-bit layers need a GPU, the model runs on {model_runner.device}")
-    layers = []
+    layers, whole = [], []
     for name, module in model_runner.compilation_config.static_forward_context.items():
         impl = getattr(module, "impl", None)
         if impl is None or getattr(impl, "num_kv_heads", None) is None or not hasattr(impl, "head_size"):
@@ -418,7 +429,12 @@ def install_batched_hooks(model_runner, num_blocks: int, key_bits: int = 3, valu
             sees = _window_of(name, impl)
             if int(impl.head_size) not in HEAD_DIMS and (idx >= exact_layers or sees[0] is not None):
                 raise ValueError(f"{name}: 8-bit layers and sliding windows take head sizes of {', '.join(map(str, HEAD_DIMS))}, got {int(impl.head_size)}")
+        elif _names_a_window(impl):
+            whole.append(name)
         layers.append((name, module, impl, sees))
+    if whole:
+        logger.warning("[TurboQuant] %d layers have a sliding window, which pages of two to four bits do not honour: %s (exact_layers and fp8_layers do)", len(whole),
+                       ", ".join(whole))
     _single.set_mode(mode)
     if initial_layers_key_bits is None:
         initial_layers_key_bits = min(key_bits + 1, 4)
