@@ -89,3 +89,39 @@ def test_factors_of_no_size(gpu, kind, d, G, runs, scale):
     q = s.query(2 * G)
     s.check(q, s.cache().attention(q.to(gpu), s.starts, s.table, s.seq_lens, scale=scale), scale)
     s.check(q, s.cache().attention(q.to(gpu), s.starts, s.table, s.seq_lens, scale=scale, window=20, sinks=3), scale, 20, 3)
+
+
+@pytest.mark.parametrize("lens,most", [([70, 300, 5], None), ([70, 300, 5], 64), ([70, 300, 0, 33], 1000), ([40], 1), ([], None), ([4200] + [20] * 30, None)])
+def test_ingesting_into_8_bits(gpu, lens, most):
+    """What the engine's blocks hold, the first tokens of every sequence: as one write of each sequence alone, and nothing else."""
+    from turboquant_amd.fp8 import Fp8PagedCache
+    from turboquant_amd.integration.batched import BatchedLayerState
+    s = Step(lens or [5], [1] * max(1, len(lens)), 2, 64, torch.bfloat16, torch.bfloat16)
+    kv = torch.stack([x.nan_to_num() for x in s.q])
+    state = BatchedLayerState(config=None, quantizer=None, pool=None, fp8=Fp8PagedCache.allocate(s.blocks, 2, 64, gpu))
+    state.ingest_paged_cache(kv, s.table, torch.tensor(lens, dtype=torch.int32), max_tokens=most)
+    want = Fp8PagedCache.allocate(s.blocks, 2, 64, gpu)
+    took = [n if most is None else min(n, most) for n in lens]
+    for b, n in enumerate(took):
+        t = torch.arange(n)
+        at = s.table_cpu[b, t // 16].long().to(gpu), (t % 16).to(gpu)
+        step = torch.tensor([0, n, n], dtype=torch.int32, device=gpu)
+        want.write(kv[0][at], kv[1][at], step[:2], s.table[b: b + 1], step[2:])
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(state.fp8.operands(), want.operands()))
+    assert state.tokens_written == sum(took)
+
+
+def test_ingesting_more_than_the_table_holds(gpu):
+    """Tokens without a block are left out."""
+    from turboquant_amd.fp8 import Fp8PagedCache
+    from turboquant_amd.integration.batched import BatchedLayerState
+    s = Step([40, 30], [1, 1], 2, 64, torch.bfloat16, torch.bfloat16)
+    kv = torch.stack([x.nan_to_num() for x in s.q])
+    table = torch.tensor([[2, -1, 1], [3, s.blocks, 0]], dtype=torch.int32, device=gpu)
+    held = []
+    for lens in ([48, 48], [1000, 50]):
+        state = BatchedLayerState(config=None, quantizer=None, pool=None, fp8=Fp8PagedCache.allocate(s.blocks, 2, 64, gpu))
+        state.ingest_paged_cache(kv, table, torch.tensor(lens))
+        held.append(state.fp8)
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(held[0].operands(), held[1].operands()))
+    assert [int(x) > 0 for x in held[0].key_scales[:, 0]][:4] == [True] * 4 and not held[0].key_scales[4:].any()

@@ -42,6 +42,7 @@ from __future__ import annotations
 import logging
 import math
 from dataclasses import dataclass
+from itertools import accumulate
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -144,26 +145,32 @@ class BatchedLayerState:
         """Compress what the engine's exact paged cache (2, num_blocks, 16, H_kv, d) already holds for the
         sequences of `block_table`: tokens [0, seq_lens[b]) of every sequence, read in place through the
         block table and written to the pages of the same numbers (the batch counterpart of
-        capture.py:187-217, without the gather copy)."""
+        capture.py:187-217, without the gather copy; 8-bit layers gather pieces of them).  max_tokens: the first tokens of every sequence only."""
         if not self.supports_hybrid:
             raise RuntimeError("an exact layer has no pages to write to")
         if self.fp8 is not None:
-            self._ingest_fp8(kv_cache, block_table, [int(n) for n in seq_lens.tolist()])
+            most = math.inf if max_tokens is None else max_tokens
+            self._ingest_fp8(kv_cache, block_table, [min(int(n), most) for n in seq_lens.tolist()])
             return
         self.pool.append_from_blocks(kv_cache[0], kv_cache[1], block_table, block_table, seq_lens,
                                      max_tokens=max_tokens)
         self.tokens_written += int(seq_lens.sum())
 
     def _ingest_fp8(self, kv_cache, block_table, lens) -> None:
-        """Sequence by sequence, 4096 tokens at a time (whole blocks: none is rounded twice), gathered from their blocks."""
-        for b, length in enumerate(lens):
-            for first in range(0, length, 4096):
-                n = min(4096, length - first)
-                t = torch.arange(first, first + n, device=block_table.device)
-                block, slot = block_table[b].long()[t // PAGE_TOKENS], t % PAGE_TOKENS
-                step = torch.tensor([0, n, first + n], dtype=torch.int32).to(block_table.device)
-                self.fp8.write(kv_cache[0][block, slot], kv_cache[1][block, slot], step[:2], block_table[b: b + 1], step[2:])
-                self.tokens_written += n
+        """All sequences together, whole blocks of each (none is rounded twice) up to 65536 rows in all, gathered from their blocks."""
+        B, device = len(lens), block_table.device
+        table, num_blocks = block_table[:B], kv_cache.shape[1]
+        piece = max(1, 65536 // PAGE_TOKENS // max(1, B)) * PAGE_TOKENS
+        for first in range(0, max(lens, default=0), piece):
+            runs = [max(0, min(n - first, piece)) for n in lens]
+            step = torch.tensor([0, *accumulate(runs), *(first + n for n in runs)], dtype=torch.int32).to(device)
+            starts, row = step[: B + 1], torch.arange(sum(runs), dtype=torch.int32, device=device)
+            b = torch.searchsorted(starts[1:].contiguous(), row, right=True)
+            t = (first + row - starts[b]).long()
+            # (tokens without a block read one that is there, and are not written)
+            block = table[b, (t // PAGE_TOKENS).clamp_max(table.shape[1] - 1)].long().clamp(0, num_blocks - 1)
+            self.fp8.write(kv_cache[0][block, t % PAGE_TOKENS], kv_cache[1][block, t % PAGE_TOKENS], starts, table, step[B + 1:])
+            self.tokens_written += sum(runs)
 
     # ---- read --------------------------------------------------------------------
     def _exact_tail(self, kv_cache, meta):
