@@ -241,3 +241,14 @@ def test_a_window_that_pages_do_not_honour_is_said(monkeypatch, caplog, window, 
         single.set_mode(before)
     said = [m.getMessage() for m in caplog.records if "sliding window" in m.getMessage()]
     assert len(said) == bool(warned) and all((name in said[0]) == (i in warned) for i, name in enumerate(states) if warned)
+
+
+def test_starts_without_memory(calls):
+    """A zero tensor of torch's own has an address of nothing, which the library takes for a step of single tokens: refused."""
+    none = torch._efficientzerotensor(3, dtype=torch.int32)
+    cache, q, k = cache8(), torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 2, 64)
+    _, table, lens = step(1, 1)
+    for call in (lambda: cache.attention(q, none, table, lens), lambda: cache.write(k, k, none, table, lens), lambda: cache.read(none, table, lens, rows=2)):
+        with pytest.raises(ValueError):
+            call()
+    assert not calls

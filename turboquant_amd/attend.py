@@ -40,6 +40,8 @@ def step_starts(device: torch.device, query_start_loc: torch.Tensor):
     """(starts, sequences): int32 on the cache's GPU, contiguous."""
     if query_start_loc.dim() != 1 or query_start_loc.shape[0] < 1:
         raise ValueError("query_start_loc must have one entry more than there are sequences")
+    if query_start_loc._is_zerotensor():
+        raise ValueError("query_start_loc must hold its values")
     return query_start_loc.to(device=device, dtype=torch.int32).contiguous().resolve_neg(), query_start_loc.shape[0] - 1
 
 
