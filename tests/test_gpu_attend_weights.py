@@ -56,3 +56,20 @@ def test_decode_steps_lose_nothing_by_their_heads(gpu, kind, d, G):
     for window, sinks in ((20, 3), (1000, 0)):
         got = s.cache().decode_attention(q.to(gpu), s.table, s.seq_lens, window=window, sinks=sinks)
         s.check(q, got, 1 / math.sqrt(d), window, sinks, weight_step=2.0 ** -21 if kind == "fp16" else 2.0 ** -15)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("runs", [[2, 1, 3, 2], [12, 40, 20, 33]])
+@pytest.mark.parametrize("n_split", [1, 3])
+def test_a_sequence_alone_has_the_same_bits(gpu, kind, runs, n_split):
+    """With a number of splits given, of the same tokens at most, and as many rows x heads that the same kernel answers (up to 16, up to 32, more), a sequence's rows do
+    not depend on who else is in the step."""
+    s = Step([500, 40, 77, 900], runs, 2, 64, *KINDS[kind])
+    q, cache, longest = s.query(6).to(gpu), s.cache(), s.table.shape[1] * 16
+    got = cache.attention(q, s.starts, s.table, s.seq_lens, n_split=n_split, max_rows=max(runs), max_len=longest)
+    at = 0
+    for b, run in enumerate(runs):
+        alone = torch.tensor([0, run], dtype=torch.int32, device=gpu)
+        one = cache.attention(q[at: at + run], alone, s.table[b: b + 1], s.seq_lens[b: b + 1], n_split=n_split, max_len=longest)
+        assert torch.equal(one, got[at: at + run]), b
+        at += run
