@@ -201,7 +201,9 @@ MIB = 1 << 20
 @pytest.mark.parametrize("call,most", [
     # single tokens of 256 sequences in a wide table: 0.27 GB are four splits of 256 x 32 rows of 128 channels 16 times over
     (dict(cache=3, starts=0, rows=256, B=256, Hq=32, Hkv=32, d=128, max_len=131072), 80), (dict(cache=2, starts=0, rows=256, B=256, Hq=16, Hkv=16, d=256, max_len=131072), 80),
-    (dict(cache=3, starts=0, rows=256, B=256, Hq=32, Hkv=8, d=128, max_len=131072), 80), (dict(cache=3, starts=0, rows=300, B=300, Hq=32, Hkv=32, d=128, max_len=1 << 20), 80),
+    (dict(cache=3, starts=0, rows=256, B=256, Hq=32, Hkv=8, d=128, max_len=131072), 80), (dict(cache=3, starts=0, rows=256, B=256, Hq=32, Hkv=32, d=128, max_len=1 << 24), 80),
+    # more sequences than are shared out anew, of which one may be far longer than the others: 256 MiB
+    (dict(cache=3, starts=0, rows=300, B=300, Hq=32, Hkv=32, d=128, max_len=1 << 20), 270), (dict(cache=2, rows=3000, B=1000, Hq=64, Hkv=8, d=256, max_len=1 << 20, max_rows=3), 800),
     # three drafted rows each
     (dict(cache=3, rows=768, B=256, Hq=16, Hkv=16, d=256, max_len=131072, max_rows=3), 160), (dict(cache=2, rows=768, B=256, Hq=64, Hkv=8, d=256, max_len=131072, max_rows=3), 400),
     # prompts: what is shared out anew is bounded whatever the number of rows, and a large part of the output only where that is small
@@ -218,7 +220,7 @@ def test_workspaces_are_bounded(call, most):
 def test_a_wider_table_takes_no_more_for_ever():
     """A workspace does not grow with the bound of the lengths once there are workgroups enough."""
     need = lambda B, n: _ffi.lib().tq_attend_bytes(2, 3, 0, B, B, 32, 8, 128, n, 1, 0, 0, 0)
-    assert need(64, 1 << 17) == need(64, 1 << 20) and need(300, 1 << 15) == need(300, 1 << 24)
+    assert need(64, 1 << 17) == need(64, 1 << 20) and need(300, 1 << 20) == need(300, 1 << 24)
 
 
 # ---- hooks --------------------------------------------------------------------------------------------------------------------------------------

@@ -125,7 +125,9 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
       // than 4096 workgroups or four splits (d 128, splits of 2048 / so: fp8, 8 heads, 32 of 65536 752 / 737, 64 of 65536 1504 / 1449, 128 of 32768 1558 / 1481; 16 heads, 256 of 4096, one split 860, two 780,
       // four 742), and of the next numbers of splits, while they leave 512 tokens, the first that leaves no compute unit without work in its last round (24 of 6000: 3 70.9, 4 62.9).
       const int64_t turn = 4 * TB * 2 * d * (cache == TQ_E4M3 ? 1 : 2), target = turn >= 65536 ? 256 : 512;
-      n = std::max((target + pairs - 1) / pairs, std::min((tokens + 2047) / 2048, std::max<int64_t>(4, 4096 / pairs)));
+      // Steps of more sequences than are shared out anew keep splits of 2048 tokens, since one may be far longer than the others, while partial results are 256 MiB at most.
+      const int64_t most = B > STEP_ROUND ? ((int64_t)256 << 20) / (4 * std::max<int64_t>(1, rows * Hq * d)) : 4096 / pairs;
+      n = std::max((target + pairs - 1) / pairs, std::min((tokens + 2047) / 2048, std::max<int64_t>(4, most)));
       double best = 0;
       for (int64_t i = n; i <= 2 * n && i <= std::max(n, tokens / 512); ++i) {
         const double full = double(pairs * i) / (256 * ((pairs * i + 255) / 256));
