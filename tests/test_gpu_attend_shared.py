@@ -18,10 +18,15 @@ UNEVEN = [61, 700, 3000, 9000]
 
 
 def check(s, q, got, window=None, sinks=0, every=1):
-    """Step.check's bounds, all rows of a sequence at once, every so many of them; rows behind the last sequence are not looked at."""
+    """Step.check's bounds, all rows of a sequence at once, every so many of them; rows behind the last sequence are not looked at.  An fp16 output of less than 2^-14
+    is rounded by up to 2^-25 whatever its size."""
     scale, step, at = 1 / math.sqrt(s.d), half_step(s.dtype), 0
     G = q.shape[1] // s.H
     for b, (n, run) in enumerate(zip(s.lens, s.runs)):
+        if run == 0 or n == 0:
+            assert (got[at: at + run] == 0).all()
+            at += run
+            continue
         pick = torch.arange(run)[(torch.arange(run) % every == 0) | (torch.arange(run) == run - 1)]
         k, v, there = (x.to(s.device) for x in s.tokens(b, n))
         p, t = (n - run + pick).to(s.device)[:, None], torch.arange(n, device=s.device)
@@ -39,7 +44,7 @@ def check(s, q, got, window=None, sinks=0, every=1):
             err = (2 * score + (n + 64) * STEP32 + 1.01 * step) * size
             mine = got[(at + pick).to(got.device), h * G: (h + 1) * G].reshape(-1, s.d).double()
             assert torch.isfinite(mine).all(), f"sequence {b} of {n}: not finite"
-            off, allowed = (mine - out).abs(), err + step * (out.abs() + err) + 1e-30
+            off, allowed = (mine - out).abs(), err + step * (out.abs() + err) + (2.0 ** -25 if s.dtype == torch.float16 else 1e-30)
             assert (off <= allowed).all(), f"sequence {b} of {n}, head {h}: off by {float((off / allowed).max()):.3g} of what is allowed"
         at += run
 

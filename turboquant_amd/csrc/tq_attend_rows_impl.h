@@ -15,15 +15,16 @@
 // Instructions of a wavefront follow one another: those of the vector unit stand between the matrix instructions (weights and values of the next sixteen tokens
 // beside the product of these; 256 channels 1541 -> 1331 us), keys are read four ahead, and turns come in pairs, so that buffers are constants in addresses
 // (64 channels 354 -> 345 us).
-// Bound by both kinds of instructions of two wavefronts on a SIMD (192 and 256 channels: one): a turn of 128 channels is 1024 cycles of matrix instructions and 160 vector ones, 32 of
+// Bound by both kinds of instructions of two wavefronts on a SIMD (192 and 256 channels: one): a turn of 128 channels is 1024 cycles of matrix instructions and 144 vector ones, 32 of
 // them exponentials.  bf16, 128 channels: 481 GFLOP in 460 us, 1.05 PFLOP/s, where a large product of the library reaches 1.40; with a window of 4096, one prompt of 8192, 413 in
-// 424; 64 channels 0.87, 192 0.79, 256 0.87 PFLOP/s; 8 bits, 128 channels 0.98 (fp16 queries with their two halves 0.71).  The clock falls as they are busier: with 16 bits straight to LDS a launch takes a fifth
+// 415; 64 channels 0.81, 192 0.83, 256 0.90 PFLOP/s; 8 bits, 128 channels 1.01 (fp16 queries with their two halves 0.73).  The clock falls as they are busier: with 16 bits straight to LDS a launch takes a fifth
 // fewer cycles and a tenth less time.  Eight wavefronts to a workgroup, which would load half as
 // often, 460 us, too; two tiles of rows to a wavefront, which would read LDS half as often, 64 channels 274, 128 627 (at one wavefront on a SIMD half of its registers are the
 // accumulators', and scores are copied out of them).  Without its reads of LDS a turn of 128 channels would take 0.78 of its time, without its loads 0.87, without exponentials 0.91.
 // With 32 tokens a turn and three wavefronts on a SIMD 128 channels take 413 us for 419 with the window and 511 for 467 without (512 workgroups at a time become 768, of 1024); the
 // next turn's scores computed ahead of this one's products take 41 - 264 registers more than there are.
-// LDS: 16-byte pieces of a row change places by the row (rows_key_turn, rows_value_turn), so that neither reads nor writes meet in a bank.
+// LDS: 16-byte pieces of a row change places by the row (rows_key_turn, rows_value_turn), so that reads do not meet in a bank, and 16 bits on their way in do not either; the stores of
+// converted 8 bits do, two to a bank (2.95e7 cycles of 1.18e8 that LDS is busy; see there).
 #pragma once
 
 #include "tq_attend.h"
@@ -73,7 +74,7 @@ __global__ void __launch_bounds__(256, (D <= 128 ? 2 : 1)) attend_rows_kernel(co
   constexpr int SIZE = F8 ? 1 : 2, ROW = D * 2;              // bytes of an element in the cache, of a row in LDS
   constexpr int LANES = D * SIZE / 16, LOADS = ROWS_TOKENS * LANES / 256;
   constexpr int KSTEPS = D / 16, TILES = D / 32, M = 128;
-    constexpr int KAHEAD = 4;                                  // reads of keys that are on their way at a time
+  constexpr int KAHEAD = 4;                                  // reads of keys that are on their way at a time
   constexpr int HALF = ROWS_TOKENS * ROW;                    // keys or values of a turn
   extern __shared__ __attribute__((aligned(16))) char s_rows[];
 
