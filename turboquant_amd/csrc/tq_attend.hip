@@ -78,7 +78,8 @@ static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 // other half of them 1.35, since some get two; two on all of them 2.05, so that the second gains little; 192 and 256 channels have one, 1.2), and a join is a launch and the
 // partial results' way out and back, 5 and 1 for 2 MB.  No split has less than four turns of 128 channels.  Measured (us; bf16, 32 query heads on 8 of 128, one sequence, 1 / 2 / 4 / 8 / 16 splits): 512
 // tokens, 512 rows 20 / 26 / 31 / 39; 1024, 1024 30 / 41 / 54 / 64; 4096, 64 rows 82 / 50 / 32 / 24 / 23, 512 rows 82 / 71 / 58 / 64 / 89; 16384, 64 rows
-// 309 / 165 / 90 / 54 / 42, 512 rows 305 / 199 / 152 / 158 / 175, 2048 rows 483 / 541 / 553 / 587 / 674.
+// 309 / 165 / 90 / 54 / 42, 512 rows 305 / 199 / 152 / 158 / 175, 2048 rows 483 / 541 / 553 / 587 / 674.  Other types and sizes go by the same numbers: bf16 and 8 bits, bf16 and fp16 queries, 64, 128 and 256 channels, 512
+// rows of 512, 64 and 512 of 4096 and 16384: never more than 9 % above the best of 1 .. 32 splits; 64 rows of 2048 at 256 channels, where the bound of four turns leaves four, 35 (fp16 queries over 8 bits 47) for 30 (35) with eight.
 static int64_t attend_rows_splits(int64_t pairs, int64_t blocks, int64_t rows, int d) {
   const int64_t most = std::min<int64_t>(blocks * 128 / (4 * std::max(d, 128)), JOIN_MAX_SPLITS);
   const double channels = d / 128.0, mb = (double)rows * d * 4e-6;

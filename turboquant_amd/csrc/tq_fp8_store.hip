@@ -2,7 +2,8 @@
 //
 // A wavefront takes one block of 16 tokens of one KV head, keys or values: its lanes hold the block's rows 8 neighbouring channels at a time (16 bytes of
 // 16-bit input, 8 of the cache), which is all of it, so that the largest value is a reduction over the wavefront and the block is read once.
-// Tokens that a block held before the step keep their bytes unless the block's exponent grows: then they are rounded again from what they stand for.
+// Tokens that a block held before the step keep their bytes unless the block's exponent grows: then they are rounded again from what they stand for.  It never shrinks before the
+// block starts anew: what was rounded away for a token that is written over later does not come back.
 // No two wavefronts write to one block of a head: a block belongs to one sequence.
 // Bound by the memory system where there are prompts (32768 rows, 8 heads of 128, bf16: write 44 us, 201 MB in and out, read 38, a launch each: 403 MB in 84 us, 4.8 TB/s; a
 // large copy reaches 5.1), by the chain of starts, lengths, table entry and rows where there are tokens (64 tokens: 4.6 and 5.2 us, of which a launch that does nothing is 2).

@@ -81,7 +81,8 @@ class Fp8PagedCache:
 
         A block's scale is the smallest power of two that brings its largest finite value to 448 at most; infinite values become the largest that
         it holds, NaN stays.  Tokens that a block holds already are rounded again where a new one needs a larger scale; a block whose first slot is written
-        starts anew.  A sequence's blocks must be its own while it writes to them; rows in front of token 0, behind the table or in blocks outside
+        starts anew.  (A sequence that steps back behind a refused token and writes another in its place keeps the scale that it had raised, and the bits that the block's
+        earlier tokens lost by it.)  A sequence's blocks must be its own while it writes to them; rows in front of token 0, behind the table or in blocks outside
         the cache are left out."""
         fast = _ffi.native()
         if fast is not None and fast.fp8_write(key, value, query_start_loc, block_table, seq_lens, *self.operands()):
