@@ -254,3 +254,15 @@ def test_starts_without_memory(calls):
         with pytest.raises(ValueError):
             call()
     assert not calls
+
+
+@pytest.mark.parametrize("table", [torch.zeros(1, 4, dtype=torch.int32), torch.zeros(4, dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int64), torch.zeros(2, 0, dtype=torch.int32)])
+def test_ingesting_needs_a_table_for_every_sequence(calls, table):
+    from turboquant_amd.integration.batched import BatchedLayerState
+    state = BatchedLayerState(config=None, quantizer=None, pool=None, fp8=cache8())
+    kv, lens = torch.zeros(2, 4, 16, 2, 64, dtype=torch.bfloat16), torch.tensor([20, 30])
+    with pytest.raises(ValueError):
+        state.ingest_paged_cache(kv, table, lens)
+    assert not calls and state.tokens_written == 0
+    state.ingest_paged_cache(kv, torch.zeros(3, 4, dtype=torch.int32), lens)
+    assert [name for name, _ in calls] == ["tq_fp8_write"] and state.tokens_written == 50

@@ -158,7 +158,9 @@ class BatchedLayerState:
 
     def _ingest_fp8(self, kv_cache, block_table, lens) -> None:
         """All sequences together, whole blocks of each (none is rounded twice) up to 65536 rows in all, gathered from their blocks."""
-        B, device = len(lens), block_table.device
+        B, device = len(lens), self.fp8.device
+        if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] < B or block_table.shape[1] == 0 or block_table.device != device:
+            raise ValueError(f"block_table must be int32 ({B}, max_pages) on {device}")
         table, num_blocks = block_table[:B], kv_cache.shape[1]
         piece = max(1, 65536 // PAGE_TOKENS // max(1, B)) * PAGE_TOKENS
         for first in range(0, max(lens, default=0), piece):
