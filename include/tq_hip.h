@@ -480,7 +480,7 @@ int tq_fp8_read(void *k_out, void *v_out, int dtype, int64_t rows, const int32_t
  * unused) or TQ_E4M3; d 64, 128, 192 or 256; Hq / Hkv any whole number up to 1024.  A row that sees nothing is zeros; tokens without a block in the cache have no weight.
  * query_start_loc null: a row per sequence (rows == B).  max_len bounds seq_lens and max_rows the rows of a sequence, for the plan: what exceeds them is right, too, and
  * slower.  n_split: 0, or how many workgroups share a row's tokens, up to 1024.  fill as tq_fp8_read.  workspace: tq_attend_bytes bytes (starts: whether there is a
- * query_start_loc), 16-byte aligned, of this call alone until it has run.  0: sizes out of range.                                   */
+ * query_start_loc), 16-byte aligned, of this call alone until it has run.  0: sizes out of range.  sm_scale: below 2^127.            */
 size_t tq_attend_bytes(int dtype, int cache, int starts, int64_t rows, int B, int Hq, int Hkv, int d, int64_t max_len, int64_t max_rows,
                        int64_t window, int sinks, int n_split);
 int tq_attend(const void *q, int dtype, int64_t rows, const int32_t *query_start_loc, int B, int Hq, int Hkv, int d, int cache,

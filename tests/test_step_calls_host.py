@@ -11,9 +11,16 @@ from turboquant_amd.fp8 import Fp8PagedCache
 from turboquant_amd.rotary import inverse_frequencies, rotate_heads
 
 
+_LIBRARY = _ffi.lib()
+
+
+def real_attend():
+    return _LIBRARY.tq_attend
+
+
 @pytest.fixture
 def calls(monkeypatch):
-    got, real = [], _ffi.lib()
+    got, real = [], _LIBRARY
 
     class Library:
         def __getattr__(self, name):
@@ -266,3 +273,20 @@ def test_ingesting_needs_a_table_for_every_sequence(calls, table):
     assert not calls and state.tokens_written == 0
     state.ingest_paged_cache(kv, torch.zeros(3, 4, dtype=torch.int32), lens)
     assert [name for name, _ in calls] == ["tq_fp8_write"] and state.tokens_written == 50
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 2.0 ** 127, -1e300])
+def test_a_factor_that_is_no_number_is_refused(calls, scale):
+    """Masked scores are -inf: times NaN or times infinity less infinity rows that see nothing would not be zeros."""
+    from tests.test_step_host import attend_args
+    assert real_attend()(*attend_args(scale=scale if abs(scale) < 1e39 else float("inf"))) == -1
+    cache, q = cache8(), torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    starts, table, lens = step(1, 1)
+    k = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    for call in (lambda: cache.attention(q, starts, table, lens, scale=scale), lambda: cache.decode_attention(q, table, lens, scale=scale),
+                 lambda: ExactPagedCache(k, k.clone()).decode_attention(q, table, lens, scale=scale, window=4)):
+        with pytest.raises(ValueError, match="scale"):
+            call()
+    assert not calls
+    cache.attention(q, starts, table, lens, scale=2.0 ** 126)
+    assert len(calls) == 1

@@ -18,6 +18,7 @@ from .paged import PAGE_TOKENS
 
 HEAD_DIMS = (64, 128, 192, 256)
 MAX_SPLITS = 1024
+MAX_SCALE = 2.0 ** 127              # (times log2 e it is a number in 32 bits)
 
 
 def sequences(device: torch.device, block_table: torch.Tensor, seq_lens: torch.Tensor, batch: int):
@@ -122,6 +123,8 @@ def attend(what: str, cache, query: torch.Tensor, query_start_loc: Optional[torc
         goes_by["query_start_loc"] = starts
     if scale is None:
         scale = 1.0 / math.sqrt(d)
+    elif not abs(scale) < MAX_SCALE:
+        raise ValueError(f"scale must be a number below 2^127, got {scale}")
     query = query.contiguous().resolve_neg()
     if query.data_ptr() % 16:
         query = query.clone()

@@ -195,6 +195,7 @@ extern "C" int tq_attend(const void* q, int dtype, int64_t rows, const int32_t* 
   if (!q || !out || !k_cache || !v_cache) return TQ_ENULL;
   AttendPlan p;
   if (!attend_plan(&p, dtype, cache, query_start_loc != nullptr, rows, B, Hq, Hkv, d, max_len, max_rows, window, sinks, n_split)) return TQ_EINVAL;
+  if (!(sm_scale > -0x1p127f && sm_scale < 0x1p127f)) return TQ_EINVAL;      // (masked scores are -inf, which a factor of NaN or infinity would not leave so)
   Attend a{};
   if (const int rc = step_init(&a.s, query_start_loc, rows, B, seq_lens, block_table, bt_stride, num_blocks)) return rc;
   if (cache == TQ_E4M3) {
