@@ -17,7 +17,6 @@ from .eviction import memory_of
 from .paged import PAGE_TOKENS
 
 HEAD_DIMS = (64, 128, 192, 256)
-MAX_SPLITS = 1024
 MAX_SCALE = 2.0 ** 127              # (times log2 e it is a number in 32 bits)
 
 
