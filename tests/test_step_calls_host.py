@@ -290,3 +290,16 @@ def test_a_factor_that_is_no_number_is_refused(calls, scale):
     assert not calls
     cache.attention(q, starts, table, lens, scale=2.0 ** 126)
     assert len(calls) == 1
+
+
+@pytest.mark.parametrize("planned", [16400, 32784, 100000, 1 << 20])
+def test_a_workspace_serves_narrower_tables(calls, planned):
+    """A workspace for up to so many tokens is enough for steps of that bound, however wide the table is that they come with."""
+    q = torch.zeros(1, 16, 256, dtype=torch.bfloat16)
+    cache = cache8(H=2, d=256)
+    work, rows = cache.workspace(1, 16, planned), cache.workspace(1, 16, planned, B=1)
+    for pages in (1, 64, 1000, 1024, 2048, planned // 16 + 1):
+        table, lens, starts = torch.zeros(1, pages, dtype=torch.int32), torch.tensor([10], dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32)
+        cache.decode_attention(q, table, lens, workspace=work, max_len=planned)
+        cache.attention(q, starts, table, lens, workspace=rows, max_len=planned)
+    assert len(calls) == 12

@@ -139,7 +139,8 @@ def attend(what: str, cache, query: torch.Tensor, query_start_loc: Optional[torc
             if overlaps(out, t):
                 raise ValueError(f"out must be memory of its own, it overlaps {name}")
     longest = table.shape[-1] * PAGE_TOKENS
-    max_len = longest if max_len is None else min(int(max_len), longest)
+    # (a plan for fewer tokens may take more memory: with a workspace of its own a call is planned by what it says, as the workspace was)
+    max_len = longest if max_len is None else (min(int(max_len), longest) if workspace is None else int(max_len))
     max_rows = rows if max_rows is None else int(max_rows)
     if rows == 0:
         return out

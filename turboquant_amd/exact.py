@@ -179,7 +179,8 @@ class ExactPagedCache:
 
         max_len and max_rows bound the lengths and a sequence's rows for the plan of the splits (without them the table's width and all rows
         do).  Of up to 32 rows x heads on a KV head and in decode steps the softmax's weights go into the product with the values as two numbers of the cache's
-        type, otherwise as one, half a step off.  The `workspace` of a step (`step_workspace()`) belongs to it alone until it has run: graphs that may run at the same time need one each."""
+        type, otherwise as one, half a step off.  The `workspace` of a step (`step_workspace()` of the same sizes and bounds) belongs to it alone until it has run: graphs that may
+        run at the same time need one each."""
         return attend("attention", self, query, query_start_loc, block_table, seq_lens, scale, window, sinks, n_split, workspace, out, max_len, max_rows)
 
     def step_workspace(self, rows: int, Hq: int, max_len: int, B: Optional[int] = None, max_rows: Optional[int] = None, window: Optional[int] = None,

@@ -187,7 +187,8 @@ class Fp8PagedCache:
 
         max_len and max_rows bound the lengths and a sequence's rows for the plan of the splits (without them the table's width and all rows
         do).  Of up to 32 rows x heads on a KV head, in decode steps and for fp16 queries the softmax's weights go into the product with the values as two
-        numbers of 16 bits, 2^-15 of a weight off, otherwise as one of the query's type, half a step off.  The `workspace` of a step (`workspace()`) belongs to it alone until it has run: graphs that may run at the same time need one each."""
+        numbers of 16 bits, 2^-15 of a weight off, otherwise as one of the query's type, half a step off.  The `workspace` of a step (`workspace()` of the
+        same sizes and bounds) belongs to it alone until it has run: graphs that may run at the same time need one each."""
         return attend("attention", self, query, query_start_loc, block_table, seq_lens, scale, window, sinks, n_split, workspace, out, max_len, max_rows)
 
     def workspace(self, rows: int, Hq: int, max_len: int, B: Optional[int] = None, max_rows: Optional[int] = None, window: Optional[int] = None,
