@@ -303,3 +303,14 @@ def test_a_workspace_serves_narrower_tables(calls, planned):
         cache.decode_attention(q, table, lens, workspace=work, max_len=planned)
         cache.attention(q, starts, table, lens, workspace=rows, max_len=planned)
     assert len(calls) == 12
+
+
+def test_more_workgroups_than_a_launch_has():
+    """A launch has less than 2^32 threads, 2^24 workgroups of 256: what takes more is refused in front of it."""
+    from tests.test_step_host import read_args, rotate_args, write_args
+    lib = _LIBRARY
+    assert lib.tq_rotate_heads(*rotate_args(rows=1 << 26)) == -1
+    assert lib.tq_fp8_write(*write_args(rows=1 << 28)) == -1 and lib.tq_fp8_read(*read_args(rows=1 << 28)) == -1
+    need = lambda rows, **kw: lib.tq_attend_bytes(*{**dict(dtype=2, cache=2, starts=1, rows=rows, B=4, Hq=32, Hkv=8, d=256, max_len=1 << 16, max_rows=rows, window=0, sinks=0, n_split=0), **kw}.values())
+    assert need(1 << 20) > 0 and need(1 << 17, n_split=128) == 0 and need(1 << 17, n_split=64) > 0                 # (the join of over 64 splits: a workgroup for 64 channels of a row)
+    assert need(1 << 24, Hkv=32, max_rows=1 << 24) == 0 and need(1 << 22, B=1 << 22, Hq=8, d=64, max_rows=1, max_len=16) == 0

@@ -176,7 +176,8 @@ static bool attend_plan(AttendPlan* p, int dtype, int cache, bool starts, int64_
   p->ml_at = at;      at = round256(at + places * sizeof(float2));
   p->acc_at = at;     at = round256(at + places * d * sizeof(float));
   p->bytes = std::max<size_t>(at, 256);
-  return p->grid <= INT32_MAX && (int64_t)all * (d / 64) <= INT32_MAX;
+  const int64_t joins = most <= 1 ? 0 : (p->few ? (int64_t)(all + 4 * p->few - 1) / (4 * p->few) : (int64_t)all * (d / 64));
+  return p->grid <= STEP_MAX_GROUPS && joins <= STEP_MAX_GROUPS && (int64_t)all * (d / 64) <= INT32_MAX;
 }
 
 }  // namespace tq

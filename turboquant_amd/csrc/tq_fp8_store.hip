@@ -236,7 +236,7 @@ static int store(Fp8Store& a, int dtype, bool write, hipStream_t st) {
   if (a.s.rows == 0) return TQ_OK;
   const int64_t units = store_units(a.s.rows, a.s.B);
   a.parts = store_parts(units, a.c.H, a.c.d, dtype);
-  if (units * a.parts > INT32_MAX) return TQ_EINVAL;
+  if (units * a.parts > STEP_MAX_GROUPS) return TQ_EINVAL;
   switch (dtype) {
     case TQ_F32: return launch_store<TQ_F32>(a, write, units * a.parts, st);
     case TQ_F16: return launch_store<TQ_F16>(a, write, units * a.parts, st);

@@ -8,7 +8,7 @@
 // first heads.  In turns and 64 bits, position * (inv_freq / 2 pi) less its whole turns: at position 2^20 an angle in 32 bits would be 0.03 off.
 // All sums, norms and rotations in 32 bits, one rounding at the end.  Bound by the memory system: 16384 tokens, 40 and 8 heads of 128, bf16 with norms, 403 MB in 80 us,
 // 5.0 TB/s (a large copy: 5.1); with four pairs a lane, 8 bytes a load, 145 us.  A step of 64 tokens, 5.8 us, is a launch, the positions' latency and the sines.
-#include "tq_common.h"
+#include "tq_step.h"
 
 #include <algorithm>
 
@@ -233,6 +233,7 @@ extern "C" int tq_rotate_heads(const void* q, const void* k, int dtype, int64_t 
   // Few tokens: one a workgroup, so that there are workgroups for the compute units; the sines of many are worked out 256 at a time.
   Rotate a{{q, k}, {q_out, k_out}, {q_weight, k_weight}, {qs_t, ks_t}, {qs_h, ks_h}, {qo_t, ko_t}, {qo_h, ko_h}, positions, inv_freq, rows, {Hq, Hkv}, d,
            rotary_dim, wide_positions, rows < 1024 ? 1 : ROTATE_TOKENS, eps};
+  if ((rows + a.tokens - 1) / a.tokens > STEP_MAX_GROUPS) return TQ_EINVAL;
   const unsigned grid = (unsigned)((rows + a.tokens - 1) / a.tokens);
   hipStream_t st = (hipStream_t)stream;
   bool wide = d % 16 == 0 && rotary_dim % 16 == 0 && ((uintptr_t)q | (uintptr_t)k | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)q_weight | (uintptr_t)k_weight) % 16 == 0;

@@ -6,6 +6,8 @@
 
 namespace tq {
 
+constexpr int64_t STEP_MAX_GROUPS = (1 << 24) - 1;      // of 256: a launch has less than 2^32 threads
+
 struct Step {
   const int32_t* starts;   // B + 1; null: one row per sequence
   const int32_t* lens;
